@@ -6,6 +6,7 @@
 // the call fails with a message instead of computing on the host.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -1031,6 +1032,204 @@ extern "C" int fh3_hip_attention_qkv_dev(const float *d_qkv, int n, int heads, i
     const int64_t inner = (int64_t)heads * hd;
     return attention_dev(d_qkv, d_qkv + inner, d_qkv + 2 * inner, 3 * inner, n, heads, hd, d_qnorm_w, d_knorm_w, eps,
                          d_cos, d_sin, rot_dim, d_o, stream, fn);
+}
+
+// ---------------------------------------------------------------------------
+// Packed sequences and the key/value cache (fh3_seqs.hip, fh3_kv.hip)
+// ---------------------------------------------------------------------------
+static size_t value_bytes(int type) {
+    return type == FH3_QUANT_F32 ? 4 : type == FH3_QUANT_F16 || type == FH3_QUANT_BF16 ? 2 : 0;
+}
+
+// One of the arrays of rows: its pointer and its row stride (0 = dense).
+static int check_rows(const void *p, int64_t *ld, int64_t width, int type, const char *what, const char *fn) {
+    if (!p) return set_err(FH3_E_INVALID, "%s: NULL %s", fn, what);
+    if (*ld == 0) *ld = width;
+    if ((uintptr_t)p & 15u || *ld < width || *ld > ((int64_t)1 << 32) || *ld * value_bytes(type) % 16)
+        return set_err(FH3_E_INVALID, "%s: rows of %s must be 16-byte aligned and not overlap", fn, what);
+    return FH3_OK;
+}
+
+static int check_seqs(Fh3kSeqs s, const char *fn) {
+    if (s.n_tok <= 0 || s.n_tok > (1 << 24) || s.n_seq <= 0 || s.n_seq > (1 << 20))
+        return set_err(FH3_E_INVALID, "%s: n_tok must be from 1 to 2^24 and n_seq from 1 to 2^20", fn);
+    if (s.first ? ((uintptr_t)s.first & 3u) != 0 : s.n_tok % s.n_seq != 0)
+        return set_err(FH3_E_INVALID, "%s: d_first misaligned, or NULL where n_tok is no multiple of n_seq", fn);
+    return FH3_OK;
+}
+
+static int check_attn(const Fh3AttnCfg *c, int n_tok, Fh3kAttn *a, const char *fn) {
+    if (!c || c->heads <= 0 || c->kv_heads <= 0 || c->heads % c->kv_heads || c->heads / c->kv_heads > 128)
+        return set_err(FH3_E_INVALID, "%s: heads must be a multiple of kv_heads, at most 128 to each", fn);
+    if (!fh3k_attn_head_dim_ok(c->head_dim))
+        return set_err(FH3_E_INVALID, "%s: head_dim %d is not supported (64 or 128)", fn, c->head_dim);
+    if (!value_bytes(c->type)) return set_err(FH3_E_INVALID, "%s: type %d is not F32, F16 or BF16", fn, c->type);
+    if (!(c->scale >= 0.f && c->scale <= 1e30f) || !(c->softcap >= 0.f && c->softcap <= 1e30f))
+        return set_err(FH3_E_INVALID, "%s: scale and softcap must be finite and not negative", fn);
+    if ((uintptr_t)c->d_slopes & 3u) return set_err(FH3_E_INVALID, "%s: d_slopes misaligned", fn);
+    if (n_tok > 0 && (int64_t)n_tok > ((int64_t)1 << 30) / c->heads)
+        return set_err(FH3_E_INVALID, "%s: n_tok * heads too large", fn);
+    *a = {c->heads, c->kv_heads, c->head_dim, c->type, c->causal != 0,
+          c->scale > 0.f ? c->scale : 1.0f / sqrtf((float)c->head_dim), c->softcap, c->d_slopes};
+    return FH3_OK;
+}
+
+static size_t kv_bytes_of(int kv_heads, int hd, int pages) { return (size_t)pages * kv_heads * 2 * FH3_KV_PAGE * hd; }
+
+extern "C" size_t fh3_hip_kv_pool_bytes(int kv_heads, int head_dim, int pages) {
+    if (kv_heads <= 0 || kv_heads > 4096 || pages <= 0 || !fh3k_attn_head_dim_ok(head_dim)) return 0;
+    return kv_bytes_of(kv_heads, head_dim, pages) + (size_t)pages * kv_heads * 2 * sizeof(float);
+}
+
+static int check_kv(const Fh3KvCache *kv, Fh3kKv *c, const char *fn) {
+    if (!kv || !fh3_hip_kv_pool_bytes(kv->kv_heads, kv->head_dim, kv->pages))
+        return set_err(FH3_E_INVALID, "%s: kv_heads from 1 to 4096, head_dim 64 or 128 and pages above 0 are needed", fn);
+    if (kv->max_pages <= 0 || kv->max_pages > (1 << 24))
+        return set_err(FH3_E_INVALID, "%s: max_pages must be from 1 to 2^24", fn);
+    if (!kv->d_pool || !kv->d_table || !kv->d_len || (uintptr_t)kv->d_pool & 15u || (uintptr_t)kv->d_table & 3u ||
+        (uintptr_t)kv->d_len & 3u)
+        return set_err(FH3_E_INVALID, "%s: pool, table and lengths must be set and aligned", fn);
+    uint8_t *pool = (uint8_t *)kv->d_pool;
+    *c = {kv->kv_heads, kv->head_dim, kv->pages, kv->max_pages, pool,
+          (float *)(pool + kv_bytes_of(kv->kv_heads, kv->head_dim, kv->pages)), kv->d_table, kv->d_len};
+    return FH3_OK;
+}
+
+// bytes from the first to the end of the last of n rows
+static size_t span(int64_t n, int64_t ld, int64_t width, int type) {
+    return (size_t)((n - 1) * ld + width) * value_bytes(type);
+}
+
+extern "C" int fh3_hip_attention_seqs_dev(const Fh3AttnCfg *c, const void *d_q, int64_t ldq, const void *d_k,
+                                          int64_t ldk, const void *d_v, int64_t ldv, void *d_o, int64_t ldo,
+                                          int n_tok, int n_seq, const int *d_first, const int *d_prefix,
+                                          void *stream) {
+    const char *fn = "fh3_hip_attention_seqs_dev";
+    Fh3kAttn a;
+    const Fh3kSeqs s = {d_first, n_tok, n_seq};
+    int rc = check_attn(c, n_tok, &a, fn);
+    if (rc == FH3_OK) rc = check_seqs(s, fn);
+    if (rc != FH3_OK) return rc;
+    const int64_t wq = (int64_t)a.heads * a.hd, wk = (int64_t)a.kv_heads * a.hd;
+    if ((rc = check_rows(d_q, &ldq, wq, a.type, "q", fn)) != FH3_OK) return rc;
+    if ((rc = check_rows(d_k, &ldk, wk, a.type, "k", fn)) != FH3_OK) return rc;
+    if ((rc = check_rows(d_v, &ldv, wk, a.type, "v", fn)) != FH3_OK) return rc;
+    if ((rc = check_rows(d_o, &ldo, wq, a.type, "o", fn)) != FH3_OK) return rc;
+    if ((uintptr_t)d_prefix & 3u) return set_err(FH3_E_INVALID, "%s: d_prefix misaligned", fn);
+    const size_t on = span(n_tok, ldo, wq, a.type);
+    if (overlap(d_o, on, d_q, span(n_tok, ldq, wq, a.type)) || overlap(d_o, on, d_k, span(n_tok, ldk, wk, a.type)) ||
+        overlap(d_o, on, d_v, span(n_tok, ldv, wk, a.type)))
+        return set_err(FH3_E_INVALID, "%s: o overlaps an input", fn);
+    if ((rc = ensure_init()) != FH3_OK) return rc;
+    FragRt::On on_device(g.device);
+    FH3_HIPCALL(fh3k_attn_seqs(&a, d_q, ldq, d_k, ldk, d_v, ldv, d_o, ldo, s, d_prefix,
+                               stream ? (hipStream_t)stream : g.stream));
+    return FH3_OK;
+}
+
+extern "C" int fh3_hip_kv_extend_dev(const Fh3KvCache *kv, int n_tok, int n_seq, const int *d_first, void *stream) {
+    const char *fn = "fh3_hip_kv_extend_dev";
+    Fh3kKv k;
+    const Fh3kSeqs s = {d_first, n_tok, n_seq};
+    int rc = check_kv(kv, &k, fn);
+    if (rc == FH3_OK) rc = check_seqs(s, fn);
+    if (rc == FH3_OK) rc = ensure_init();
+    if (rc != FH3_OK) return rc;
+    FragRt::On on_device(g.device);
+    FH3_HIPCALL(fh3k_kv_extend(kv->d_len, s, stream ? (hipStream_t)stream : g.stream));
+    return FH3_OK;
+}
+
+static int kv_rows(const Fh3KvCache *kv, int type, const void *d_k, int64_t *ldk, const void *d_v, int64_t *ldv,
+                   Fh3kSeqs s, Fh3kKv *k, const char *fn) {
+    int rc = check_kv(kv, k, fn);
+    if (rc == FH3_OK) rc = check_seqs(s, fn);
+    if (rc != FH3_OK) return rc;
+    if (!value_bytes(type)) return set_err(FH3_E_INVALID, "%s: type %d is not F32, F16 or BF16", fn, type);
+    if ((int64_t)s.n_tok > ((int64_t)1 << 30) / k->kv_heads)
+        return set_err(FH3_E_INVALID, "%s: n_tok * kv_heads too large", fn);
+    const int64_t w = (int64_t)k->kv_heads * k->hd;
+    if (d_k && (rc = check_rows(d_k, ldk, w, type, "k", fn)) != FH3_OK) return rc;
+    if (d_v && (rc = check_rows(d_v, ldv, w, type, "v", fn)) != FH3_OK) return rc;
+    return FH3_OK;
+}
+
+extern "C" int fh3_hip_kv_append_dev(const Fh3KvCache *kv, int type, const void *d_k, int64_t ldk, const void *d_v,
+                                     int64_t ldv, int n_tok, int n_seq, const int *d_first, void *stream) {
+    const char *fn = "fh3_hip_kv_append_dev";
+    Fh3kKv k;
+    const Fh3kSeqs s = {d_first, n_tok, n_seq};
+    int rc = kv_rows(kv, type, d_k, &ldk, d_v, &ldv, s, &k, fn);
+    if (rc != FH3_OK) return rc;
+    if (!d_k || !d_v) return set_err(FH3_E_INVALID, "%s: NULL k or v", fn);
+    if ((rc = ensure_init()) != FH3_OK) return rc;
+    FragRt::On on_device(g.device);
+    FH3_HIPCALL(fh3k_kv_append(&k, type, d_k, ldk, d_v, ldv, s, stream ? (hipStream_t)stream : g.stream));
+    return FH3_OK;
+}
+
+extern "C" int fh3_hip_kv_read_dev(const Fh3KvCache *kv, int type, void *d_k, int64_t ldk, void *d_v, int64_t ldv,
+                                   int n_tok, int n_seq, const int *d_first, void *stream) {
+    const char *fn = "fh3_hip_kv_read_dev";
+    Fh3kKv k;
+    const Fh3kSeqs s = {d_first, n_tok, n_seq};
+    int rc = kv_rows(kv, type, d_k, &ldk, d_v, &ldv, s, &k, fn);
+    if (rc != FH3_OK) return rc;
+    if (!d_k && !d_v) return set_err(FH3_E_INVALID, "%s: NULL k and v", fn);
+    if ((rc = ensure_init()) != FH3_OK) return rc;
+    FragRt::On on_device(g.device);
+    FH3_HIPCALL(fh3k_kv_read(&k, type, d_k, ldk, d_v, ldv, s, stream ? (hipStream_t)stream : g.stream));
+    return FH3_OK;
+}
+
+// The checks that the workspace's size depends on.
+static int check_kv_attn(const Fh3AttnCfg *c, const Fh3KvCache *kv, Fh3kSeqs s, Fh3kAttn *a, const char *fn) {
+    int rc = check_attn(c, s.n_tok, a, fn);
+    if (rc == FH3_OK) rc = check_seqs(s, fn);
+    if (rc != FH3_OK) return rc;
+    if (!kv || kv->kv_heads != a->kv_heads || kv->head_dim != a->hd || kv->max_pages <= 0 ||
+        kv->max_pages > (1 << 24))
+        return set_err(FH3_E_INVALID, "%s: the cache's heads, head_dim or max_pages do not fit", fn);
+    return FH3_OK;
+}
+
+extern "C" size_t fh3_hip_kv_attention_workspace_bytes(const Fh3AttnCfg *c, const Fh3KvCache *kv, int n_tok,
+                                                       int n_seq) {
+    Fh3kAttn a;
+    // the size does not depend on how the rows are shared out, so any alignment of d_first stands for it
+    static const int some[1] = {0};
+    const Fh3kSeqs s = {some, n_tok, n_seq};
+    if (check_kv_attn(c, kv, s, &a, "fh3_hip_kv_attention_workspace_bytes") != FH3_OK) return 0;
+    const Fh3kKv k = {kv->kv_heads, kv->head_dim, kv->pages, kv->max_pages, nullptr, nullptr, nullptr, nullptr};
+    return fh3k_kv_attn_ws_bytes(&a, &k, s);
+}
+
+extern "C" int fh3_hip_kv_attention_dev(const Fh3AttnCfg *c, const Fh3KvCache *kv, const void *d_q, int64_t ldq,
+                                        void *d_o, int64_t ldo, int n_tok, int n_seq, const int *d_first, void *d_ws,
+                                        size_t ws_bytes, void *stream) {
+    const char *fn = "fh3_hip_kv_attention_dev";
+    Fh3kAttn a;
+    Fh3kKv k;
+    const Fh3kSeqs s = {d_first, n_tok, n_seq};
+    int rc = check_kv_attn(c, kv, s, &a, fn);
+    if (rc == FH3_OK) rc = check_kv(kv, &k, fn);
+    if (rc != FH3_OK) return rc;
+    const int64_t w = (int64_t)a.heads * a.hd;
+    if ((rc = check_rows(d_q, &ldq, w, a.type, "q", fn)) != FH3_OK) return rc;
+    if ((rc = check_rows(d_o, &ldo, w, a.type, "o", fn)) != FH3_OK) return rc;
+    const size_t need = fh3k_kv_attn_ws_bytes(&a, &k, s), on = span(n_tok, ldo, w, a.type);
+    if (ws_bytes < need || (need && (!d_ws || (uintptr_t)d_ws & 15u)))
+        return set_err(FH3_E_INVALID, "%s: a 16-byte aligned workspace of %zu bytes is needed (%zu given)", fn, need,
+                       ws_bytes);
+    const size_t pool = fh3_hip_kv_pool_bytes(k.kv_heads, k.hd, k.pages);
+    if (overlap(d_o, on, d_q, span(n_tok, ldq, w, a.type)) || overlap(d_o, on, kv->d_pool, pool) ||
+        (need && (overlap(d_ws, need, d_q, span(n_tok, ldq, w, a.type)) || overlap(d_ws, need, d_o, on) ||
+                  overlap(d_ws, need, kv->d_pool, pool))))
+        return set_err(FH3_E_INVALID, "%s: o or the workspace overlaps another array", fn);
+    if ((rc = ensure_init()) != FH3_OK) return rc;
+    FragRt::On on_device(g.device);
+    FH3_HIPCALL(fh3k_kv_attn(&a, &k, d_q, ldq, d_o, ldo, s, d_ws, stream ? (hipStream_t)stream : g.stream));
+    return FH3_OK;
 }
 
 // ---------------------------------------------------------------------------

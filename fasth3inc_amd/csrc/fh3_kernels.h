@@ -171,6 +171,34 @@ hipError_t fh3k_vsa_attention(const float *q, const float *k, const float *v, in
                               const int *gather, const int *cnt, int T, int P, int kv, int all, float scale, void *ws,
                               hipStream_t st);
 
+// Packed sequences (fh3_seqs.hip, fh3_kv.hip): the rows of each, as fh3_hip.h
+// says; first may be NULL.  Arguments are checked by the callers.
+typedef struct Fh3kSeqs {
+    const int *first;
+    int n_tok, n_seq;
+} Fh3kSeqs;
+typedef struct Fh3kAttn {
+    int heads, kv_heads, hd, type, causal;
+    float scale, softcap;
+    const float *slopes;
+} Fh3kAttn;
+typedef struct Fh3kKv {
+    int kv_heads, hd, pages, max_pages;
+    uint8_t *pool;
+    float *scales;
+    const int *table, *len;
+} Fh3kKv;
+hipError_t fh3k_attn_seqs(const Fh3kAttn *a, const void *q, int64_t ldq, const void *k, int64_t ldk, const void *v,
+                          int64_t ldv, void *o, int64_t ldo, Fh3kSeqs s, const int *prefix, hipStream_t st);
+hipError_t fh3k_kv_extend(int *len, Fh3kSeqs s, hipStream_t st);
+hipError_t fh3k_kv_append(const Fh3kKv *c, int type, const void *k, int64_t ldk, const void *v, int64_t ldv,
+                          Fh3kSeqs s, hipStream_t st);
+hipError_t fh3k_kv_read(const Fh3kKv *c, int type, void *k, int64_t ldk, void *v, int64_t ldv, Fh3kSeqs s,
+                        hipStream_t st);
+size_t fh3k_kv_attn_ws_bytes(const Fh3kAttn *a, const Fh3kKv *c, Fh3kSeqs s);
+hipError_t fh3k_kv_attn(const Fh3kAttn *a, const Fh3kKv *c, const void *q, int64_t ldq, void *o, int64_t ldo,
+                        Fh3kSeqs s, void *ws, hipStream_t st);
+
 // Largest in-dimension (K) the activation preparation handles.
 int fh3k_max_in(void);
 

@@ -74,6 +74,18 @@ class Fh3Seq(ctypes.Structure):          # include/fh3/fh3.h (the reference's la
                 ("pos", ctypes.c_void_p), ("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p)]
 
 
+class Fh3AttnCfg(ctypes.Structure):      # include/fh3/fh3_hip.h
+    _fields_ = [("heads", ctypes.c_int), ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("type", ctypes.c_int), ("causal", ctypes.c_int), ("scale", ctypes.c_float),
+                ("softcap", ctypes.c_float), ("d_slopes", ctypes.c_void_p)]
+
+
+class Fh3KvCache(ctypes.Structure):      # include/fh3/fh3_hip.h
+    _fields_ = [("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("pages", ctypes.c_int),
+                ("max_pages", ctypes.c_int), ("d_pool", ctypes.c_void_p), ("d_table", ctypes.c_void_p),
+                ("d_len", ctypes.c_void_p)]
+
+
 class Fh3LayerView(ctypes.Structure):
     _fields_ = [(n, Fh3W) for n in LAYER_TENSORS]
 
@@ -180,6 +192,20 @@ SIGNATURES = {
                                        _c_void_p]),
     "fh3_hip_attention_qkv_dev": (_c_int, [_c_void_p, _c_int, _c_int, _c_int, _c_void_p, _c_void_p, ctypes.c_float,
                                            _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p]),
+    "fh3_hip_attention_seqs_dev": (_c_int, [ctypes.POINTER(Fh3AttnCfg), _c_void_p, _c_i64, _c_void_p, _c_i64,
+                                            _c_void_p, _c_i64, _c_void_p, _c_i64, _c_int, _c_int, _c_void_p,
+                                            _c_void_p, _c_void_p]),
+    "fh3_hip_kv_pool_bytes": (_c_size, [_c_int, _c_int, _c_int]),
+    "fh3_hip_kv_extend_dev": (_c_int, [ctypes.POINTER(Fh3KvCache), _c_int, _c_int, _c_void_p, _c_void_p]),
+    "fh3_hip_kv_append_dev": (_c_int, [ctypes.POINTER(Fh3KvCache), _c_int, _c_void_p, _c_i64, _c_void_p, _c_i64,
+                                       _c_int, _c_int, _c_void_p, _c_void_p]),
+    "fh3_hip_kv_read_dev": (_c_int, [ctypes.POINTER(Fh3KvCache), _c_int, _c_void_p, _c_i64, _c_void_p, _c_i64,
+                                     _c_int, _c_int, _c_void_p, _c_void_p]),
+    "fh3_hip_kv_attention_workspace_bytes": (_c_size, [ctypes.POINTER(Fh3AttnCfg), ctypes.POINTER(Fh3KvCache),
+                                                       _c_int, _c_int]),
+    "fh3_hip_kv_attention_dev": (_c_int, [ctypes.POINTER(Fh3AttnCfg), ctypes.POINTER(Fh3KvCache), _c_void_p, _c_i64,
+                                          _c_void_p, _c_i64, _c_int, _c_int, _c_void_p, _c_void_p, _c_size,
+                                          _c_void_p]),
     "fh3_hip_vsa_attention_dev": (_c_int, [ctypes.POINTER(Fh3VsaCfg), _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                                            _c_void_p, ctypes.POINTER(Fh3Seq), _c_int, _c_int, _c_void_p]),
     "fh3_hip_vsa_attention_qkv_dev": (_c_int, [ctypes.POINTER(Fh3VsaCfg), _c_void_p, _c_void_p, _c_void_p,
@@ -459,6 +485,60 @@ def attention_host(q, k, v):
     n, heads, hd = q.shape
     lib().fh3_attention(_p(q), _p(k), _p(v), _p(o), n, heads, hd)
     return o
+
+
+KV_PAGE = 64   # FH3_KV_PAGE
+
+
+def attn_cfg(heads, kv_heads, hd, qtype=FH3_QUANT_F32, causal=True, scale=0.0, softcap=0.0, d_slopes=None):
+    """An Fh3AttnCfg; d_slopes: device fp32 [heads], kept alive by the caller."""
+    return Fh3AttnCfg(heads, kv_heads, hd, qtype, int(causal), scale, softcap, _ptr_of(d_slopes))
+
+
+def attention_seqs_dev(cfg, d_q, d_k, d_v, d_o, n_tok, n_seq=1, d_first=None, d_prefix=None, ldq=0, ldk=0, ldv=0,
+                       ldo=0, stream_ptr=None):
+    """fh3_hip_attention_seqs_dev: attention within packed sequences, shared key heads."""
+    _check(lib().fh3_hip_attention_seqs_dev(ctypes.byref(cfg), _ptr_of(d_q), ldq, _ptr_of(d_k), ldk, _ptr_of(d_v),
+                                            ldv, _ptr_of(d_o), ldo, n_tok, n_seq, _ptr_of(d_first),
+                                            _ptr_of(d_prefix), stream_ptr), "fh3_hip_attention_seqs_dev")
+
+
+def kv_pool_bytes(kv_heads, hd, pages):
+    return lib().fh3_hip_kv_pool_bytes(kv_heads, hd, pages)
+
+
+def kv_cache(kv_heads, hd, pages, max_pages, d_pool, d_table, d_len):
+    """An Fh3KvCache over device buffers that the caller keeps alive."""
+    return Fh3KvCache(kv_heads, hd, pages, max_pages, _ptr_of(d_pool), _ptr_of(d_table), _ptr_of(d_len))
+
+
+def kv_extend_dev(kv, n_tok, n_seq, d_first=None, stream_ptr=None):
+    """fh3_hip_kv_extend_dev: every sequence's length grows by its new rows."""
+    _check(lib().fh3_hip_kv_extend_dev(ctypes.byref(kv), n_tok, n_seq, _ptr_of(d_first), stream_ptr),
+           "fh3_hip_kv_extend_dev")
+
+
+def kv_append_dev(kv, qtype, d_k, d_v, n_tok, n_seq, d_first=None, ldk=0, ldv=0, stream_ptr=None):
+    """fh3_hip_kv_append_dev: new rows quantised into the cache."""
+    _check(lib().fh3_hip_kv_append_dev(ctypes.byref(kv), qtype, _ptr_of(d_k), ldk, _ptr_of(d_v), ldv, n_tok, n_seq,
+                                       _ptr_of(d_first), stream_ptr), "fh3_hip_kv_append_dev")
+
+
+def kv_read_dev(kv, qtype, d_k, d_v, n_tok, n_seq, d_first=None, ldk=0, ldv=0, stream_ptr=None):
+    """fh3_hip_kv_read_dev: the rows' cached values."""
+    _check(lib().fh3_hip_kv_read_dev(ctypes.byref(kv), qtype, _ptr_of(d_k), ldk, _ptr_of(d_v), ldv, n_tok, n_seq,
+                                     _ptr_of(d_first), stream_ptr), "fh3_hip_kv_read_dev")
+
+
+def kv_attention_workspace_bytes(cfg, kv, n_tok, n_seq):
+    return lib().fh3_hip_kv_attention_workspace_bytes(ctypes.byref(cfg), ctypes.byref(kv), n_tok, n_seq)
+
+
+def kv_attention_dev(cfg, kv, d_q, d_o, n_tok, n_seq, d_ws, ws_bytes, d_first=None, ldq=0, ldo=0, stream_ptr=None):
+    """fh3_hip_kv_attention_dev: the new rows' attention over the cache."""
+    _check(lib().fh3_hip_kv_attention_dev(ctypes.byref(cfg), ctypes.byref(kv), _ptr_of(d_q), ldq, _ptr_of(d_o), ldo,
+                                          n_tok, n_seq, _ptr_of(d_first), _ptr_of(d_ws), ws_bytes, stream_ptr),
+           "fh3_hip_kv_attention_dev")
 
 
 def seq_of(n, num_text=0, num_audio=0, num_video=None, grid=(0, 0, 0)):

@@ -189,6 +189,123 @@ int fh3_hip_vsa_attention_qkv_dev(const Fh3VsaCfg *c, const float *d_qkv, const 
                                   int rot_dim, const float *d_gate, float *d_o, const Fh3Seq *seq, int heads,
                                   int head_dim, void *stream);
 
+/* Attention over packed sequences (a text encoder's layer; the reference's is
+ * the causal attention of src/model/fh3_te.c:242-302).  Query head h reads key
+ * head h / (heads / kv_heads); row i of a sequence gets
+ *   o_i = sum_j softmax_j(s_ij) v_j,  s_ij = scale * q_i . k_j,
+ * over the keys j of its own sequence that it sees, where s_ij is replaced by
+ * softcap * tanh(s_ij / softcap) when softcap > 0 and d_slopes[h] * |i - j| is
+ * then subtracted when d_slopes is set.  A row that sees no key gets zeros.
+ *   heads, kv_heads  heads % kv_heads == 0, heads / kv_heads <= 128
+ *   head_dim         64 or 128
+ *   type             of q, k, v and o: FH3_QUANT_F32, _F16 or _BF16
+ *   causal           non-zero: row i sees keys j <= i (and the prefix); zero: all
+ *   scale            0 means 1 / sqrt(head_dim)
+ *   softcap          0 means none
+ *   d_slopes         NULL, or device [heads]
+ * F16 and BF16 operands enter the matrix products as they are, F32 ones as two
+ * 16-bit terms each (the result is that of fp32 arithmetic to about 1e-6);
+ * softmax and sums are fp32, the weights are rounded to the operand type for the
+ * second product (F32: two terms).  Deterministic. */
+typedef struct Fh3AttnCfg {
+    int heads;
+    int kv_heads;
+    int head_dim;
+    int type;
+    int causal;
+    float scale;
+    float softcap;
+    const float *d_slopes;
+} Fh3AttnCfg;
+
+/* q [n_tok][heads][head_dim], k and v [n_tok][kv_heads][head_dim], o as q, at
+ * ldq, ldk, ldv, ldo values per token (0 = dense), so that q, k and v may be
+ * parts of one projection's output.  Sequence s is the rows d_first[s] ..
+ * d_first[s + 1] - 1 (device [n_seq + 1], non-decreasing, within n_tok); with
+ * d_first NULL the rows are n_seq sequences of n_tok / n_seq.  Rows behind the
+ * last sequence are neither read nor written.  d_prefix (NULL, or device
+ * [n_seq]): the first d_prefix[s] tokens are seen by every row of sequence s,
+ * causal or not.  Pointers and row starts 16-byte aligned; o must not overlap
+ * the inputs.  A NaN or infinity in a key or value makes the rows that see it
+ * non-finite (at the least in the channels that hold it) and no other row.  No
+ * workspace: calls on different streams do not disturb each other. */
+int fh3_hip_attention_seqs_dev(const Fh3AttnCfg *c, const void *d_q, int64_t ldq, const void *d_k, int64_t ldk,
+                               const void *d_v, int64_t ldv, void *d_o, int64_t ldo, int n_tok, int n_seq,
+                               const int *d_first, const int *d_prefix, void *stream);
+
+/* A key/value cache in 8 bits for n_seq sequences of one layer.  Tokens stand
+ * in pages of FH3_KV_PAGE; a page holds, for each key head, K and V as integers
+ * q in [-127, 127] with one fp32 scale each, a power of two: value = q * scale.
+ *   pages      pages in the pool
+ *   max_pages  columns of d_table
+ *   d_pool     fh3_hip_kv_pool_bytes(...) device bytes, 16-byte aligned
+ *   d_table    device [n_seq][max_pages]: the page that holds tokens
+ *              FH3_KV_PAGE * p .. of a sequence; an entry outside the pool is a
+ *              page that holds nothing (not written, not seen, read as zeros)
+ *   d_len      device [n_seq]: tokens held, the new ones of this step among them
+ * The table and the lengths are shared by all layers of a model, the pool is
+ * one layer's.  Pages may be shared between sequences as long as no call appends
+ * to them.
+ * Layout: pages in order, in each its heads, of each the K and then the V bytes
+ * (q + 128); behind all pages the scales [pages][kv_heads][K, V].  K of token
+ * 16 t + i, channel 64 c + 16 g + b is byte ((t * head_dim / 64 + c) * 4 + g) *
+ * 256 + 16 i + b; V of token 16 t + 4 g + r, channel 16 c + i is byte (4 c + g) *
+ * 256 + 16 i + 4 t + r: the orders in which the matrix cores take them. */
+#define FH3_KV_PAGE 64
+typedef struct Fh3KvCache {
+    int kv_heads;
+    int head_dim;
+    int pages;
+    int max_pages;
+    void *d_pool;
+    const int *d_table;
+    int *d_len;
+} Fh3KvCache;
+
+/* 0 for sizes that are not supported. */
+size_t fh3_hip_kv_pool_bytes(int kv_heads, int head_dim, int pages);
+
+/* In the calls below sequence s has the rows d_first[s] .. d_first[s + 1] - 1 of
+ * the n_tok given (or n_tok / n_seq each with d_first NULL), as above; they are
+ * its last tokens, at positions d_len[s] - count .. d_len[s] - 1.  Tokens whose
+ * position is negative or past the table's end are not held.  All are enqueued
+ * on `stream` without synchronising, allocate nothing and may be captured; a
+ * captured call reads the lengths and the table anew at each replay.
+ *
+ * fh3_hip_kv_extend_dev: d_len[s] += count (once a step, before the layers).
+ *
+ * fh3_hip_kv_append_dev: write the rows k and v ([n_tok][kv_heads][head_dim] of
+ * `type` F32, F16 or BF16, ldk and ldv values per token, 0 = dense) to the
+ * cache.  The scale of a page, head and K or V is the least 2^e, e >= -100, with
+ * amax <= 127 * 2^e over the finite values of its tokens; q = value / scale
+ * rounded to nearest even, an infinity +-127, a NaN 0.  Where new tokens raise
+ * the scale of a page that holds earlier ones, those are rounded again to it.
+ * Appending the same rows at the same positions again changes nothing.
+ *
+ * fh3_hip_kv_read_dev: the rows' cached values as `type` (for export, or a
+ * prefix that another program attends to).  K or V may be NULL. */
+int fh3_hip_kv_extend_dev(const Fh3KvCache *kv, int n_tok, int n_seq, const int *d_first, void *stream);
+int fh3_hip_kv_append_dev(const Fh3KvCache *kv, int type, const void *d_k, int64_t ldk, const void *d_v, int64_t ldv,
+                          int n_tok, int n_seq, const int *d_first, void *stream);
+int fh3_hip_kv_read_dev(const Fh3KvCache *kv, int type, void *d_k, int64_t ldk, void *d_v, int64_t ldv, int n_tok,
+                        int n_seq, const int *d_first, void *stream);
+
+/* The rows' attention over the cache: q and o as in fh3_hip_attention_seqs_dev,
+ * keys and values of the row's sequence from the cache (the row's own among
+ * them: append first), distances between positions.  causal: a row sees the
+ * positions up to its own; otherwise all d_len[s].  The cached integers are exact in
+ * the fp16 matrix products; q is scaled by a power of two for each row and
+ * rounded to fp16 (F16 and BF16: exact but for values 2^-24 below the row's
+ * largest; F32: two terms), the weights too (F32: two terms).  The work is split
+ * over the keys by the lengths on the device; d_ws (16-byte aligned,
+ * fh3_hip_kv_attention_workspace_bytes, may be 0) holds the parts until a
+ * second kernel joins them in order: deterministic.  Calls that may overlap need
+ * a workspace each. */
+size_t fh3_hip_kv_attention_workspace_bytes(const Fh3AttnCfg *c, const Fh3KvCache *kv, int n_tok, int n_seq);
+int fh3_hip_kv_attention_dev(const Fh3AttnCfg *c, const Fh3KvCache *kv, const void *d_q, int64_t ldq, void *d_o,
+                             int64_t ldo, int n_tok, int n_seq, const int *d_first, void *d_ws, size_t ws_bytes,
+                             void *stream);
+
 /* Weight registration (the boundary's "host data -> device pointer" hook).
  * fh3_hip_register_weights uploads [host, host + bytes) once and keeps the
  * copy on the device; the host-pointer wrappers fh3_matmul / fh3_dequant then
