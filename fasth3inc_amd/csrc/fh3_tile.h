@@ -1,0 +1,250 @@
+// fh3_tile.h -- one wavefront's 32 query rows against 64-key tiles in LDS, for
+// the kernels over packed sequences (fh3_seqs.hip) and the 8-bit cache (fh3_kv.hip).
+//
+// S^T = K Q^T and O^T = V^T P^T on 32x32x16 matrix products: a lane holds one row
+// (lane & 31) and, of each 32 keys, those with (key >> 2) & 1 == lane >> 5, so the
+// softmax needs no exchange between lanes but the last sums, and the weights go
+// from the first product's registers straight into the second's operand.  The
+// rows of a tile are (token, query head of the group) pairs of one key head, so
+// shared key heads fill the tile.
+#ifndef FH3_TILE_H
+#define FH3_TILE_H
+
+#include "fh3_seqs.h"
+
+namespace {
+
+constexpr int TILE_K = 64;   // keys per tile
+constexpr int WAVE_R = 32;   // rows per wavefront
+// Weights are exp2(t - m) where m is raised only when a tile's largest t exceeds
+// it by more than RAISE: the weights stay within 2^-OFFSET .. 2^RAISE of what a
+// fresh maximum would give, and most tiles need no rescale of the sums.  The
+// offset keeps small weights out of fp16's subnormal range (2^14 < 65504).
+constexpr float OFFSET = 6.f, RAISE = 14.f;
+constexpr float M_NONE = -1e30f;  // no key seen yet: finite, so that masked t = -inf gives 0
+
+template <class T> struct Vec;
+template <> struct Vec<_Float16> { typedef half8 v8; };
+template <> struct Vec<__bf16> { typedef bf8 v8; };
+
+__device__ __forceinline__ f32x16 mfma32(half8 a, half8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(bf8 a, bf8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// What every row of a call shares.
+struct Score {
+    float f;        // product sum -> t (log2 units), or -> 2 log2(e) x / cap before the tanh
+    float cap2;     // cap * log2(e), or 0
+    bool bias;
+};
+__device__ __forceinline__ Score score_of(const Fh3kAttn &a) {
+    Score sc;
+    sc.cap2 = a.softcap > 0.f ? a.softcap * LOG2E : 0.f;
+    sc.f = a.softcap > 0.f ? 2.f * LOG2E * (a.scale / a.softcap) : a.scale * LOG2E;
+    sc.bias = a.slopes != nullptr;
+    return sc;
+}
+// cap tanh(x / cap) from y = 2 log2(e) x / cap: tanh = 1 - 2 / (1 + e^2z)
+__device__ __forceinline__ float capped(float y, float cap2) {
+    return cap2 - 2.f * cap2 * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(y));
+}
+
+// 2^e such that amax * 2^e lies in [2^13, 2^14); 1 for zeros and values that are not finite.
+__device__ __forceinline__ float pow2_to_14(float amax) {
+    int e = 13 - ((int)(__builtin_bit_cast(uint32_t, amax) >> 23) - 127);
+    e = e > 126 ? 126 : e;
+    return amax > 0.f && amax <= 3.402823466e38f ? __builtin_bit_cast(float, (uint32_t)(e + 127) << 23) : 1.f;
+}
+
+// eight consecutive values of a row
+__device__ __forceinline__ void load8(const void *p, int type, int64_t at, float (&x)[8]) {
+    if (type == FH3K_F32) {
+        const f32x4 *q = (const f32x4 *)((const float *)p + at);
+        const f32x4 a = q[0], b = q[1];
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = a[i], x[4 + i] = b[i];
+    } else if (type == FH3K_F16) {
+        const half8 a = *(const half8 *)((const _Float16 *)p + at);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = (float)a[i];
+    } else {
+        const u32x4 a = *(const u32x4 *)((const uint16_t *)p + at);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            x[i] = __builtin_bit_cast(float, i & 1 ? a[i >> 1] & 0xFFFF0000u : a[i >> 1] << 16);
+    }
+}
+// four consecutive values of an output row
+__device__ __forceinline__ void store4(void *p, int type, int64_t at, f32x4 x) {
+    if (type == FH3K_F32) *(f32x4 *)((float *)p + at) = x;
+    else if (type == FH3K_F16) {
+        half4 h;
+#pragma unroll
+        for (int i = 0; i < 4; i++) h[i] = (_Float16)x[i];
+        *(half4 *)((_Float16 *)p + at) = h;
+    } else {
+        const u32x2 h = {__builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x[0], x[1]}, bf2)),
+                         __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x[2], x[3]}, bf2))};
+        *(u32x2 *)((uint16_t *)p + at) = h;
+    }
+}
+
+// two terms of 16 bits: x ~ hi + lo, both rounded to nearest
+template <class T> struct Two { T hi, lo; };
+template <class T> __device__ __forceinline__ Two<T> split(float x) {
+    const T hi = (T)x;
+    return {hi, (T)(x - (float)hi)};
+}
+
+__device__ __forceinline__ float half_swap(float x) { return __shfl_xor(x, 32); }
+
+// TQ: element of the first product's operands, TP: of the second's.  QT: terms of
+// q and of the weights, KT: of k and v.
+template <int HD, class TQ, class TP, int QT, int KT> struct Rows {
+    static constexpr int KS = HD / 16, DB = HD / 32;
+    static constexpr int KROW = HD + 8;  // LDS row of K
+    typedef typename Vec<TQ>::v8 q8;
+    typedef typename Vec<TP>::v8 p8;
+
+    q8 q[QT][KS];
+    f32x16 o[DB];
+    float m, l;      // of the row: the weights' offset, the sum over this lane's keys
+    float f;         // Score::f over the row's own power of two
+    float slope2;
+    int pos, lim;    // the row sees keys 0 .. lim - 1
+
+    // q's fragments: lane holds row lane & 31, channels 16 kk + 8 (lane >> 5) ..
+    // SCALED: by the row's power of two (fp32 or the cache's fp16 products)
+    template <bool SCALED> __device__ __forceinline__ void load_q(const void *qp, int type, int64_t at, const Score &sc) {
+        const int hf = (threadIdx.x >> 5) & 1;
+        f = sc.f;
+        if constexpr (!SCALED) {
+#pragma unroll
+            for (int kk = 0; kk < KS; kk++) q[0][kk] = *(const q8 *)((const TQ *)qp + at + 16 * kk + 8 * hf);
+        } else {
+            float x[KS][8], top = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < KS; kk++) {
+                load8(qp, type, at + 16 * kk + 8 * hf, x[kk]);
+#pragma unroll
+                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[kk][i]));
+            }
+            top = fmaxf(top, half_swap(top));
+            const float up = pow2_to_14(top);
+            f = sc.f / up;
+#pragma unroll
+            for (int kk = 0; kk < KS; kk++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    if constexpr (QT == 2) {
+                        const Two<TQ> y = split<TQ>(x[kk][i] * up);
+                        q[0][kk][i] = y.hi, q[1][kk][i] = y.lo;
+                    } else {
+                        q[0][kk][i] = (TQ)(x[kk][i] * up);
+                    }
+                }
+        }
+    }
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < DB; i++) o[i] = f32x16{};
+        m = M_NONE;
+        l = 0.f;
+    }
+
+    // Scores of the 64 keys from position j0 on: sk holds K's KT planes of 64
+    // rows.  kscale: one for the tile, or (PER_KEY) sks[key].  Then their weights,
+    // as the second product's operand.  seen: keys below it are seen.
+    template <bool PER_KEY>
+    __device__ __forceinline__ void weigh(const TQ *sk, const Score &sc, float kscale, const float *sks, int j0, bool cut,
+                                          int seen, p8 (&pf)[QT][4]) {
+        const int l32 = threadIdx.x & 31, hf = (threadIdx.x >> 5) & 1;
+        f32x16 s[2] = {};
+#pragma unroll
+        for (int kk = 0; kk < KS; kk++)
+#pragma unroll
+            for (int st = 0; st < 2; st++) {
+                const TQ *row = sk + (32 * st + l32) * KROW + 16 * kk + 8 * hf;
+                const q8 a = *(const q8 *)row;
+                if constexpr (KT == 2) s[st] = mfma32(*(const q8 *)(row + TILE_K * KROW), q[0][kk], s[st]);
+                if constexpr (QT == 2) s[st] = mfma32(a, q[1][kk], s[st]);
+                s[st] = mfma32(a, q[0][kk], s[st]);
+            }
+        const float c = f * kscale;
+        if (!sc.cap2 && !sc.bias) {
+#pragma unroll
+            for (int st = 0; st < 2; st++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    f32x4 ks = {c, c, c, c};
+                    if constexpr (PER_KEY) ks = *(const f32x4 *)(sks + 32 * st + 8 * g + 4 * hf) * f;
+#pragma unroll
+                    for (int v = 0; v < 4; v++) s[st][4 * g + v] *= ks[v];
+                }
+        } else {
+            const float far = (float)(pos - j0 - 4 * hf);
+#pragma unroll
+            for (int st = 0; st < 2; st++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    f32x4 ks = {c, c, c, c};
+                    if constexpr (PER_KEY) ks = *(const f32x4 *)(sks + 32 * st + 8 * g + 4 * hf) * f;
+#pragma unroll
+                    for (int v = 0; v < 4; v++) {
+                        float t = s[st][4 * g + v] * ks[v];
+                        if (sc.cap2) t = capped(t, sc.cap2);
+                        if (sc.bias) t = fmaf(-slope2, fabsf(far - (float)(32 * st + 8 * g + v)), t);
+                        s[st][4 * g + v] = t;
+                    }
+                }
+        }
+        if (cut) {
+            const int left = seen - j0 - 4 * hf;
+#pragma unroll
+            for (int st = 0; st < 2; st++)
+#pragma unroll
+                for (int v = 0; v < 16; v++) s[st][v] = left > 32 * st + 8 * (v >> 2) + (v & 3) ? s[st][v] : -INFINITY;
+        }
+        float mt = s[0][0];
+#pragma unroll
+        for (int v = 1; v < 16; v++) mt = fmaxf(mt, s[0][v]);
+#pragma unroll
+        for (int v = 0; v < 16; v++) mt = fmaxf(mt, s[1][v]);
+        if (__ballot(mt > m + RAISE)) {  // wave-uniform
+            mt = fmaxf(mt, half_swap(mt));
+            const float now = mt > m + RAISE ? mt - OFFSET : m;
+            const float keep = __builtin_amdgcn_exp2f(m - now);
+            m = now;
+            l *= keep;
+#pragma unroll
+            for (int i = 0; i < DB; i++) o[i] *= keep;
+        }
+#pragma unroll
+        for (int st = 0; st < 2; st++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) s[st][v] = __builtin_amdgcn_exp2f(s[st][v] - m);
+        float sum[4] = {};
+#pragma unroll
+        for (int tt = 0; tt < 4; tt++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float p = s[tt >> 1][8 * (tt & 1) + e];
+                sum[e & 3] += p;
+                if constexpr (QT == 2) {
+                    const Two<TP> y = split<TP>(p);
+                    pf[0][tt][e] = y.hi, pf[1][tt][e] = y.lo;
+                } else {
+                    pf[0][tt][e] = (TP)p;
+                }
+            }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    }
+};
+
+}  // namespace
+
+#endif
