@@ -1,7 +1,7 @@
 // fh3_kv.hip -- the 8-bit key/value cache: new rows written to it
 // (fh3_hip_kv_append_dev), read back (fh3_hip_kv_read_dev), lengths moved on
 // (fh3_hip_kv_extend_dev) and attention over it (fh3_hip_kv_attention_dev).
-#include "fh3_seqs.h"
+#include "fh3_tile.h"
 
 namespace {
 
@@ -152,58 +152,546 @@ __global__ __launch_bounds__(ROW_T) void k_kv_extend(int *len, Fh3kSeqs s) {
     len[i] = l < 0x7FFFFFFF - cnt ? l + cnt : 0x7FFFFFFF;
 }
 
-// One wavefront to a row and query head: 64 keys at a time, a key to a lane, then
-// HD / 64 channels to a lane.
-template <int HD>
-__global__ __launch_bounds__(64) void k_kv_rows(Fh3kAttn a, Fh3kKv c, const void *__restrict__ q, int64_t ldq,
-                                                void *__restrict__ o, int64_t ldo, Fh3kSeqs s) {
-    __shared__ float sq[HD], sp[64];
-    const int lane = threadIdx.x, h = blockIdx.y, m = h / (a.heads / a.kv_heads);
-    int seq, first, cnt, len, base;
-    int64_t at;
-    if (!find_unit(blockIdx.x, s.n_seq, [&](int i) { int b, n; seq_rows(s, i, b, n); return (int64_t)n; }, seq, at))
+// ---------------------------------------------------------------------------
+// Attention over the cache.  The work is the pages that each tile of rows looks
+// through, one after the other over all sequences ("units", the same for every
+// key head); a key head's workgroups take equal runs of units, whatever the
+// lengths are, so a run may end inside a tile: the parts then go to the workspace
+// and k_kv_join adds them in order.  Tiles of at most WHOLE pages are not divided:
+// the workgroup of their first page takes them.
+// ---------------------------------------------------------------------------
+constexpr int WHOLE = 8;
+
+struct KvWork {
+    int G, rows_per_tile;  // query heads of a key head; rows of a tile
+    int wgs;               // workgroups of a key head
+};
+// Tiles of sequence i, and pages (units) of each; a tile that sees no key has one unit.
+__device__ __forceinline__ int64_t kv_tiles(const Fh3kKv &c, const Fh3kSeqs &s, const KvWork &w, int i, int &pages) {
+    int a, cnt, len, base;
+    seq_rows(s, i, a, cnt);
+    kv_len(c, i, cnt, len, base);
+    pages = len > 0 ? (len + KV_PAGE - 1) / KV_PAGE : 1;
+    return ((int64_t)cnt * w.G + w.rows_per_tile - 1) / w.rows_per_tile;
+}
+__device__ __forceinline__ int64_t wave_sum(int64_t x) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
+    return x;
+}
+// Units of all sequences, and from them a workgroup's run.
+__device__ __forceinline__ int64_t kv_run(const Fh3kKv &c, const Fh3kSeqs &s, const KvWork &w, int64_t &units) {
+    int64_t n = 0;
+    for (int i = threadIdx.x & 63; i < s.n_seq; i += 64) {
+        int pages;
+        const int64_t t = kv_tiles(c, s, w, i, pages);
+        n += t * pages;
+    }
+    units = wave_sum(n);
+    const int64_t run = (units + w.wgs - 1) / w.wgs;
+    return run > WHOLE ? run : WHOLE;
+}
+
+// Where the parts of a divided tile stand: of each workgroup two, the end of a
+// tile begun before its run (0) and the beginning of one that goes on behind it
+// (1); rows x HD sums, then the rows' offsets and sums of weights.
+template <int HD> struct Parts {
+    float *p;
+    int rows, wgs;
+    __device__ __forceinline__ float *of(int kvh, int wg, int which) const {
+        return p + (((int64_t)kvh * wgs + wg) * 2 + which) * rows * (HD + 2);
+    }
+};
+
+__device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float lane_value(float x, int n) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), n & 63));
+}
+// Eight stored bytes -> fp16 integers: 0x64 before a byte makes 1024 + it.
+__device__ __forceinline__ half8 to_half(uint32_t a, uint32_t b) {
+    u32x4 w = {__builtin_amdgcn_perm(0x64646464u, a, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u),
+               __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)};
+    return __builtin_bit_cast(half8, w) - (half8)(_Float16)1152.f;
+}
+
+// Few rows to a sequence: tiles of 16 R rows; each of four wavefronts takes every
+// fourth page of a tile with all its rows, straight from memory into the
+// operands of 16x16x32 products (S^T = K Q^T, O^T = V^T P^T), and the four are
+// joined in LDS.  NT: 16-bit terms of q and of the weights (fp32: two).
+constexpr int FEW_W = 4;
+template <int HD, int R, int NT>
+__global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, const void *__restrict__ q, int64_t ldq,
+                                                          void *__restrict__ o, int64_t ldo, Fh3kSeqs s, KvWork work,
+                                                          float *__restrict__ ws) {
+    constexpr int ROWS = 16 * R, KU = HD / 64, DT = HD / 16, OROW = HD + 4;
+    __shared__ __align__(16) float so[FEW_W][ROWS][OROW];
+    __shared__ float sm[FEW_W][ROWS], sl[FEW_W][ROWS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, g = lane >> 4;
+    const int kvh = blockIdx.x % c.kv_heads, wg = blockIdx.x / c.kv_heads, G = work.G;
+    const Score sc = score_of(a);
+    const Parts<HD> parts = {ws, ROWS, work.wgs};
+
+    int64_t units, at;
+    const int64_t run = kv_run(c, s, work, units);
+    int64_t u = wg * run;
+    const int64_t u_end = u + run < units ? u + run : units;
+    int seq = 0, pages = 0;
+    if (u >= u_end ||
+        !find_unit(u, s.n_seq, [&](int i) { int p; const int64_t t = kv_tiles(c, s, work, i, p); return t * p; }, seq, at))
         return;
-    seq_rows(s, seq, first, cnt);
-    kv_len(c, seq, cnt, len, base);
-    const int row = first + (int)at, pos = base + (int)at;
-    for (int d = lane; d < HD; d += 64) sq[d] = value_at(q, a.type, row * ldq + h * HD + d);
-    __syncthreads();
-    const int end = a.causal && pos + 1 < len ? pos + 1 : len;
-    bool some = false;  // the row sees a key
-    float top = -INFINITY, sum = 0.f, acc[HD / 64] = {};
-    for (int j0 = 0; j0 < end; j0 += 64) {
-        const int j = j0 + lane, id = kv_page(c, seq, j0 >> 6);
-        if (id < 0) continue;
-        some = true;
-        const int64_t blk = ((int64_t)id * c.kv_heads + m) * 2;
-        const uint8_t *kp = c.pool + blk * KV_PAGE * HD, *vp = kp + KV_PAGE * HD;
-        float x = -INFINITY;
-        if (j < end) {
-            x = 0.f;
-            for (int d = 0; d < HD; d++) x = fmaf(sq[d], (float)((int)kp[k_byte<HD>(lane, d)] - 128), x);
-            x *= c.scales[blk] * a.scale;
-            if (a.softcap > 0.f) x = a.softcap * tanhf(x / a.softcap);
-            if (a.slopes) x -= a.slopes[h] * fabsf((float)(pos - j));
+    seq = __builtin_amdgcn_readfirstlane(seq);
+    int64_t tiles = kv_tiles(c, s, work, seq, pages);
+    int64_t tile = at / pages;
+    int page0 = (int)(at % pages);
+    while (u < u_end) {
+        const bool whole = pages <= WHOLE;
+        if (!(whole && page0)) {
+            const int page1 = whole || pages - page0 <= u_end - u ? pages : page0 + (int)(u_end - u);
+            int first, cnt, len, base;
+            seq_rows(s, seq, first, cnt);
+            kv_len(c, seq, cnt, len, base);
+            const int rows = cnt * G, r0 = (int)tile * ROWS;
+            auto limit = [&](int tok) { return a.causal && base + tok + 1 < len ? base + tok + 1 : len; };
+            const int lo = limit(r0 / G);  // keys that all rows see
+            // rows of this lane: R times l16; q's fragments, 16 channels of each 64
+            half8 qf[R][NT][2 * KU];
+            float f[R], m[R], l[R], slope2[R];
+            int pos[R], lim[R];
+            f32x4 acc[R][DT];
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const int row = r0 + 16 * r + l16, rc = row < rows ? row : rows - 1;
+                const int tok = rc / G, head = kvh * G + rc % G;
+                const int64_t at_q = (int64_t)(first + tok) * ldq + head * HD + 16 * g;
+                float x[2 * KU][8], top = 0.f;
+#pragma unroll
+                for (int i = 0; i < 2 * KU; i++) {
+                    load8(q, a.type, at_q + 64 * (i >> 1) + 8 * (i & 1), x[i]);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[i][e]));
+                }
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float up = pow2_to_14(top);
+                f[r] = sc.f / up;
+#pragma unroll
+                for (int i = 0; i < 2 * KU; i++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const Two<_Float16> y = split<_Float16>(x[i][e] * up);
+                        qf[r][0][i][e] = y.hi;
+                        if constexpr (NT == 2) qf[r][NT - 1][i][e] = y.lo;
+                    }
+                pos[r] = base + tok;
+                lim[r] = limit(tok);
+                slope2[r] = sc.bias ? a.slopes[head] * LOG2E : 0.f;
+                m[r] = M_NONE;
+                l[r] = 0.f;
+#pragma unroll
+                for (int d = 0; d < DT; d++) acc[r][d] = f32x4{};
+            }
+
+            // 64 of this wavefront's pages at a time, one to a lane: page and scales
+            int ids = -1;
+            f32x2 scs = {};
+            auto load_ids = [&](int n) {
+                const int p = page0 + wave + FEW_W * (n + lane);
+                ids = p < page1 ? kv_page(c, seq, p) : -1;
+                scs = f32x2{};
+                if (ids >= 0) scs = *(const f32x2 *)(c.scales + ((int64_t)ids * c.kv_heads + kvh) * 2);
+            };
+            u32x4 kr[4 * KU], vr[DT];
+            auto block = [&](int n) {  // a page that is not there: page 0, whose keys are then all cut
+                const int id = __builtin_amdgcn_readlane(ids, n & 63);
+                return (const u32x4 *)(c.pool + ((int64_t)(id < 0 ? 0 : id) * c.kv_heads + kvh) * 2 * KV_PAGE * HD) + lane;
+            };
+            const int n_pages = (page1 - page0 - wave + FEW_W - 1) / FEW_W;
+            if (n_pages > 0) {
+                load_ids(0);
+                const u32x4 *b = block(0);
+#pragma unroll
+                for (int i = 0; i < 4 * KU; i++) kr[i] = b[64 * i];
+            }
+            for (int n = 0; n < n_pages; n++) {
+                const u32x4 *b = block(n);
+#pragma unroll
+                for (int i = 0; i < DT; i++) vr[i] = b[64 * (4 * KU + i)];
+                const bool there = __builtin_amdgcn_readlane(ids, n & 63) >= 0;
+                const float ks = lane_value(scs[0], n);
+                const float vs = lane_value(scs[1], n);
+                const int j0 = (page0 + wave + FEW_W * n) * KV_PAGE;
+                f32x4 t[R][4] = {};
+#pragma unroll
+                for (int h = 0; h < KU; h++)
+#pragma unroll
+                    for (int tt = 0; tt < 4; tt++) {
+                        const u32x4 w = kr[tt * KU + h];
+                        const half8 k0 = to_half(w[0], w[1]), k1 = to_half(w[2], w[3]);
+#pragma unroll
+                        for (int r = 0; r < R; r++) {
+#pragma unroll
+                            for (int e = NT - 1; e >= 0; e--) {
+                                t[r][tt] = mfma16(k0, qf[r][e][2 * h], t[r][tt]);
+                                t[r][tt] = mfma16(k1, qf[r][e][2 * h + 1], t[r][tt]);
+                            }
+                        }
+                    }
+                if (n + 1 < n_pages) {
+                    if (((n + 1) & 63) == 0) load_ids(n + 1);
+                    const u32x4 *nb = block(n + 1);
+#pragma unroll
+                    for (int i = 0; i < 4 * KU; i++) kr[i] = nb[64 * i];
+                }
+                // lane holds keys 16 tt + 4 g + v of row l16
+                const bool cut = !there || j0 + KV_PAGE > lo;
+                half8 pf[R][NT][2];
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    const float x = f[r] * ks, far = (float)(pos[r] - j0 - 4 * g);
+                    const int left = there ? lim[r] - j0 - 4 * g : 0x80000000;
+#pragma unroll
+                    for (int tt = 0; tt < 4; tt++)
+#pragma unroll
+                        for (int v = 0; v < 4; v++) {
+                            float y = t[r][tt][v] * x;
+                            if (sc.cap2) y = capped(y, sc.cap2);
+                            if (sc.bias) y = fmaf(-slope2[r], fabsf(far - (float)(16 * tt + v)), y);
+                            t[r][tt][v] = y;
+                        }
+                    if (cut) {
+#pragma unroll
+                        for (int tt = 0; tt < 4; tt++)
+#pragma unroll
+                            for (int v = 0; v < 4; v++) t[r][tt][v] = left > 16 * tt + v ? t[r][tt][v] : -INFINITY;
+                    }
+                    float mt = t[r][0][0];
+#pragma unroll
+                    for (int i = 1; i < 16; i++) mt = fmaxf(mt, t[r][i >> 2][i & 3]);
+                    if (__ballot(mt > m[r] + RAISE)) {
+                        mt = fmaxf(mt, __shfl_xor(mt, 16));
+                        mt = fmaxf(mt, __shfl_xor(mt, 32));
+                        const float now = mt > m[r] + RAISE ? mt - OFFSET : m[r];
+                        const float keep = __builtin_amdgcn_exp2f(m[r] - now);
+                        m[r] = now;
+                        l[r] *= keep;
+#pragma unroll
+                        for (int d = 0; d < DT; d++) acc[r][d] *= keep;
+                    }
+                    float sum = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float p = __builtin_amdgcn_exp2f(t[r][i >> 2][i & 3] - m[r]);
+                        sum += p;
+                        const Two<_Float16> y = split<_Float16>(p);
+                        pf[r][0][i >> 3][i & 7] = y.hi;
+                        if constexpr (NT == 2) pf[r][NT - 1][i >> 3][i & 7] = y.lo;
+                    }
+                    l[r] += sum;
+                }
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    const half8 v0 = to_half(vr[d][0], vr[d][1]), v1 = to_half(vr[d][2], vr[d][3]);
+#pragma unroll
+                    for (int r = 0; r < R; r++) {
+                        f32x4 y = {};
+#pragma unroll
+                        for (int e = NT - 1; e >= 0; e--) {
+                            y = mfma16(v0, pf[r][e][0], y);
+                            y = mfma16(v1, pf[r][e][1], y);
+                        }
+#pragma unroll
+                        for (int v = 0; v < 4; v++) acc[r][d][v] = fmaf(y[v], vs, acc[r][d][v]);
+                    }
+                }
+            }
+
+            // the four wavefronts' parts, in order
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                l[r] += __shfl_xor(l[r], 16);
+                l[r] += __shfl_xor(l[r], 32);
+                const int row = 16 * r + l16;
+                if (g == 0) sm[wave][row] = m[r], sl[wave][row] = l[r];
+#pragma unroll
+                for (int d = 0; d < DT; d++) *(f32x4 *)&so[wave][row][16 * d + 4 * g] = acc[r][d];
+            }
+            __syncthreads();
+            const bool done = page0 == 0 && page1 == pages;
+            float *part = done ? nullptr : parts.of(kvh, wg, page0 == 0);
+            for (int e = tid; e < ROWS * HD / 4; e += 64 * FEW_W) {
+                const int row = e / (HD / 4), d = e % (HD / 4) * 4;
+                float top = sm[0][row];
+#pragma unroll
+                for (int w = 1; w < FEW_W; w++) top = fmaxf(top, sm[w][row]);
+                float sum = 0.f;
+                f32x4 x = {};
+#pragma unroll
+                for (int w = 0; w < FEW_W; w++) {
+                    const float keep = __builtin_amdgcn_exp2f(sm[w][row] - top);
+                    sum += sl[w][row] * keep;
+                    const f32x4 y = *(const f32x4 *)&so[w][row][d];
+#pragma unroll
+                    for (int v = 0; v < 4; v++) x[v] = fmaf(y[v], keep, x[v]);
+                }
+                if (!done) {
+                    *(f32x4 *)(part + row * HD + d) = x;
+                    if (d == 0) part[ROWS * HD + row] = top, part[ROWS * (HD + 1) + row] = sum;
+                } else if (r0 + row < rows) {
+                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                    const int tok = (r0 + row) / G, head = kvh * G + (r0 + row) % G;
+#pragma unroll
+                    for (int v = 0; v < 4; v++) x[v] *= inv;
+                    store4(o, a.type, (int64_t)(first + tok) * ldo + head * HD + d, x);
+                }
+            }
+            __syncthreads();
+            u += page1 - page0;
+        } else {
+            u += pages - page0;
         }
-        float t = x;
-        for (int w = 1; w < 64; w <<= 1) t = fmaxf(t, __shfl_xor(t, w));
-        t = fmaxf(t, top);
-        const float keep = top == -INFINITY ? 0.f : expf(top - t);
-        const float p = j < end ? expf(x - t) : 0.f;
-        top = t;
-        sum = sum * keep + p;
-        __syncthreads();
-        sp[lane] = p * c.scales[blk + 1];
-        __syncthreads();
-        for (int e = 0; e < HD / 64; e++) {
-            acc[e] *= keep;
-            for (int l = 0; l < 64 && j0 + l < end; l++)
-                acc[e] = fmaf(sp[l], (float)((int)vp[v_byte<HD>(l, 64 * e + lane)] - 128), acc[e]);
+        page0 = 0;
+        if (++tile >= tiles) {
+            tile = 0;
+            do {
+                if (++seq >= s.n_seq) return;
+                tiles = kv_tiles(c, s, work, seq, pages);
+            } while (tiles == 0);
         }
     }
-    for (int w = 1; w < 64; w <<= 1) sum += __shfl_xor(sum, w);
-    for (int e = 0; e < HD / 64; e++)
-        put_value(o, a.type, row * ldo + h * HD + 64 * e + lane, some ? acc[e] / sum : 0.f);
+}
+
+// One workgroup to a tile and key head: where the tile was divided, its parts in order.
+template <int HD>
+__global__ __launch_bounds__(256) void k_kv_join(Fh3kAttn a, Fh3kKv c, void *__restrict__ o, int64_t ldo, Fh3kSeqs s,
+                                                 KvWork work, const float *__restrict__ ws) {
+    const int tid = threadIdx.x, kvh = blockIdx.y, G = work.G, ROWS = work.rows_per_tile;
+    int seq, pages, first, cnt;
+    int64_t tile, units;
+    if (!find_unit(blockIdx.x, s.n_seq, [&](int i) { int p; return kv_tiles(c, s, work, i, p); }, seq, tile)) return;
+    kv_tiles(c, s, work, seq, pages);
+    if (pages <= WHOLE) return;
+    const int64_t run = kv_run(c, s, work, units);
+    int64_t u0 = 0;  // units before the tile
+    for (int i = tid & 63; i < seq; i += 64) {
+        int p;
+        const int64_t t = kv_tiles(c, s, work, i, p);
+        u0 += t * p;
+    }
+    u0 = wave_sum(u0) + tile * pages;
+    const int w0 = (int)(u0 / run), w1 = (int)((u0 + pages - 1) / run);
+    if (w0 == w1) return;
+    seq_rows(s, seq, first, cnt);
+    const int rows = cnt * G, r0 = (int)tile * ROWS;
+    const Parts<HD> parts = {(float *)ws, ROWS, work.wgs};
+    for (int e = tid; e < ROWS * HD / 4; e += 256) {
+        const int row = e / (HD / 4), d = e % (HD / 4) * 4;
+        if (r0 + row >= rows) break;
+        float top = M_NONE, sum = 0.f;
+        f32x4 x = {};
+        for (int w = w0; w <= w1; w++) {
+            const float *p = parts.of(kvh, w, w == w0);
+            const float pm = p[ROWS * HD + row], now = fmaxf(top, pm);
+            const float keep = __builtin_amdgcn_exp2f(top - now), add = __builtin_amdgcn_exp2f(pm - now);
+            const f32x4 y = *(const f32x4 *)(p + row * HD + d);
+            top = now;
+            sum = sum * keep + p[ROWS * (HD + 1) + row] * add;
+#pragma unroll
+            for (int v = 0; v < 4; v++) x[v] = x[v] * keep + y[v] * add;
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const int tok = (r0 + row) / G, head = kvh * G + (r0 + row) % G;
+#pragma unroll
+        for (int v = 0; v < 4; v++) x[v] *= inv;
+        store4(o, a.type, (int64_t)(first + tok) * ldo + head * HD + d, x);
+    }
+}
+
+// Many rows to a sequence: tiles of 128, 32 to a wavefront.  A page is turned
+// into fp16 once for all of them, through double-buffered LDS: K as rows, V
+// transposed with the keys of each 16 in the order of the first product's
+// accumulator (0-3, 8-11, 4-7, 12-15).
+constexpr int MANY_W = 4;
+template <int HD, int NT>
+__global__ __launch_bounds__(64 * MANY_W, 2) void k_kv_many(Fh3kAttn a, Fh3kKv c, const void *__restrict__ q,
+                                                            int64_t ldq, void *__restrict__ o, int64_t ldo, Fh3kSeqs s,
+                                                            KvWork work, float *__restrict__ ws) {
+    typedef Rows<HD, _Float16, _Float16, NT, 1> R;
+    constexpr int ROWS = WAVE_R * MANY_W, NTH = 64 * MANY_W, KU = HD / 64, VROW = KV_PAGE + 8;
+    constexpr int CH = KV_PAGE * HD / 16 / NTH;  // 16-byte pieces of K, and of V, to a thread
+    __shared__ __align__(16) _Float16 sk[2][KV_PAGE][R::KROW];
+    __shared__ __align__(16) _Float16 sv[2][HD][VROW];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l32 = lane & 31, hf = lane >> 5;
+    const int kvh = blockIdx.x % c.kv_heads, wg = blockIdx.x / c.kv_heads, G = work.G;
+    const Score sc = score_of(a);
+    const Parts<HD> parts = {ws, ROWS, work.wgs};
+
+    int64_t units, at;
+    const int64_t run = kv_run(c, s, work, units);
+    int64_t u = wg * run;
+    const int64_t u_end = u + run < units ? u + run : units;
+    int seq = 0, pages = 0;
+    if (u >= u_end ||
+        !find_unit(u, s.n_seq, [&](int i) { int p; const int64_t t = kv_tiles(c, s, work, i, p); return t * p; }, seq, at))
+        return;
+    seq = __builtin_amdgcn_readfirstlane(seq);
+    int64_t tiles = kv_tiles(c, s, work, seq, pages);
+    int64_t tile = at / pages;
+    int page0 = (int)(at % pages);
+    while (u < u_end) {
+        const bool whole = pages <= WHOLE;
+        if (!(whole && page0)) {
+            const int page1 = whole || pages - page0 <= u_end - u ? pages : page0 + (int)(u_end - u);
+            int first, cnt, len, base;
+            seq_rows(s, seq, first, cnt);
+            kv_len(c, seq, cnt, len, base);
+            const int rows = cnt * G, r0 = (int)tile * ROWS;
+            auto limit = [&](int tok) { return a.causal && base + tok + 1 < len ? base + tok + 1 : len; };
+            const int row = r0 + WAVE_R * wave + l32, rc = row < rows ? row : rows - 1;
+            const int tok = rc / G, head = kvh * G + rc % G;
+            R w;
+            w.template load_q<true>(q, a.type, (int64_t)(first + tok) * ldq + head * HD, sc);
+            w.clear();
+            w.pos = base + tok;
+            w.lim = limit(tok);
+            w.slope2 = sc.bias ? a.slopes[head] * LOG2E : 0.f;
+            const bool active = r0 + WAVE_R * wave < rows;
+            const int lo = __builtin_amdgcn_readfirstlane(w.lim), hi = __builtin_amdgcn_readlane(w.lim, 31);
+            const int seen = limit((r0 + ROWS < rows ? r0 + ROWS - 1 : rows - 1) / G);  // by the tile's last row
+            const int page_n = seen <= page0 * KV_PAGE ? page0 : seen >= page1 * KV_PAGE ? page1 : (seen + KV_PAGE - 1) / KV_PAGE;
+            float ref = 0.f;  // the sums are in units of this value scale
+
+            int ids = -1;
+            f32x2 scs = {};
+            auto load_ids = [&](int n) {  // 64 pages at a time, one to a lane
+                const int p = page0 + n + lane;
+                ids = p < page_n ? kv_page(c, seq, p) : -1;
+                scs = f32x2{};
+                if (ids >= 0) scs = *(const f32x2 *)(c.scales + ((int64_t)ids * c.kv_heads + kvh) * 2);
+            };
+            u32x4 rk[CH], rv[CH];
+            auto load = [&](int n) {
+                const int id = __builtin_amdgcn_readlane(ids, n & 63);
+                const u32x4 *b = (const u32x4 *)(c.pool + ((int64_t)(id < 0 ? 0 : id) * c.kv_heads + kvh) * 2 * KV_PAGE * HD) + tid;
+#pragma unroll
+                for (int i = 0; i < CH; i++) rk[i] = b[NTH * i], rv[i] = b[NTH * (CH + i)];
+            };
+            auto store = [&](int n) {
+#pragma unroll
+                for (int i = 0; i < CH; i++) {
+                    const int p = tid + NTH * i, x = p & 15, g = (p >> 4) & 3, b = p >> 6;
+                    _Float16 *kd = &sk[n & 1][16 * (b / KU) + x][64 * (b % KU) + 16 * g];
+                    *(half8 *)kd = to_half(rk[i][0], rk[i][1]);
+                    *(half8 *)(kd + 8) = to_half(rk[i][2], rk[i][3]);
+                    _Float16 *vd = &sv[n & 1][16 * b + x][8 * (g & 1) + 4 * (g >> 1)];
+                    const u32x4 lo4 = __builtin_bit_cast(u32x4, to_half(rv[i][0], rv[i][1]));
+                    const u32x4 hi4 = __builtin_bit_cast(u32x4, to_half(rv[i][2], rv[i][3]));
+                    *(u32x2 *)vd = u32x2{lo4[0], lo4[1]};
+                    *(u32x2 *)(vd + 16) = u32x2{lo4[2], lo4[3]};
+                    *(u32x2 *)(vd + 32) = u32x2{hi4[0], hi4[1]};
+                    *(u32x2 *)(vd + 48) = u32x2{hi4[2], hi4[3]};
+                }
+            };
+            const int n_pages = page_n - page0;
+            float ks = 0.f, vs = 0.f;
+            bool there = false;
+            auto scales = [&](int n) {
+                there = __builtin_amdgcn_readlane(ids, n & 63) >= 0;
+                ks = lane_value(scs[0], n);
+                vs = lane_value(scs[1], n);
+            };
+            __syncthreads();  // the last tile's readers are done
+            if (n_pages > 0) {
+                load_ids(0);
+                load(0);
+                scales(0);
+                store(0);
+            }
+            __syncthreads();
+            for (int n = 0; n < n_pages; n++) {
+                const int j0 = (page0 + n) * KV_PAGE;
+                const float ks_n = ks, vs_n = vs;
+                const bool there_n = there;
+                if (n + 1 < n_pages) {
+                    if (((n + 1) & 63) == 0) load_ids(n + 1);
+                    load(n + 1);
+                    scales(n + 1);
+                }
+                if (active && there_n && j0 < hi) {
+                    half8 pf[NT][4];
+                    w.template weigh<false>(&sk[n & 1][0][0], sc, ks_n, nullptr, j0, j0 + KV_PAGE > lo, w.lim, pf);
+                    // pages of the same scale add up in the product's accumulator
+                    if (vs_n > ref) {
+                        const float down = ref / vs_n;
+                        ref = vs_n;
+#pragma unroll
+                        for (int i = 0; i < R::DB; i++) w.o[i] *= down;
+                    }
+                    if (vs_n == ref) {
+#pragma unroll
+                        for (int db = 0; db < R::DB; db++)
+#pragma unroll
+                            for (int tt = 0; tt < 4; tt++) {
+                                const half8 x = *(const half8 *)&sv[n & 1][32 * db + l32][16 * tt + 8 * hf];
+#pragma unroll
+                                for (int e = NT - 1; e >= 0; e--) w.o[db] = mfma32(x, pf[e][tt], w.o[db]);
+                            }
+                    } else {
+                        const float down = vs_n / ref;
+#pragma unroll
+                        for (int db = 0; db < R::DB; db++) {
+                            f32x16 y = {};
+#pragma unroll
+                            for (int tt = 0; tt < 4; tt++) {
+                                const half8 x = *(const half8 *)&sv[n & 1][32 * db + l32][16 * tt + 8 * hf];
+#pragma unroll
+                                for (int e = NT - 1; e >= 0; e--) y = mfma32(x, pf[e][tt], y);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 16; i++) w.o[db][i] = fmaf(y[i], down, w.o[db][i]);
+                        }
+                    }
+                }
+                if (n + 1 < n_pages) store(n + 1);
+                __syncthreads();
+            }
+
+            const float l = w.l + half_swap(w.l);
+            if (row < rows) {
+                const bool done = page0 == 0 && page1 == pages;
+                float *part = done ? nullptr : parts.of(kvh, wg, page0 == 0);
+                const float inv = done ? (l == 0.f ? 0.f : ref / l) : ref;
+                const int64_t at_o = (int64_t)(first + tok) * ldo + head * HD;
+                const int r = WAVE_R * wave + l32;
+                if (!done && hf == 0) part[ROWS * HD + r] = w.m, part[ROWS * (HD + 1) + r] = l;
+#pragma unroll
+                for (int db = 0; db < R::DB; db++)
+#pragma unroll
+                    for (int g = 0; g < 4; g++) {
+                        const int d = 32 * db + 8 * g + 4 * hf;
+                        f32x4 x;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) x[i] = w.o[db][4 * g + i] * inv;
+                        if (done) store4(o, a.type, at_o + d, x);
+                        else *(f32x4 *)(part + r * HD + d) = x;
+                    }
+            }
+            u += page1 - page0;
+        } else {
+            u += pages - page0;
+        }
+        page0 = 0;
+        if (++tile >= tiles) {
+            tile = 0;
+            do {
+                if (++seq >= s.n_seq) return;
+                tiles = kv_tiles(c, s, work, seq, pages);
+            } while (tiles == 0);
+        }
+    }
 }
 
 }  // namespace
@@ -233,14 +721,57 @@ extern "C" hipError_t fh3k_kv_read(const Fh3kKv *c, int type, void *k, int64_t l
     return hipGetLastError();
 }
 
-extern "C" size_t fh3k_kv_attn_ws_bytes(const Fh3kAttn *, const Fh3kKv *, Fh3kSeqs) { return 0; }
+// How the rows of a call are tiled: by the average sequence, which is what the
+// host knows (any tiling is right for any sequence).
+struct KvForm {
+    KvWork work;
+    int64_t tiles;  // of all sequences at most
+    bool few, join;
+};
+static KvForm kv_form(const Fh3kAttn &a, const Fh3kKv &c, const Fh3kSeqs &s) {
+    KvForm f;
+    const int64_t G = a.heads / a.kv_heads, rows = s.n_tok * G, avg = (rows + s.n_seq - 1) / s.n_seq;
+    f.few = avg <= 32;
+    const int R = avg <= 16 ? 16 : avg <= 32 ? 32 : WAVE_R * MANY_W;
+    f.tiles = rows / R + (s.n_seq < s.n_tok ? s.n_seq : s.n_tok);
+    const int64_t runs = (f.tiles * c.max_pages + WHOLE - 1) / WHOLE, most = (512 + a.kv_heads - 1) / a.kv_heads;
+    f.work = {(int)G, R, (int)(runs < most ? runs : most)};
+    f.join = c.max_pages > WHOLE && f.work.wgs > 1;
+    return f;
+}
+
+extern "C" size_t fh3k_kv_attn_ws_bytes(const Fh3kAttn *a, const Fh3kKv *c, Fh3kSeqs s) {
+    const KvForm f = kv_form(*a, *c, s);
+    return f.join ? (size_t)a->kv_heads * f.work.wgs * 2 * f.work.rows_per_tile * (a->hd + 2) * sizeof(float) : 0;
+}
+
+template <int HD>
+static hipError_t kv_attn(const Fh3kAttn &a, const Fh3kKv &c, const void *q, int64_t ldq, void *o, int64_t ldo,
+                          const Fh3kSeqs &s, float *ws, hipStream_t st) {
+    const KvForm f = kv_form(a, c, s);
+    if (f.tiles > 0x7FFFFF) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)f.work.wgs * a.kv_heads);
+    const bool two = a.type == FH3K_F32;
+#define FH3K_KV(K, W) hipLaunchKernelGGL(K, grid, dim3(64 * W), 0, st, a, c, q, ldq, o, ldo, s, f.work, ws)
+    if (f.work.rows_per_tile == 16) {
+        if (two) FH3K_KV((k_kv_few<HD, 1, 2>), FEW_W);
+        else FH3K_KV((k_kv_few<HD, 1, 1>), FEW_W);
+    } else if (f.few) {
+        if (two) FH3K_KV((k_kv_few<HD, 2, 2>), FEW_W);
+        else FH3K_KV((k_kv_few<HD, 2, 1>), FEW_W);
+    } else {
+        if (two) FH3K_KV((k_kv_many<HD, 2>), MANY_W);
+        else FH3K_KV((k_kv_many<HD, 1>), MANY_W);
+    }
+#undef FH3K_KV
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !f.join) return e;
+    hipLaunchKernelGGL(k_kv_join<HD>, dim3((unsigned)f.tiles, a.kv_heads), dim3(256), 0, st, a, c, o, ldo, s, f.work, ws);
+    return hipGetLastError();
+}
 
 extern "C" hipError_t fh3k_kv_attn(const Fh3kAttn *a, const Fh3kKv *c, const void *q, int64_t ldq, void *o,
-                                   int64_t ldo, Fh3kSeqs s, void *, hipStream_t st) {
-    const dim3 grid(s.n_tok, a->heads);
-    if (a->hd == 128)
-        hipLaunchKernelGGL(k_kv_rows<128>, grid, dim3(64), 0, st, *a, *c, q, ldq, o, ldo, s);
-    else
-        hipLaunchKernelGGL(k_kv_rows<64>, grid, dim3(64), 0, st, *a, *c, q, ldq, o, ldo, s);
-    return hipGetLastError();
+                                   int64_t ldo, Fh3kSeqs s, void *ws, hipStream_t st) {
+    return a->hd == 128 ? kv_attn<128>(*a, *c, q, ldq, o, ldo, s, (float *)ws, st)
+                        : kv_attn<64>(*a, *c, q, ldq, o, ldo, s, (float *)ws, st);
 }
