@@ -6,13 +6,13 @@
 namespace {
 
 // Pages that a sequence's cnt rows touch at most, and the touched pages of sequence i.
-__host__ __device__ __forceinline__ int64_t most_pages(int64_t cnt) { return cnt > 0 ? (cnt + 62) / 64 + 1 : 0; }
-__device__ __forceinline__ int64_t touched_pages(const Fh3kKv &c, const Fh3kSeqs &s, int i, int &p0) {
+int64_t most_pages(int64_t cnt) { return cnt > 0 ? (cnt + 62) / 64 + 1 : 0; }
+__device__ __forceinline__ int touched_pages(const Fh3kKv &c, const Fh3kSeqs &s, int i, int &p0) {
     int a, cnt, len, base;
     seq_rows(s, i, a, cnt);
     kv_len(c, i, cnt, len, base);
     p0 = base >> 6;  // base may be negative: rows that no page holds
-    return cnt > 0 ? (int64_t)((base + cnt - 1) >> 6) - p0 + 1 : 0;
+    return cnt > 0 ? ((base + cnt - 1) >> 6) - p0 + 1 : 0;
 }
 int64_t touched_most(Fh3kSeqs s) {  // over all sequences: at least one row to a page
     if (!s.first) return s.n_seq * most_pages(s.n_tok / s.n_seq);
@@ -54,17 +54,17 @@ __global__ __launch_bounds__(ROW_T) void k_kv_append(Fh3kKv c, int type, const v
     __shared__ __align__(16) float sx[KV_PAGE * LD];
     __shared__ float smax[ROW_T / 64];
     const int t = threadIdx.x, h = blockIdx.y >> 1, which = blockIdx.y & 1;
-    int seq, a, cnt, len, base, p0;
-    int64_t at;
+    int seq, a, cnt, len, base, p0, at;
     if (!find_unit(blockIdx.x, s.n_seq, [&](int i) { int p; return touched_pages(c, s, i, p); }, seq, at)) return;
     seq_rows(s, seq, a, cnt);
     kv_len(c, seq, cnt, len, base);
     touched_pages(c, s, seq, p0);
-    const int p = p0 + (int)at, id = kv_page(c, seq, p);
+    const int p = p0 + at, id = kv_page(c, seq, p);
     if (id < 0) return;
     const int64_t pos0 = (int64_t)p * KV_PAGE;
     const int lo = (int)(base > pos0 ? base - pos0 : 0);  // slots lo .. hi - 1 are new, those below lo held
     const int hi = (int)(base + cnt < pos0 + KV_PAGE ? base + cnt - pos0 : KV_PAGE);
+    if (hi <= lo) return;
     const void *x = which ? v : k;
     const int64_t ld = which ? ldv : ldk;
     float m = 0.f;
@@ -122,13 +122,12 @@ __global__ __launch_bounds__(ROW_T) void k_kv_read(Fh3kKv c, int type, void *__r
     const int t = threadIdx.x, h = blockIdx.y >> 1, which = blockIdx.y & 1;
     void *x = which ? v : k;
     if (!x) return;
-    int seq, a, cnt, len, base, p0;
-    int64_t at;
+    int seq, a, cnt, len, base, p0, at;
     if (!find_unit(blockIdx.x, s.n_seq, [&](int i) { int p; return touched_pages(c, s, i, p); }, seq, at)) return;
     seq_rows(s, seq, a, cnt);
     kv_len(c, seq, cnt, len, base);
     touched_pages(c, s, seq, p0);
-    const int p = p0 + (int)at, id = kv_page(c, seq, p);
+    const int p = p0 + at, id = kv_page(c, seq, p);
     const int64_t pos0 = (int64_t)p * KV_PAGE, ld = which ? ldv : ldk;
     const int lo = (int)(base > pos0 ? base - pos0 : 0);
     const int hi = (int)(base + cnt < pos0 + KV_PAGE ? base + cnt - pos0 : KV_PAGE);
@@ -163,45 +162,87 @@ __global__ __launch_bounds__(ROW_T) void k_kv_extend(int *len, Fh3kSeqs s) {
 constexpr int WHOLE = 8;
 
 struct KvWork {
-    int G, rows_per_tile;  // query heads of a key head; rows of a tile
-    int wgs;               // workgroups of a key head
+    int G;      // query heads of a key head
+    int shift;  // tiles of 2^shift rows
+    int wgs;    // workgroups of a key head
 };
 // Tiles of sequence i, and pages (units) of each; a tile that sees no key has one unit.
-__device__ __forceinline__ int64_t kv_tiles(const Fh3kKv &c, const Fh3kSeqs &s, const KvWork &w, int i, int &pages) {
+__device__ __forceinline__ int kv_tiles(const Fh3kKv &c, const Fh3kSeqs &s, const KvWork &w, int i, int &pages) {
     int a, cnt, len, base;
     seq_rows(s, i, a, cnt);
     kv_len(c, i, cnt, len, base);
     pages = len > 0 ? (len + KV_PAGE - 1) / KV_PAGE : 1;
-    return ((int64_t)cnt * w.G + w.rows_per_tile - 1) / w.rows_per_tile;
+    return (cnt * w.G + (1 << w.shift) - 1) >> w.shift;
 }
-__device__ __forceinline__ int64_t wave_sum(int64_t x) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-    return x;
-}
-// Units of all sequences, and from them a workgroup's run.
-__device__ __forceinline__ int64_t kv_run(const Fh3kKv &c, const Fh3kSeqs &s, const KvWork &w, int64_t &units) {
-    int64_t n = 0;
-    for (int i = threadIdx.x & 63; i < s.n_seq; i += 64) {
+// A workgroup's run of units u .. end - 1 and the sequence, tile and page of the first.
+struct KvRun {
+    int size, u, end, seq, tiles, pages, tile, page;
+};
+__device__ __forceinline__ bool kv_run(const Fh3kKv &c, const Fh3kSeqs &s, const KvWork &w, int wg, KvRun &r) {
+    auto units = [&](int i) {
         int pages;
-        const int64_t t = kv_tiles(c, s, w, i, pages);
-        n += t * pages;
+        const int t = kv_tiles(c, s, w, i, pages);
+        return t * pages;
+    };
+    const int lane = threadIdx.x & 63;
+    int all = 0, mine = 0, end = 0;
+    for (int s0 = 0; s0 < s.n_seq; s0 += 64) {
+        mine = s0 + lane < s.n_seq ? units(s0 + lane) : 0;
+        end = wave_scan(mine);
+        all += __builtin_amdgcn_readlane(end, 63);
     }
-    units = wave_sum(n);
-    const int64_t run = (units + w.wgs - 1) / w.wgs;
-    return run > WHOLE ? run : WHOLE;
+    const int even = (all + w.wgs - 1) / w.wgs;
+    r.size = __builtin_amdgcn_readfirstlane(even > WHOLE ? even : WHOLE);
+    // wg * size may pass 2^31 only where it also passes all
+    if ((int64_t)wg * r.size >= all) return false;
+    r.u = wg * r.size;
+    r.end = all - r.u < r.size ? all : r.u + r.size;
+    int at = 0;
+    if (s.n_seq <= 64) {
+        const int l = __builtin_ctzll(__ballot(end > r.u));
+        r.seq = l;
+        at = r.u - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(mine, l));
+    } else {
+        if (!find_unit(r.u, s.n_seq, units, r.seq, at)) return false;
+    }
+    r.tiles = kv_tiles(c, s, w, r.seq, r.pages);
+    r.tile = at / r.pages;
+    r.page = at - r.tile * r.pages;
+    return true;
+}
+// The next tile after r.tile is done; false behind the last.
+__device__ __forceinline__ bool kv_next(const Fh3kKv &c, const Fh3kSeqs &s, const KvWork &w, KvRun &r) {
+    r.page = 0;
+    if (++r.tile < r.tiles) return true;
+    r.tile = 0;
+    do {
+        if (++r.seq >= s.n_seq) return false;
+        r.tiles = kv_tiles(c, s, w, r.seq, r.pages);
+    } while (r.tiles == 0);
+    return true;
 }
 
 // Where the parts of a divided tile stand: of each workgroup two, the end of a
 // tile begun before its run (0) and the beginning of one that goes on behind it
-// (1); rows x HD sums, then the rows' offsets and sums of weights.
+// (1); rows x HD sums, then the rows' offsets and sums of weights.  What k_kv_join
+// has to know of the second, the workgroup that begins the tile writes down.
+struct Begun {
+    int last;               // the workgroup that ends it, or 0: there is none
+    int first, r0, rows;    // the sequence's first row in q and o, the tile's row in it, its rows
+};
 template <int HD> struct Parts {
     float *p;
-    int rows, wgs;
+    int rows, kv_heads, wgs;
     __device__ __forceinline__ float *of(int kvh, int wg, int which) const {
         return p + (((int64_t)kvh * wgs + wg) * 2 + which) * rows * (HD + 2);
     }
+    __device__ __forceinline__ Begun *begun(int kvh, int wg) const {
+        return (Begun *)(p + (int64_t)kv_heads * wgs * 2 * rows * (HD + 2)) + (kvh * wgs + wg);
+    }
 };
+__host__ __device__ constexpr int64_t parts_bytes(int hd, int rows, int kv_heads, int wgs) {
+    return (int64_t)kv_heads * wgs * (2 * rows * (hd + 2) * (int)sizeof(float) + (int)sizeof(Begun));
+}
 
 __device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -232,68 +273,23 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
     const int l16 = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.x % c.kv_heads, wg = blockIdx.x / c.kv_heads, G = work.G;
     const Score sc = score_of(a);
-    const Parts<HD> parts = {ws, ROWS, work.wgs};
-
-    int64_t units, at;
-    const int64_t run = kv_run(c, s, work, units);
-    int64_t u = wg * run;
-    const int64_t u_end = u + run < units ? u + run : units;
-    int seq = 0, pages = 0;
-    if (u >= u_end ||
-        !find_unit(u, s.n_seq, [&](int i) { int p; const int64_t t = kv_tiles(c, s, work, i, p); return t * p; }, seq, at))
-        return;
-    seq = __builtin_amdgcn_readfirstlane(seq);
-    int64_t tiles = kv_tiles(c, s, work, seq, pages);
-    int64_t tile = at / pages;
-    int page0 = (int)(at % pages);
-    while (u < u_end) {
+    const Parts<HD> parts = {ws, ROWS, c.kv_heads, work.wgs};
+    KvRun run;
+    const bool any = kv_run(c, s, work, wg, run);
+    if (ws && tid == 0) parts.begun(kvh, wg)->last = 0;
+    if (!any) return;
+    do {
+        const int page0 = run.page, pages = run.pages;
         const bool whole = pages <= WHOLE;
         if (!(whole && page0)) {
-            const int page1 = whole || pages - page0 <= u_end - u ? pages : page0 + (int)(u_end - u);
+            const int page1 = whole || pages - page0 <= run.end - run.u ? pages : page0 + run.end - run.u;
+            const int seq = run.seq;
             int first, cnt, len, base;
             seq_rows(s, seq, first, cnt);
             kv_len(c, seq, cnt, len, base);
-            const int rows = cnt * G, r0 = (int)tile * ROWS;
+            const int rows = cnt * G, r0 = run.tile * ROWS;
             auto limit = [&](int tok) { return a.causal && base + tok + 1 < len ? base + tok + 1 : len; };
             const int lo = limit(r0 / G);  // keys that all rows see
-            // rows of this lane: R times l16; q's fragments, 16 channels of each 64
-            half8 qf[R][NT][2 * KU];
-            float f[R], m[R], l[R], slope2[R];
-            int pos[R], lim[R];
-            f32x4 acc[R][DT];
-#pragma unroll
-            for (int r = 0; r < R; r++) {
-                const int row = r0 + 16 * r + l16, rc = row < rows ? row : rows - 1;
-                const int tok = rc / G, head = kvh * G + rc % G;
-                const int64_t at_q = (int64_t)(first + tok) * ldq + head * HD + 16 * g;
-                float x[2 * KU][8], top = 0.f;
-#pragma unroll
-                for (int i = 0; i < 2 * KU; i++) {
-                    load8(q, a.type, at_q + 64 * (i >> 1) + 8 * (i & 1), x[i]);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[i][e]));
-                }
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                const float up = pow2_to_14(top);
-                f[r] = sc.f / up;
-#pragma unroll
-                for (int i = 0; i < 2 * KU; i++)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const Two<_Float16> y = split<_Float16>(x[i][e] * up);
-                        qf[r][0][i][e] = y.hi;
-                        if constexpr (NT == 2) qf[r][NT - 1][i][e] = y.lo;
-                    }
-                pos[r] = base + tok;
-                lim[r] = limit(tok);
-                slope2[r] = sc.bias ? a.slopes[head] * LOG2E : 0.f;
-                m[r] = M_NONE;
-                l[r] = 0.f;
-#pragma unroll
-                for (int d = 0; d < DT; d++) acc[r][d] = f32x4{};
-            }
-
             // 64 of this wavefront's pages at a time, one to a lane: page and scales
             int ids = -1;
             f32x2 scs = {};
@@ -309,11 +305,55 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
                 return (const u32x4 *)(c.pool + ((int64_t)(id < 0 ? 0 : id) * c.kv_heads + kvh) * 2 * KV_PAGE * HD) + lane;
             };
             const int n_pages = (page1 - page0 - wave + FEW_W - 1) / FEW_W;
+            // rows of this lane: R times l16; q's fragments, 16 channels of each 64.
+            // q, the first pages and their K are on their way before any is used.
+            Raw8 raw[R][2 * KU];
+            float f[R], m[R], l[R], slope2[R];
+            int pos[R], lim[R];
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const int row = r0 + 16 * r + l16, rc = row < rows ? row : rows - 1;
+                const int tok = rc / G, head = kvh * G + rc % G;
+                const int64_t at_q = (int64_t)(first + tok) * ldq + head * HD + 16 * g;
+#pragma unroll
+                for (int i = 0; i < 2 * KU; i++) raw[r][i] = load8(q, a.type, at_q + 64 * (i >> 1) + 8 * (i & 1));
+                pos[r] = base + tok;
+                lim[r] = limit(tok);
+                slope2[r] = sc.bias ? a.slopes[head] * LOG2E : 0.f;
+            }
             if (n_pages > 0) {
                 load_ids(0);
                 const u32x4 *b = block(0);
 #pragma unroll
                 for (int i = 0; i < 4 * KU; i++) kr[i] = b[64 * i];
+            }
+            half8 qf[R][NT][2 * KU];
+            f32x4 acc[R][DT];
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                float x[2 * KU][8], top = 0.f;
+#pragma unroll
+                for (int i = 0; i < 2 * KU; i++) {
+                    values8(raw[r][i], a.type, x[i]);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[i][e]));
+                }
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float up = pow2_to_14(top);
+                f[r] = sc.f / up;
+#pragma unroll
+                for (int i = 0; i < 2 * KU; i++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const Two<_Float16> y = split<_Float16>(x[i][e] * up);
+                        qf[r][0][i][e] = y.hi;
+                        if constexpr (NT == 2) qf[r][NT - 1][i][e] = y.lo;
+                    }
+                m[r] = M_NONE;
+                l[r] = 0.f;
+#pragma unroll
+                for (int d = 0; d < DT; d++) acc[r][d] = f32x4{};
             }
             for (int n = 0; n < n_pages; n++) {
                 const u32x4 *b = block(n);
@@ -421,6 +461,8 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
             __syncthreads();
             const bool done = page0 == 0 && page1 == pages;
             float *part = done ? nullptr : parts.of(kvh, wg, page0 == 0);
+            if (!done && page0 == 0 && tid == 0)
+                *parts.begun(kvh, wg) = {(run.u + pages - 1) / run.size, first, r0, rows};
             for (int e = tid; e < ROWS * HD / 4; e += 64 * FEW_W) {
                 const int row = e / (HD / 4), d = e % (HD / 4) * 4;
                 float top = sm[0][row];
@@ -448,65 +490,64 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
                 }
             }
             __syncthreads();
-            u += page1 - page0;
+            run.u += page1 - page0;
         } else {
-            u += pages - page0;
+            run.u += pages - page0;
         }
-        page0 = 0;
-        if (++tile >= tiles) {
-            tile = 0;
-            do {
-                if (++seq >= s.n_seq) return;
-                tiles = kv_tiles(c, s, work, seq, pages);
-            } while (tiles == 0);
-        }
-    }
+    } while (run.u < run.end && kv_next(c, s, work, run));
 }
 
-// One workgroup to a tile and key head: where the tile was divided, its parts in order.
-template <int HD>
-__global__ __launch_bounds__(256) void k_kv_join(Fh3kAttn a, Fh3kKv c, void *__restrict__ o, int64_t ldo, Fh3kSeqs s,
-                                                 KvWork work, const float *__restrict__ ws) {
-    const int tid = threadIdx.x, kvh = blockIdx.y, G = work.G, ROWS = work.rows_per_tile;
-    int seq, pages, first, cnt;
-    int64_t tile, units;
-    if (!find_unit(blockIdx.x, s.n_seq, [&](int i) { int p; return kv_tiles(c, s, work, i, p); }, seq, tile)) return;
-    kv_tiles(c, s, work, seq, pages);
-    if (pages <= WHOLE) return;
-    const int64_t run = kv_run(c, s, work, units);
-    int64_t u0 = 0;  // units before the tile
-    for (int i = tid & 63; i < seq; i += 64) {
-        int p;
-        const int64_t t = kv_tiles(c, s, work, i, p);
-        u0 += t * p;
+// Joins the parts of a divided tile in order.  A workgroup takes RB rows of the tile
+// that workgroup blockIdx.x of key head blockIdx.y began; SB groups of threads take
+// every SB-th part each.
+template <int HD, int SB>
+__global__ __launch_bounds__(256) void k_kv_join(Fh3kAttn a, Fh3kKv c, void *__restrict__ o, int64_t ldo, KvWork work,
+                                                 const float *__restrict__ ws) {
+    constexpr int RB = 1024 / HD / SB;
+    __shared__ __align__(16) float so[SB][RB * HD];
+    __shared__ float sm[SB][RB], sl[SB][RB];
+    const int tid = threadIdx.x, wg = blockIdx.x, kvh = blockIdx.y, G = work.G, ROWS = 1 << work.shift;
+    const Parts<HD> parts = {(float *)ws, ROWS, c.kv_heads, work.wgs};
+    const Begun b = *parts.begun(kvh, wg);
+    const int row0 = blockIdx.z * RB;
+    if (b.last == 0 || b.r0 + row0 >= b.rows) return;
+    const int grp = tid / (256 / SB), t = tid % (256 / SB), r = t / (HD / 4), d = t % (HD / 4) * 4, row = row0 + r;
+    float top = M_NONE, sum = 0.f;
+    f32x4 x = {};
+#pragma unroll 4
+    for (int w = wg + grp; w <= b.last; w += SB) {
+        const float *p = parts.of(kvh, w, w == wg);
+        const float pm = p[ROWS * HD + row], pl = p[ROWS * (HD + 1) + row];
+        const f32x4 y = *(const f32x4 *)(p + row * HD + d);
+        const float now = fmaxf(top, pm);
+        const float keep = __builtin_amdgcn_exp2f(top - now), add = __builtin_amdgcn_exp2f(pm - now);
+        top = now;
+        sum = sum * keep + pl * add;
+#pragma unroll
+        for (int v = 0; v < 4; v++) x[v] = x[v] * keep + y[v] * add;
     }
-    u0 = wave_sum(u0) + tile * pages;
-    const int w0 = (int)(u0 / run), w1 = (int)((u0 + pages - 1) / run);
-    if (w0 == w1) return;
-    seq_rows(s, seq, first, cnt);
-    const int rows = cnt * G, r0 = (int)tile * ROWS;
-    const Parts<HD> parts = {(float *)ws, ROWS, work.wgs};
-    for (int e = tid; e < ROWS * HD / 4; e += 256) {
-        const int row = e / (HD / 4), d = e % (HD / 4) * 4;
-        if (r0 + row >= rows) break;
-        float top = M_NONE, sum = 0.f;
-        f32x4 x = {};
-        for (int w = w0; w <= w1; w++) {
-            const float *p = parts.of(kvh, w, w == w0);
-            const float pm = p[ROWS * HD + row], now = fmaxf(top, pm);
+    if constexpr (SB > 1) {
+        *(f32x4 *)&so[grp][r * HD + d] = x;
+        if (d == 0) sm[grp][r] = top, sl[grp][r] = sum;
+        __syncthreads();
+        if (grp) return;
+#pragma unroll
+        for (int e = 1; e < SB; e++) {
+            const float pm = sm[e][r], now = fmaxf(top, pm);
             const float keep = __builtin_amdgcn_exp2f(top - now), add = __builtin_amdgcn_exp2f(pm - now);
-            const f32x4 y = *(const f32x4 *)(p + row * HD + d);
+            const f32x4 y = *(const f32x4 *)&so[e][r * HD + d];
             top = now;
-            sum = sum * keep + p[ROWS * (HD + 1) + row] * add;
+            sum = sum * keep + sl[e][r] * add;
 #pragma unroll
             for (int v = 0; v < 4; v++) x[v] = x[v] * keep + y[v] * add;
         }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const int tok = (r0 + row) / G, head = kvh * G + (r0 + row) % G;
-#pragma unroll
-        for (int v = 0; v < 4; v++) x[v] *= inv;
-        store4(o, a.type, (int64_t)(first + tok) * ldo + head * HD + d, x);
     }
+    if (b.r0 + row >= b.rows) return;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int tok = (b.r0 + row) / G, head = kvh * G + (b.r0 + row) % G;
+#pragma unroll
+    for (int v = 0; v < 4; v++) x[v] *= inv;
+    store4(o, a.type, (int64_t)(b.first + tok) * ldo + head * HD + d, x);
 }
 
 // Many rows to a sequence: tiles of 128, 32 to a wavefront.  A page is turned
@@ -527,28 +568,21 @@ __global__ __launch_bounds__(64 * MANY_W, 2) void k_kv_many(Fh3kAttn a, Fh3kKv c
     const int l32 = lane & 31, hf = lane >> 5;
     const int kvh = blockIdx.x % c.kv_heads, wg = blockIdx.x / c.kv_heads, G = work.G;
     const Score sc = score_of(a);
-    const Parts<HD> parts = {ws, ROWS, work.wgs};
-
-    int64_t units, at;
-    const int64_t run = kv_run(c, s, work, units);
-    int64_t u = wg * run;
-    const int64_t u_end = u + run < units ? u + run : units;
-    int seq = 0, pages = 0;
-    if (u >= u_end ||
-        !find_unit(u, s.n_seq, [&](int i) { int p; const int64_t t = kv_tiles(c, s, work, i, p); return t * p; }, seq, at))
-        return;
-    seq = __builtin_amdgcn_readfirstlane(seq);
-    int64_t tiles = kv_tiles(c, s, work, seq, pages);
-    int64_t tile = at / pages;
-    int page0 = (int)(at % pages);
-    while (u < u_end) {
+    const Parts<HD> parts = {ws, ROWS, c.kv_heads, work.wgs};
+    KvRun run;
+    const bool any = kv_run(c, s, work, wg, run);
+    if (ws && tid == 0) parts.begun(kvh, wg)->last = 0;
+    if (!any) return;
+    do {
+        const int page0 = run.page, pages = run.pages;
         const bool whole = pages <= WHOLE;
         if (!(whole && page0)) {
-            const int page1 = whole || pages - page0 <= u_end - u ? pages : page0 + (int)(u_end - u);
+            const int page1 = whole || pages - page0 <= run.end - run.u ? pages : page0 + run.end - run.u;
+            const int seq = run.seq;
             int first, cnt, len, base;
             seq_rows(s, seq, first, cnt);
             kv_len(c, seq, cnt, len, base);
-            const int rows = cnt * G, r0 = (int)tile * ROWS;
+            const int rows = cnt * G, r0 = run.tile * ROWS;
             auto limit = [&](int tok) { return a.causal && base + tok + 1 < len ? base + tok + 1 : len; };
             const int row = r0 + WAVE_R * wave + l32, rc = row < rows ? row : rows - 1;
             const int tok = rc / G, head = kvh * G + rc % G;
@@ -660,8 +694,10 @@ __global__ __launch_bounds__(64 * MANY_W, 2) void k_kv_many(Fh3kAttn a, Fh3kKv c
             }
 
             const float l = w.l + half_swap(w.l);
+            const bool done = page0 == 0 && page1 == pages;
+            if (!done && page0 == 0 && tid == 0)
+                *parts.begun(kvh, wg) = {(run.u + pages - 1) / run.size, first, r0, rows};
             if (row < rows) {
-                const bool done = page0 == 0 && page1 == pages;
                 float *part = done ? nullptr : parts.of(kvh, wg, page0 == 0);
                 const float inv = done ? (l == 0.f ? 0.f : ref / l) : ref;
                 const int64_t at_o = (int64_t)(first + tok) * ldo + head * HD;
@@ -679,19 +715,11 @@ __global__ __launch_bounds__(64 * MANY_W, 2) void k_kv_many(Fh3kAttn a, Fh3kKv c
                         else *(f32x4 *)(part + r * HD + d) = x;
                     }
             }
-            u += page1 - page0;
+            run.u += page1 - page0;
         } else {
-            u += pages - page0;
+            run.u += pages - page0;
         }
-        page0 = 0;
-        if (++tile >= tiles) {
-            tile = 0;
-            do {
-                if (++seq >= s.n_seq) return;
-                tiles = kv_tiles(c, s, work, seq, pages);
-            } while (tiles == 0);
-        }
-    }
+    } while (run.u < run.end && kv_next(c, s, work, run));
 }
 
 }  // namespace
@@ -732,28 +760,29 @@ static KvForm kv_form(const Fh3kAttn &a, const Fh3kKv &c, const Fh3kSeqs &s) {
     KvForm f;
     const int64_t G = a.heads / a.kv_heads, rows = s.n_tok * G, avg = (rows + s.n_seq - 1) / s.n_seq;
     f.few = avg <= 32;
-    const int R = avg <= 16 ? 16 : avg <= 32 ? 32 : WAVE_R * MANY_W;
-    f.tiles = rows / R + (s.n_seq < s.n_tok ? s.n_seq : s.n_tok);
+    static_assert(WAVE_R * MANY_W == 1 << 7, "");
+    const int shift = avg <= 16 ? 4 : avg <= 32 ? 5 : 7;
+    f.tiles = (rows >> shift) + (s.n_seq < s.n_tok ? s.n_seq : s.n_tok);
     const int64_t runs = (f.tiles * c.max_pages + WHOLE - 1) / WHOLE, most = (512 + a.kv_heads - 1) / a.kv_heads;
-    f.work = {(int)G, R, (int)(runs < most ? runs : most)};
+    f.work = {(int)G, shift, (int)(runs < most ? runs : most)};
     f.join = c.max_pages > WHOLE && f.work.wgs > 1;
     return f;
 }
 
 extern "C" size_t fh3k_kv_attn_ws_bytes(const Fh3kAttn *a, const Fh3kKv *c, Fh3kSeqs s) {
     const KvForm f = kv_form(*a, *c, s);
-    return f.join ? (size_t)a->kv_heads * f.work.wgs * 2 * f.work.rows_per_tile * (a->hd + 2) * sizeof(float) : 0;
+    return f.join ? (size_t)parts_bytes(a->hd, 1 << f.work.shift, a->kv_heads, f.work.wgs) : 0;
 }
 
 template <int HD>
 static hipError_t kv_attn(const Fh3kAttn &a, const Fh3kKv &c, const void *q, int64_t ldq, void *o, int64_t ldo,
                           const Fh3kSeqs &s, float *ws, hipStream_t st) {
     const KvForm f = kv_form(a, c, s);
-    if (f.tiles > 0x7FFFFF) return hipErrorInvalidValue;
+    if (f.tiles * c.max_pages > 0x7FFFFFFF) return hipErrorInvalidValue;
     const dim3 grid((unsigned)f.work.wgs * a.kv_heads);
     const bool two = a.type == FH3K_F32;
-#define FH3K_KV(K, W) hipLaunchKernelGGL(K, grid, dim3(64 * W), 0, st, a, c, q, ldq, o, ldo, s, f.work, ws)
-    if (f.work.rows_per_tile == 16) {
+#define FH3K_KV(K, W) hipLaunchKernelGGL(K, grid, dim3(64 * W), 0, st, a, c, q, ldq, o, ldo, s, f.work, f.join ? ws : nullptr)
+    if (f.work.shift == 4) {
         if (two) FH3K_KV((k_kv_few<HD, 1, 2>), FEW_W);
         else FH3K_KV((k_kv_few<HD, 1, 1>), FEW_W);
     } else if (f.few) {
@@ -766,7 +795,11 @@ static hipError_t kv_attn(const Fh3kAttn &a, const Fh3kKv &c, const void *q, int
 #undef FH3K_KV
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !f.join) return e;
-    hipLaunchKernelGGL(k_kv_join<HD>, dim3((unsigned)f.tiles, a.kv_heads), dim3(256), 0, st, a, c, o, ldo, s, f.work, ws);
+    // few rows: divided among up to 64 workgroups; many: between two or three
+    const int rb = 1024 / HD / (f.few ? 4 : 1);
+    const dim3 jg(f.work.wgs, a.kv_heads, (1 << f.work.shift) / rb);
+    if (f.few) hipLaunchKernelGGL((k_kv_join<HD, 4>), jg, dim3(256), 0, st, a, c, o, ldo, f.work, ws);
+    else hipLaunchKernelGGL((k_kv_join<HD, 1>), jg, dim3(256), 0, st, a, c, o, ldo, f.work, ws);
     return hipGetLastError();
 }
 

@@ -50,27 +50,32 @@ __device__ __forceinline__ void seq_rows(const Fh3kSeqs &s, int i, int &a, int &
     }
 }
 
-// Work unit w when sequence i has units(i) of them: its sequence and its place
-// there, or false past the last.  Every lane of a wavefront calls it with the
-// same w; 64 sequences at a time.
-template <class F> __device__ __forceinline__ bool find_unit(int64_t w, int n_seq, F units, int &seq, int64_t &at) {
+// Sums over the lanes below and this one.
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast 15, 31
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+    return x;
+}
+// Work unit w when sequence i has units(i) of them (fewer than 2^31 in all): its
+// sequence and its place there, or false past the last.  Every lane of a
+// wavefront calls it with the same w; 64 sequences at a time.
+template <class F> __device__ __forceinline__ bool find_unit(int w, int n_seq, F units, int &seq, int &at) {
     const int lane = threadIdx.x & 63;
     for (int s0 = 0; s0 < n_seq; s0 += 64) {
-        const int64_t u = s0 + lane < n_seq ? units(s0 + lane) : 0;
-        int64_t end = u;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int64_t o = __shfl_up(end, d);
-            end += lane >= d ? o : 0;
-        }
+        const int u = s0 + lane < n_seq ? units(s0 + lane) : 0;
+        const int end = wave_scan(u);
         const uint64_t past = __ballot(end > w);
         if (past) {
             const int l = __builtin_ctzll(past);
             seq = s0 + l;
-            at = w - (__shfl(end, l) - __shfl(u, l));
+            at = w - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(u, l));
             return true;
         }
-        w -= __shfl(end, 63);
+        w -= __builtin_amdgcn_readlane(end, 63);
     }
     return false;
 }

@@ -81,16 +81,15 @@ __global__ __launch_bounds__(64 * Operand<TY>::NW, 2) void k_attn_seqs(
     // sequence see most keys and go first.
     const int kvh = blockIdx.x % a.kv_heads, G = a.heads / a.kv_heads;
     int seq, first, cnt;
-    int64_t at;
-    if (!find_unit(tiles - 1 - (int)(blockIdx.x / a.kv_heads), s.n_seq, [&](int i) {
+    int at;
+    if (!find_unit(tiles - 1 - (int)blockIdx.x / a.kv_heads, s.n_seq, [&](int i) {
             int b, n;
             seq_rows(s, i, b, n);
-            return ((int64_t)n * G + ROWS - 1) / ROWS;
+            return (n * G + ROWS - 1) / ROWS;
         }, seq, at))
         return;
-    seq = __builtin_amdgcn_readfirstlane(seq);
     seq_rows(s, seq, first, cnt);
-    const int rows = cnt * G, r0 = (int)at * ROWS;
+    const int rows = cnt * G, r0 = at * ROWS;
     int pre = a.causal ? (prefix ? prefix[seq] : 0) : cnt;
     pre = pre < cnt ? pre : cnt;
     auto limit = [&](int i) { return i + 1 > pre ? i + 1 : pre; };  // keys that token i sees

@@ -59,22 +59,34 @@ __device__ __forceinline__ float pow2_to_14(float amax) {
     return amax > 0.f && amax <= 3.402823466e38f ? __builtin_bit_cast(float, (uint32_t)(e + 127) << 23) : 1.f;
 }
 
-// eight consecutive values of a row
-__device__ __forceinline__ void load8(const void *p, int type, int64_t at, float (&x)[8]) {
+// Eight consecutive values of a row: as they stand in memory (so that the load can
+// be on its way while other work is done), and as fp32.
+struct Raw8 {
+    u32x4 a, b;  // b: fp32 only
+};
+__device__ __forceinline__ Raw8 load8(const void *p, int type, int64_t at) {
+    Raw8 r = {};
     if (type == FH3K_F32) {
-        const f32x4 *q = (const f32x4 *)((const float *)p + at);
-        const f32x4 a = q[0], b = q[1];
+        const u32x4 *q = (const u32x4 *)((const float *)p + at);
+        r.a = q[0], r.b = q[1];
+    } else {
+        r.a = *(const u32x4 *)((const uint16_t *)p + at);
+    }
+    return r;
+}
+__device__ __forceinline__ void values8(const Raw8 &r, int type, float (&x)[8]) {
+    if (type == FH3K_F32) {
+        const f32x4 a = __builtin_bit_cast(f32x4, r.a), b = __builtin_bit_cast(f32x4, r.b);
 #pragma unroll
         for (int i = 0; i < 4; i++) x[i] = a[i], x[4 + i] = b[i];
     } else if (type == FH3K_F16) {
-        const half8 a = *(const half8 *)((const _Float16 *)p + at);
+        const half8 a = __builtin_bit_cast(half8, r.a);
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] = (float)a[i];
     } else {
-        const u32x4 a = *(const u32x4 *)((const uint16_t *)p + at);
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            x[i] = __builtin_bit_cast(float, i & 1 ? a[i >> 1] & 0xFFFF0000u : a[i >> 1] << 16);
+            x[i] = __builtin_bit_cast(float, i & 1 ? r.a[i >> 1] & 0xFFFF0000u : r.a[i >> 1] << 16);
     }
 }
 // four consecutive values of an output row
@@ -128,7 +140,7 @@ template <int HD, class TQ, class TP, int QT, int KT> struct Rows {
             float x[KS][8], top = 0.f;
 #pragma unroll
             for (int kk = 0; kk < KS; kk++) {
-                load8(qp, type, at + 16 * kk + 8 * hf, x[kk]);
+                values8(load8(qp, type, at + 16 * kk + 8 * hf), type, x[kk]);
 #pragma unroll
                 for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[kk][i]));
             }
