@@ -1045,7 +1045,7 @@ static size_t value_bytes(int type) {
 static int check_rows(const void *p, int64_t *ld, int64_t width, int type, const char *what, const char *fn) {
     if (!p) return set_err(FH3_E_INVALID, "%s: NULL %s", fn, what);
     if (*ld == 0) *ld = width;
-    if ((uintptr_t)p & 15u || *ld < width || *ld > ((int64_t)1 << 32) || *ld * value_bytes(type) % 16)
+    if ((uintptr_t)p & 15u || *ld < width || *ld > ((int64_t)1 << 23) || *ld * value_bytes(type) % 16)
         return set_err(FH3_E_INVALID, "%s: rows of %s must be 16-byte aligned and not overlap", fn, what);
     return FH3_OK;
 }

@@ -39,6 +39,19 @@ template <class V8, int VROW> __device__ __forceinline__ V8 v_frag(const uint16_
     return __builtin_bit_cast(V8, w);
 }
 
+template <int CTRL> __device__ __forceinline__ float dpp_max(float x) {
+    const int y = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xF, 0xF, true);
+    return fmaxf(x, __builtin_bit_cast(float, y));
+}
+// The largest of N = 16 or 32 neighbouring lanes' values, in all of them.
+template <int N> __device__ __forceinline__ float row_max(float x) {
+    x = dpp_max<0xB1>(x);   // quad_perm 1 0 3 2
+    x = dpp_max<0x4E>(x);   // quad_perm 2 3 0 1
+    x = dpp_max<0x141>(x);  // row_half_mirror
+    x = dpp_max<0x140>(x);  // row_mirror
+    return N == 32 ? fmaxf(x, __shfl_xor(x, 16)) : x;
+}
+
 // Whether any of 16 bytes of values is infinite or NaN (all exponent bits set);
 // those become 0.
 template <int TYPE> __device__ __forceinline__ bool not_finite(u32x4 &w) {
@@ -112,15 +125,26 @@ __global__ __launch_bounds__(64 * Operand<TY>::NW, 2) void k_attn_seqs(
     // The next tile's rows, on their way from memory while this one is in work.
     constexpr int VAL = TY == 2 ? 4 : 8, CPR = HD / VAL, CH = TILE_K * CPR / NT;  // 16-byte pieces
     u32x4 rk[CH], rv[CH];
-    const int64_t k0 = (int64_t)first * ldk + kvh * HD, v0 = (int64_t)first * ldv + kvh * HD;
-    auto load = [&](int j0) {
+    const char *kp = (const char *)k + ((int64_t)first * ldk + kvh * HD) * (16 / VAL);
+    const char *vp = (const char *)v + ((int64_t)first * ldv + kvh * HD) * (16 / VAL);
+    uint32_t ko[CH], vo[CH];  // of this thread's pieces in a tile
 #pragma unroll
-        for (int i = 0; i < CH; i++) {
-            const int c = tid + i * NT, key = j0 + c / CPR, d = c % CPR * VAL;
-            rk[i] = rv[i] = u32x4{};
-            if (key < cnt) {  // rows behind belong to another sequence
-                rk[i] = *(const u32x4 *)((const char *)k + (k0 + key * ldk + d) * (16 / VAL));
-                rv[i] = *(const u32x4 *)((const char *)v + (v0 + key * ldv + d) * (16 / VAL));
+    for (int i = 0; i < CH; i++) {
+        const int c = tid + i * NT;
+        ko[i] = ((uint32_t)(c / CPR) * (uint32_t)ldk + c % CPR * VAL) * (16 / VAL);
+        vo[i] = ((uint32_t)(c / CPR) * (uint32_t)ldv + c % CPR * VAL) * (16 / VAL);
+    }
+    auto load = [&](int j0) {
+        const char *kt = kp + j0 * ldk * (16 / VAL), *vt = vp + j0 * ldv * (16 / VAL);
+        if (j0 + TILE_K <= cnt) {
+#pragma unroll
+            for (int i = 0; i < CH; i++) rk[i] = *(const u32x4 *)(kt + ko[i]), rv[i] = *(const u32x4 *)(vt + vo[i]);
+        } else {  // past the sequence its last row again: no row sees those keys
+#pragma unroll
+            for (int i = 0; i < CH; i++) {
+                const int c = tid + i * NT, key = j0 + c / CPR < cnt ? c / CPR : cnt - 1 - j0;
+                rk[i] = *(const u32x4 *)(kt + (key * ldk + c % CPR * VAL) * (16 / VAL));
+                rv[i] = *(const u32x4 *)(vt + (key * ldv + c % CPR * VAL) * (16 / VAL));
             }
         }
     };
@@ -144,8 +168,7 @@ __global__ __launch_bounds__(64 * Operand<TY>::NW, 2) void k_attn_seqs(
             } else {
                 const f32x4 x = __builtin_bit_cast(f32x4, rk[i]), y = __builtin_bit_cast(f32x4, rv[i]);
                 float top = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-#pragma unroll
-                for (int e = 1; e < CPR; e <<= 1) top = fmaxf(top, __shfl_xor(top, e));
+                top = row_max<CPR>(top);
                 const float up = pow2_to_14(top);
                 if (c % CPR == 0) t.ks[key] = 1.f / up;
                 TQ kh[4], kl[4];
@@ -200,7 +223,7 @@ __global__ __launch_bounds__(64 * Operand<TY>::NW, 2) void k_attn_seqs(
                 for (int db = 0; db < R::DB; db++)
 #pragma unroll
                     for (int g = 0; g < 4; g++) {
-                        const int64_t at_v = v0 + j * ldv + 32 * db + 8 * g + 4 * hf;
+                        const int64_t at_v = (first + j) * ldv + kvh * HD + 32 * db + 8 * g + 4 * hf;
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             const float x = value_at(v, Op::TYPE, at_v + i);

@@ -24,8 +24,26 @@ constexpr float OFFSET = 6.f, RAISE = 14.f;
 constexpr float M_NONE = -1e30f;  // no key seen yet: finite, so that masked t = -inf gives 0
 
 template <class T> struct Vec;
-template <> struct Vec<_Float16> { typedef half8 v8; };
-template <> struct Vec<__bf16> { typedef bf8 v8; };
+template <> struct Vec<_Float16> {
+    typedef half8 v8;
+    static __device__ __forceinline__ uint32_t pair(float a, float b) {
+        uint32_t w = __builtin_bit_cast(uint32_t, half2v{(_Float16)a, (_Float16)b});
+        asm("" : "+v"(w));  // one pair, not converted once for each use
+        return w;
+    }
+    static __device__ __forceinline__ float sum(uint32_t w, float c) {
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, w), half2v{1, 1}, c, false);
+    }
+};
+template <> struct Vec<__bf16> {
+    typedef bf8 v8;
+    static __device__ __forceinline__ uint32_t pair(float a, float b) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf2));
+    }
+    static __device__ __forceinline__ float sum(uint32_t w, float c) {
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf2, w), bf2{1.f, 1.f}, c, false);
+    }
+};
 
 __device__ __forceinline__ f32x16 mfma32(half8 a, half8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
@@ -186,33 +204,29 @@ template <int HD, class TQ, class TP, int QT, int KT> struct Rows {
                 if constexpr (QT == 2) s[st] = mfma32(a, q[1][kk], s[st]);
                 s[st] = mfma32(a, q[0][kk], s[st]);
             }
-        const float c = f * kscale;
-        if (!sc.cap2 && !sc.bias) {
+        if constexpr (PER_KEY) {
 #pragma unroll
             for (int st = 0; st < 2; st++)
 #pragma unroll
                 for (int g = 0; g < 4; g++) {
-                    f32x4 ks = {c, c, c, c};
-                    if constexpr (PER_KEY) ks = *(const f32x4 *)(sks + 32 * st + 8 * g + 4 * hf) * f;
+                    const f32x4 ks = *(const f32x4 *)(sks + 32 * st + 8 * g + 4 * hf);
 #pragma unroll
                     for (int v = 0; v < 4; v++) s[st][4 * g + v] *= ks[v];
                 }
-        } else {
+        }
+        float c = f * kscale;  // t = c s, unless there is more to do
+        if (sc.cap2 || sc.bias) {
             const float far = (float)(pos - j0 - 4 * hf);
 #pragma unroll
             for (int st = 0; st < 2; st++)
 #pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    f32x4 ks = {c, c, c, c};
-                    if constexpr (PER_KEY) ks = *(const f32x4 *)(sks + 32 * st + 8 * g + 4 * hf) * f;
-#pragma unroll
-                    for (int v = 0; v < 4; v++) {
-                        float t = s[st][4 * g + v] * ks[v];
-                        if (sc.cap2) t = capped(t, sc.cap2);
-                        if (sc.bias) t = fmaf(-slope2, fabsf(far - (float)(32 * st + 8 * g + v)), t);
-                        s[st][4 * g + v] = t;
-                    }
+                for (int v = 0; v < 16; v++) {
+                    float t = s[st][v] * c;
+                    if (sc.cap2) t = capped(t, sc.cap2);
+                    if (sc.bias) t = fmaf(-slope2, fabsf(far - (float)(32 * st + 8 * (v >> 2) + (v & 3))), t);
+                    s[st][v] = t;
                 }
+            c = 1.f;
         }
         if (cut) {
             const int left = seen - j0 - 4 * hf;
@@ -221,11 +235,10 @@ template <int HD, class TQ, class TP, int QT, int KT> struct Rows {
 #pragma unroll
                 for (int v = 0; v < 16; v++) s[st][v] = left > 32 * st + 8 * (v >> 2) + (v & 3) ? s[st][v] : -INFINITY;
         }
-        float mt = s[0][0];
+        float mt = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-        for (int v = 1; v < 16; v++) mt = fmaxf(mt, s[0][v]);
-#pragma unroll
-        for (int v = 0; v < 16; v++) mt = fmaxf(mt, s[1][v]);
+        for (int v = 1; v < 16; v++) mt = fmaxf(fmaxf(mt, s[0][v]), s[1][v]);
+        mt *= c;
         if (__ballot(mt > m + RAISE)) {  // wave-uniform
             mt = fmaxf(mt, half_swap(mt));
             const float now = mt > m + RAISE ? mt - OFFSET : m;
@@ -235,25 +248,31 @@ template <int HD, class TQ, class TP, int QT, int KT> struct Rows {
 #pragma unroll
             for (int i = 0; i < DB; i++) o[i] *= keep;
         }
+        const float nm = -m;
+        float sum[2] = {};
 #pragma unroll
-        for (int st = 0; st < 2; st++)
+        for (int tt = 0; tt < 4; tt++) {
+            float p[8];
 #pragma unroll
-            for (int v = 0; v < 16; v++) s[st][v] = __builtin_amdgcn_exp2f(s[st][v] - m);
-        float sum[4] = {};
+            for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(fmaf(s[tt >> 1][8 * (tt & 1) + e], c, nm));
+            if constexpr (QT == 2) {
 #pragma unroll
-        for (int tt = 0; tt < 4; tt++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float p = s[tt >> 1][8 * (tt & 1) + e];
-                sum[e & 3] += p;
-                if constexpr (QT == 2) {
-                    const Two<TP> y = split<TP>(p);
+                for (int e = 0; e < 8; e++) {
+                    sum[e & 1] += p[e];
+                    const Two<TP> y = split<TP>(p[e]);
                     pf[0][tt][e] = y.hi, pf[1][tt][e] = y.lo;
-                } else {
-                    pf[0][tt][e] = (TP)p;
                 }
+            } else {  // the sum is of the rounded weights, which the product takes
+                u32x4 w;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    w[e] = Vec<TP>::pair(p[2 * e], p[2 * e + 1]);
+                    sum[e & 1] = Vec<TP>::sum(w[e], sum[e & 1]);
+                }
+                pf[0][tt] = __builtin_bit_cast(p8, w);
             }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        }
+        l += sum[0] + sum[1];
     }
 };
 

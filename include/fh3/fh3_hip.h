@@ -219,8 +219,8 @@ typedef struct Fh3AttnCfg {
 } Fh3AttnCfg;
 
 /* q [n_tok][heads][head_dim], k and v [n_tok][kv_heads][head_dim], o as q, at
- * ldq, ldk, ldv, ldo values per token (0 = dense), so that q, k and v may be
- * parts of one projection's output.  Sequence s is the rows d_first[s] ..
+ * ldq, ldk, ldv, ldo values per token (0 = dense, at most 2^23), so that q, k and
+ * v may be parts of one projection's output.  Sequence s is the rows d_first[s] ..
  * d_first[s + 1] - 1 (device [n_seq + 1], non-decreasing, within n_tok); with
  * d_first NULL the rows are n_seq sequences of n_tok / n_seq.  Rows behind the
  * last sequence are neither read nor written.  d_prefix (NULL, or device
