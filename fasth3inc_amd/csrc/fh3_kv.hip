@@ -656,7 +656,9 @@ __global__ __launch_bounds__(64 * MANY_W, 2) void k_kv_many(Fh3kAttn a, Fh3kKv c
                 }
                 if (active && there_n && j0 < hi) {
                     half8 pf[NT][4];
-                    w.template weigh<false>(&sk[n & 1][0][0], sc, ks_n, nullptr, j0, j0 + KV_PAGE > lo, w.lim, pf);
+                    f32x16 x[2];
+                    w.products(&sk[n & 1][0][0], x);
+                    w.weights(x, w.template scores<false>(x, sc, ks_n, nullptr, j0, j0 + KV_PAGE > lo, w.lim), pf);
                     // pages of the same scale add up in the product's accumulator
                     if (vs_n > ref) {
                         const float down = ref / vs_n;

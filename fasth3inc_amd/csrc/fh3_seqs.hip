@@ -5,24 +5,24 @@ namespace {
 
 // How the three value types enter the matrix products.
 template <int TY> struct Operand;
-template <> struct Operand<0> { typedef _Float16 TQ, TP; static constexpr int T = 1, NW = 4, TYPE = FH3K_F16; };
-template <> struct Operand<1> { typedef __bf16 TQ, TP; static constexpr int T = 1, NW = 4, TYPE = FH3K_BF16; };
+template <> struct Operand<0> { typedef _Float16 TQ, TP; static constexpr int NW = 4, TYPE = FH3K_F16; };
+template <> struct Operand<1> { typedef __bf16 TQ, TP; static constexpr int NW = 4, TYPE = FH3K_BF16; };
 // fp32 as two 16-bit terms: q and k fp16 after a power of two for each row (22
 // bits), v and the weights bf16 (16 bits, any exponent); three products each
 template <> struct Operand<2> {
     typedef _Float16 TQ;
     typedef __bf16 TP;
-    static constexpr int T = 2, NW = 8, TYPE = FH3K_F32;
+    static constexpr int NW = 8, TYPE = FH3K_F32;
 };
 
-// A tile of K and V in LDS: T planes of K [64][HD + 8], of V [64][HD + 32] (the
+// A tile of fp32 K and V in LDS: two planes of K [64][HD + 8], of V [64][HD + 32] (the
 // transposing reads take 4 rows x 64 bytes at once: rows 64 bytes apart modulo the
-// banks), and for fp32 one factor per key.
-template <int HD, int TY> struct TileLds {
-    static constexpr int T = Operand<TY>::T, KROW = HD + 8, VROW = HD + 32;
-    uint16_t k[T][TILE_K][KROW];
-    uint16_t v[T][TILE_K][VROW];
-    float ks[T == 2 ? TILE_K : 4];
+// banks), and one factor per key.
+template <int HD> struct TileLds {
+    static constexpr int KROW = HD + 8, VROW = HD + 32;
+    uint16_t k[2][TILE_K][KROW];
+    uint16_t v[2][TILE_K][VROW];
+    float ks[TILE_K];
 };
 
 // V^T operand of channels 32 db .. and keys 16 tt ..: two transposing reads of
@@ -72,123 +72,316 @@ template <int TYPE> __device__ __forceinline__ bool not_finite(u32x4 &w) {
     return any;
 }
 
+struct SeqsArgs {
+    Fh3kAttn a;
+    const void *q, *k, *v;
+    void *o;
+    int64_t ldq, ldk, ldv, ldo;
+    Fh3kSeqs s;
+    const int *prefix;
+    int tiles;  // of all sequences at most
+};
+
+// A workgroup's tile of rows.
+struct Place {
+    int kvh, G, first, cnt, rows, r0;
+    int pre;  // tokens that every row sees
+    __device__ __forceinline__ int limit(int tok) const { return tok + 1 > pre ? tok + 1 : pre; }  // keys that it sees
+};
+// Workgroups next to each other run on different XCDs: with the key head as the
+// fastest index an XCD keeps to few heads' K and V.  The last rows of a sequence see
+// most keys and go first.
+template <int ROWS> __device__ __forceinline__ bool place(const SeqsArgs &g, Place &p) {
+    p.kvh = blockIdx.x % g.a.kv_heads;
+    p.G = g.a.heads / g.a.kv_heads;
+    int seq, at;
+    if (!find_unit(g.tiles - 1 - (int)blockIdx.x / g.a.kv_heads, g.s.n_seq, [&](int i) {
+            int b, n;
+            seq_rows(g.s, i, b, n);
+            return (n * p.G + ROWS - 1) / ROWS;
+        }, seq, at))
+        return false;
+    seq_rows(g.s, seq, p.first, p.cnt);
+    p.rows = p.cnt * p.G;
+    p.r0 = at * ROWS;
+    const int pre = g.a.causal ? (g.prefix ? g.prefix[seq] : 0) : p.cnt;
+    p.pre = pre < p.cnt ? pre : p.cnt;
+    return true;
+}
+
+// A value that is not finite must not reach rows that do not see it (their weight
+// of 0 would make it NaN): in tiles that some row of the workgroup sees only in part
+// it enters as 0, and here the channels of the rows that do see it are lost.
+template <int HD, int TYPE, class R>
+__device__ __forceinline__ void lose(R &w, const SeqsArgs &g, const Place &p, int from, int to) {
+    const int hf = (threadIdx.x >> 5) & 1;
+    uint64_t gone = 0;
+    for (int j = from; j < to; j++)
+        if (j < w.lim)
+#pragma unroll 1
+            for (int c = 0; c < HD / 8; c++)
+                for (int i = 0; i < 4; i++) {
+                    const float x = value_at(g.v, TYPE, (p.first + j) * g.ldv + p.kvh * HD + 8 * c + 4 * hf + i);
+                    gone |= (uint64_t)!(fabsf(x) <= 3.402823466e38f) << (4 * c + i);
+                }
+    if (__ballot(gone != 0)) {
+#pragma unroll
+        for (int db = 0; db < R::DB; db++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) w.o[db][v] = gone >> (16 * db + v) & 1 ? __builtin_nanf("") : w.o[db][v];
+    }
+}
+
+template <int HD, int TYPE, class R>
+__device__ __forceinline__ void put_rows(const R &w, const SeqsArgs &g, const Place &p, int row, int head) {
+    const int hf = (threadIdx.x >> 5) & 1;
+    const float l = w.l + half_swap(w.l), inv = l == 0.f ? 0.f : 1.f / l;
+    if (row >= p.rows) return;
+    const int64_t at = (int64_t)(p.first + w.pos) * g.ldo + head * HD + 4 * hf;
+#pragma unroll
+    for (int db = 0; db < R::DB; db++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            f32x4 x;
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = w.o[db][4 * c + i] * inv;
+            store4(g.o, TYPE, at + 32 * db + 8 * c, x);
+        }
+}
+
+// F16 and BF16.  K and V go from memory to LDS without registers (16 bytes a lane),
+// rows unpadded, their 16-byte (K) or 64-byte (V) pieces permuted by the row
+// so that the reads meet no bank twice.  The next tile's scores are computed
+// while this one's weights are (matrix and vector instructions alternate), so K
+// is a tile ahead of V.
 template <int HD, int TY>
-__global__ __launch_bounds__(64 * Operand<TY>::NW, 2) void k_attn_seqs(
-    Fh3kAttn a, const void *__restrict__ q, int64_t ldq, const void *__restrict__ k, int64_t ldk,
-    const void *__restrict__ v, int64_t ldv, void *__restrict__ o, int64_t ldo, Fh3kSeqs s,
-    const int *__restrict__ prefix, int tiles) {
+__global__ __launch_bounds__(256, 2) void k_attn_seqs16(SeqsArgs g) {
     typedef Operand<TY> Op;
-    typedef typename Op::TQ TQ;
-    typedef typename Op::TP TP;
-    constexpr int T = Op::T, NT = 64 * Op::NW, ROWS = WAVE_R * Op::NW;
-    typedef Rows<HD, TQ, TP, T, T> R;
-    typedef typename R::p8 p8;
-    typedef TileLds<HD, TY> Lds;
-    __shared__ __align__(16) Lds lds[2];
+    typedef typename Op::TQ T;
+    constexpr int NW = 4, ROWS = WAVE_R * NW, RB = HD * 2, TILE_B = TILE_K * RB, PPR = RB / 16;  // pieces per row
+    constexpr int CH = TILE_B / (1024 * NW);  // a wavefront's loads of a tile
+    typedef Rows<HD, T, T, 1, 1> R;
+    typedef typename R::q8 v8;
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4 *lds4;
+    typedef __attribute__((address_space(3))) void lds_void;
+    // Four arrays, not one: reads of one then need not wait for the loads into another.
+    __shared__ __align__(16) char sk0[TILE_B], sk1[TILE_B], sv0[TILE_B], sv1[TILE_B];
     __shared__ int lost;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, hf = lane >> 5;
-    // workgroups next to each other run on different XCDs: with the key head as
-    // the fastest index an XCD keeps to few heads' K and V.  The last rows of a
-    // sequence see most keys and go first.
-    const int kvh = blockIdx.x % a.kv_heads, G = a.heads / a.kv_heads;
-    int seq, first, cnt;
-    int at;
-    if (!find_unit(tiles - 1 - (int)blockIdx.x / a.kv_heads, s.n_seq, [&](int i) {
-            int b, n;
-            seq_rows(s, i, b, n);
-            return (n * G + ROWS - 1) / ROWS;
-        }, seq, at))
-        return;
-    seq_rows(s, seq, first, cnt);
-    const int rows = cnt * G, r0 = at * ROWS;
-    int pre = a.causal ? (prefix ? prefix[seq] : 0) : cnt;
-    pre = pre < cnt ? pre : cnt;
-    auto limit = [&](int i) { return i + 1 > pre ? i + 1 : pre; };  // keys that token i sees
+    Place p;
+    if (!place<ROWS>(g, p)) return;
+    if (tid == 0) lost = 0;
+    __syncthreads();
 
-    const int row = r0 + WAVE_R * wave + l32, rc = row < rows ? row : rows - 1;
-    const int tok = rc / G, head = kvh * G + rc % G;
-    const Score sc = score_of(a);
-    R w;
-    w.template load_q<TY == 2>(q, Op::TYPE, (int64_t)(first + tok) * ldq + head * HD, sc);
-    w.clear();
-    w.pos = tok;
-    w.lim = limit(tok);
-    w.slope2 = sc.bias ? a.slopes[head] * LOG2E : 0.f;
-    const bool active = r0 + WAVE_R * wave < rows;
-    const int lo = __builtin_amdgcn_readfirstlane(w.lim), hi = __builtin_amdgcn_readlane(w.lim, 31);
-    const int last = r0 + ROWS < rows ? r0 + ROWS - 1 : rows - 1;
-    const int end = limit(last / G);
-    const int n_tiles = (end + TILE_K - 1) / TILE_K;
-
-    // The next tile's rows, on their way from memory while this one is in work.
-    constexpr int VAL = TY == 2 ? 4 : 8, CPR = HD / VAL, CH = TILE_K * CPR / NT;  // 16-byte pieces
-    u32x4 rk[CH], rv[CH];
-    const char *kp = (const char *)k + ((int64_t)first * ldk + kvh * HD) * (16 / VAL);
-    const char *vp = (const char *)v + ((int64_t)first * ldv + kvh * HD) * (16 / VAL);
-    uint32_t ko[CH], vo[CH];  // of this thread's pieces in a tile
+    // DMA: lane's piece of the wavefront's 1024 bytes i: row (CH wave + i) (64 / PPR) + lane / PPR
+    int kc[CH], vc[CH];  // its channel in K and V
 #pragma unroll
     for (int i = 0; i < CH; i++) {
-        const int c = tid + i * NT;
-        ko[i] = ((uint32_t)(c / CPR) * (uint32_t)ldk + c % CPR * VAL) * (16 / VAL);
-        vo[i] = ((uint32_t)(c / CPR) * (uint32_t)ldv + c % CPR * VAL) * (16 / VAL);
+        const int r = (CH * wave + i) * (64 / PPR) + lane / PPR, at = lane % PPR;
+        kc[i] = 8 * (HD == 128 ? at ^ (r & 15) : at ^ ((r >> 1) & 7));
+        vc[i] = 8 * (HD == 128 ? at ^ ((r & 3) << 2) : at ^ ((r & 2) << 1));
     }
-    auto load = [&](int j0) {
-        const char *kt = kp + j0 * ldk * (16 / VAL), *vt = vp + j0 * ldv * (16 / VAL);
-        if (j0 + TILE_K <= cnt) {
+    auto dma = [&](const void *x, int64_t ld, const int (&c)[CH], int j0, char *to) {
+        const char *base = (const char *)x + ((p.first + j0) * ld + p.kvh * HD) * 2;
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, 0xFFFFFFFF, 0x00020000);
+        const int rows = p.cnt - j0;  // past the sequence its last row again: no row sees those keys
 #pragma unroll
-            for (int i = 0; i < CH; i++) rk[i] = *(const u32x4 *)(kt + ko[i]), rv[i] = *(const u32x4 *)(vt + vo[i]);
-        } else {  // past the sequence its last row again: no row sees those keys
+        for (int i = 0; i < CH; i++) {
+            int row = (CH * wave + i) * (64 / PPR) + lane / PPR;
+            if (rows < TILE_K) row = row < rows ? row : rows - 1;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)(to + (CH * wave + i) * 1024), 16,
+                                                     (int)((uint32_t)row * (uint32_t)ld + c[i]) * 2, 0, 0, 0);
+        }
+    };
+    auto load_k = [&](int e, char *to) { dma(g.k, g.ldk, kc, e * TILE_K, to); };
+    auto load_v = [&](int e, char *to) { dma(g.v, g.ldv, vc, e * TILE_K, to); };
+    const int whole = p.limit(p.r0 / p.G);  // keys that every row sees
+    const int last = p.r0 + ROWS < p.rows ? p.r0 + ROWS - 1 : p.rows - 1;
+    const int end = p.limit(last / p.G), n_tiles = (end + TILE_K - 1) / TILE_K;
+    load_k(0, sk0);
+    load_v(0, sv0);
+    if (n_tiles > 1) load_k(1, sk1);
+
+    const int row = p.r0 + WAVE_R * wave + l32, rc = row < p.rows ? row : p.rows - 1;
+    const int tok = rc / p.G, head = p.kvh * p.G + rc % p.G;
+    const Score sc = score_of(g.a);
+    R w;
+    w.template load_q<false>(g.q, Op::TYPE, (int64_t)(p.first + tok) * g.ldq + head * HD, sc);
+    w.clear();
+    w.pos = tok;
+    w.lim = p.limit(tok);
+    w.slope2 = sc.bias ? g.a.slopes[head] * LOG2E : 0.f;
+    const bool active = p.r0 + WAVE_R * wave < p.rows;
+    const int lo = __builtin_amdgcn_readfirstlane(w.lim);
+    const int hi = active ? __builtin_amdgcn_readlane(w.lim, 31) : 0;
+
+    const int k_at = l32 * RB + ((hf ^ (HD == 128 ? l32 & 15 : (l32 >> 1) & 7)) << 4);
+    auto products = [&](const char *b, f32x16 (&s)[2]) {
+        s[0] = s[1] = f32x16{};
 #pragma unroll
-            for (int i = 0; i < CH; i++) {
-                const int c = tid + i * NT, key = j0 + c / CPR < cnt ? c / CPR : cnt - 1 - j0;
-                rk[i] = *(const u32x4 *)(kt + (key * ldk + c % CPR * VAL) * (16 / VAL));
-                rv[i] = *(const u32x4 *)(vt + (key * ldv + c % CPR * VAL) * (16 / VAL));
+        for (int kk = 0; kk < R::KS; kk++) {
+            const char *at = b + (k_at ^ (kk << 5));
+#pragma unroll
+            for (int st = 0; st < 2; st++) s[st] = mfma32(*(const v8 *)(at + 32 * st * RB), w.q[0][kk], s[st]);
+        }
+    };
+    // V^T operand of channels 32 db .. and keys 16 tt ..: two transposing reads of
+    // four keys each; the lane gets channel 32 db + l32, keys 16 tt + 4 hf + 0..3
+    // and 16 tt + 8 + 4 hf + 0..3, the order of the first product's accumulator.
+    const int v_at = (4 * hf + ((lane & 15) >> 2)) * RB + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+    const int v_x = HD == 128 ? (lane & 15) >> 2 : (lane >> 3) & 1;
+    auto product2 = [&](const char *b, const v8 (&pf)[1][4]) {
+#pragma unroll
+        for (int db = 0; db < R::DB; db++) {
+            const char *at = b + v_at + ((db ^ v_x) << 6);
+#pragma unroll
+            for (int tt = 0; tt < 4; tt++) {
+                struct { s4 a, b; } x;
+                x.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 16 * tt * RB));
+                x.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + (16 * tt + 8) * RB));
+                w.o[db] = mfma32(__builtin_bit_cast(v8, x), pf[0][tt], w.o[db]);
             }
         }
     };
-    // A value that is not finite must not reach rows that do not see it (their
-    // weight of 0 would make it NaN): in tiles that some row sees in part it enters
-    // as 0, and the rows that do see it are put right at the end.
-    const int whole = limit(r0 / G);  // keys that every row of the workgroup sees
+    // a wavefront's own pieces of V's tile e, once they are there
+    auto clean_v = [&](int e, char *b) {
+        if ((e + 1) * TILE_K <= whole) return;
+        bool any = false;
+#pragma unroll 1
+        for (int i = 0; i < CH; i++) {
+            u32x4 *at = (u32x4 *)(b + (CH * wave + i) * 1024 + 16 * lane);
+            u32x4 x = *at;
+            if (not_finite<Op::TYPE>(x)) *at = x, any = true;
+        }
+        if (any) lost = 1;
+    };
+    auto wait = [&](int e, char *b) {  // for tile e of V and e + 1 of K
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+        clean_v(e, b);
+        __syncthreads();
+    };
+
+    f32x16 s0[2], s1[2];
+    auto step = [&](int e, f32x16 (&s)[2], f32x16 (&next)[2], char *ke, char *kn, char *ve, char *vn) {
+        const int j0 = e * TILE_K;
+        if (e + 2 < n_tiles) load_k(e + 2, ke);
+        if (e + 1 < n_tiles) load_v(e + 1, vn);
+        if (j0 < hi) {
+            v8 pf[1][4];
+            const float c = w.template scores<false>(s, sc, 1.f, nullptr, j0, j0 + TILE_K > lo, w.lim);
+            products(kn, next);  // past the last tile: what is there, not used
+            w.weights(s, c, pf);
+            product2(ve, pf);
+            constexpr int M1 = 2 * R::KS, M2 = 4 * R::DB;  // matrix instructions of the two products
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);  // LDS reads, four ahead
+#pragma unroll
+            for (int i = 0; i < M1; i++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);        // matrix
+                __builtin_amdgcn_sched_group_barrier(0x402, 96 / M1, 0);  // vector
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                if (i >= M1 - 4) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < M2; i++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            }
+        }
+        if (e + 1 < n_tiles) wait(e + 1, vn);
+    };
+    wait(0, sv0);
+    if (hi > 0) products(sk0, s0);
+    __syncthreads();  // before the third tile's K takes the first's place
+    for (int e = 0; e < n_tiles; e += 2) {
+        step(e, s0, s1, sk0, sk1, sv0, sv1);
+        if (e + 1 < n_tiles) step(e + 1, s1, s0, sk1, sk0, sv1, sv0);
+    }
+    if (lost) lose<HD, Op::TYPE>(w, g, p, whole & ~(TILE_K - 1), end);
+    put_rows<HD, Op::TYPE>(w, g, p, row, head);
+}
+
+// F32: every operand is two 16-bit terms, made on the way to LDS.
+template <int HD>
+__global__ __launch_bounds__(512, 2) void k_attn_seqs32(SeqsArgs g) {
+    typedef Operand<2> Op;
+    typedef Op::TQ TQ;
+    typedef Op::TP TP;
+    constexpr int NT = 512, ROWS = WAVE_R * 8;
+    typedef Rows<HD, TQ, TP, 2, 2> R;
+    typedef typename R::p8 p8;
+    typedef TileLds<HD> Lds;
+    __shared__ __align__(16) Lds lds[2];
+    __shared__ int lost;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l32 = lane & 31;
+    Place p;
+    if (!place<ROWS>(g, p)) return;
+    if (tid == 0) lost = 0;
+
+    // The next tile's rows, on their way from memory while this one is in work.
+    constexpr int CPR = HD / 4, CH = TILE_K * CPR / NT;  // 16-byte pieces of a row; of a tile, to a thread
+    u32x4 rk[CH], rv[CH];
+    const float *kp = (const float *)g.k + (int64_t)p.first * g.ldk + p.kvh * HD;
+    const float *vp = (const float *)g.v + (int64_t)p.first * g.ldv + p.kvh * HD;
+    auto load = [&](int j0) {
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            const int c = tid + i * NT;
+            // past the sequence its last row again: no row sees those keys
+            const int key = j0 + c / CPR < p.cnt ? j0 + c / CPR : p.cnt - 1;
+            rk[i] = *(const u32x4 *)(kp + key * g.ldk + c % CPR * 4);
+            rv[i] = *(const u32x4 *)(vp + key * g.ldv + c % CPR * 4);
+        }
+    };
+    const int whole = p.limit(p.r0 / p.G);  // keys that every row sees
     auto store = [&](Lds &t, int j0) {
         if (j0 + TILE_K > whole) {
             bool any = false;
 #pragma unroll
-            for (int i = 0; i < CH; i++) any = not_finite<Op::TYPE>(rv[i]) || any;
+            for (int i = 0; i < CH; i++) any = not_finite<FH3K_F32>(rv[i]) || any;
             if (any) lost = 1;
         }
 #pragma unroll
         for (int i = 0; i < CH; i++) {
-            const int c = tid + i * NT, key = c / CPR, d = c % CPR * VAL;
-            if constexpr (TY != 2) {
-                *(u32x4 *)&t.k[0][key][d] = rk[i];
-                *(u32x4 *)&t.v[0][key][d] = rv[i];
-            } else {
-                const f32x4 x = __builtin_bit_cast(f32x4, rk[i]), y = __builtin_bit_cast(f32x4, rv[i]);
-                float top = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-                top = row_max<CPR>(top);
-                const float up = pow2_to_14(top);
-                if (c % CPR == 0) t.ks[key] = 1.f / up;
-                TQ kh[4], kl[4];
-                TP vh[4], vl[4];
+            const int c = tid + i * NT, key = c / CPR, d = c % CPR * 4;
+            const f32x4 x = __builtin_bit_cast(f32x4, rk[i]), y = __builtin_bit_cast(f32x4, rv[i]);
+            const float top = row_max<CPR>(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
+            const float up = pow2_to_14(top);
+            if (c % CPR == 0) t.ks[key] = 1.f / up;
+            TQ kh[4], kl[4];
+            TP vh[4], vl[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const Two<TQ> kt = split<TQ>(x[e] * up);
-                    const Two<TP> vt = split<TP>(y[e]);
-                    kh[e] = kt.hi, kl[e] = kt.lo, vh[e] = vt.hi, vl[e] = vt.lo;
-                }
-                *(u32x2 *)&t.k[0][key][d] = *(const u32x2 *)kh;
-                *(u32x2 *)&t.k[T - 1][key][d] = *(const u32x2 *)kl;
-                *(u32x2 *)&t.v[0][key][d] = *(const u32x2 *)vh;
-                *(u32x2 *)&t.v[T - 1][key][d] = *(const u32x2 *)vl;
+            for (int e = 0; e < 4; e++) {
+                const Two<TQ> kt = split<TQ>(x[e] * up);
+                const Two<TP> vt = split<TP>(y[e]);
+                kh[e] = kt.hi, kl[e] = kt.lo, vh[e] = vt.hi, vl[e] = vt.lo;
             }
+            *(u32x2 *)&t.k[0][key][d] = *(const u32x2 *)kh;
+            *(u32x2 *)&t.k[1][key][d] = *(const u32x2 *)kl;
+            *(u32x2 *)&t.v[0][key][d] = *(const u32x2 *)vh;
+            *(u32x2 *)&t.v[1][key][d] = *(const u32x2 *)vl;
         }
     };
-
-    if (tid == 0) lost = 0;
     load(0);
+
+    const int row = p.r0 + WAVE_R * wave + l32, rc = row < p.rows ? row : p.rows - 1;
+    const int tok = rc / p.G, head = p.kvh * p.G + rc % p.G;
+    const Score sc = score_of(g.a);
+    R w;
+    w.template load_q<true>(g.q, Op::TYPE, (int64_t)(p.first + tok) * g.ldq + head * HD, sc);
+    w.clear();
+    w.pos = tok;
+    w.lim = p.limit(tok);
+    w.slope2 = sc.bias ? g.a.slopes[head] * LOG2E : 0.f;
+    const bool active = p.r0 + WAVE_R * wave < p.rows;
+    const int lo = __builtin_amdgcn_readfirstlane(w.lim), hi = __builtin_amdgcn_readlane(w.lim, 31);
+    const int last = p.r0 + ROWS < p.rows ? p.r0 + ROWS - 1 : p.rows - 1;
+    const int end = p.limit(last / p.G), n_tiles = (end + TILE_K - 1) / TILE_K;
+
     __syncthreads();
     store(lds[0], 0);
     __syncthreads();
@@ -197,53 +390,25 @@ __global__ __launch_bounds__(64 * Operand<TY>::NW, 2) void k_attn_seqs(
         const int j0 = e * TILE_K;
         if (e + 1 < n_tiles) load(j0 + TILE_K);
         if (active && j0 < hi) {
-            const bool cut = j0 + TILE_K > lo;  // some row does not see all of it
-            p8 pf[T][4];
-            w.template weigh<TY == 2>((const TQ *)&t.k[0][0][0], sc, 1.f, t.ks, j0, cut, w.lim, pf);
+            p8 pf[2][4];
+            f32x16 x[2];
+            w.products((const TQ *)&t.k[0][0][0], x);
+            w.weights(x, w.template scores<true>(x, sc, 1.f, t.ks, j0, j0 + TILE_K > lo, w.lim), pf);
 #pragma unroll
             for (int db = 0; db < R::DB; db++)
 #pragma unroll
                 for (int tt = 0; tt < 4; tt++) {
-                    const p8 x = v_frag<p8, Lds::VROW>(&t.v[0][0][0], db, tt);
-                    if constexpr (T == 2) {
-                        w.o[db] = mfma32(v_frag<p8, Lds::VROW>(&t.v[T - 1][0][0], db, tt), pf[0][tt], w.o[db]);
-                        w.o[db] = mfma32(x, pf[T - 1][tt], w.o[db]);
-                    }
-                    w.o[db] = mfma32(x, pf[0][tt], w.o[db]);
+                    const p8 y = v_frag<p8, Lds::VROW>(&t.v[0][0][0], db, tt);
+                    w.o[db] = mfma32(v_frag<p8, Lds::VROW>(&t.v[1][0][0], db, tt), pf[0][tt], w.o[db]);
+                    w.o[db] = mfma32(y, pf[1][tt], w.o[db]);
+                    w.o[db] = mfma32(y, pf[0][tt], w.o[db]);
                 }
         }
         if (e + 1 < n_tiles) store(lds[(e & 1) ^ 1], j0 + TILE_K);
         __syncthreads();
     }
-
-    if (lost) {
-        for (int j = whole & ~(TILE_K - 1); j < end; j++)
-            if (j < w.lim)
-#pragma unroll
-                for (int db = 0; db < R::DB; db++)
-#pragma unroll
-                    for (int g = 0; g < 4; g++) {
-                        const int64_t at_v = (first + j) * ldv + kvh * HD + 32 * db + 8 * g + 4 * hf;
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float x = value_at(v, Op::TYPE, at_v + i);
-                            if (!(fabsf(x) <= 3.402823466e38f)) w.o[db][4 * g + i] = __builtin_nanf("");
-                        }
-                    }
-    }
-    const float l = w.l + half_swap(w.l), inv = l == 0.f ? 0.f : 1.f / l;
-    if (row < rows) {
-        const int64_t at_o = (int64_t)(first + tok) * ldo + head * HD;
-#pragma unroll
-        for (int db = 0; db < R::DB; db++)
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-                f32x4 x;
-#pragma unroll
-                for (int i = 0; i < 4; i++) x[i] = w.o[db][4 * g + i] * inv;
-                store4(o, Op::TYPE, at_o + 32 * db + 8 * g + 4 * hf, x);
-            }
-    }
+    if (lost) lose<HD, Op::TYPE>(w, g, p, whole & ~(TILE_K - 1), end);
+    put_rows<HD, Op::TYPE>(w, g, p, row, head);
 }
 
 template <int HD, int TY>
@@ -255,8 +420,10 @@ hipError_t launch_seqs(const Fh3kAttn &a, const void *q, int64_t ldq, const void
     const int64_t tiles = s.first ? s.n_tok * G / ROWS + (s.n_seq < s.n_tok ? s.n_seq : s.n_tok)
                                   : (int64_t)s.n_seq * ((s.n_tok / s.n_seq * G + ROWS - 1) / ROWS);
     if (tiles * a.kv_heads > 0x7FFFFF) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_attn_seqs<HD, TY>), dim3((unsigned)(tiles * a.kv_heads)), dim3(64 * NW), 0, st, a, q, ldq, k,
-                       ldk, v, ldv, o, ldo, s, prefix, (int)tiles);
+    const SeqsArgs g = {a, q, k, v, o, ldq, ldk, ldv, ldo, s, prefix, (int)tiles};
+    const dim3 grid((unsigned)(tiles * a.kv_heads));
+    if constexpr (TY == 2) hipLaunchKernelGGL(k_attn_seqs32<HD>, grid, dim3(64 * NW), 0, st, g);
+    else hipLaunchKernelGGL((k_attn_seqs16<HD, TY>), grid, dim3(64 * NW), 0, st, g);
     return hipGetLastError();
 }
 

@@ -186,14 +186,10 @@ template <int HD, class TQ, class TP, int QT, int KT> struct Rows {
         l = 0.f;
     }
 
-    // Scores of the 64 keys from position j0 on: sk holds K's KT planes of 64
-    // rows.  kscale: one for the tile, or (PER_KEY) sks[key].  Then their weights,
-    // as the second product's operand.  seen: keys below it are seen.
-    template <bool PER_KEY>
-    __device__ __forceinline__ void weigh(const TQ *sk, const Score &sc, float kscale, const float *sks, int j0, bool cut,
-                                          int seen, p8 (&pf)[QT][4]) {
+    // S^T of 64 keys; sk holds K's KT planes of 64 rows.
+    __device__ __forceinline__ void products(const TQ *sk, f32x16 (&s)[2]) {
         const int l32 = threadIdx.x & 31, hf = (threadIdx.x >> 5) & 1;
-        f32x16 s[2] = {};
+        s[0] = s[1] = f32x16{};
 #pragma unroll
         for (int kk = 0; kk < KS; kk++)
 #pragma unroll
@@ -204,6 +200,15 @@ template <int HD, class TQ, class TP, int QT, int KT> struct Rows {
                 if constexpr (QT == 2) s[st] = mfma32(a, q[1][kk], s[st]);
                 s[st] = mfma32(a, q[0][kk], s[st]);
             }
+    }
+
+    // From the products to scores t = c s (c is returned), their offset m raised
+    // where one asks for it.  The keys are those from position j0 on; kscale: one
+    // scale for the tile, or (PER_KEY) sks[key]; cut: keys from `seen` on are not seen.
+    template <bool PER_KEY>
+    __device__ __forceinline__ float scores(f32x16 (&s)[2], const Score &sc, float kscale, const float *sks, int j0,
+                                            bool cut, int seen) {
+        const int hf = (threadIdx.x >> 5) & 1;
         if constexpr (PER_KEY) {
 #pragma unroll
             for (int st = 0; st < 2; st++)
@@ -248,6 +253,11 @@ template <int HD, class TQ, class TP, int QT, int KT> struct Rows {
 #pragma unroll
             for (int i = 0; i < DB; i++) o[i] *= keep;
         }
+        return c;
+    }
+
+    // The weights exp2(t - m) as the second product's operand, and their sum.
+    __device__ __forceinline__ void weights(const f32x16 (&s)[2], float c, p8 (&pf)[QT][4]) {
         const float nm = -m;
         float sum[2] = {};
 #pragma unroll
