@@ -338,18 +338,21 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
 #pragma unroll
                     for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[i][e]));
                 }
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
+                top = max32(max16(top));
                 const float up = pow2_to_14(top);
                 f[r] = sc.f / up;
 #pragma unroll
-                for (int i = 0; i < 2 * KU; i++)
+                for (int i = 0; i < 2 * KU; i++) {
+                    u32x4 h, l4;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const Two<_Float16> y = split<_Float16>(x[i][e] * up);
-                        qf[r][0][i][e] = y.hi;
-                        if constexpr (NT == 2) qf[r][NT - 1][i][e] = y.lo;
+                    for (int e = 0; e < 4; e++) {
+                        uint32_t hi, lo;
+                        split2(x[i][2 * e], x[i][2 * e + 1], up, hi, lo, _Float16());
+                        h[e] = hi, l4[e] = lo;
                     }
+                    qf[r][0][i] = __builtin_bit_cast(half8, h);
+                    if constexpr (NT == 2) qf[r][NT - 1][i] = __builtin_bit_cast(half8, l4);
+                }
                 m[r] = M_NONE;
                 l[r] = 0.f;
 #pragma unroll
@@ -411,8 +414,7 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
 #pragma unroll
                     for (int i = 1; i < 16; i++) mt = fmaxf(mt, t[r][i >> 2][i & 3]);
                     if (__ballot(mt > m[r] + RAISE)) {
-                        mt = fmaxf(mt, __shfl_xor(mt, 16));
-                        mt = fmaxf(mt, __shfl_xor(mt, 32));
+                        mt = max32(max16(mt));
                         const float now = mt > m[r] + RAISE ? mt - OFFSET : m[r];
                         const float keep = __builtin_amdgcn_exp2f(m[r] - now);
                         m[r] = now;
@@ -422,12 +424,20 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
                     }
                     float sum = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const float p = __builtin_amdgcn_exp2f(t[r][i >> 2][i & 3] - m[r]);
-                        sum += p;
-                        const Two<_Float16> y = split<_Float16>(p);
-                        pf[r][0][i >> 3][i & 7] = y.hi;
-                        if constexpr (NT == 2) pf[r][NT - 1][i >> 3][i & 7] = y.lo;
+                    for (int u = 0; u < 2; u++) {
+                        u32x4 h, l4;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int i = 8 * u + 2 * e;
+                            const float p0 = __builtin_amdgcn_exp2f(t[r][i >> 2][i & 3] - m[r]);
+                            const float p1 = __builtin_amdgcn_exp2f(t[r][i >> 2][(i & 3) + 1] - m[r]);
+                            uint32_t hi, lo;
+                            split2(p0, p1, 1.f, hi, lo, _Float16());
+                            h[e] = hi, l4[e] = lo;
+                            sum += p0 + p1;
+                        }
+                        pf[r][0][u] = __builtin_bit_cast(half8, h);
+                        if constexpr (NT == 2) pf[r][NT - 1][u] = __builtin_bit_cast(half8, l4);
                     }
                     l[r] += sum;
                 }
@@ -451,8 +461,7 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
             // the four wavefronts' parts, in order
 #pragma unroll
             for (int r = 0; r < R; r++) {
-                l[r] += __shfl_xor(l[r], 16);
-                l[r] += __shfl_xor(l[r], 32);
+                l[r] = sum32(sum16(l[r]));
                 const int row = 16 * r + l16;
                 if (g == 0) sm[wave][row] = m[r], sl[wave][row] = l[r];
 #pragma unroll
@@ -695,7 +704,7 @@ __global__ __launch_bounds__(64 * MANY_W, 2) void k_kv_many(Fh3kAttn a, Fh3kKv c
                 __syncthreads();
             }
 
-            const float l = w.l + half_swap(w.l);
+            const float l = sum32(w.l);
             const bool done = page0 == 0 && page1 == pages;
             if (!done && page0 == 0 && tid == 0)
                 *parts.begun(kvh, wg) = {(run.u + pages - 1) / run.size, first, r0, rows};

@@ -12,17 +12,19 @@ template <> struct Operand<1> { typedef __bf16 TQ, TP; static constexpr int NW =
 template <> struct Operand<2> {
     typedef _Float16 TQ;
     typedef __bf16 TP;
-    static constexpr int NW = 8, TYPE = FH3K_F32;
+    static constexpr int NW = 4, TYPE = FH3K_F32;
 };
 
-// A tile of fp32 K and V in LDS: two planes of K [64][HD + 8], of V [64][HD + 32] (the
+// Tiles of fp32 K and V in LDS: two planes of K [64][HD + 8], of V [64][HD + 32] (the
 // transposing reads take 4 rows x 64 bytes at once: rows 64 bytes apart modulo the
-// banks), and one factor per key.
-template <int HD> struct TileLds {
-    static constexpr int KROW = HD + 8, VROW = HD + 32;
-    uint16_t k[2][TILE_K][KROW];
-    uint16_t v[2][TILE_K][VROW];
-    float ks[TILE_K];
+// banks).
+template <int HD> struct KLds {
+    static constexpr int ROW = HD + 8;
+    uint16_t x[2][TILE_K][ROW];
+};
+template <int HD> struct VLds {
+    static constexpr int ROW = HD + 32;
+    uint16_t x[2][TILE_K][ROW];
 };
 
 // V^T operand of channels 32 db .. and keys 16 tt ..: two transposing reads of
@@ -49,7 +51,7 @@ template <int N> __device__ __forceinline__ float row_max(float x) {
     x = dpp_max<0x4E>(x);   // quad_perm 2 3 0 1
     x = dpp_max<0x141>(x);  // row_half_mirror
     x = dpp_max<0x140>(x);  // row_mirror
-    return N == 32 ? fmaxf(x, __shfl_xor(x, 16)) : x;
+    return N == 32 ? max16(x) : x;
 }
 
 // Whether any of 16 bytes of values is infinite or NaN (all exponent bits set);
@@ -135,7 +137,7 @@ __device__ __forceinline__ void lose(R &w, const SeqsArgs &g, const Place &p, in
 template <int HD, int TYPE, class R>
 __device__ __forceinline__ void put_rows(const R &w, const SeqsArgs &g, const Place &p, int row, int head) {
     const int hf = (threadIdx.x >> 5) & 1;
-    const float l = w.l + half_swap(w.l), inv = l == 0.f ? 0.f : 1.f / l;
+    const float l = sum32(w.l), inv = l == 0.f ? 0.f : 1.f / l;
     if (row >= p.rows) return;
     const int64_t at = (int64_t)(p.first + w.pos) * g.ldo + head * HD + 4 * hf;
 #pragma unroll
@@ -303,17 +305,24 @@ __global__ __launch_bounds__(256, 2) void k_attn_seqs16(SeqsArgs g) {
     put_rows<HD, Op::TYPE>(w, g, p, row, head);
 }
 
-// F32: every operand is two 16-bit terms, made on the way to LDS.
+// F32: every operand is two 16-bit terms, made on the way to LDS.  One wavefront to
+// a SIMD (its registers and the LDS tiles leave no room for two), so everything
+// stands between matrix instructions: the terms of the next V beside the first
+// product, the weights and the terms of the next K beside the second.
 template <int HD>
-__global__ __launch_bounds__(512, 2) void k_attn_seqs32(SeqsArgs g) {
+__global__ __launch_bounds__(256, 1) void k_attn_seqs32(SeqsArgs g) {
     typedef Operand<2> Op;
     typedef Op::TQ TQ;
     typedef Op::TP TP;
-    constexpr int NT = 512, ROWS = WAVE_R * 8;
+    constexpr int NT = 256, ROWS = WAVE_R * 4;
     typedef Rows<HD, TQ, TP, 2, 2> R;
     typedef typename R::p8 p8;
-    typedef TileLds<HD> Lds;
-    __shared__ __align__(16) Lds lds[2];
+    typedef KLds<HD> LK;
+    typedef VLds<HD> LV;
+    // (arrays of their own, so that writes to one need not wait for reads of another)
+    __shared__ __align__(16) LK lk0, lk1;
+    __shared__ __align__(16) LV lv0, lv1;
+    __shared__ __align__(16) float ks0[2 * TILE_K], ks1[2 * TILE_K];  // each key's factor; the other half is not read
     __shared__ int lost;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -322,51 +331,77 @@ __global__ __launch_bounds__(512, 2) void k_attn_seqs32(SeqsArgs g) {
     if (!place<ROWS>(g, p)) return;
     if (tid == 0) lost = 0;
 
-    // The next tile's rows, on their way from memory while this one is in work.
     constexpr int CPR = HD / 4, CH = TILE_K * CPR / NT;  // 16-byte pieces of a row; of a tile, to a thread
-    u32x4 rk[CH], rv[CH];
-    const float *kp = (const float *)g.k + (int64_t)p.first * g.ldk + p.kvh * HD;
-    const float *vp = (const float *)g.v + (int64_t)p.first * g.ldv + p.kvh * HD;
-    auto load = [&](int j0) {
+    const int key0 = tid / CPR, d0 = tid % CPR * 4;      // the first; the others NT / CPR keys on
+    const int whole = p.limit(p.r0 / p.G);               // keys that every row sees
+    const int last = p.r0 + ROWS < p.rows ? p.r0 + ROWS - 1 : p.rows - 1;
+    const int end = p.limit(last / p.G), n_tiles = (end + TILE_K - 1) / TILE_K;
+    auto load = [&](const void *x, int64_t ld, int e, u32x4 (&r)[CH]) {
+        const float *base = (const float *)x + (p.first + e * TILE_K) * ld + p.kvh * HD;
+        const int keys = p.cnt - e * TILE_K;  // past the sequence its last row again: no row sees those keys
 #pragma unroll
         for (int i = 0; i < CH; i++) {
-            const int c = tid + i * NT;
-            // past the sequence its last row again: no row sees those keys
-            const int key = j0 + c / CPR < p.cnt ? j0 + c / CPR : p.cnt - 1;
-            rk[i] = *(const u32x4 *)(kp + key * g.ldk + c % CPR * 4);
-            rv[i] = *(const u32x4 *)(vp + key * g.ldv + c % CPR * 4);
+            int key = key0 + i * (NT / CPR);
+            if (keys < TILE_K) key = key < keys ? key : keys - 1;
+            r[i] = *(const u32x4 *)(base + (uint32_t)((uint32_t)key * (uint32_t)ld + d0));
         }
     };
-    const int whole = p.limit(p.r0 / p.G);  // keys that every row sees
-    auto store = [&](Lds &t, int j0) {
-        if (j0 + TILE_K > whole) {
-            bool any = false;
-#pragma unroll
-            for (int i = 0; i < CH; i++) any = not_finite<FH3K_F32>(rv[i]) || any;
-            if (any) lost = 1;
-        }
+    // Powers of two for this thread's pieces of K.  With values below 2^15 and one of
+    // 2^-5 at least in each row 1 will do (fp16's second term then reaches down to
+    // 2^-25, 2^-20 of the row's largest); otherwise the row's largest gives it.
+    auto scales = [&](const u32x4 (&r)[CH], float (&up)[CH]) {
+        float top[CH];
+        uint64_t fine = ~0ull;
 #pragma unroll
         for (int i = 0; i < CH; i++) {
-            const int c = tid + i * NT, key = c / CPR, d = c % CPR * 4;
-            const f32x4 x = __builtin_bit_cast(f32x4, rk[i]), y = __builtin_bit_cast(f32x4, rv[i]);
-            const float top = row_max<CPR>(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
-            const float up = pow2_to_14(top);
-            if (c % CPR == 0) t.ks[key] = 1.f / up;
-            TQ kh[4], kl[4];
-            TP vh[4], vl[4];
+            const f32x4 x = __builtin_bit_cast(f32x4, r[i]);
+            top[i] = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+            up[i] = 1.f;
+            uint64_t some = __ballot(top[i] >= 0.03125f);  // any lane of a row
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const Two<TQ> kt = split<TQ>(x[e] * up);
-                const Two<TP> vt = split<TP>(y[e]);
-                kh[e] = kt.hi, kl[e] = kt.lo, vh[e] = vt.hi, vl[e] = vt.lo;
+            for (int e = 1; e < CPR; e <<= 1) some |= some >> e;
+            constexpr uint64_t FIRST = CPR == 32 ? 0x0000000100000001ull : 0x0001000100010001ull;
+            fine &= (some & FIRST) == FIRST && !__ballot(!(top[i] < 32768.f)) ? ~0ull : 0;
+        }
+        if (!fine) {
+#pragma unroll
+            for (int i = 0; i < CH; i++) {
+                const float m = row_max<CPR>(top[i]);  // each row for itself
+                up[i] = m >= 0.03125f && m < 32768.f ? 1.f : pow2_to_14(m);
             }
-            *(u32x2 *)&t.k[0][key][d] = *(const u32x2 *)kh;
-            *(u32x2 *)&t.k[1][key][d] = *(const u32x2 *)kl;
-            *(u32x2 *)&t.v[0][key][d] = *(const u32x2 *)vh;
-            *(u32x2 *)&t.v[1][key][d] = *(const u32x2 *)vl;
         }
     };
-    load(0);
+    // a piece of K, of V, as two terms
+    auto put_k = [&](const u32x4 &r, float up, int i, LK &to, float *ks) {
+        const int key = key0 + i * (NT / CPR);
+        const f32x4 x = __builtin_bit_cast(f32x4, r);
+        uint32_t h0, h1, l0, l1;
+        split2(x[0], x[1], up, h0, l0, TQ());
+        split2(x[2], x[3], up, h1, l1, TQ());
+        *(u32x2 *)&to.x[0][key][d0] = u32x2{h0, h1};
+        *(u32x2 *)&to.x[1][key][d0] = u32x2{l0, l1};
+        ks[d0 ? TILE_K + key : key] = __builtin_bit_cast(float, 0x7F000000u - __builtin_bit_cast(uint32_t, up));  // 1 / up
+    };
+    auto put_v = [&](const u32x4 &r, int i, LV &to) {
+        const int key = key0 + i * (NT / CPR);
+        const f32x4 x = __builtin_bit_cast(f32x4, r);
+        uint32_t h0, h1, l0, l1;
+        split2(x[0], x[1], 1.f, h0, l0, TP());
+        split2(x[2], x[3], 1.f, h1, l1, TP());
+        *(u32x2 *)&to.x[0][key][d0] = u32x2{h0, h1};
+        *(u32x2 *)&to.x[1][key][d0] = u32x2{l0, l1};
+    };
+    auto clean = [&](u32x4 (&r)[CH], int e) {
+        if ((e + 1) * TILE_K <= whole) return;
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < CH; i++) any = not_finite<FH3K_F32>(r[i]) || any;
+        if (any) lost = 1;
+    };
+    auto tile = [&](int e) { return e < n_tiles ? e : n_tiles - 1; };
+    u32x4 rk[CH], rv[CH];
+    load(g.k, g.ldk, 0, rk);
+    load(g.v, g.ldv, 0, rv);
 
     const int row = p.r0 + WAVE_R * wave + l32, rc = row < p.rows ? row : p.rows - 1;
     const int tok = rc / p.G, head = p.kvh * p.G + rc % p.G;
@@ -377,35 +412,93 @@ __global__ __launch_bounds__(512, 2) void k_attn_seqs32(SeqsArgs g) {
     w.pos = tok;
     w.lim = p.limit(tok);
     w.slope2 = sc.bias ? g.a.slopes[head] * LOG2E : 0.f;
-    const bool active = p.r0 + WAVE_R * wave < p.rows;
-    const int lo = __builtin_amdgcn_readfirstlane(w.lim), hi = __builtin_amdgcn_readlane(w.lim, 31);
-    const int last = p.r0 + ROWS < p.rows ? p.r0 + ROWS - 1 : p.rows - 1;
-    const int end = p.limit(last / p.G), n_tiles = (end + TILE_K - 1) / TILE_K;
+    const int lo = __builtin_amdgcn_readfirstlane(w.lim);
 
+    float up[CH];
     __syncthreads();
-    store(lds[0], 0);
+    clean(rv, 0);
+    scales(rk, up);
+#pragma unroll
+    for (int i = 0; i < CH; i++) put_k(rk[i], up[i], i, lk0, ks0), put_v(rv[i], i, lv0);
+    load(g.k, g.ldk, tile(1), rk);
+    load(g.v, g.ldv, tile(1), rv);
     __syncthreads();
-    for (int e = 0; e < n_tiles; e++) {
-        const Lds &t = lds[e & 1];
+    // Rows that see nothing of a tile have weights of 0: the workgroup waits for
+    // those that do either way.  Past the last tile that one is made again, not read.
+    auto step = [&](int e, const LK &k_now, LK &k_next, const LV &v_now, LV &v_next, const float *ks, float *ks_next) {
         const int j0 = e * TILE_K;
-        if (e + 1 < n_tiles) load(j0 + TILE_K);
-        if (active && j0 < hi) {
-            p8 pf[2][4];
-            f32x16 x[2];
-            w.products((const TQ *)&t.k[0][0][0], x);
-            w.weights(x, w.template scores<true>(x, sc, 1.f, t.ks, j0, j0 + TILE_K > lo, w.lim), pf);
+        clean(rv, e + 1);
+        f32x16 s[2] = {};
+        constexpr int N1 = 2 * R::KS, N2 = 4 * R::DB;
+        typedef typename R::q8 q8;
+        auto k_frag = [&](int i, int plane) {
+            return *(const q8 *)&k_now.x[plane][32 * (i & 1) + l32][16 * (i >> 1) + 8 * (lane >> 5)];
+        };
+        q8 a0 = k_frag(0, 0), a1 = k_frag(0, 1);
 #pragma unroll
-            for (int db = 0; db < R::DB; db++)
+        for (int i = 0; i < N1; i++) {
+            const q8 c0 = a0, c1 = a1;
+            if (i + 1 < N1) a0 = k_frag(i + 1, 0), a1 = k_frag(i + 1, 1);
+            s[i & 1] = mfma32(c1, w.q[0][i >> 1], s[i & 1]);
+            s[i & 1] = mfma32(c0, w.q[1][i >> 1], s[i & 1]);
+            s[i & 1] = mfma32(c0, w.q[0][i >> 1], s[i & 1]);
+            if (i * CH % N1 < CH) put_v(rv[i * CH / N1], i * CH / N1, v_next);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
 #pragma unroll
-                for (int tt = 0; tt < 4; tt++) {
-                    const p8 y = v_frag<p8, Lds::VROW>(&t.v[0][0][0], db, tt);
-                    w.o[db] = mfma32(v_frag<p8, Lds::VROW>(&t.v[1][0][0], db, tt), pf[0][tt], w.o[db]);
-                    w.o[db] = mfma32(y, pf[1][tt], w.o[db]);
-                    w.o[db] = mfma32(y, pf[0][tt], w.o[db]);
-                }
+            for (int x = 0; x < 3; x++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix
+                __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);  // vector
+            }
+            __builtin_amdgcn_sched_group_barrier(0x200, 2, 0);  // LDS writes
         }
-        if (e + 1 < n_tiles) store(lds[(e & 1) ^ 1], j0 + TILE_K);
+        load(g.v, g.ldv, tile(e + 2), rv);
+        const float c = w.template scores<true>(s, sc, 1.f, ks, j0, j0 + TILE_K > lo, w.lim), nm = -w.m;
+        scales(rk, up);
+        float sum[2] = {};
+        u32x4 ph[4], pl[4];
+        auto weigh = [&](int tt, int x) {  // two keys' weights
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[tt >> 1][8 * (tt & 1) + 2 * x], c, nm));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[tt >> 1][8 * (tt & 1) + 2 * x + 1], c, nm));
+            uint32_t hi, lw;
+            split2(p0, p1, 1.f, hi, lw, TP());
+            ph[tt][x] = hi, pl[tt][x] = lw;
+            sum[0] += p0, sum[1] += p1;
+        };
+#pragma unroll
+        for (int x = 0; x < 4; x++) weigh(0, x);
+        p8 y0 = v_frag<p8, LV::ROW>(&v_now.x[0][0][0], 0, 0), y1 = v_frag<p8, LV::ROW>(&v_now.x[1][0][0], 0, 0);
+#pragma unroll
+        for (int i = 0; i < N2; i++) {
+            const int tt = i / R::DB, db = i % R::DB, n = i + 1;
+            const p8 c0 = y0, c1 = y1;
+            if (n < N2) {
+                y0 = v_frag<p8, LV::ROW>(&v_now.x[0][0][0], n % R::DB, n / R::DB);
+                y1 = v_frag<p8, LV::ROW>(&v_now.x[1][0][0], n % R::DB, n / R::DB);
+            }
+            const p8 p0 = __builtin_bit_cast(p8, ph[tt]), p1 = __builtin_bit_cast(p8, pl[tt]);
+            w.o[db] = mfma32(c1, p0, w.o[db]);
+            w.o[db] = mfma32(c0, p1, w.o[db]);
+            w.o[db] = mfma32(c0, p0, w.o[db]);
+            if (tt < 3)
+#pragma unroll
+                for (int x = db * 4 / R::DB; x < (db + 1) * 4 / R::DB; x++) weigh(tt + 1, x);
+            if (i * CH % N2 < CH) put_k(rk[i * CH / N2], up[i * CH / N2], i * CH / N2, k_next, ks_next);
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+            for (int x = 0; x < 3; x++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x402, 10, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x200, 3, 0);
+        }
+        w.l += sum[0] + sum[1];
+        load(g.k, g.ldk, tile(e + 2), rk);
         __syncthreads();
+    };
+#pragma unroll 1
+    for (int e = 0; e < n_tiles; e += 2) {
+        step(e, lk0, lk1, lv0, lv1, ks0, ks1);
+        if (e + 1 < n_tiles) step(e + 1, lk1, lk0, lv1, lv0, ks1, ks0);
     }
     if (lost) lose<HD, Op::TYPE>(w, g, p, whole & ~(TILE_K - 1), end);
     put_rows<HD, Op::TYPE>(w, g, p, row, head);

@@ -123,14 +123,49 @@ __device__ __forceinline__ void store4(void *p, int type, int64_t at, f32x4 x) {
 }
 
 // two terms of 16 bits: x ~ hi + lo, both rounded to nearest
-template <class T> struct Two { T hi, lo; };
-template <class T> __device__ __forceinline__ Two<T> split(float x) {
-    const T hi = (T)x;
-    return {hi, (T)(x - (float)hi)};
+// Two values as two terms of 16 bits each, x ~ hi + lo, all rounded to nearest; x
+// is x * scale for fp16 (a power of two).
+__device__ __forceinline__ void split2(float a, float b, float scale, uint32_t &hi, uint32_t &lo, _Float16) {
+    const half2v h = __builtin_convertvector(f32x2{a * scale, b * scale}, half2v);
+    const f32x2 l = {fmaf(a, scale, -(float)h[0]), fmaf(b, scale, -(float)h[1])};
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(l, half2v));
+}
+__device__ __forceinline__ void split2(float a, float b, float, uint32_t &hi, uint32_t &lo, __bf16) {
+    hi = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf2));
+    const float ha = __builtin_bit_cast(float, hi << 16), hb = __builtin_bit_cast(float, hi & 0xFFFF0000u);
+    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a - ha, b - hb}, bf2));
 }
 
-__device__ __forceinline__ float half_swap(float x) { return __shfl_xor(x, 32); }
-
+// The lanes 32 (16) apart: the larger value, the sum, in both.
+__device__ __forceinline__ f32x2 swap32(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    const uint32_t lo = r[0], hi = r[1];
+    return {__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi)};
+}
+__device__ __forceinline__ f32x2 swap16(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    const uint32_t lo = r[0], hi = r[1];
+    return {__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi)};
+}
+__device__ __forceinline__ float max32(float x) {
+    const f32x2 r = swap32(x);
+    return fmaxf(r[0], r[1]);
+}
+__device__ __forceinline__ float sum32(float x) {
+    const f32x2 r = swap32(x);
+    return r[0] + r[1];
+}
+__device__ __forceinline__ float max16(float x) {
+    const f32x2 r = swap16(x);
+    return fmaxf(r[0], r[1]);
+}
+__device__ __forceinline__ float sum16(float x) {
+    const f32x2 r = swap16(x);
+    return r[0] + r[1];
+}
 // TQ: element of the first product's operands, TP: of the second's.  QT: terms of
 // q and of the weights, KT: of k and v.
 template <int HD, class TQ, class TP, int QT, int KT> struct Rows {
@@ -162,20 +197,25 @@ template <int HD, class TQ, class TP, int QT, int KT> struct Rows {
 #pragma unroll
                 for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[kk][i]));
             }
-            top = fmaxf(top, half_swap(top));
+            top = max32(top);
             const float up = pow2_to_14(top);
             f = sc.f / up;
 #pragma unroll
-            for (int kk = 0; kk < KS; kk++)
+            for (int kk = 0; kk < KS; kk++) {
+                if constexpr (QT == 2) {
+                    u32x4 h, l4;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    if constexpr (QT == 2) {
-                        const Two<TQ> y = split<TQ>(x[kk][i] * up);
-                        q[0][kk][i] = y.hi, q[1][kk][i] = y.lo;
-                    } else {
-                        q[0][kk][i] = (TQ)(x[kk][i] * up);
+                    for (int i = 0; i < 4; i++) {
+                        uint32_t hi, lo;
+                        split2(x[kk][2 * i], x[kk][2 * i + 1], up, hi, lo, TQ());
+                        h[i] = hi, l4[i] = lo;
                     }
+                    q[0][kk] = __builtin_bit_cast(q8, h), q[QT - 1][kk] = __builtin_bit_cast(q8, l4);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) q[0][kk][i] = (TQ)(x[kk][i] * up);
                 }
+            }
         }
     }
 
@@ -245,7 +285,7 @@ template <int HD, class TQ, class TP, int QT, int KT> struct Rows {
         for (int v = 1; v < 16; v++) mt = fmaxf(fmaxf(mt, s[0][v]), s[1][v]);
         mt *= c;
         if (__ballot(mt > m + RAISE)) {  // wave-uniform
-            mt = fmaxf(mt, half_swap(mt));
+            mt = max32(mt);
             const float now = mt > m + RAISE ? mt - OFFSET : m;
             const float keep = __builtin_amdgcn_exp2f(m - now);
             m = now;
@@ -266,12 +306,15 @@ template <int HD, class TQ, class TP, int QT, int KT> struct Rows {
 #pragma unroll
             for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(fmaf(s[tt >> 1][8 * (tt & 1) + e], c, nm));
             if constexpr (QT == 2) {
+                u32x4 h, l4;
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    sum[e & 1] += p[e];
-                    const Two<TP> y = split<TP>(p[e]);
-                    pf[0][tt][e] = y.hi, pf[1][tt][e] = y.lo;
+                for (int e = 0; e < 4; e++) {
+                    uint32_t hi, lo;
+                    split2(p[2 * e], p[2 * e + 1], 1.f, hi, lo, TP());
+                    h[e] = hi, l4[e] = lo;
+                    sum[0] += p[2 * e], sum[1] += p[2 * e + 1];
                 }
+                pf[0][tt] = __builtin_bit_cast(p8, h), pf[QT - 1][tt] = __builtin_bit_cast(p8, l4);
             } else {  // the sum is of the rounded weights, which the product takes
                 u32x4 w;
 #pragma unroll
