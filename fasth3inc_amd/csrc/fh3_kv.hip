@@ -32,113 +32,164 @@ __device__ __forceinline__ float finite_abs(float x) {
     const float y = fabsf(x);
     return y <= 3.402823466e38f ? y : 0.f;
 }
-// x / s as a stored byte; the clamp takes infinities, a NaN becomes 0.
+// x / s as a stored byte in the low eight bits: 1.5 * 2^23 + 128 leaves the integer
+// nearest (ties to even) there; the clamp takes infinities, a NaN becomes 0.
 __device__ __forceinline__ uint32_t to_byte(float x, float inv) {
-    const float y = x == x ? fminf(fmaxf(rintf(x * inv), -127.f), 127.f) : 0.f;
-    return (uint32_t)((int)y + 128);
+    const float y = x == x ? fminf(fmaxf(x * inv, -127.f), 127.f) : 0.f;
+    return __builtin_bit_cast(uint32_t, y + 12583040.f);
 }
-// A stored byte at a new scale: ratio = old / new <= 1, exactly a power of two.
-__device__ __forceinline__ uint32_t again(uint32_t b, float ratio) {
-    return (uint32_t)((int)fminf(fmaxf(rintf((float)((int)b - 128) * ratio), -127.f), 127.f) + 128);
+// the low bytes of four words
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0C0C0400u), __builtin_amdgcn_perm(b, a, 0x0C0C0400u), 0x05040100u);
+}
+__device__ __forceinline__ float byte_value(uint32_t w, int e) { return (float)(w >> (8 * e) & 255) - 128.f; }
+// Four stored bytes at a new scale: ratio = old / new <= 1, exactly a power of two.
+__device__ __forceinline__ uint32_t again4(uint32_t w, float ratio) {
+    return pack4(to_byte(byte_value(w, 0), ratio), to_byte(byte_value(w, 1), ratio), to_byte(byte_value(w, 2), ratio),
+                 to_byte(byte_value(w, 3), ratio));
 }
 
 constexpr int ROW_T = 256;  // threads of the kernels that move rows
 
-// One workgroup to a page that new rows touch, a head, and K or V (blockIdx.y).
-// The rows go through LDS as fp32: their largest finite value gives the scale,
-// then each thread makes whole 16-byte pieces of the page.
+// A page that new rows touch (work unit), of a head, K or V: blockIdx.y.
+struct RowPage {
+    int h, which, seq, id;
+    int64_t row0;  // the row of slot 0, were it one
+    int lo, hi;    // its rows are slots lo .. hi - 1
+};
+__device__ __forceinline__ bool row_page(const Fh3kKv &c, const Fh3kSeqs &s, RowPage &r) {
+    int a, cnt, len, base, p0, at;
+    r.h = blockIdx.y >> 1, r.which = blockIdx.y & 1;
+    if (!find_unit(blockIdx.x, s.n_seq, [&](int i) { int p; return touched_pages(c, s, i, p); }, r.seq, at)) return false;
+    seq_rows(s, r.seq, a, cnt);
+    kv_len(c, r.seq, cnt, len, base);
+    const int p = (base >> 6) + at;
+    r.id = kv_page(c, r.seq, p);
+    const int64_t pos0 = (int64_t)p * KV_PAGE;
+    r.row0 = a + (pos0 - base);
+    r.lo = (int)(base > pos0 ? base - pos0 : 0);
+    r.hi = (int)(base + cnt < pos0 + KV_PAGE ? base + cnt - pos0 : KV_PAGE);
+    return r.lo < r.hi;
+}
+
+// The rows go through LDS as fp32: their largest finite value gives the scale, then
+// a whole page is made in 16-byte pieces, part of one in the smallest that its
+// rows fill (K: 16 channels of a slot; V: four slots of a channel).
 template <int HD>
 __global__ __launch_bounds__(ROW_T) void k_kv_append(Fh3kKv c, int type, const void *__restrict__ k, int64_t ldk,
                                                      const void *__restrict__ v, int64_t ldv, Fh3kSeqs s) {
-    constexpr int LD = HD + 4;
+    constexpr int LD = HD + 4, PPR = HD / 8, PIECES = KV_PAGE * PPR / ROW_T;
     __shared__ __align__(16) float sx[KV_PAGE * LD];
     __shared__ float smax[ROW_T / 64];
-    const int t = threadIdx.x, h = blockIdx.y >> 1, which = blockIdx.y & 1;
-    int seq, a, cnt, len, base, p0, at;
-    if (!find_unit(blockIdx.x, s.n_seq, [&](int i) { int p; return touched_pages(c, s, i, p); }, seq, at)) return;
-    seq_rows(s, seq, a, cnt);
-    kv_len(c, seq, cnt, len, base);
-    touched_pages(c, s, seq, p0);
-    const int p = p0 + at, id = kv_page(c, seq, p);
-    if (id < 0) return;
-    const int64_t pos0 = (int64_t)p * KV_PAGE;
-    const int lo = (int)(base > pos0 ? base - pos0 : 0);  // slots lo .. hi - 1 are new, those below lo held
-    const int hi = (int)(base + cnt < pos0 + KV_PAGE ? base + cnt - pos0 : KV_PAGE);
-    if (hi <= lo) return;
-    const void *x = which ? v : k;
-    const int64_t ld = which ? ldv : ldk;
-    float m = 0.f;
-    for (int e = t; e < (hi - lo) * HD; e += ROW_T) {
-        const int slot = lo + e / HD, d = e % HD;
-        const float y = value_at(x, type, (a + (pos0 + slot - base)) * ld + h * HD + d);
-        sx[slot * LD + d] = y;
-        m = fmaxf(m, finite_abs(y));
+    const int t = threadIdx.x;
+    RowPage r;
+    if (!row_page(c, s, r) || r.id < 0) return;
+    const int lo = r.lo, hi = r.hi;
+    const void *x = r.which ? v : k;
+    const int64_t ld = r.which ? ldv : ldk, at0 = r.row0 * ld + r.h * HD;
+    const int64_t blk = ((int64_t)r.id * c.kv_heads + r.h) * 2 + r.which;
+    const float before = c.scales[blk];
+    Raw8 raw[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; i++) {
+        const int e = t + ROW_T * i, slot = lo + e / PPR, d = e % PPR * 8;
+        if (slot < hi) raw[i] = load8(x, type, at0 + slot * ld + d);
     }
-    float *scale = c.scales + ((int64_t)id * c.kv_heads + h) * 2 + which;
-    const float before = *scale;
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < PIECES; i++) {
+        const int e = t + ROW_T * i, slot = lo + e / PPR, d = e % PPR * 8;
+        if (slot < hi) {
+            float y[8];
+            values8(raw[i], type, y);
+#pragma unroll
+            for (int j = 0; j < 8; j++) m = fmaxf(m, finite_abs(y[j]));
+            *(f32x4 *)&sx[slot * LD + d] = f32x4{y[0], y[1], y[2], y[3]};
+            *(f32x4 *)&sx[slot * LD + d + 4] = f32x4{y[4], y[5], y[6], y[7]};
+        }
+    }
 #pragma unroll
     for (int w = 1; w < 64; w <<= 1) m = fmaxf(m, __shfl_xor(m, w));
     if ((t & 63) == 0) smax[t >> 6] = m;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < ROW_T / 64; w++) m = fmaxf(m, smax[w]);
+    m = fmaxf(fmaxf(smax[0], smax[1]), fmaxf(smax[2], smax[3]));
     float now = page_scale(m);
     if (lo > 0) now = fmaxf(now, before);
     const float inv = 1.f / now, ratio = before * inv;
     const bool redo = lo > 0 && before != now;
-    if (t == 0) *scale = now;
-    u32x4 *page = (u32x4 *)(c.pool + (((int64_t)id * c.kv_heads + h) * 2 + which) * KV_PAGE * HD);
-    for (int u = t; u < KV_PAGE * HD / 16; u += ROW_T) {
-        // K: 16 channels of slot; V: slots 16 b + 4 g + r of a channel
-        const int i = u & 15, g = (u >> 4) & 3, b = u >> 6;
-        const int slot = which ? 4 * g : 16 * (b / (HD / 64)) + i;
-        const int d = which ? 16 * b + i : 64 * (b % (HD / 64)) + 16 * g;
-        uint32_t any = 0;  // bit e: byte e is written
+    if (t == 0) c.scales[blk] = now;
+    uint8_t *page = c.pool + blk * KV_PAGE * HD;
+    if (lo == 0 && hi == KV_PAGE) {
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const int sl = which ? slot + 16 * (e >> 2) + (e & 3) : slot;
-            any |= (uint32_t)((sl >= lo && sl < hi) || (redo && sl < lo)) << e;
-        }
-        if (!any) continue;
-        u32x4 w = {};
-        if (any != 0xFFFF || redo) w = page[u];
+        for (int u = 0; u < KV_PAGE * HD / 16 / ROW_T; u++) {
+            const int p = t + ROW_T * u, i = p & 15, g = (p >> 4) & 3, b = p >> 6;
+            const float *at = r.which ? &sx[4 * g * LD + 16 * b + i] : &sx[(16 * (b / (HD / 64)) + i) * LD + 64 * (b % (HD / 64)) + 16 * g];
+            u32x4 w;
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const int sl = which ? slot + 16 * (e >> 2) + (e & 3) : slot;
-            const uint32_t old = (w[e >> 2] >> (8 * (e & 3))) & 255;
-            uint32_t y = old;
-            if (sl >= lo && sl < hi) y = to_byte(sx[sl * LD + (which ? d : d + e)], inv);
-            else if (redo && sl < lo) y = again(old, ratio);
-            w[e >> 2] ^= (y ^ old) << (8 * (e & 3));
+            for (int e = 0; e < 4; e++) {
+                const int o = r.which ? 16 * e * LD : 4 * e, n = r.which ? LD : 1;
+                w[e] = pack4(to_byte(at[o], inv), to_byte(at[o + n], inv), to_byte(at[o + 2 * n], inv), to_byte(at[o + 3 * n], inv));
+            }
+            *(u32x4 *)(page + 16 * p) = w;
         }
-        page[u] = w;
+    } else if (r.which == 0) {
+        const int from = redo ? 0 : lo;
+        for (int e = t; e < (hi - from) * (HD / 16); e += ROW_T) {
+            const int slot = from + e / (HD / 16), d = e % (HD / 16) * 16;
+            u32x4 *at = (u32x4 *)(page + k_byte<HD>(slot, d)), w;
+            if (slot < lo) {
+                w = *at;
+                for (int i = 0; i < 4; i++) w[i] = again4(w[i], ratio);
+            } else {
+                const float *y = &sx[slot * LD + d];
+                for (int i = 0; i < 4; i++)
+                    w[i] = pack4(to_byte(y[4 * i], inv), to_byte(y[4 * i + 1], inv), to_byte(y[4 * i + 2], inv), to_byte(y[4 * i + 3], inv));
+            }
+            *at = w;
+        }
+    } else {
+        const int from = redo ? 0 : lo >> 2, to = (hi + 3) >> 2;  // fours of slots
+        for (int e = t; e < (to - from) * HD; e += ROW_T) {
+            const int slot = 4 * (from + e / HD), d = e % HD;
+            uint32_t *at = (uint32_t *)(page + v_byte<HD>(slot, d)), w = 0;
+            if (slot < lo || slot + 4 > hi) w = *at;
+            if (redo && slot < lo) w = again4(w, ratio);  // (of slots from lo on too: they are replaced)
+            for (int i = 0; i < 4; i++)
+                if (slot + i >= lo && slot + i < hi)
+                    w = (w & ~(255u << 8 * i)) | (to_byte(sx[(slot + i) * LD + d], inv) & 255) << 8 * i;
+            *at = w;
+        }
     }
 }
 
-// The same pages read back as rows; rows that no page holds become zeros.
+// The same pages read back as rows; rows that no page holds become zeros.  A thread
+// takes four slots x four channels, so that rows are written in order.
 template <int HD>
 __global__ __launch_bounds__(ROW_T) void k_kv_read(Fh3kKv c, int type, void *__restrict__ k, int64_t ldk,
                                                    void *__restrict__ v, int64_t ldv, Fh3kSeqs s) {
-    const int t = threadIdx.x, h = blockIdx.y >> 1, which = blockIdx.y & 1;
-    void *x = which ? v : k;
-    if (!x) return;
-    int seq, a, cnt, len, base, p0, at;
-    if (!find_unit(blockIdx.x, s.n_seq, [&](int i) { int p; return touched_pages(c, s, i, p); }, seq, at)) return;
-    seq_rows(s, seq, a, cnt);
-    kv_len(c, seq, cnt, len, base);
-    touched_pages(c, s, seq, p0);
-    const int p = p0 + at, id = kv_page(c, seq, p);
-    const int64_t pos0 = (int64_t)p * KV_PAGE, ld = which ? ldv : ldk;
-    const int lo = (int)(base > pos0 ? base - pos0 : 0);
-    const int hi = (int)(base + cnt < pos0 + KV_PAGE ? base + cnt - pos0 : KV_PAGE);
-    const int64_t blk = ((int64_t)id * c.kv_heads + h) * 2 + which;
-    const float scale = id >= 0 ? c.scales[blk] : 0.f;
+    void *x = blockIdx.y & 1 ? v : k;
+    RowPage r;
+    if (!x || !row_page(c, s, r)) return;
+    const int64_t ld = r.which ? ldv : ldk, at0 = r.row0 * ld + r.h * HD;
+    const int64_t blk = ((int64_t)(r.id < 0 ? 0 : r.id) * c.kv_heads + r.h) * 2 + r.which;
+    const float scale = r.id < 0 ? 0.f : c.scales[blk];
     const uint8_t *page = c.pool + blk * KV_PAGE * HD;
-    for (int e = t; e < (hi - lo) * HD; e += ROW_T) {
-        const int slot = lo + e / HD, d = e % HD;
-        const float y = id >= 0 ? (float)((int)page[which ? v_byte<HD>(slot, d) : k_byte<HD>(slot, d)] - 128) * scale
-                                : 0.f;
-        put_value(x, type, (a + (pos0 + slot - base)) * ld + h * HD + d, y);
+    const int from = r.lo >> 2, to = (r.hi + 3) >> 2;
+    for (int e = threadIdx.x; e < (to - from) * (HD / 4); e += ROW_T) {
+        const int slot = 4 * (from + e / (HD / 4)), d = e % (HD / 4) * 4;
+        uint32_t w[4];  // K: of a slot; V: of a channel
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            w[i] = *(const uint32_t *)(page + (r.which ? v_byte<HD>(slot, d + i) : k_byte<HD>(slot + i, d)));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (slot + i < r.lo || slot + i >= r.hi) continue;
+            f32x4 y;
+#pragma unroll
+            for (int j = 0; j < 4; j++) y[j] = byte_value(r.which ? w[j] : w[i], r.which ? i : j) * scale;
+            if (r.id < 0) y = f32x4{};
+            store4(x, type, at0 + (slot + i) * ld + d, y);
+        }
     }
 }
 
