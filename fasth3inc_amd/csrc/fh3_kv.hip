@@ -5,15 +5,8 @@
 
 namespace {
 
-// Pages that a sequence's cnt rows touch at most, and the touched pages of sequence i.
+// Pages that a sequence's cnt rows touch at most.
 int64_t most_pages(int64_t cnt) { return cnt > 0 ? (cnt + 62) / 64 + 1 : 0; }
-__device__ __forceinline__ int touched_pages(const Fh3kKv &c, const Fh3kSeqs &s, int i, int &p0) {
-    int a, cnt, len, base;
-    seq_rows(s, i, a, cnt);
-    kv_len(c, i, cnt, len, base);
-    p0 = base >> 6;  // base may be negative: rows that no page holds
-    return cnt > 0 ? ((base + cnt - 1) >> 6) - p0 + 1 : 0;
-}
 int64_t touched_most(Fh3kSeqs s) {  // over all sequences: at least one row to a page
     if (!s.first) return s.n_seq * most_pages(s.n_tok / s.n_seq);
     const int64_t n = (int64_t)s.n_tok / 64 + 2 * (int64_t)s.n_seq;
@@ -58,11 +51,16 @@ struct RowPage {
     int lo, hi;    // its rows are slots lo .. hi - 1
 };
 __device__ __forceinline__ bool row_page(const Fh3kKv &c, const Fh3kSeqs &s, RowPage &r) {
-    int a, cnt, len, base, p0, at;
+    int a = 0, cnt = 0, len, base = 0, at;
     r.h = blockIdx.y >> 1, r.which = blockIdx.y & 1;
-    if (!find_unit(blockIdx.x, s.n_seq, [&](int i) { int p; return touched_pages(c, s, i, p); }, r.seq, at)) return false;
-    seq_rows(s, r.seq, a, cnt);
-    kv_len(c, r.seq, cnt, len, base);
+    if (!find_unit(blockIdx.x, s.n_seq, [&](int i) {
+            seq_rows(s, i, a, cnt);
+            kv_len(c, i, cnt, len, base);
+            // base may be negative: rows that no page holds
+            return cnt > 0 ? ((base + cnt - 1) >> 6) - (base >> 6) + 1 : 0;
+        }, r.seq, at))
+        return false;
+    a = of_lane(a, r.seq), cnt = of_lane(cnt, r.seq), base = of_lane(base, r.seq);
     const int p = (base >> 6) + at;
     r.id = kv_page(c, r.seq, p);
     const int64_t pos0 = (int64_t)p * KV_PAGE;
@@ -217,23 +215,29 @@ struct KvWork {
     int shift;  // tiles of 2^shift rows
     int wgs;    // workgroups of a key head
 };
-// Tiles of sequence i, and pages (units) of each; a tile that sees no key has one unit.
-__device__ __forceinline__ int kv_tiles(const Fh3kKv &c, const Fh3kSeqs &s, const KvWork &w, int i, int &pages) {
-    int a, cnt, len, base;
-    seq_rows(s, i, a, cnt);
-    kv_len(c, i, cnt, len, base);
-    pages = len > 0 ? (len + KV_PAGE - 1) / KV_PAGE : 1;
-    return (cnt * w.G + (1 << w.shift) - 1) >> w.shift;
+// A sequence: its rows first .. first + cnt - 1, tokens held, position of the first
+// row, tiles, and pages (units) of each; a tile that sees no key has one unit.
+struct KvSeq {
+    int first, cnt, len, base, tiles, pages;
+};
+__device__ __forceinline__ KvSeq kv_seq(const Fh3kKv &c, const Fh3kSeqs &s, const KvWork &w, int i) {
+    KvSeq q;
+    seq_rows(s, i, q.first, q.cnt);
+    kv_len(c, i, q.cnt, q.len, q.base);
+    q.pages = q.len > 0 ? (q.len + KV_PAGE - 1) / KV_PAGE : 1;
+    q.tiles = (q.cnt * w.G + (1 << w.shift) - 1) >> w.shift;
+    return q;
 }
 // A workgroup's run of units u .. end - 1 and the sequence, tile and page of the first.
 struct KvRun {
-    int size, u, end, seq, tiles, pages, tile, page;
+    int size, u, end, seq, tile, page;
+    KvSeq q;
 };
 __device__ __forceinline__ bool kv_run(const Fh3kKv &c, const Fh3kSeqs &s, const KvWork &w, int wg, KvRun &r) {
+    KvSeq q = {};
     auto units = [&](int i) {
-        int pages;
-        const int t = kv_tiles(c, s, w, i, pages);
-        return t * pages;
+        q = kv_seq(c, s, w, i);
+        return q.tiles * q.pages;
     };
     const int lane = threadIdx.x & 63;
     int all = 0, mine = 0, end = 0;
@@ -250,26 +254,26 @@ __device__ __forceinline__ bool kv_run(const Fh3kKv &c, const Fh3kSeqs &s, const
     r.end = all - r.u < r.size ? all : r.u + r.size;
     int at = 0;
     if (s.n_seq <= 64) {
-        const int l = __builtin_ctzll(__ballot(end > r.u));
-        r.seq = l;
-        at = r.u - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(mine, l));
+        r.seq = __builtin_ctzll(__ballot(end > r.u));
+        at = r.u - (of_lane(end, r.seq) - of_lane(mine, r.seq));
     } else {
         if (!find_unit(r.u, s.n_seq, units, r.seq, at)) return false;
     }
-    r.tiles = kv_tiles(c, s, w, r.seq, r.pages);
-    r.tile = at / r.pages;
-    r.page = at - r.tile * r.pages;
+    r.q = {of_lane(q.first, r.seq), of_lane(q.cnt, r.seq), of_lane(q.len, r.seq), of_lane(q.base, r.seq),
+           of_lane(q.tiles, r.seq), of_lane(q.pages, r.seq)};
+    r.tile = at / r.q.pages;
+    r.page = at - r.tile * r.q.pages;
     return true;
 }
 // The next tile after r.tile is done; false behind the last.
 __device__ __forceinline__ bool kv_next(const Fh3kKv &c, const Fh3kSeqs &s, const KvWork &w, KvRun &r) {
     r.page = 0;
-    if (++r.tile < r.tiles) return true;
+    if (++r.tile < r.q.tiles) return true;
     r.tile = 0;
     do {
         if (++r.seq >= s.n_seq) return false;
-        r.tiles = kv_tiles(c, s, w, r.seq, r.pages);
-    } while (r.tiles == 0);
+        r.q = kv_seq(c, s, w, r.seq);
+    } while (r.q.tiles == 0);
     return true;
 }
 
@@ -330,14 +334,11 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
     if (ws && tid == 0) parts.begun(kvh, wg)->last = 0;
     if (!any) return;
     do {
-        const int page0 = run.page, pages = run.pages;
+        const int page0 = run.page, pages = run.q.pages;
         const bool whole = pages <= WHOLE;
         if (!(whole && page0)) {
             const int page1 = whole || pages - page0 <= run.end - run.u ? pages : page0 + run.end - run.u;
-            const int seq = run.seq;
-            int first, cnt, len, base;
-            seq_rows(s, seq, first, cnt);
-            kv_len(c, seq, cnt, len, base);
+            const int seq = run.seq, first = run.q.first, cnt = run.q.cnt, len = run.q.len, base = run.q.base;
             const int rows = cnt * G, r0 = run.tile * ROWS;
             auto limit = [&](int tok) { return a.causal && base + tok + 1 < len ? base + tok + 1 : len; };
             const int lo = limit(r0 / G);  // keys that all rows see
@@ -447,14 +448,16 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
                     const float x = f[r] * ks, far = (float)(pos[r] - j0 - 4 * g);
                     const int left = there ? lim[r] - j0 - 4 * g : 0x80000000;
 #pragma unroll
-                    for (int tt = 0; tt < 4; tt++)
+                    for (int i = 0; i < 16; i++) t[r][i >> 2][i & 3] *= x;
+                    if (sc.cap2) {
 #pragma unroll
-                        for (int v = 0; v < 4; v++) {
-                            float y = t[r][tt][v] * x;
-                            if (sc.cap2) y = capped(y, sc.cap2);
-                            if (sc.bias) y = fmaf(-slope2[r], fabsf(far - (float)(16 * tt + v)), y);
-                            t[r][tt][v] = y;
-                        }
+                        for (int i = 0; i < 16; i++) t[r][i >> 2][i & 3] = capped(t[r][i >> 2][i & 3], sc.cap2);
+                    }
+                    if (sc.bias) {
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            t[r][i >> 2][i & 3] = fmaf(-slope2[r], fabsf(far - (float)(16 * (i >> 2) + (i & 3))), t[r][i >> 2][i & 3]);
+                    }
                     if (cut) {
 #pragma unroll
                         for (int tt = 0; tt < 4; tt++)
@@ -634,14 +637,11 @@ __global__ __launch_bounds__(64 * MANY_W, 2) void k_kv_many(Fh3kAttn a, Fh3kKv c
     if (ws && tid == 0) parts.begun(kvh, wg)->last = 0;
     if (!any) return;
     do {
-        const int page0 = run.page, pages = run.pages;
+        const int page0 = run.page, pages = run.q.pages;
         const bool whole = pages <= WHOLE;
         if (!(whole && page0)) {
             const int page1 = whole || pages - page0 <= run.end - run.u ? pages : page0 + run.end - run.u;
-            const int seq = run.seq;
-            int first, cnt, len, base;
-            seq_rows(s, seq, first, cnt);
-            kv_len(c, seq, cnt, len, base);
+            const int seq = run.seq, first = run.q.first, cnt = run.q.cnt, len = run.q.len, base = run.q.base;
             const int rows = cnt * G, r0 = run.tile * ROWS;
             auto limit = [&](int tok) { return a.causal && base + tok + 1 < len ? base + tok + 1 : len; };
             const int row = r0 + WAVE_R * wave + l32, rc = row < rows ? row : rows - 1;
@@ -718,6 +718,12 @@ __global__ __launch_bounds__(64 * MANY_W, 2) void k_kv_many(Fh3kAttn a, Fh3kKv c
                     half8 pf[NT][4];
                     f32x16 x[2];
                     w.products(&sk[n & 1][0][0], x);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);  // LDS reads, four ahead
+#pragma unroll
+                    for (int i = 0; i < 2 * R::KS; i++) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, NT, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    }
                     w.weights(x, w.template scores<false>(x, sc, ks_n, nullptr, j0, j0 + KV_PAGE > lo, w.lim), pf);
                     // pages of the same scale add up in the product's accumulator
                     if (vs_n > ref) {
@@ -735,6 +741,12 @@ __global__ __launch_bounds__(64 * MANY_W, 2) void k_kv_many(Fh3kAttn a, Fh3kKv c
 #pragma unroll
                                 for (int e = NT - 1; e >= 0; e--) w.o[db] = mfma32(x, pf[e][tt], w.o[db]);
                             }
+                        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+                        for (int i = 0; i < 4 * R::DB; i++) {
+                            __builtin_amdgcn_sched_group_barrier(0x008, NT, 0);
+                            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                        }
                     } else {
                         const float down = vs_n / ref;
 #pragma unroll

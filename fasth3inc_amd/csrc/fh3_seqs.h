@@ -62,7 +62,9 @@ __device__ __forceinline__ int wave_scan(int x) {
 }
 // Work unit w when sequence i has units(i) of them (fewer than 2^31 in all): its
 // sequence and its place there, or false past the last.  Every lane of a
-// wavefront calls it with the same w; 64 sequences at a time.
+// wavefront calls it with the same w; 64 sequences at a time.  What units() noted of
+// its sequence is then in lane seq % 64 (of_lane), and need not be read again.
+__device__ __forceinline__ int of_lane(int x, int seq) { return __builtin_amdgcn_readlane(x, seq & 63); }
 template <class F> __device__ __forceinline__ bool find_unit(int w, int n_seq, F units, int &seq, int &at) {
     const int lane = threadIdx.x & 63;
     for (int s0 = 0; s0 < n_seq; s0 += 64) {

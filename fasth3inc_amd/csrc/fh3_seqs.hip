@@ -96,17 +96,18 @@ struct Place {
 template <int ROWS> __device__ __forceinline__ bool place(const SeqsArgs &g, Place &p) {
     p.kvh = blockIdx.x % g.a.kv_heads;
     p.G = g.a.heads / g.a.kv_heads;
-    int seq, at;
+    int seq, at, b = 0, n = 0, pre = 0;
     if (!find_unit(g.tiles - 1 - (int)blockIdx.x / g.a.kv_heads, g.s.n_seq, [&](int i) {
-            int b, n;
+            if (g.a.causal && g.prefix) pre = g.prefix[i];
             seq_rows(g.s, i, b, n);
             return (n * p.G + ROWS - 1) / ROWS;
         }, seq, at))
         return false;
-    seq_rows(g.s, seq, p.first, p.cnt);
+    p.first = of_lane(b, seq);
+    p.cnt = of_lane(n, seq);
+    pre = g.a.causal ? of_lane(pre, seq) : p.cnt;
     p.rows = p.cnt * p.G;
     p.r0 = at * ROWS;
-    const int pre = g.a.causal ? (g.prefix ? g.prefix[seq] : 0) : p.cnt;
     p.pre = pre < p.cnt ? pre : p.cnt;
     return true;
 }

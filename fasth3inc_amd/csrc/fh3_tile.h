@@ -260,17 +260,30 @@ template <int HD, class TQ, class TP, int QT, int KT> struct Rows {
                 }
         }
         float c = f * kscale;  // t = c s, unless there is more to do
-        if (sc.cap2 || sc.bias) {
-            const float far = (float)(pos - j0 - 4 * hf);
+        // (two loops and two branches: in one loop both would be computed and selected)
+        if (sc.cap2) {
 #pragma unroll
             for (int st = 0; st < 2; st++)
 #pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    float t = s[st][v] * c;
-                    if (sc.cap2) t = capped(t, sc.cap2);
-                    if (sc.bias) t = fmaf(-slope2, fabsf(far - (float)(32 * st + 8 * (v >> 2) + (v & 3))), t);
-                    s[st][v] = t;
-                }
+                for (int v = 0; v < 16; v++) s[st][v] = capped(s[st][v] * c, sc.cap2);
+            c = 1.f;
+        }
+        if (sc.bias) {
+            const float far = (float)(pos - j0 - 4 * hf);
+            if (!__ballot(pos < j0 + TILE_K - 1)) {  // no row has a key behind it
+                const float at = -slope2 * far;
+#pragma unroll
+                for (int st = 0; st < 2; st++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++)
+                        s[st][v] = fmaf(s[st][v], c, fmaf(slope2, (float)(32 * st + 8 * (v >> 2) + (v & 3)), at));
+            } else {
+#pragma unroll
+                for (int st = 0; st < 2; st++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++)
+                        s[st][v] = fmaf(-slope2, fabsf(far - (float)(32 * st + 8 * (v >> 2) + (v & 3))), s[st][v] * c);
+            }
             c = 1.f;
         }
         if (cut) {
