@@ -15,16 +15,17 @@ template <> struct Operand<2> {
     static constexpr int NW = 4, TYPE = FH3K_F32;
 };
 
-// Tiles of fp32 K and V in LDS: two planes of K [64][HD + 8], of V [64][HD + 32] (the
+// Tiles of fp32 K and V in LDS: two planes of K [32][HD + 8], of V [32][HD + 32] (the
 // transposing reads take 4 rows x 64 bytes at once: rows 64 bytes apart modulo the
 // banks).
+constexpr int TILE_32 = 32;
 template <int HD> struct KLds {
     static constexpr int ROW = HD + 8;
-    uint16_t x[2][TILE_K][ROW];
+    uint16_t x[2][TILE_32][ROW];
 };
 template <int HD> struct VLds {
     static constexpr int ROW = HD + 32;
-    uint16_t x[2][TILE_K][ROW];
+    uint16_t x[2][TILE_32][ROW];
 };
 
 // V^T operand of channels 32 db .. and keys 16 tt ..: two transposing reads of
@@ -306,12 +307,13 @@ __global__ __launch_bounds__(256, 2) void k_attn_seqs16(SeqsArgs g) {
     put_rows<HD, Op::TYPE>(w, g, p, row, head);
 }
 
-// F32: every operand is two 16-bit terms, made on the way to LDS.  One wavefront to
-// a SIMD (its registers and the LDS tiles leave no room for two), so everything
-// stands between matrix instructions: the terms of the next V beside the first
-// product, the weights and the terms of the next K beside the second.
+// F32: every operand is two 16-bit terms, made on the way to LDS: the terms of the
+// next V beside the first product, the weights and the terms of the next K beside
+// the second.  Tiles of 32 keys, so that two workgroups fit a CU and nothing has
+// to be moved to accumulation registers (64 keys, one workgroup: 600 tokens x 64
+// heads 52.6 us; a third of the instructions were such moves).
 template <int HD>
-__global__ __launch_bounds__(256, 1) void k_attn_seqs32(SeqsArgs g) {
+__global__ __launch_bounds__(256, 2) void k_attn_seqs32(SeqsArgs g) {
     typedef Operand<2> Op;
     typedef Op::TQ TQ;
     typedef Op::TP TP;
@@ -323,7 +325,7 @@ __global__ __launch_bounds__(256, 1) void k_attn_seqs32(SeqsArgs g) {
     // (arrays of their own, so that writes to one need not wait for reads of another)
     __shared__ __align__(16) LK lk0, lk1;
     __shared__ __align__(16) LV lv0, lv1;
-    __shared__ __align__(16) float ks0[2 * TILE_K], ks1[2 * TILE_K];  // each key's factor; the other half is not read
+    __shared__ __align__(16) float ks0[2 * TILE_32], ks1[2 * TILE_32];  // each key's factor; the other half is not read
     __shared__ int lost;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -332,18 +334,18 @@ __global__ __launch_bounds__(256, 1) void k_attn_seqs32(SeqsArgs g) {
     if (!place<ROWS>(g, p)) return;
     if (tid == 0) lost = 0;
 
-    constexpr int CPR = HD / 4, CH = TILE_K * CPR / NT;  // 16-byte pieces of a row; of a tile, to a thread
+    constexpr int CPR = HD / 4, CH = TILE_32 * CPR / NT;  // 16-byte pieces of a row; of a tile, to a thread
     const int key0 = tid / CPR, d0 = tid % CPR * 4;      // the first; the others NT / CPR keys on
     const int whole = p.limit(p.r0 / p.G);               // keys that every row sees
     const int last = p.r0 + ROWS < p.rows ? p.r0 + ROWS - 1 : p.rows - 1;
-    const int end = p.limit(last / p.G), n_tiles = (end + TILE_K - 1) / TILE_K;
+    const int end = p.limit(last / p.G), n_tiles = (end + TILE_32 - 1) / TILE_32;
     auto load = [&](const void *x, int64_t ld, int e, u32x4 (&r)[CH]) {
-        const float *base = (const float *)x + (p.first + e * TILE_K) * ld + p.kvh * HD;
-        const int keys = p.cnt - e * TILE_K;  // past the sequence its last row again: no row sees those keys
+        const float *base = (const float *)x + (p.first + e * TILE_32) * ld + p.kvh * HD;
+        const int keys = p.cnt - e * TILE_32;  // past the sequence its last row again: no row sees those keys
 #pragma unroll
         for (int i = 0; i < CH; i++) {
             int key = key0 + i * (NT / CPR);
-            if (keys < TILE_K) key = key < keys ? key : keys - 1;
+            if (keys < TILE_32) key = key < keys ? key : keys - 1;
             r[i] = *(const u32x4 *)(base + (uint32_t)((uint32_t)key * (uint32_t)ld + d0));
         }
     };
@@ -381,7 +383,7 @@ __global__ __launch_bounds__(256, 1) void k_attn_seqs32(SeqsArgs g) {
         split2(x[2], x[3], up, h1, l1, TQ());
         *(u32x2 *)&to.x[0][key][d0] = u32x2{h0, h1};
         *(u32x2 *)&to.x[1][key][d0] = u32x2{l0, l1};
-        ks[d0 ? TILE_K + key : key] = __builtin_bit_cast(float, 0x7F000000u - __builtin_bit_cast(uint32_t, up));  // 1 / up
+        ks[d0 ? TILE_32 + key : key] = __builtin_bit_cast(float, 0x7F000000u - __builtin_bit_cast(uint32_t, up));  // 1 / up
     };
     auto put_v = [&](const u32x4 &r, int i, LV &to) {
         const int key = key0 + i * (NT / CPR);
@@ -393,7 +395,7 @@ __global__ __launch_bounds__(256, 1) void k_attn_seqs32(SeqsArgs g) {
         *(u32x2 *)&to.x[1][key][d0] = u32x2{l0, l1};
     };
     auto clean = [&](u32x4 (&r)[CH], int e) {
-        if ((e + 1) * TILE_K <= whole) return;
+        if ((e + 1) * TILE_32 <= whole) return;
         bool any = false;
 #pragma unroll
         for (int i = 0; i < CH; i++) any = not_finite<FH3K_F32>(r[i]) || any;
@@ -427,22 +429,22 @@ __global__ __launch_bounds__(256, 1) void k_attn_seqs32(SeqsArgs g) {
     // Rows that see nothing of a tile have weights of 0: the workgroup waits for
     // those that do either way.  Past the last tile that one is made again, not read.
     auto step = [&](int e, const LK &k_now, LK &k_next, const LV &v_now, LV &v_next, const float *ks, float *ks_next) {
-        const int j0 = e * TILE_K;
+        const int j0 = e * TILE_32;
         clean(rv, e + 1);
-        f32x16 s[2] = {};
-        constexpr int N1 = 2 * R::KS, N2 = 4 * R::DB;
+        f32x16 s[1] = {};
+        constexpr int N1 = R::KS, N2 = 2 * R::DB;
         typedef typename R::q8 q8;
         auto k_frag = [&](int i, int plane) {
-            return *(const q8 *)&k_now.x[plane][32 * (i & 1) + l32][16 * (i >> 1) + 8 * (lane >> 5)];
+            return *(const q8 *)&k_now.x[plane][l32][16 * i + 8 * (lane >> 5)];
         };
         q8 a0 = k_frag(0, 0), a1 = k_frag(0, 1);
 #pragma unroll
         for (int i = 0; i < N1; i++) {
             const q8 c0 = a0, c1 = a1;
             if (i + 1 < N1) a0 = k_frag(i + 1, 0), a1 = k_frag(i + 1, 1);
-            s[i & 1] = mfma32(c1, w.q[0][i >> 1], s[i & 1]);
-            s[i & 1] = mfma32(c0, w.q[1][i >> 1], s[i & 1]);
-            s[i & 1] = mfma32(c0, w.q[0][i >> 1], s[i & 1]);
+            s[0] = mfma32(c1, w.q[0][i], s[0]);
+            s[0] = mfma32(c0, w.q[1][i], s[0]);
+            s[0] = mfma32(c0, w.q[0][i], s[0]);
             if (i * CH % N1 < CH) put_v(rv[i * CH / N1], i * CH / N1, v_next);
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
 #pragma unroll
@@ -453,13 +455,13 @@ __global__ __launch_bounds__(256, 1) void k_attn_seqs32(SeqsArgs g) {
             __builtin_amdgcn_sched_group_barrier(0x200, 2, 0);  // LDS writes
         }
         load(g.v, g.ldv, tile(e + 2), rv);
-        const float c = w.template scores<true>(s, sc, 1.f, ks, j0, j0 + TILE_K > lo, w.lim), nm = -w.m;
+        const float c = w.template scores<true>(s, sc, 1.f, ks, j0, j0 + TILE_32 > lo, w.lim), nm = -w.m;
         scales(rk, up);
         float sum[2] = {};
-        u32x4 ph[4], pl[4];
+        u32x4 ph[2], pl[2];
         auto weigh = [&](int tt, int x) {  // two keys' weights
-            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[tt >> 1][8 * (tt & 1) + 2 * x], c, nm));
-            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[tt >> 1][8 * (tt & 1) + 2 * x + 1], c, nm));
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[0][8 * tt + 2 * x], c, nm));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][8 * tt + 2 * x + 1], c, nm));
             uint32_t hi, lw;
             split2(p0, p1, 1.f, hi, lw, TP());
             ph[tt][x] = hi, pl[tt][x] = lw;
@@ -480,7 +482,7 @@ __global__ __launch_bounds__(256, 1) void k_attn_seqs32(SeqsArgs g) {
             w.o[db] = mfma32(c1, p0, w.o[db]);
             w.o[db] = mfma32(c0, p1, w.o[db]);
             w.o[db] = mfma32(c0, p0, w.o[db]);
-            if (tt < 3)
+            if (tt < 1)
 #pragma unroll
                 for (int x = db * 4 / R::DB; x < (db + 1) * 4 / R::DB; x++) weigh(tt + 1, x);
             if (i * CH % N2 < CH) put_k(rk[i * CH / N2], up[i * CH / N2], i * CH / N2, k_next, ks_next);
@@ -501,7 +503,7 @@ __global__ __launch_bounds__(256, 1) void k_attn_seqs32(SeqsArgs g) {
         step(e, lk0, lk1, lv0, lv1, ks0, ks1);
         if (e + 1 < n_tiles) step(e + 1, lk1, lk0, lv1, lv0, ks1, ks0);
     }
-    if (lost) lose<HD, Op::TYPE>(w, g, p, whole & ~(TILE_K - 1), end);
+    if (lost) lose<HD, Op::TYPE>(w, g, p, whole & ~(TILE_32 - 1), end);
     put_rows<HD, Op::TYPE>(w, g, p, row, head);
 }
 

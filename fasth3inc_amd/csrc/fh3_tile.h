@@ -243,15 +243,15 @@ template <int HD, class TQ, class TP, int QT, int KT> struct Rows {
     }
 
     // From the products to scores t = c s (c is returned), their offset m raised
-    // where one asks for it.  The keys are those from position j0 on; kscale: one
+    // where one asks for it.  The 32 NS keys are those from position j0 on; kscale: one
     // scale for the tile, or (PER_KEY) sks[key]; cut: keys from `seen` on are not seen.
-    template <bool PER_KEY>
-    __device__ __forceinline__ float scores(f32x16 (&s)[2], const Score &sc, float kscale, const float *sks, int j0,
+    template <bool PER_KEY, int NS>
+    __device__ __forceinline__ float scores(f32x16 (&s)[NS], const Score &sc, float kscale, const float *sks, int j0,
                                             bool cut, int seen) {
         const int hf = (threadIdx.x >> 5) & 1;
         if constexpr (PER_KEY) {
 #pragma unroll
-            for (int st = 0; st < 2; st++)
+            for (int st = 0; st < NS; st++)
 #pragma unroll
                 for (int g = 0; g < 4; g++) {
                     const f32x4 ks = *(const f32x4 *)(sks + 32 * st + 8 * g + 4 * hf);
@@ -263,23 +263,23 @@ template <int HD, class TQ, class TP, int QT, int KT> struct Rows {
         // (two loops and two branches: in one loop both would be computed and selected)
         if (sc.cap2) {
 #pragma unroll
-            for (int st = 0; st < 2; st++)
+            for (int st = 0; st < NS; st++)
 #pragma unroll
                 for (int v = 0; v < 16; v++) s[st][v] = capped(s[st][v] * c, sc.cap2);
             c = 1.f;
         }
         if (sc.bias) {
             const float far = (float)(pos - j0 - 4 * hf);
-            if (!__ballot(pos < j0 + TILE_K - 1)) {  // no row has a key behind it
+            if (!__ballot(pos < j0 + 32 * NS - 1)) {  // no row has a key behind it
                 const float at = -slope2 * far;
 #pragma unroll
-                for (int st = 0; st < 2; st++)
+                for (int st = 0; st < NS; st++)
 #pragma unroll
                     for (int v = 0; v < 16; v++)
                         s[st][v] = fmaf(s[st][v], c, fmaf(slope2, (float)(32 * st + 8 * (v >> 2) + (v & 3)), at));
             } else {
 #pragma unroll
-                for (int st = 0; st < 2; st++)
+                for (int st = 0; st < NS; st++)
 #pragma unroll
                     for (int v = 0; v < 16; v++)
                         s[st][v] = fmaf(-slope2, fabsf(far - (float)(32 * st + 8 * (v >> 2) + (v & 3))), s[st][v] * c);
@@ -289,13 +289,13 @@ template <int HD, class TQ, class TP, int QT, int KT> struct Rows {
         if (cut) {
             const int left = seen - j0 - 4 * hf;
 #pragma unroll
-            for (int st = 0; st < 2; st++)
+            for (int st = 0; st < NS; st++)
 #pragma unroll
                 for (int v = 0; v < 16; v++) s[st][v] = left > 32 * st + 8 * (v >> 2) + (v & 3) ? s[st][v] : -INFINITY;
         }
-        float mt = fmaxf(s[0][0], s[1][0]);
+        float mt = fmaxf(s[0][0], s[NS - 1][15]);
 #pragma unroll
-        for (int v = 1; v < 16; v++) mt = fmaxf(fmaxf(mt, s[0][v]), s[1][v]);
+        for (int i = 1; i < 16 * NS - 1; i += 2) mt = fmaxf(fmaxf(mt, s[i >> 4][i & 15]), s[(i + 1) >> 4][(i + 1) & 15]);
         mt *= c;
         if (__ballot(mt > m + RAISE)) {  // wave-uniform
             mt = max32(mt);
