@@ -153,6 +153,38 @@ __device__ __forceinline__ void put_rows(const R &w, const SeqsArgs &g, const Pl
         }
 }
 
+// Two halves of the workgroup that took every other tile of keys: the second's sums
+// go through LDS (in a and b, DB / 2 blocks of 16 KB each; offsets and sums of weights
+// in c) to the first.
+template <class R> __device__ __forceinline__ void join_halves(R &w, int half, int wave, char *a, char *b, char *c) {
+    const int lane = threadIdx.x & 63;
+    float *ml = (float *)c + wave * 64 + lane;
+    auto at = [&](int db, int q) {
+        return (f32x4 *)((db < R::DB / 2 ? a : b) + db % (R::DB / 2) * 16384) + (q * 4 + wave) * 64 + lane;
+    };
+    __syncthreads();
+    if (half) {
+        ml[0] = w.m, ml[256] = w.l;
+#pragma unroll
+        for (int db = 0; db < R::DB; db++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) *at(db, q) = f32x4{w.o[db][4 * q], w.o[db][4 * q + 1], w.o[db][4 * q + 2], w.o[db][4 * q + 3]};
+    }
+    __syncthreads();
+    if (half) return;
+    const float m = ml[0], now = fmaxf(w.m, m), x = __builtin_amdgcn_exp2f(w.m - now), y = __builtin_amdgcn_exp2f(m - now);
+    w.m = now;
+    w.l = w.l * x + ml[256] * y;
+#pragma unroll
+    for (int db = 0; db < R::DB; db++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const f32x4 z = *at(db, q);
+#pragma unroll
+            for (int i = 0; i < 4; i++) w.o[db][4 * q + i] = w.o[db][4 * q + i] * x + z[i] * y;
+        }
+}
+
 // F16 and BF16.  K and V go from memory to LDS without registers (16 bytes a lane),
 // rows unpadded, their 16-byte (K) or 64-byte (V) pieces permuted by the row
 // so that the reads meet no bank twice.  The next tile's scores are computed
@@ -181,27 +213,33 @@ __global__ __launch_bounds__(256, 2) void k_attn_seqs16(SeqsArgs g) {
     __syncthreads();
 
     // DMA: lane's piece of the wavefront's 1024 bytes i: row (CH wave + i) (64 / PPR) + lane / PPR
-    int kc[CH], vc[CH];  // its channel in K and V
+    int ko[CH], vo[CH];  // its offset in a tile of K and V
 #pragma unroll
     for (int i = 0; i < CH; i++) {
         const int r = (CH * wave + i) * (64 / PPR) + lane / PPR, at = lane % PPR;
-        kc[i] = 8 * (HD == 128 ? at ^ (r & 15) : at ^ ((r >> 1) & 7));
-        vc[i] = 8 * (HD == 128 ? at ^ ((r & 3) << 2) : at ^ ((r & 2) << 1));
+        ko[i] = (r * (int)g.ldk + 8 * (HD == 128 ? at ^ (r & 15) : at ^ ((r >> 1) & 7))) * 2;
+        vo[i] = (r * (int)g.ldv + 8 * (HD == 128 ? at ^ ((r & 3) << 2) : at ^ ((r & 2) << 1))) * 2;
     }
-    auto dma = [&](const void *x, int64_t ld, const int (&c)[CH], int j0, char *to) {
+    auto dma = [&](const void *x, int64_t ld, const int (&o)[CH], int j0, char *to) {
         const char *base = (const char *)x + ((p.first + j0) * ld + p.kvh * HD) * 2;
         const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, 0xFFFFFFFF, 0x00020000);
-        const int rows = p.cnt - j0;  // past the sequence its last row again: no row sees those keys
+        const int rows = p.cnt - j0;
+        auto get = [&](int i, int at) {
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)(to + (CH * wave + i) * 1024), 16, at, 0, 0, 0);
+        };
+        if (rows >= TILE_K) {
 #pragma unroll
-        for (int i = 0; i < CH; i++) {
-            int row = (CH * wave + i) * (64 / PPR) + lane / PPR;
-            if (rows < TILE_K) row = row < rows ? row : rows - 1;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)(to + (CH * wave + i) * 1024), 16,
-                                                     (int)((uint32_t)row * (uint32_t)ld + c[i]) * 2, 0, 0, 0);
+            for (int i = 0; i < CH; i++) get(i, o[i]);
+        } else {  // past the sequence its last row again: no row sees those keys
+#pragma unroll
+            for (int i = 0; i < CH; i++) {
+                const int over = (CH * wave + i) * (64 / PPR) + lane / PPR - rows + 1;
+                get(i, o[i] - (over > 0 ? over * (int)ld * 2 : 0));
+            }
         }
     };
-    auto load_k = [&](int e, char *to) { dma(g.k, g.ldk, kc, e * TILE_K, to); };
-    auto load_v = [&](int e, char *to) { dma(g.v, g.ldv, vc, e * TILE_K, to); };
+    auto load_k = [&](int e, char *to) { dma(g.k, g.ldk, ko, e * TILE_K, to); };
+    auto load_v = [&](int e, char *to) { dma(g.v, g.ldv, vo, e * TILE_K, to); };
     const int whole = p.limit(p.r0 / p.G);  // keys that every row sees
     const int last = p.r0 + ROWS < p.rows ? p.r0 + ROWS - 1 : p.rows - 1;
     const int end = p.limit(last / p.G), n_tiles = (end + TILE_K - 1) / TILE_K;
@@ -311,9 +349,10 @@ __global__ __launch_bounds__(256, 2) void k_attn_seqs16(SeqsArgs g) {
 // next V beside the first product, the weights and the terms of the next K beside
 // the second.  Tiles of 32 keys, so that two workgroups fit a CU and nothing has
 // to be moved to accumulation registers (64 keys, one workgroup: 600 tokens x 64
-// heads 52.6 us; a third of the instructions were such moves).
-template <int HD>
-__global__ __launch_bounds__(256, 2) void k_attn_seqs32(SeqsArgs g) {
+// heads 52.6 us; a third of the instructions were such moves).  KH = 2: eight
+// wavefronts, two to a SIMD, each four with every other tile of keys.
+template <int HD, int KH>
+__global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
     typedef Operand<2> Op;
     typedef Op::TQ TQ;
     typedef Op::TP TP;
@@ -323,12 +362,13 @@ __global__ __launch_bounds__(256, 2) void k_attn_seqs32(SeqsArgs g) {
     typedef KLds<HD> LK;
     typedef VLds<HD> LV;
     // (arrays of their own, so that writes to one need not wait for reads of another)
-    __shared__ __align__(16) LK lk0, lk1;
-    __shared__ __align__(16) LV lv0, lv1;
-    __shared__ __align__(16) float ks0[2 * TILE_32], ks1[2 * TILE_32];  // each key's factor; the other half is not read
+    __shared__ __align__(16) LK lk0[KH], lk1[KH];
+    __shared__ __align__(16) LV lv0[KH], lv1[KH];
+    __shared__ __align__(16) float ks0[KH][2 * TILE_32], ks1[KH][2 * TILE_32];  // each key's factor; the other half is not read
     __shared__ int lost;
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tid = threadIdx.x % NT, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int half = KH == 2 ? __builtin_amdgcn_readfirstlane(threadIdx.x / NT) : 0;
     const int l32 = lane & 31;
     Place p;
     if (!place<ROWS>(g, p)) return;
@@ -401,10 +441,12 @@ __global__ __launch_bounds__(256, 2) void k_attn_seqs32(SeqsArgs g) {
         for (int i = 0; i < CH; i++) any = not_finite<FH3K_F32>(r[i]) || any;
         if (any) lost = 1;
     };
-    auto tile = [&](int e) { return e < n_tiles ? e : n_tiles - 1; };
+    const int steps = (n_tiles + KH - 1) / KH;
+    auto tile = [&](int e) { return e * KH + half; };  // of this half's step e
+    auto there = [&](int t) { return t < n_tiles ? t : n_tiles - 1; };  // past the last tile that one again, all cut
     u32x4 rk[CH], rv[CH];
-    load(g.k, g.ldk, 0, rk);
-    load(g.v, g.ldv, 0, rv);
+    load(g.k, g.ldk, there(tile(0)), rk);
+    load(g.v, g.ldv, there(tile(0)), rv);
 
     const int row = p.r0 + WAVE_R * wave + l32, rc = row < p.rows ? row : p.rows - 1;
     const int tok = rc / p.G, head = p.kvh * p.G + rc % p.G;
@@ -419,18 +461,18 @@ __global__ __launch_bounds__(256, 2) void k_attn_seqs32(SeqsArgs g) {
 
     float up[CH];
     __syncthreads();
-    clean(rv, 0);
+    clean(rv, tile(0));
     scales(rk, up);
 #pragma unroll
-    for (int i = 0; i < CH; i++) put_k(rk[i], up[i], i, lk0, ks0), put_v(rv[i], i, lv0);
-    load(g.k, g.ldk, tile(1), rk);
-    load(g.v, g.ldv, tile(1), rv);
+    for (int i = 0; i < CH; i++) put_k(rk[i], up[i], i, lk0[half], ks0[half]), put_v(rv[i], i, lv0[half]);
+    load(g.k, g.ldk, there(tile(1)), rk);
+    load(g.v, g.ldv, there(tile(1)), rv);
     __syncthreads();
     // Rows that see nothing of a tile have weights of 0: the workgroup waits for
     // those that do either way.  Past the last tile that one is made again, not read.
     auto step = [&](int e, const LK &k_now, LK &k_next, const LV &v_now, LV &v_next, const float *ks, float *ks_next) {
-        const int j0 = e * TILE_32;
-        clean(rv, e + 1);
+        const int j0 = tile(e) * TILE_32;
+        clean(rv, tile(e + 1));
         f32x16 s[1] = {};
         constexpr int N1 = R::KS, N2 = 2 * R::DB;
         typedef typename R::q8 q8;
@@ -454,7 +496,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_seqs32(SeqsArgs g) {
             }
             __builtin_amdgcn_sched_group_barrier(0x200, 2, 0);  // LDS writes
         }
-        load(g.v, g.ldv, tile(e + 2), rv);
+        load(g.v, g.ldv, there(tile(e + 2)), rv);
         const float c = w.template scores<true>(s, sc, 1.f, ks, j0, j0 + TILE_32 > lo, w.lim), nm = -w.m;
         scales(rk, up);
         float sum[2] = {};
@@ -495,17 +537,30 @@ __global__ __launch_bounds__(256, 2) void k_attn_seqs32(SeqsArgs g) {
             __builtin_amdgcn_sched_group_barrier(0x200, 3, 0);
         }
         w.l += sum[0] + sum[1];
-        load(g.k, g.ldk, tile(e + 2), rk);
+        load(g.k, g.ldk, there(tile(e + 2)), rk);
         __syncthreads();
     };
 #pragma unroll 1
-    for (int e = 0; e < n_tiles; e += 2) {
-        step(e, lk0, lk1, lv0, lv1, ks0, ks1);
-        if (e + 1 < n_tiles) step(e + 1, lk1, lk0, lv1, lv0, ks1, ks0);
+    for (int e = 0; e < steps; e += 2) {
+        step(e, lk0[half], lk1[half], lv0[half], lv1[half], ks0[half], ks1[half]);
+        if (e + 1 < steps) step(e + 1, lk1[half], lk0[half], lv1[half], lv0[half], ks1[half], ks0[half]);
+    }
+    if constexpr (KH == 2) {
+        static_assert(sizeof lk0 >= R::DB / 2 * 16384 && sizeof lv0 >= 2048, "");
+        join_halves(w, half, wave, (char *)lk0, (char *)lk1, (char *)lv0);
+        if (half) return;
     }
     if (lost) lose<HD, Op::TYPE>(w, g, p, whole & ~(TILE_32 - 1), end);
     put_rows<HD, Op::TYPE>(w, g, p, row, head);
 }
+
+// F32 with every other tile of keys to four more wavefronts, against four wavefronts
+// alone, us: one sequence at 64 heads over 8, hd 128, 37 tokens 15.5 / 11.0, 300
+// tokens 27.9 / 30.4, 600 tokens 45.7 / 54.1, 900 tokens 77 / 79, 1200 tokens (608
+// workgroups) 116 / 110; 16 heads over 16, hd 64, 500 tokens 20.9 / 26.7, 2000 tokens
+// 63 / 88, 4000 tokens (512 workgroups) 144 / 178, 5060 tokens (672) 106 / 106.
+// (16 bits: 0.7 to 0.9 as fast at hd 128, 0.8 to 1.1 at hd 64, so not there.)
+constexpr int SPLIT_TO = 512, SPLIT_FROM = 128;
 
 template <int HD, int TY>
 hipError_t launch_seqs(const Fh3kAttn &a, const void *q, int64_t ldq, const void *k, int64_t ldk, const void *v,
@@ -518,8 +573,15 @@ hipError_t launch_seqs(const Fh3kAttn &a, const void *q, int64_t ldq, const void
     if (tiles * a.kv_heads > 0x7FFFFF) return hipErrorInvalidValue;
     const SeqsArgs g = {a, q, k, v, o, ldq, ldk, ldv, ldo, s, prefix, (int)tiles};
     const dim3 grid((unsigned)(tiles * a.kv_heads));
-    if constexpr (TY == 2) hipLaunchKernelGGL(k_attn_seqs32<HD>, grid, dim3(64 * NW), 0, st, g);
-    else hipLaunchKernelGGL((k_attn_seqs16<HD, TY>), grid, dim3(64 * NW), 0, st, g);
+    if constexpr (TY == 2) {
+        // Few workgroups with more than a few tiles of keys: eight wavefronts each, so
+        // that a SIMD has two and a row half as many steps.
+        if (tiles * a.kv_heads <= SPLIT_TO && (int64_t)s.n_tok >= (int64_t)SPLIT_FROM * s.n_seq)
+            hipLaunchKernelGGL((k_attn_seqs32<HD, 2>), grid, dim3(512), 0, st, g);
+        else
+            hipLaunchKernelGGL((k_attn_seqs32<HD, 1>), grid, dim3(256), 0, st, g);
+    } else
+        hipLaunchKernelGGL((k_attn_seqs16<HD, TY>), grid, dim3(256), 0, st, g);
     return hipGetLastError();
 }
 

@@ -89,6 +89,19 @@ def test_long_and_peaked(gpu, t, hd):
 
 
 @pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("heads,kv,hd", [(16, 16, 64), (16, 8, 128)])
+def test_many_sequences(gpu, t, heads, kv, hd):
+    """More than 64 sequences, some empty, one long: more workgroups than the card holds at once."""
+    lens = [int(x) for x in np.random.default_rng(17).integers(0, 40, 150)]
+    lens[97] = 500
+    first = _offsets(lens)
+    arrays = _case(18, t, first[-1], heads, kv, hd)
+    got = _run(gpu, arrays, t, first, heads, kv, hd)
+    o, a, big = R.attention(*(R.from_type(x, t) for x in arrays), first, heads, kv, hd)
+    R.check(got, t, o, a, big, hd, 500, "many")
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
 def test_rows_behind_the_last_sequence(gpu, t):
     heads, kv, hd = 4, 2, 64
     arrays = _case(5, t, 90, heads, kv, hd)
