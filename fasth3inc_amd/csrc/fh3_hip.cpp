@@ -1151,6 +1151,10 @@ static int kv_rows(const Fh3KvCache *kv, int type, const void *d_k, int64_t *ldk
     const int64_t w = (int64_t)k->kv_heads * k->hd;
     if (d_k && (rc = check_rows(d_k, ldk, w, type, "k", fn)) != FH3_OK) return rc;
     if (d_v && (rc = check_rows(d_v, ldv, w, type, "v", fn)) != FH3_OK) return rc;
+    const size_t pool = fh3_hip_kv_pool_bytes(k->kv_heads, k->hd, k->pages);
+    if ((d_k && overlap(kv->d_pool, pool, d_k, span(s.n_tok, *ldk, w, type))) ||
+        (d_v && overlap(kv->d_pool, pool, d_v, span(s.n_tok, *ldv, w, type))))
+        return set_err(FH3_E_INVALID, "%s: the rows overlap the pool", fn);
     return FH3_OK;
 }
 

@@ -232,6 +232,10 @@ __device__ __forceinline__ KvSeq kv_seq(const Fh3kKv &c, const Fh3kSeqs &s, cons
 struct KvRun {
     int size, u, end, seq, tile, page;
     KvSeq q;
+    __device__ __forceinline__ int ends(int pages, int wgs) const {  // the workgroup that ends a tile begun at u
+        const int w = (u + pages - 1) / size;
+        return w < wgs ? w : wgs - 1;
+    }
 };
 __device__ __forceinline__ bool kv_run(const Fh3kKv &c, const Fh3kSeqs &s, const KvWork &w, int wg, KvRun &r) {
     KvSeq q = {};
@@ -525,7 +529,7 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
             const bool done = page0 == 0 && page1 == pages;
             float *part = done ? nullptr : parts.of(kvh, wg, page0 == 0);
             if (!done && page0 == 0 && tid == 0)
-                *parts.begun(kvh, wg) = {(run.u + pages - 1) / run.size, first, r0, rows};
+                *parts.begun(kvh, wg) = {run.ends(pages, work.wgs), first, r0, rows};
             for (int e = tid; e < ROWS * HD / 4; e += 64 * FEW_W) {
                 const int row = e / (HD / 4), d = e % (HD / 4) * 4;
                 float top = sm[0][row];
@@ -622,7 +626,7 @@ template <int HD, int NT>
 __global__ __launch_bounds__(64 * MANY_W, 2) void k_kv_many(Fh3kAttn a, Fh3kKv c, const void *__restrict__ q,
                                                             int64_t ldq, void *__restrict__ o, int64_t ldo, Fh3kSeqs s,
                                                             KvWork work, float *__restrict__ ws) {
-    typedef Rows<HD, _Float16, _Float16, NT, 1> R;
+    typedef Rows<HD, _Float16, _Float16, NT> R;
     constexpr int ROWS = WAVE_R * MANY_W, NTH = 64 * MANY_W, KU = HD / 64, VROW = KV_PAGE + 8;
     constexpr int CH = KV_PAGE * HD / 16 / NTH;  // 16-byte pieces of K, and of V, to a thread
     __shared__ __align__(16) _Float16 sk[2][KV_PAGE][R::KROW];
@@ -770,7 +774,7 @@ __global__ __launch_bounds__(64 * MANY_W, 2) void k_kv_many(Fh3kAttn a, Fh3kKv c
             const float l = sum32(w.l);
             const bool done = page0 == 0 && page1 == pages;
             if (!done && page0 == 0 && tid == 0)
-                *parts.begun(kvh, wg) = {(run.u + pages - 1) / run.size, first, r0, rows};
+                *parts.begun(kvh, wg) = {run.ends(pages, work.wgs), first, r0, rows};
             if (row < rows) {
                 float *part = done ? nullptr : parts.of(kvh, wg, page0 == 0);
                 const float inv = done ? (l == 0.f ? 0.f : ref / l) : ref;

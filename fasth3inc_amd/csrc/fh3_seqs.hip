@@ -7,13 +7,9 @@ namespace {
 template <int TY> struct Operand;
 template <> struct Operand<0> { typedef _Float16 TQ, TP; static constexpr int NW = 4, TYPE = FH3K_F16; };
 template <> struct Operand<1> { typedef __bf16 TQ, TP; static constexpr int NW = 4, TYPE = FH3K_BF16; };
-// fp32 as two 16-bit terms: q and k fp16 after a power of two for each row (22
-// bits), v and the weights bf16 (16 bits, any exponent); three products each
-template <> struct Operand<2> {
-    typedef _Float16 TQ;
-    typedef __bf16 TP;
-    static constexpr int NW = 4, TYPE = FH3K_F32;
-};
+// fp32 as two fp16 terms (22 bits) after a power of two for each row of q, k and
+// v; three products each
+template <> struct Operand<2> { typedef _Float16 TQ, TP; static constexpr int NW = 4, TYPE = FH3K_F32; };
 
 // Tiles of fp32 K and V in LDS: two planes of K [32][HD + 8], of V [32][HD + 32] (the
 // transposing reads take 4 rows x 64 bytes at once: rows 64 bytes apart modulo the
@@ -137,9 +133,9 @@ __device__ __forceinline__ void lose(R &w, const SeqsArgs &g, const Place &p, in
 }
 
 template <int HD, int TYPE, class R>
-__device__ __forceinline__ void put_rows(const R &w, const SeqsArgs &g, const Place &p, int row, int head) {
+__device__ __forceinline__ void put_rows(const R &w, const SeqsArgs &g, const Place &p, int row, int head, float unit) {
     const int hf = (threadIdx.x >> 5) & 1;
-    const float l = sum32(w.l), inv = l == 0.f ? 0.f : 1.f / l;
+    const float l = sum32(w.l), inv = l == 0.f ? 0.f : unit / l;
     if (row >= p.rows) return;
     const int64_t at = (int64_t)(p.first + w.pos) * g.ldo + head * HD + 4 * hf;
 #pragma unroll
@@ -154,9 +150,10 @@ __device__ __forceinline__ void put_rows(const R &w, const SeqsArgs &g, const Pl
 }
 
 // Two halves of the workgroup that took every other tile of keys: the second's sums
-// go through LDS (in a and b, DB / 2 blocks of 16 KB each; offsets and sums of weights
-// in c) to the first.
-template <class R> __device__ __forceinline__ void join_halves(R &w, int half, int wave, char *a, char *b, char *c) {
+// go through LDS (in a and b, DB / 2 blocks of 16 KB each; offsets, sums of weights
+// and units in c) to the first.
+template <class R>
+__device__ __forceinline__ void join_halves(R &w, float &unit, float first, int half, int wave, char *a, char *b, char *c) {
     const int lane = threadIdx.x & 63;
     float *ml = (float *)c + wave * 64 + lane;
     auto at = [&](int db, int q) {
@@ -164,7 +161,7 @@ template <class R> __device__ __forceinline__ void join_halves(R &w, int half, i
     };
     __syncthreads();
     if (half) {
-        ml[0] = w.m, ml[256] = w.l;
+        ml[0] = w.m, ml[256] = w.l, ml[512] = unit;
 #pragma unroll
         for (int db = 0; db < R::DB; db++)
 #pragma unroll
@@ -172,7 +169,12 @@ template <class R> __device__ __forceinline__ void join_halves(R &w, int half, i
     }
     __syncthreads();
     if (half) return;
-    const float m = ml[0], now = fmaxf(w.m, m), x = __builtin_amdgcn_exp2f(w.m - now), y = __builtin_amdgcn_exp2f(m - now);
+    const float m = ml[0], now = fmaxf(w.m, m), other = ml[512];
+    const float x = __builtin_amdgcn_exp2f(w.m - now), y = __builtin_amdgcn_exp2f(m - now);
+    // (a half that saw nothing has no say in the unit)
+    const float mine = unit >= 0.f ? unit : max32(w.l) > 0.f ? first : 0.f, its = other >= 0.f ? other : max32(ml[256]) > 0.f ? first : 0.f;
+    const float u = fmaxf(mine, its), ox = u > 0.f ? x * (mine / u) : 0.f, oy = u > 0.f ? y * (its / u) : 0.f;
+    unit = u;
     w.m = now;
     w.l = w.l * x + ml[256] * y;
 #pragma unroll
@@ -181,7 +183,7 @@ template <class R> __device__ __forceinline__ void join_halves(R &w, int half, i
         for (int q = 0; q < 4; q++) {
             const f32x4 z = *at(db, q);
 #pragma unroll
-            for (int i = 0; i < 4; i++) w.o[db][4 * q + i] = w.o[db][4 * q + i] * x + z[i] * y;
+            for (int i = 0; i < 4; i++) w.o[db][4 * q + i] = w.o[db][4 * q + i] * ox + z[i] * oy;
         }
 }
 
@@ -196,7 +198,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_seqs16(SeqsArgs g) {
     typedef typename Op::TQ T;
     constexpr int NW = 4, ROWS = WAVE_R * NW, RB = HD * 2, TILE_B = TILE_K * RB, PPR = RB / 16;  // pieces per row
     constexpr int CH = TILE_B / (1024 * NW);  // a wavefront's loads of a tile
-    typedef Rows<HD, T, T, 1, 1> R;
+    typedef Rows<HD, T, T, 1> R;
     typedef typename R::q8 v8;
     typedef short s4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s4 *lds4;
@@ -342,12 +344,13 @@ __global__ __launch_bounds__(256, 2) void k_attn_seqs16(SeqsArgs g) {
         if (e + 1 < n_tiles) step(e + 1, s1, s0, sk1, sk0, sv1, sv0);
     }
     if (lost) lose<HD, Op::TYPE>(w, g, p, whole & ~(TILE_K - 1), end);
-    put_rows<HD, Op::TYPE>(w, g, p, row, head);
+    put_rows<HD, Op::TYPE>(w, g, p, row, head, 1.f);
 }
 
-// F32: every operand is two 16-bit terms, made on the way to LDS: the terms of the
+// F32: every operand is two fp16 terms, made on the way to LDS: the terms of the
 // next V beside the first product, the weights and the terms of the next K beside
-// the second.  Tiles of 32 keys, so that two workgroups fit a CU and nothing has
+// the second.  (V and weights as two bf16 terms, which need no power of two: 600
+// tokens 46 us for 53, but 4e-6 off for 4e-7.)  Tiles of 32 keys, so that two workgroups fit a CU and nothing has
 // to be moved to accumulation registers (64 keys, one workgroup: 600 tokens x 64
 // heads 52.6 us; a third of the instructions were such moves).  KH = 2: eight
 // wavefronts, two to a SIMD, each four with every other tile of keys.
@@ -357,7 +360,7 @@ __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
     typedef Op::TQ TQ;
     typedef Op::TP TP;
     constexpr int NT = 256, ROWS = WAVE_R * 4;
-    typedef Rows<HD, TQ, TP, 2, 2> R;
+    typedef Rows<HD, TQ, TP, 2> R;
     typedef typename R::p8 p8;
     typedef KLds<HD> LK;
     typedef VLds<HD> LV;
@@ -365,14 +368,15 @@ __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
     __shared__ __align__(16) LK lk0[KH], lk1[KH];
     __shared__ __align__(16) LV lv0[KH], lv1[KH];
     __shared__ __align__(16) float ks0[KH][2 * TILE_32], ks1[KH][2 * TILE_32];  // each key's factor; the other half is not read
-    __shared__ int lost;
+    __shared__ __align__(16) float vs0[KH][2 * TILE_32], vs1[KH][2 * TILE_32];
+    __shared__ int lost, odd;  // odd: some factor of V so far is not 1 / V_UP
 
     const int tid = threadIdx.x % NT, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int half = KH == 2 ? __builtin_amdgcn_readfirstlane(threadIdx.x / NT) : 0;
     const int l32 = lane & 31;
     Place p;
     if (!place<ROWS>(g, p)) return;
-    if (tid == 0) lost = 0;
+    if (tid == 0) lost = odd = 0;
 
     constexpr int CPR = HD / 4, CH = TILE_32 * CPR / NT;  // 16-byte pieces of a row; of a tile, to a thread
     const int key0 = tid / CPR, d0 = tid % CPR * 4;      // the first; the others NT / CPR keys on
@@ -389,24 +393,27 @@ __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
             r[i] = *(const u32x4 *)(base + (uint32_t)((uint32_t)key * (uint32_t)ld + d0));
         }
     };
-    // Powers of two for this thread's pieces of K.  With values below 2^15 and one of
-    // 2^-5 at least in each row 1 will do (fp16's second term then reaches down to
-    // 2^-25, 2^-20 of the row's largest); otherwise the row's largest gives it.
+    // 0 where each row of a piece has a value of 2^-5 at least and none of `limit` or more.
+    auto largest = [&](const u32x4 &r) {
+        const f32x4 x = __builtin_bit_cast(f32x4, r);
+        return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+    };
+    auto rows_odd = [&](float top, float limit) {
+        uint64_t some = __ballot(top >= 0.03125f);  // any lane of a row
+#pragma unroll
+        for (int e = 1; e < CPR; e <<= 1) some |= some >> e;
+        constexpr uint64_t FIRST = CPR == 32 ? 0x0000000100000001ull : 0x0001000100010001ull;
+        return (~some & FIRST) | __ballot(!(top < limit));
+    };
+    // Powers of two for this thread's pieces of K: 1 for such rows (fp16's second term
+    // then reaches down to 2^-25, 2^-20 of the row's largest); otherwise the row's
+    // largest gives it.
     auto scales = [&](const u32x4 (&r)[CH], float (&up)[CH]) {
         float top[CH];
-        uint64_t fine = ~0ull;
+        uint64_t other = 0;
 #pragma unroll
-        for (int i = 0; i < CH; i++) {
-            const f32x4 x = __builtin_bit_cast(f32x4, r[i]);
-            top[i] = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-            up[i] = 1.f;
-            uint64_t some = __ballot(top[i] >= 0.03125f);  // any lane of a row
-#pragma unroll
-            for (int e = 1; e < CPR; e <<= 1) some |= some >> e;
-            constexpr uint64_t FIRST = CPR == 32 ? 0x0000000100000001ull : 0x0001000100010001ull;
-            fine &= (some & FIRST) == FIRST && !__ballot(!(top[i] < 32768.f)) ? ~0ull : 0;
-        }
-        if (!fine) {
+        for (int i = 0; i < CH; i++) top[i] = largest(r[i]), up[i] = 1.f, other |= rows_odd(top[i], 32768.f);
+        if (other) {
 #pragma unroll
             for (int i = 0; i < CH; i++) {
                 const float m = row_max<CPR>(top[i]);  // each row for itself
@@ -425,14 +432,37 @@ __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
         *(u32x2 *)&to.x[1][key][d0] = u32x2{l0, l1};
         ks[d0 ? TILE_32 + key : key] = __builtin_bit_cast(float, 0x7F000000u - __builtin_bit_cast(uint32_t, up));  // 1 / up
     };
-    auto put_v = [&](const u32x4 &r, int i, LV &to) {
+    // V's rows enter times V_UP (down to 2^-29 of the row's largest).  Where one is not
+    // as above put_v says so, and again_v gives each row of the pieces, written once
+    // more, a power of two of its own where it needs one: the largest of a small row
+    // comes to 2^3 .. 2^4 and of a large one to 2^14 .. 2^15, next to the least and the
+    // greatest that the rows left alone have, so that the weights' least step in the
+    // other's units is 2^-25 of the larger row's.  The way back is the key's factor; 0
+    // for a row of zeros.
+    constexpr float V_UP = 512.f;
+    auto v_terms = [&](const u32x4 &r, float up, float back, int i, LV &to, float *vs) {
         const int key = key0 + i * (NT / CPR);
         const f32x4 x = __builtin_bit_cast(f32x4, r);
         uint32_t h0, h1, l0, l1;
-        split2(x[0], x[1], 1.f, h0, l0, TP());
-        split2(x[2], x[3], 1.f, h1, l1, TP());
+        split2(x[0], x[1], up, h0, l0, TP());
+        split2(x[2], x[3], up, h1, l1, TP());
         *(u32x2 *)&to.x[0][key][d0] = u32x2{h0, h1};
         *(u32x2 *)&to.x[1][key][d0] = u32x2{l0, l1};
+        vs[d0 ? TILE_32 + key : key] = back;
+    };
+    auto put_v = [&](const u32x4 &r, int i, LV &to, float *vs) {
+        v_terms(r, V_UP, 1.f / V_UP, i, to, vs);
+        return rows_odd(largest(r), 64.f);
+    };
+    auto again_v = [&](const u32x4 (&r)[CH], LV &to, float *vs) {
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            const float m = row_max<CPR>(largest(r[i]));
+            const bool leave = (m >= 0.03125f && m < 64.f) || !(m <= 3.402823466e38f);
+            const float up = leave ? V_UP : pow2_to_14(m) * (m < 1.f ? 0x1p-10f : 2.f);
+            v_terms(r[i], up, m == 0.f ? 0.f : __builtin_bit_cast(float, 0x7F000000u - __builtin_bit_cast(uint32_t, up)), i, to, vs);
+        }
+        odd = 1;
     };
     auto clean = [&](u32x4 (&r)[CH], int e) {
         if ((e + 1) * TILE_32 <= whole) return;
@@ -459,20 +489,55 @@ __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
     w.slope2 = sc.bias ? g.a.slopes[head] * LOG2E : 0.f;
     const int lo = __builtin_amdgcn_readfirstlane(w.lim);
 
-    float up[CH];
+    float up[CH], unit = -1.f;  // the row's sums of weighted V are in units of this (-1: of 1 / V_UP until a key has another factor)
     __syncthreads();
     clean(rv, tile(0));
     scales(rk, up);
+    uint64_t other = 0;
 #pragma unroll
-    for (int i = 0; i < CH; i++) put_k(rk[i], up[i], i, lk0[half], ks0[half]), put_v(rv[i], i, lv0[half]);
+    for (int i = 0; i < CH; i++) {
+        put_k(rk[i], up[i], i, lk0[half], ks0[half]);
+        other |= put_v(rv[i], i, lv0[half], vs0[half]);
+    }
+    if (other) again_v(rv, lv0[half], vs0[half]);
     load(g.k, g.ldk, there(tile(1)), rk);
     load(g.v, g.ldv, there(tile(1)), rv);
     __syncthreads();
+    // Keys whose V stands there by a factor: it goes to the weight, in units of the
+    // largest one that a key with a weight has had (2^-25 of that one's weights is
+    // the least that fp16 holds).
+    auto units = [&](f32x16 &s, float c, float nm, const float *vs) {
+        vs += 4 * (lane >> 5);
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            if (fmaf(s[i], c, nm) > -25.f) top = fmaxf(top, vs[8 * (i >> 2) + (i & 3)]);
+        top = max32(top);
+        const float was = unit >= 0.f ? unit : max32(w.l) > 0.f ? 1.f / V_UP : 0.f;
+        unit = fmaxf(was, top);
+        if (was < unit) {
+            const float down = was / unit;
+#pragma unroll
+            for (int db = 0; db < R::DB; db++) w.o[db] *= down;
+        }
+        float full = 0.f, left = 0.f;  // the weights' sum, and the one that the second product's will give
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const float r = fminf(vs[8 * (i >> 2) + (i & 3)] / unit, 1.f);
+            full += __builtin_amdgcn_exp2f(fmaf(s[i], c, nm));
+            s[i] = r > 0.f ? s[i] + __builtin_amdgcn_logf(r) / c : -INFINITY;  // (0: zeros, or too small beside the unit)
+            left += __builtin_amdgcn_exp2f(fmaf(s[i], c, nm));
+        }
+        w.l += full - left;
+    };
     // Rows that see nothing of a tile have weights of 0: the workgroup waits for
     // those that do either way.  Past the last tile that one is made again, not read.
-    auto step = [&](int e, const LK &k_now, LK &k_next, const LV &v_now, LV &v_next, const float *ks, float *ks_next) {
+    auto step = [&](int e, const LK &k_now, LK &k_next, const LV &v_now, LV &v_next, const float *ks, float *ks_next,
+                    const float *vs, float *vs_next) {
         const int j0 = tile(e) * TILE_32;
+        const int some_odd = odd;
         clean(rv, tile(e + 1));
+        uint64_t other = 0;
         f32x16 s[1] = {};
         constexpr int N1 = R::KS, N2 = 2 * R::DB;
         typedef typename R::q8 q8;
@@ -487,7 +552,7 @@ __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
             s[0] = mfma32(c1, w.q[0][i], s[0]);
             s[0] = mfma32(c0, w.q[1][i], s[0]);
             s[0] = mfma32(c0, w.q[0][i], s[0]);
-            if (i * CH % N1 < CH) put_v(rv[i * CH / N1], i * CH / N1, v_next);
+            if (i * CH % N1 < CH) other |= put_v(rv[i * CH / N1], i * CH / N1, v_next, vs_next);
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
 #pragma unroll
             for (int x = 0; x < 3; x++) {
@@ -496,8 +561,10 @@ __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
             }
             __builtin_amdgcn_sched_group_barrier(0x200, 2, 0);  // LDS writes
         }
+        if (other) again_v(rv, v_next, vs_next);
         load(g.v, g.ldv, there(tile(e + 2)), rv);
         const float c = w.template scores<true>(s, sc, 1.f, ks, j0, j0 + TILE_32 > lo, w.lim), nm = -w.m;
+        if (__builtin_amdgcn_readfirstlane(some_odd)) units(s[0], c, nm, vs);
         scales(rk, up);
         float sum[2] = {};
         u32x4 ph[2], pl[2];
@@ -542,23 +609,23 @@ __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
     };
 #pragma unroll 1
     for (int e = 0; e < steps; e += 2) {
-        step(e, lk0[half], lk1[half], lv0[half], lv1[half], ks0[half], ks1[half]);
-        if (e + 1 < steps) step(e + 1, lk1[half], lk0[half], lv1[half], lv0[half], ks1[half], ks0[half]);
+        step(e, lk0[half], lk1[half], lv0[half], lv1[half], ks0[half], ks1[half], vs0[half], vs1[half]);
+        if (e + 1 < steps) step(e + 1, lk1[half], lk0[half], lv1[half], lv0[half], ks1[half], ks0[half], vs1[half], vs0[half]);
     }
     if constexpr (KH == 2) {
-        static_assert(sizeof lk0 >= R::DB / 2 * 16384 && sizeof lv0 >= 2048, "");
-        join_halves(w, half, wave, (char *)lk0, (char *)lk1, (char *)lv0);
+        static_assert(sizeof lk0 >= R::DB / 2 * 16384 && sizeof lv0 >= 3072, "");
+        join_halves(w, unit, 1.f / V_UP, half, wave, (char *)lk0, (char *)lk1, (char *)lv0);
         if (half) return;
     }
     if (lost) lose<HD, Op::TYPE>(w, g, p, whole & ~(TILE_32 - 1), end);
-    put_rows<HD, Op::TYPE>(w, g, p, row, head);
+    put_rows<HD, Op::TYPE>(w, g, p, row, head, unit < 0.f ? 1.f / V_UP : unit);
 }
 
 // F32 with every other tile of keys to four more wavefronts, against four wavefronts
 // alone, us: one sequence at 64 heads over 8, hd 128, 37 tokens 15.5 / 11.0, 300
-// tokens 27.9 / 30.4, 600 tokens 45.7 / 54.1, 900 tokens 77 / 79, 1200 tokens (608
-// workgroups) 116 / 110; 16 heads over 16, hd 64, 500 tokens 20.9 / 26.7, 2000 tokens
-// 63 / 88, 4000 tokens (512 workgroups) 144 / 178, 5060 tokens (672) 106 / 106.
+// tokens 32 / 36, 600 tokens 53 / 66, 900 tokens 89 / 95, 1200 tokens (608
+// workgroups) 134 / 127; 16 heads over 16, hd 64, 500 tokens 22 / 28, 2000 tokens
+// 65 / 92, 4000 tokens (512 workgroups) 150 / 182, 5060 tokens (672) 101 / 100.
 // (16 bits: 0.7 to 0.9 as fast at hd 128, 0.8 to 1.1 at hd 64, so not there.)
 constexpr int SPLIT_TO = 512, SPLIT_FROM = 128;
 

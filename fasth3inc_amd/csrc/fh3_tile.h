@@ -167,8 +167,8 @@ __device__ __forceinline__ float sum16(float x) {
     return r[0] + r[1];
 }
 // TQ: element of the first product's operands, TP: of the second's.  QT: terms of
-// q and of the weights, KT: of k and v.
-template <int HD, class TQ, class TP, int QT, int KT> struct Rows {
+// q and of the weights.
+template <int HD, class TQ, class TP, int QT> struct Rows {
     static constexpr int KS = HD / 16, DB = HD / 32;
     static constexpr int KROW = HD + 8;  // LDS row of K
     typedef typename Vec<TQ>::v8 q8;
@@ -226,7 +226,7 @@ template <int HD, class TQ, class TP, int QT, int KT> struct Rows {
         l = 0.f;
     }
 
-    // S^T of 64 keys; sk holds K's KT planes of 64 rows.
+    // S^T of the 64 keys whose rows sk holds.
     __device__ __forceinline__ void products(const TQ *sk, f32x16 (&s)[2]) {
         const int l32 = threadIdx.x & 31, hf = (threadIdx.x >> 5) & 1;
         s[0] = s[1] = f32x16{};
@@ -236,7 +236,6 @@ template <int HD, class TQ, class TP, int QT, int KT> struct Rows {
             for (int st = 0; st < 2; st++) {
                 const TQ *row = sk + (32 * st + l32) * KROW + 16 * kk + 8 * hf;
                 const q8 a = *(const q8 *)row;
-                if constexpr (KT == 2) s[st] = mfma32(*(const q8 *)(row + TILE_K * KROW), q[0][kk], s[st]);
                 if constexpr (QT == 2) s[st] = mfma32(a, q[1][kk], s[st]);
                 s[st] = mfma32(a, q[0][kk], s[st]);
             }

@@ -204,9 +204,10 @@ int fh3_hip_vsa_attention_qkv_dev(const Fh3VsaCfg *c, const float *d_qkv, const 
  *   softcap          0 means none
  *   d_slopes         NULL, or device [heads]
  * F16 and BF16 operands enter the matrix products as they are, F32 ones as two
- * 16-bit terms each (the result is that of fp32 arithmetic to about 1e-6);
- * softmax and sums are fp32, the weights are rounded to the operand type for the
- * second product (F32: two terms).  Deterministic. */
+ * fp16 terms each after a power of two for each row (relative error about 4e-7;
+ * beside a value of v of size V nothing below 2^-30 V counts); softmax and sums
+ * are fp32, the weights are rounded to the operand type for the second product
+ * (F32: two terms).  Deterministic. */
 typedef struct Fh3AttnCfg {
     int heads;
     int kv_heads;
@@ -228,7 +229,9 @@ typedef struct Fh3AttnCfg {
  * causal or not.  Pointers and row starts 16-byte aligned; o must not overlap
  * the inputs.  A NaN or infinity in a key or value makes the rows that see it
  * non-finite (at the least in the channels that hold it) and no other row.  No
- * workspace: calls on different streams do not disturb each other. */
+ * workspace: calls on different streams do not disturb each other.  n_tok at most
+ * 2^24, n_seq 2^20, n_tok * heads 2^30, n_tok * heads / 128 + n_seq * kv_heads
+ * below 2^23; larger calls are refused. */
 int fh3_hip_attention_seqs_dev(const Fh3AttnCfg *c, const void *d_q, int64_t ldq, const void *d_k, int64_t ldk,
                                const void *d_v, int64_t ldv, void *d_o, int64_t ldo, int n_tok, int n_seq,
                                const int *d_first, const int *d_prefix, void *stream);
@@ -279,7 +282,9 @@ size_t fh3_hip_kv_pool_bytes(int kv_heads, int head_dim, int pages);
  * cache.  The scale of a page, head and K or V is the least 2^e, e >= -100, with
  * amax <= 127 * 2^e over the finite values of its tokens; q = value / scale
  * rounded to nearest even, an infinity +-127, a NaN 0.  Where new tokens raise
- * the scale of a page that holds earlier ones, those are rounded again to it.
+ * the scale of a page that holds earlier ones, those are rounded again to it;
+ * where they replace a page's later tokens (d_len was lowered) it keeps at least
+ * the scale it had.  The rows must not overlap the pool.
  * Appending the same rows at the same positions again changes nothing.
  *
  * fh3_hip_kv_read_dev: the rows' cached values as `type` (for export, or a
@@ -300,7 +305,8 @@ int fh3_hip_kv_read_dev(const Fh3KvCache *kv, int type, void *d_k, int64_t ldk, 
  * over the keys by the lengths on the device; d_ws (16-byte aligned,
  * fh3_hip_kv_attention_workspace_bytes, may be 0) holds the parts until a
  * second kernel joins them in order: deterministic.  Calls that may overlap need
- * a workspace each. */
+ * a workspace each.  Sizes as in fh3_hip_attention_seqs_dev; tiles of rows (up
+ * to 128) times max_pages below 2^31. */
 size_t fh3_hip_kv_attention_workspace_bytes(const Fh3AttnCfg *c, const Fh3KvCache *kv, int n_tok, int n_seq);
 int fh3_hip_kv_attention_dev(const Fh3AttnCfg *c, const Fh3KvCache *kv, const void *d_q, int64_t ldq, void *d_o,
                              int64_t ldo, int n_tok, int n_seq, const int *d_first, void *d_ws, size_t ws_bytes,

@@ -94,10 +94,10 @@ def bound(t, o, a, big, hd, keys):
 FRO = {F32: 1e-5, F16: 2.0 ** -11, BF16: 2.0 ** -8}
 
 
-def check(got, t, o, a, big, hd, keys, what):
+def check(got, t, o, a, big, hd, keys, what, floor=0.0):
     got = from_type(got, t)
     off = np.abs(got - o)
-    lim = bound(t, o, a, big, hd, keys)
+    lim = bound(t, o, a, big, hd, keys) + floor
     worst = float((off / lim).max(initial=0.0))
     norm = np.linalg.norm(o)
     fro = float(np.linalg.norm(got - o) / norm) if norm else float(off.max(initial=0.0))

@@ -89,8 +89,15 @@ class Held:
     def check_attend(self, t, q, first, heads, what, slopes=None, causal=True, softcap=0.0):
         got = self.attend(t, q, first, heads, slopes=slopes, causal=causal, softcap=softcap)
         o, a, big = self.model.attention(R.from_type(q, t), first, self.lens, heads, causal, None, softcap, slopes)
-        n = first[-1]
-        R.check(got[:n], t, o[:n], a[:n], big, self.model.hd, max(self.lens), what)
+        n, m = first[-1], self.model
+        # Weights enter as fp16 (F32: two terms), whose least step is 2^-24: each is off by up to 2^-25 more where it
+        # is small, beside a largest of at least 2^6, so the output by 2^-31 of the sum of the |v| of all keys.  That
+        # matters where the key that a row is about has a 0 in a channel.
+        vs = [m.values(s, 0, n_k)[1] for s, n_k in enumerate(self.lens)]
+        floor = np.zeros_like(o)
+        for s, v in enumerate(vs):
+            floor[first[s]:first[s + 1]] = np.repeat(np.abs(v).sum(0), heads // m.kv, 0).ravel() * 2.0 ** -31 if len(v) else 0
+        R.check(got[:n], t, o[:n], a[:n], big, m.hd, max(self.lens), what, floor[:n])
         return got
 
 
@@ -248,6 +255,40 @@ def test_long_and_ragged(gpu, t, new):
     h = Held(gpu, kv, hd, lens, 41)
     first = _offsets([new] * len(lens))
     h.check_attend(t, _rows(42, t, first[-1], heads * hd, 1.5), first, heads, "ragged, %d new" % new)
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_chunk_of_peaked_scores(gpu, t, hd):
+    """Scores that pass the running offset in either half of a page, pages of different value scales."""
+    kv, heads, lens, new = 1, 2, [1500, 130], [100, 70]
+    h = Held(gpu, kv, hd, lens, 61)
+    first = _offsets(new)
+    h.check_attend(t, _rows(62, t, first[-1], heads * hd, 8.0), first, heads, "peaked chunk")
+
+
+@pytest.mark.parametrize("new", [1, 60])
+def test_shared_pages(gpu, new):
+    """Three sequences with the same first pages, one after the other and one behind what the table holds."""
+    kv, hd, heads, lens = 2, 128, 8, [190, 150, 129]
+    table = np.asarray([[5, 3, 1], [5, 3, 0], [5, 3, 2]], np.int64)
+    h = Held(gpu, kv, hd, lens, 63, pages=6, table=table, max_pages=3)
+    first = _offsets([new] * 3)
+    h.check_attend(F16, _rows(64, F16, first[-1], heads * hd), first, heads, "shared pages, %d new" % new)
+
+
+def test_lengths_lowered(gpu):
+    """Tokens taken back and others put in their place: the page keeps at least its scale, the tokens before them theirs."""
+    kv, hd, lens = 2, 64, [70]
+    h = Held(gpu, kv, hd, lens, 65)
+    h.append(F32, _rows(66, F32, 6, kv * hd, 50.0), _rows(67, F32, 6, kv * hd, 9.0), [0, 6])
+    h.same()
+    for length, new in ((67, 2), (66, 1), (65, 1), (65, 65)):   # (65, 65: all of it from the start)
+        h.lens = [length]
+        h.len = gpu.DeviceBuffer.from_array(np.asarray(h.lens, np.int32))
+        h.kv = gpu.kv_cache(kv, hd, h.model.pages, h.model.table.shape[1], h.pool, h.table, h.len)
+        h.append(F32, _rows(68, F32, new, kv * hd, 0.1), _rows(69, F32, new, kv * hd, 100.0), [0, new])
+        h.same()
 
 
 def test_many_sequences(gpu):

@@ -207,6 +207,34 @@ def test_values_far_from_one(gpu):
         R.check(got, F32, o, a, big, hd, n, "q %g k %g v %g" % (qs, ks, vs))
 
 
+@pytest.mark.parametrize("hd,lens", [(128, [230]), (64, [230]), (128, [40, 230] + [20] * 130)])
+@pytest.mark.parametrize("sizes", [(1.0, 1e-9), (1e-9, 1.0), (1.0, 1e5), (1e5, 1.0), (0.0, 1e-12), (1e-12, 0.0), (1e-20, 1e20),
+                                   (30.0, 500.0, 1e-3), (1.0, 1e30, 1e-30), (1e-30, 1e30, 1.0)])
+def test_rows_of_v_of_different_sizes(gpu, hd, lens, sizes):
+    """fp32 V whose rows change size from run to run of keys, zeros among them, with rows that see one size only.
+
+    V and the weights enter as two fp16 terms, whose least step is 2^-24.  A row of V is off by 2^-25 in units in
+    which its largest is 2^3 at least (2^4 at 2^-5 times 512), so by 2^-28 of its largest.  A weight is off by 2^-25
+    beside a largest of 2^6 at least, in units of the largest factor seen: times a row whose largest is 2^15 at most
+    where that of the factor's is 2^14 at least (large rows) or 2^4 where it is 2^3 (small ones and those left alone: 2^4),
+    so by 2^-30 of the largest row for every key."""
+    heads, kv = 16, 8
+    first = _offsets(lens)
+    q, k, v = _case(19, F32, first[-1], heads, kv, hd)
+    for s, n in enumerate(lens):
+        for j in range(n):
+            v[first[s] + j] *= sizes[min(j // 50, len(sizes) - 1)] if n > 50 else sizes[s % len(sizes)]
+    got = _run(gpu, (q, k, v), F32, first, heads, kv, hd)
+    o, a, big = R.attention(*(x.astype(np.float64) for x in (q, k, v)), first, heads, kv, hd)
+    floor = np.zeros_like(o)
+    top = np.repeat(np.abs(v.reshape(-1, kv, hd)).max(2).astype(np.float64), heads // kv, 1)
+    for s, n in enumerate(lens):
+        for j in range(n):
+            m = top[first[s]:first[s] + j + 1].max(0)
+            floor[first[s] + j] = np.repeat(m * (2.0 ** -28 + (j + 1) * 2.0 ** -30), hd)
+    R.check(got, F32, o, a, big, hd, max(lens), "sizes %s" % (sizes,), floor)
+
+
 def test_replays_and_streams(gpu):
     """Captured and replayed, with other eager work between, and on a stream of its own: the eager bits."""
     F, t, heads, kv, hd = gpu, BF16, 16, 2, 128

@@ -94,6 +94,13 @@ def test_rows_refused(F, change):
     _refused(F, F.kv_read_dev, kv, args)
 
 
+def test_rows_in_the_pool_refused(F):
+    kv, pool = F.kv_cache(2, 64, 4, 3, at(5), at(6), at(7)), F.kv_pool_bytes(2, 64, 4)
+    for d_k, d_v in ((at(5), at(1)), (at(0), at(5)), (at(0), at(5, pool - 16)), (at(5, 16 - 3 * 128 * 4), at(1))):
+        _refused(F, F.kv_append_dev, kv, 0, d_k, d_v, 3, 3)
+        _refused(F, F.kv_read_dev, kv, 0, d_k, d_v, 3, 3)
+
+
 def test_missing_rows_refused(F):
     kv = F.kv_cache(2, 64, 4, 3, at(5), at(6), at(7))
     _refused(F, F.kv_append_dev, kv, 0, None, at(1), 3, 3)
