@@ -453,7 +453,10 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
                     const int left = there ? lim[r] - j0 - 4 * g : 0x80000000;
 #pragma unroll
                     for (int i = 0; i < 16; i++) t[r][i >> 2][i & 3] *= x;
-                    if (sc.cap2) {
+                    if (sc.cap2 && sc.fine) {
+#pragma unroll
+                        for (int i = 0; i < 16; i++) t[r][i >> 2][i & 3] = capped_fine(t[r][i >> 2][i & 3], sc.cap2);
+                    } else if (sc.cap2) {
 #pragma unroll
                         for (int i = 0; i < 16; i++) t[r][i >> 2][i & 3] = capped(t[r][i >> 2][i & 3], sc.cap2);
                     }

@@ -56,18 +56,31 @@ __device__ __forceinline__ f32x16 mfma32(bf8 a, bf8 b, f32x16 c) {
 struct Score {
     float f;        // product sum -> t (log2 units), or -> 2 log2(e) x / cap before the tanh
     float cap2;     // cap * log2(e), or 0
+    bool fine;      // the cap's tanh to fp32's last bits
     bool bias;
 };
 __device__ __forceinline__ Score score_of(const Fh3kAttn &a) {
     Score sc;
     sc.cap2 = a.softcap > 0.f ? a.softcap * LOG2E : 0.f;
     sc.f = a.softcap > 0.f ? 2.f * LOG2E * (a.scale / a.softcap) : a.scale * LOG2E;
+    sc.fine = a.type == FH3K_F32 || a.softcap > 64.f;
     sc.bias = a.slopes != nullptr;
     return sc;
 }
-// cap tanh(x / cap) from y = 2 log2(e) x / cap: tanh = 1 - 2 / (1 + e^2z)
+// cap tanh(z), z = x / cap, from y = 2 log2(e) z: tanh = 1 - 2 / (1 + e^2z).  Its error is
+// 10^-7 of the cap, whatever x is: enough for 16-bit rows and caps to 64 (10^-5).
 __device__ __forceinline__ float capped(float y, float cap2) {
     return cap2 - 2.f * cap2 * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(y));
+}
+// Otherwise up to |z| = 1 by the continued fraction z / (1 + z^2 / (3 + z^2 / (5 + ..)))
+// cut after 9, z (945 + 105 z^2 + z^4) / (945 + 420 z^2 + 15 z^4), which is off by 6 10^-8 of
+// itself at most; the reciprocal by one Newton step.
+__device__ __forceinline__ float capped_fine(float y, float cap2) {
+    const float z = y * 0.34657359f, z2 = z * z;
+    const float num = fmaf(z2, z2 + 105.f, 945.f), den = fmaf(z2, fmaf(15.f, z2, 420.f), 945.f);
+    float r = __builtin_amdgcn_rcpf(den);
+    r = fmaf(fmaf(-den, r, 1.f), r, r);
+    return fabsf(z) < 1.f ? cap2 * z * (num * r) : capped(y, cap2);
 }
 
 // 2^e such that amax * 2^e lies in [2^13, 2^14); 1 for zeros and values that are not finite.
@@ -261,10 +274,17 @@ template <int HD, class TQ, class TP, int QT> struct Rows {
         float c = f * kscale;  // t = c s, unless there is more to do
         // (two loops and two branches: in one loop both would be computed and selected)
         if (sc.cap2) {
+            if (sc.fine) {
 #pragma unroll
-            for (int st = 0; st < NS; st++)
+                for (int st = 0; st < NS; st++)
 #pragma unroll
-                for (int v = 0; v < 16; v++) s[st][v] = capped(s[st][v] * c, sc.cap2);
+                    for (int v = 0; v < 16; v++) s[st][v] = capped_fine(s[st][v] * c, sc.cap2);
+            } else {
+#pragma unroll
+                for (int st = 0; st < NS; st++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++) s[st][v] = capped(s[st][v] * c, sc.cap2);
+            }
             c = 1.f;
         }
         if (sc.bias) {

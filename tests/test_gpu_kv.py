@@ -267,6 +267,16 @@ def test_chunk_of_peaked_scores(gpu, t, hd):
     h.check_attend(t, _rows(62, t, first[-1], heads * hd, 8.0), first, heads, "peaked chunk")
 
 
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("cap", [0.5, 64.0, 65.0, 1e8, 1e30])
+def test_caps_of_any_size(gpu, t, cap):
+    kv, hd, heads, lens = 2, 64, 4, [150, 70]
+    h = Held(gpu, kv, hd, lens, 71)
+    for new in (1, 40):
+        first = _offsets([new, new])
+        h.check_attend(t, _rows(72, t, first[-1], heads * hd), first, heads, "cap %g, %d new" % (cap, new), softcap=cap)
+
+
 @pytest.mark.parametrize("new", [1, 60])
 def test_shared_pages(gpu, new):
     """Three sequences with the same first pages, one after the other and one behind what the table holds."""

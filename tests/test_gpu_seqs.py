@@ -196,6 +196,18 @@ def test_closed_forms(gpu):
     assert np.abs(got[0] - v[0]).max() <= 2.0 ** -16 * np.abs(v).max()
 
 
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("cap", [0.5, 64.0, 65.0, 1e4, 1e8, 1e30])
+def test_caps_of_any_size(gpu, t, cap):
+    """A cap far above the scores leaves them as they are, one far below makes them +-cap."""
+    heads, kv, hd, lens = 4, 2, 64, [130, 20]
+    first = _offsets(lens)
+    arrays = _case(23, t, first[-1], heads, kv, hd)
+    got = _run(gpu, arrays, t, first, heads, kv, hd, softcap=cap)
+    o, a, big = R.attention(*(R.from_type(x, t) for x in arrays), first, heads, kv, hd, True, None, cap)
+    R.check(got, t, o, a, big, hd, max(lens), "cap %g" % cap)
+
+
 def test_values_far_from_one(gpu):
     """fp32 operands of any size: keys and values near the ends of fp32 and of fp16's range."""
     heads, kv, hd, n = 2, 1, 128, 90
