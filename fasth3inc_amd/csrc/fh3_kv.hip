@@ -72,7 +72,10 @@ __device__ __forceinline__ bool row_page(const Fh3kKv &c, const Fh3kSeqs &s, Row
 
 // The rows go through LDS as fp32: their largest finite value gives the scale, then
 // a whole page is made in 16-byte pieces, part of one in the smallest that its
-// rows fill (K: 16 channels of a slot; V: four slots of a channel).
+// rows fill (K: 16 channels of a slot; V: four slots of a channel).  Prompts are bound
+// by memory (with the read-back 88 MB in 26 us, 3.4 TB/s), one token of 64 sequences by
+// the loads that wait for each other: length, page, rows (4-5 us of 14 with the
+// read-back).
 template <int HD>
 __global__ __launch_bounds__(ROW_T) void k_kv_append(Fh3kKv c, int type, const void *__restrict__ k, int64_t ldk,
                                                      const void *__restrict__ v, int64_t ldv, Fh3kSeqs s) {
@@ -319,7 +322,10 @@ __device__ __forceinline__ half8 to_half(uint32_t a, uint32_t b) {
 // Few rows to a sequence: tiles of 16 R rows; each of four wavefronts takes every
 // fourth page of a tile with all its rows, straight from memory into the
 // operands of 16x16x32 products (S^T = K Q^T, O^T = V^T P^T), and the four are
-// joined in LDS.  NT: 16-bit terms of q and of the weights (fp32: two).
+// joined in LDS.  NT: 16-bit terms of q and of the weights (fp32: two).  16 KB are on
+// their way to each wavefront, 128 KB to a CU, so that memory bounds it: 0.5 GB of cache
+// in 94 us and 102 with the join (5.0 TB/s; a device copy moves 4.8), 140 MB in 31
+// and 39.  One token of one sequence takes 8 us, launch and latencies.
 constexpr int FEW_W = 4;
 template <int HD, int R, int NT>
 __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, const void *__restrict__ q, int64_t ldq,
@@ -567,7 +573,7 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
     } while (run.u < run.end && kv_next(c, s, work, run));
 }
 
-// Joins the parts of a divided tile in order.  A workgroup takes RB rows of the tile
+// Joins the parts of a divided tile in order, 4-5 us.  A workgroup takes RB rows of the tile
 // that workgroup blockIdx.x of key head blockIdx.y began; SB groups of threads take
 // every SB-th part each.
 template <int HD, int SB>
@@ -623,7 +629,9 @@ __global__ __launch_bounds__(256) void k_kv_join(Fh3kAttn a, Fh3kKv c, void *__r
 // Many rows to a sequence: tiles of 128, 32 to a wavefront.  A page is turned
 // into fp16 once for all of them, through double-buffered LDS: K as rows, V
 // transposed with the keys of each 16 in the order of the first product's
-// accumulator (0-3, 8-11, 4-7, 12-15).
+// accumulator (0-3, 8-11, 4-7, 12-15).  Bound by the vector instructions of the softmax and
+// the conversion beside the matrix ones: 1000 tokens of 64 heads behind 31000 in
+// 550 us, 0.82 PFLOP/s.
 constexpr int MANY_W = 4;
 template <int HD, int NT>
 __global__ __launch_bounds__(64 * MANY_W, 2) void k_kv_many(Fh3kAttn a, Fh3kKv c, const void *__restrict__ q,
@@ -831,7 +839,10 @@ extern "C" hipError_t fh3k_kv_read(const Fh3kKv *c, int type, void *k, int64_t l
 }
 
 // How the rows of a call are tiled: by the average sequence, which is what the
-// host knows (any tiling is right for any sequence).
+// host knows (any tiling is right for any sequence).  fp16, 8 key heads of 128, 16
+// sequences of 4000 tokens, us with tiles of 16 / 32 / 128 rows: 8 rows each 31 / 37
+// / 48, 16 rows 33 / 38 / 49, 18 rows - / 38 / 50, 32 rows - / 42 / 52; 40 rows in 128
+// 58.  Two sequences of 16000: 8 rows 21 / 23 / 33, 16 rows 22 / 27 / 33, 32 rows - / 31 / 34.
 struct KvForm {
     KvWork work;
     int64_t tiles;  // of all sequences at most
