@@ -1116,6 +1116,7 @@ extern "C" int fh3_hip_attention_seqs_dev(const Fh3AttnCfg *c, const void *d_q, 
     if ((rc = check_rows(d_v, &ldv, wk, a.type, "v", fn)) != FH3_OK) return rc;
     if ((rc = check_rows(d_o, &ldo, wq, a.type, "o", fn)) != FH3_OK) return rc;
     if ((uintptr_t)d_prefix & 3u) return set_err(FH3_E_INVALID, "%s: d_prefix misaligned", fn);
+    if (!fh3k_attn_seqs_fits(&a, s)) return set_err(FH3_E_INVALID, "%s: too many tiles of rows for one launch", fn);
     const size_t on = span(n_tok, ldo, wq, a.type);
     if (overlap(d_o, on, d_q, span(n_tok, ldq, wq, a.type)) || overlap(d_o, on, d_k, span(n_tok, ldk, wk, a.type)) ||
         overlap(d_o, on, d_v, span(n_tok, ldv, wk, a.type)))
@@ -1194,6 +1195,9 @@ static int check_kv_attn(const Fh3AttnCfg *c, const Fh3KvCache *kv, Fh3kSeqs s, 
     if (!kv || kv->kv_heads != a->kv_heads || kv->head_dim != a->hd || kv->max_pages <= 0 ||
         kv->max_pages > (1 << 24))
         return set_err(FH3_E_INVALID, "%s: the cache's heads, head_dim or max_pages do not fit", fn);
+    const Fh3kKv sizes = {kv->kv_heads, kv->head_dim, kv->pages, kv->max_pages, nullptr, nullptr, nullptr, nullptr};
+    if (!fh3k_kv_attn_fits(a, &sizes, s))
+        return set_err(FH3_E_INVALID, "%s: tiles of rows times max_pages must be below 2^31", fn);
     return FH3_OK;
 }
 

@@ -188,6 +188,9 @@ typedef struct Fh3kKv {
     float *scales;
     const int *table, *len;
 } Fh3kKv;
+// Whether a launch can number the call's tiles (and its pages, over the cache).
+int fh3k_attn_seqs_fits(const Fh3kAttn *a, Fh3kSeqs s);
+int fh3k_kv_attn_fits(const Fh3kAttn *a, const Fh3kKv *c, Fh3kSeqs s);
 hipError_t fh3k_attn_seqs(const Fh3kAttn *a, const void *q, int64_t ldq, const void *k, int64_t ldk, const void *v,
                           int64_t ldv, void *o, int64_t ldo, Fh3kSeqs s, const int *prefix, hipStream_t st);
 hipError_t fh3k_kv_extend(int *len, Fh3kSeqs s, hipStream_t st);

@@ -861,6 +861,10 @@ static KvForm kv_form(const Fh3kAttn &a, const Fh3kKv &c, const Fh3kSeqs &s) {
     return f;
 }
 
+extern "C" int fh3k_kv_attn_fits(const Fh3kAttn *a, const Fh3kKv *c, Fh3kSeqs s) {
+    return kv_form(*a, *c, s).tiles * c->max_pages <= 0x7FFFFFFF;
+}
+
 extern "C" size_t fh3k_kv_attn_ws_bytes(const Fh3kAttn *a, const Fh3kKv *c, Fh3kSeqs s) {
     const KvForm f = kv_form(*a, *c, s);
     return f.join ? (size_t)parts_bytes(a->hd, 1 << f.work.shift, a->kv_heads, f.work.wgs) : 0;
@@ -870,7 +874,6 @@ template <int HD>
 static hipError_t kv_attn(const Fh3kAttn &a, const Fh3kKv &c, const void *q, int64_t ldq, void *o, int64_t ldo,
                           const Fh3kSeqs &s, float *ws, hipStream_t st) {
     const KvForm f = kv_form(a, c, s);
-    if (f.tiles * c.max_pages > 0x7FFFFFFF) return hipErrorInvalidValue;
     const dim3 grid((unsigned)f.work.wgs * a.kv_heads);
     const bool two = a.type == FH3K_F32;
 #define FH3K_KV(K, W) hipLaunchKernelGGL(K, grid, dim3(64 * W), 0, st, a, c, q, ldq, o, ldo, s, f.work, f.join ? ws : nullptr)

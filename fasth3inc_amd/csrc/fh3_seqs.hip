@@ -5,11 +5,11 @@ namespace {
 
 // How the three value types enter the matrix products.
 template <int TY> struct Operand;
-template <> struct Operand<0> { typedef _Float16 TQ, TP; static constexpr int NW = 4, TYPE = FH3K_F16; };
-template <> struct Operand<1> { typedef __bf16 TQ, TP; static constexpr int NW = 4, TYPE = FH3K_BF16; };
+template <> struct Operand<0> { typedef _Float16 TQ, TP; static constexpr int TYPE = FH3K_F16; };
+template <> struct Operand<1> { typedef __bf16 TQ, TP; static constexpr int TYPE = FH3K_BF16; };
 // fp32 as two fp16 terms (22 bits) after a power of two for each row of q, k and
 // v; three products each
-template <> struct Operand<2> { typedef _Float16 TQ, TP; static constexpr int NW = 4, TYPE = FH3K_F32; };
+template <> struct Operand<2> { typedef _Float16 TQ, TP; static constexpr int TYPE = FH3K_F32; };
 
 // Tiles of fp32 K and V in LDS: two planes of K [32][HD + 8], of V [32][HD + 32] (the
 // transposing reads take 4 rows x 64 bytes at once: rows 64 bytes apart modulo the
@@ -632,15 +632,18 @@ __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
 // (16 bits: 0.7 to 0.9 as fast at hd 128, 0.8 to 1.1 at hd 64, so not there.)
 constexpr int SPLIT_TO = 512, SPLIT_FROM = 128;
 
+// Tiles of all sequences at most: each may have one that is not full.
+int64_t most_tiles(const Fh3kAttn &a, const Fh3kSeqs &s) {
+    constexpr int ROWS = WAVE_R * 4;
+    const int64_t G = a.heads / a.kv_heads;
+    return s.first ? s.n_tok * G / ROWS + (s.n_seq < s.n_tok ? s.n_seq : s.n_tok)
+                   : (int64_t)s.n_seq * ((s.n_tok / s.n_seq * G + ROWS - 1) / ROWS);
+}
+
 template <int HD, int TY>
 hipError_t launch_seqs(const Fh3kAttn &a, const void *q, int64_t ldq, const void *k, int64_t ldk, const void *v,
                        int64_t ldv, void *o, int64_t ldo, const Fh3kSeqs &s, const int *prefix, hipStream_t st) {
-    constexpr int NW = Operand<TY>::NW, ROWS = WAVE_R * NW;
-    const int64_t G = a.heads / a.kv_heads;
-    // tiles of all sequences at most: each may have one that is not full
-    const int64_t tiles = s.first ? s.n_tok * G / ROWS + (s.n_seq < s.n_tok ? s.n_seq : s.n_tok)
-                                  : (int64_t)s.n_seq * ((s.n_tok / s.n_seq * G + ROWS - 1) / ROWS);
-    if (tiles * a.kv_heads > 0x7FFFFF) return hipErrorInvalidValue;
+    const int64_t tiles = most_tiles(a, s);
     const SeqsArgs g = {a, q, k, v, o, ldq, ldk, ldv, ldo, s, prefix, (int)tiles};
     const dim3 grid((unsigned)(tiles * a.kv_heads));
     if constexpr (TY == 2) {
@@ -656,6 +659,8 @@ hipError_t launch_seqs(const Fh3kAttn &a, const void *q, int64_t ldq, const void
 }
 
 }  // namespace
+
+extern "C" int fh3k_attn_seqs_fits(const Fh3kAttn *a, Fh3kSeqs s) { return most_tiles(*a, s) * a->kv_heads <= 0x7FFFFF; }
 
 extern "C" hipError_t fh3k_attn_seqs(const Fh3kAttn *a, const void *q, int64_t ldq, const void *k, int64_t ldk,
                                      const void *v, int64_t ldv, void *o, int64_t ldo, Fh3kSeqs s, const int *prefix,

@@ -305,8 +305,10 @@ int fh3_hip_kv_read_dev(const Fh3KvCache *kv, int type, void *d_k, int64_t ldk, 
  * over the keys by the lengths on the device; d_ws (16-byte aligned,
  * fh3_hip_kv_attention_workspace_bytes, may be 0) holds the parts until a
  * second kernel joins them in order: deterministic.  Calls that may overlap need
- * a workspace each.  Sizes as in fh3_hip_attention_seqs_dev; tiles of rows (up
- * to 128) times max_pages below 2^31. */
+ * a workspace each.  Sizes as in fh3_hip_attention_seqs_dev; (rows / T + n_seq) *
+ * max_pages below 2^31, where rows is n_tok * heads / kv_heads and a tile has T = 16
+ * of them up to 16 to an average sequence, 32 up to 32, otherwise 128.  Larger
+ * calls are refused (a workspace size of 0). */
 size_t fh3_hip_kv_attention_workspace_bytes(const Fh3AttnCfg *c, const Fh3KvCache *kv, int n_tok, int n_seq);
 int fh3_hip_kv_attention_dev(const Fh3AttnCfg *c, const Fh3KvCache *kv, const void *d_q, int64_t ldq, void *d_o,
                              int64_t ldo, int n_tok, int n_seq, const int *d_first, void *d_ws, size_t ws_bytes,
