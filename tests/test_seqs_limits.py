@@ -28,3 +28,22 @@ def test_more_pages_than_a_cache_call_counts(F, n_tok, n_seq, max_pages):
     cfg, kv = F.attn_cfg(8, 2, 64), F.kv_cache(2, 64, 4, max_pages, at(5), at(6), at(7))
     assert F.kv_attention_workspace_bytes(cfg, kv, n_tok, n_seq) == 0
     _refused(F, F.kv_attention_dev, cfg, kv, dict(d_q=at(0), d_o=at(1), n_tok=n_tok, n_seq=n_seq, d_ws=at(2), ws_bytes=STEP))
+
+
+def test_workspaces_refused(F):
+    """A cache long enough that tiles are divided: the workspace is needed, and looked at."""
+    cfg, kv = F.attn_cfg(8, 2, 64), F.kv_cache(2, 64, 40, 30, at(5), at(6), at(7))
+    need = F.kv_attention_workspace_bytes(cfg, kv, 3, 3)
+    assert need > 0 and need % 16 == 0
+    good = dict(d_q=at(0), d_o=at(1), n_tok=3, n_seq=3, d_ws=at(2), ws_bytes=need)
+    pool, rows = F.kv_pool_bytes(2, 64, 40), 3 * 8 * 64 * 4
+    for change in (dict(ws_bytes=need - 1), dict(ws_bytes=0), dict(d_ws=None), dict(d_ws=at(2, 4)), dict(d_ws=at(2, 8)),
+                   dict(d_ws=at(1)), dict(d_ws=at(1, rows - 16)), dict(d_ws=at(1, 16 - need)),       # o
+                   dict(d_ws=at(0)), dict(d_ws=at(0, rows - 16)), dict(d_ws=at(0, -16)),             # q
+                   dict(d_ws=at(5)), dict(d_ws=at(5, pool - 16)), dict(d_ws=at(5, 16 - need))):      # the pool
+        assert "workspace" in _refused(F, F.kv_attention_dev, cfg, kv, {**good, **change}), change
+    for hd, heads, n in ((64, 8, 40), (128, 32, 7), (128, 2, 300)):   # few and many rows
+        cfg, kv = F.attn_cfg(heads, 2, hd), F.kv_cache(2, hd, 400, 200, at(5), at(6), at(7))
+        need = F.kv_attention_workspace_bytes(cfg, kv, n, 1)
+        assert need > 0
+        _refused(F, F.kv_attention_dev, cfg, kv, dict(d_q=at(0), d_o=at(1), n_tok=n, n_seq=1, d_ws=at(2), ws_bytes=need - 1))
