@@ -1100,6 +1100,14 @@ static size_t span(int64_t n, int64_t ld, int64_t width, int type) {
     return (size_t)((n - 1) * ld + width) * value_bytes(type);
 }
 
+// Whether rows of a and of b, n each, meet (rows of one pitch may stand between each other).
+static bool rows_meet(const void *a, int64_t lda, const void *b, int64_t ldb, int64_t n, int64_t width, int type) {
+    if (!overlap(a, span(n, lda, width, type), b, span(n, ldb, width, type))) return false;
+    const uintptr_t pitch = (uintptr_t)lda * value_bytes(type), w = (uintptr_t)width * value_bytes(type);
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b, off = (x > y ? x - y : y - x) % pitch;
+    return lda != ldb || off < w || off > pitch - w;
+}
+
 extern "C" int fh3_hip_attention_seqs_dev(const Fh3AttnCfg *c, const void *d_q, int64_t ldq, const void *d_k,
                                           int64_t ldk, const void *d_v, int64_t ldv, void *d_o, int64_t ldo,
                                           int n_tok, int n_seq, const int *d_first, const int *d_prefix,
@@ -1181,6 +1189,8 @@ extern "C" int fh3_hip_kv_read_dev(const Fh3KvCache *kv, int type, void *d_k, in
     int rc = kv_rows(kv, type, d_k, &ldk, d_v, &ldv, s, &k, fn);
     if (rc != FH3_OK) return rc;
     if (!d_k && !d_v) return set_err(FH3_E_INVALID, "%s: NULL k and v", fn);
+    if (d_k && d_v && rows_meet(d_k, ldk, d_v, ldv, n_tok, (int64_t)k.kv_heads * k.hd, type))
+        return set_err(FH3_E_INVALID, "%s: the rows of k and v overlap", fn);
     if ((rc = ensure_init()) != FH3_OK) return rc;
     FragRt::On on_device(g.device);
     FH3_HIPCALL(fh3k_kv_read(&k, type, d_k, ldk, d_v, ldv, s, stream ? (hipStream_t)stream : g.stream));

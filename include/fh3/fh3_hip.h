@@ -288,7 +288,8 @@ size_t fh3_hip_kv_pool_bytes(int kv_heads, int head_dim, int pages);
  * Appending the same rows at the same positions again changes nothing.
  *
  * fh3_hip_kv_read_dev: the rows' cached values as `type` (for export, or a
- * prefix that another program attends to).  K or V may be NULL. */
+ * prefix that another program attends to).  K or V may be NULL; their rows must
+ * not overlap each other or the pool, but may stand between each other. */
 int fh3_hip_kv_extend_dev(const Fh3KvCache *kv, int n_tok, int n_seq, const int *d_first, void *stream);
 int fh3_hip_kv_append_dev(const Fh3KvCache *kv, int type, const void *d_k, int64_t ldk, const void *d_v, int64_t ldv,
                           int n_tok, int n_seq, const int *d_first, void *stream);

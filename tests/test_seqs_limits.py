@@ -47,3 +47,11 @@ def test_workspaces_refused(F):
         need = F.kv_attention_workspace_bytes(cfg, kv, n, 1)
         assert need > 0
         _refused(F, F.kv_attention_dev, cfg, kv, dict(d_q=at(0), d_o=at(1), n_tok=n, n_seq=1, d_ws=at(2), ws_bytes=need - 1))
+
+
+def test_read_back_onto_itself(F):
+    """K and V read back to rows that overlap: whichever came last would stand there."""
+    kv, w = F.kv_cache(2, 64, 4, 3, at(5), at(6), at(7)), 2 * 64
+    for d_v, ld in ((at(0), 0), (at(0, 16), 0), (at(0, 2 * w * 4), 0), (at(0, w * 4 - 16), 2 * w), (at(0, w * 4 + 16), 2 * w)):
+        _refused(F, F.kv_read_dev, kv, 0, at(0), d_v, dict(n_tok=3, n_seq=3, ldk=ld, ldv=ld))
+    _refused(F, F.kv_read_dev, kv, 0, at(0), at(0, w * 4), dict(n_tok=3, n_seq=3, ldk=2 * w, ldv=3 * w))
