@@ -1069,8 +1069,11 @@ static int check_attn(const Fh3AttnCfg *c, int n_tok, Fh3kAttn *a, const char *f
     if ((uintptr_t)c->d_slopes & 3u) return set_err(FH3_E_INVALID, "%s: d_slopes misaligned", fn);
     if (n_tok > 0 && (int64_t)n_tok > ((int64_t)1 << 30) / c->heads)
         return set_err(FH3_E_INVALID, "%s: n_tok * heads too large", fn);
-    *a = {c->heads, c->kv_heads, c->head_dim, c->type, c->causal != 0,
-          c->scale > 0.f ? c->scale : 1.0f / sqrtf((float)c->head_dim), c->softcap, c->d_slopes};
+    const float scale = c->scale > 0.f ? c->scale : 1.0f / sqrtf((float)c->head_dim);
+    // one fp32 factor takes a product to its part of the cap: 2 log2(e) scale / softcap, over q's power of two
+    if (c->softcap > 0.f && !((double)c->softcap <= scale * 0x1p106 && (double)c->softcap >= scale * 0x1p-100))
+        return set_err(FH3_E_INVALID, "%s: softcap must be from 2^-100 to 2^106 times the scale", fn);
+    *a = {c->heads, c->kv_heads, c->head_dim, c->type, c->causal != 0, scale, c->softcap, c->d_slopes};
     return FH3_OK;
 }
 

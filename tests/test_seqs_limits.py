@@ -55,3 +55,10 @@ def test_read_back_onto_itself(F):
     for d_v, ld in ((at(0), 0), (at(0, 16), 0), (at(0, 2 * w * 4), 0), (at(0, w * 4 - 16), 2 * w), (at(0, w * 4 + 16), 2 * w)):
         _refused(F, F.kv_read_dev, kv, 0, at(0), d_v, dict(n_tok=3, n_seq=3, ldk=ld, ldv=ld))
     _refused(F, F.kv_read_dev, kv, 0, at(0), at(0, w * 4), dict(n_tok=3, n_seq=3, ldk=2 * w, ldv=3 * w))
+
+
+@pytest.mark.parametrize("scale,softcap", [(1e-20, 1e30), (1e-44, 1e-3), (1e30, 1e-3), (1.0, 1e-44), (0.0, 1e-38)])
+def test_caps_too_far_from_the_scale(F, scale, softcap):
+    """scale / softcap is one fp32 factor of the product: past its range every score would be 0, or the cap."""
+    cfg = F.attn_cfg(8, 2, 64, scale=scale, softcap=softcap)
+    _refused(F, F.attention_seqs_dev, cfg, SEQS)
