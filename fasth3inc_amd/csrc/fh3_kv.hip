@@ -286,7 +286,7 @@ __device__ __forceinline__ bool kv_next(const Fh3kKv &c, const Fh3kSeqs &s, cons
 
 // Where the parts of a divided tile stand: of each workgroup two, the end of a
 // tile begun before its run (0) and the beginning of one that goes on behind it
-// (1); rows x HD sums, then the rows' offsets and sums of weights.  What k_kv_join
+// (1); rows x HD sums, then the rows' sums of weights and their offsets' two terms.  What k_kv_join
 // has to know of the second, the workgroup that begins the tile writes down.
 struct Begun {
     int last;               // the workgroup that ends it, or 0: there is none
@@ -296,14 +296,14 @@ template <int HD> struct Parts {
     float *p;
     int rows, kv_heads, wgs;
     __device__ __forceinline__ float *of(int kvh, int wg, int which) const {
-        return p + (((int64_t)kvh * wgs + wg) * 2 + which) * rows * (HD + 2);
+        return p + (((int64_t)kvh * wgs + wg) * 2 + which) * rows * (HD + 3);
     }
     __device__ __forceinline__ Begun *begun(int kvh, int wg) const {
-        return (Begun *)(p + (int64_t)kv_heads * wgs * 2 * rows * (HD + 2)) + (kvh * wgs + wg);
+        return (Begun *)(p + (int64_t)kv_heads * wgs * 2 * rows * (HD + 3)) + (kvh * wgs + wg);
     }
 };
 __host__ __device__ constexpr int64_t parts_bytes(int hd, int rows, int kv_heads, int wgs) {
-    return (int64_t)kv_heads * wgs * (2 * rows * (hd + 2) * (int)sizeof(float) + (int)sizeof(Begun));
+    return (int64_t)kv_heads * wgs * (2 * rows * (hd + 3) * (int)sizeof(float) + (int)sizeof(Begun));
 }
 
 __device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c) {
@@ -333,7 +333,7 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
                                                           float *__restrict__ ws) {
     constexpr int ROWS = 16 * R, KU = HD / 64, DT = HD / 16, OROW = HD + 4;
     __shared__ __align__(16) float so[FEW_W][ROWS][OROW];
-    __shared__ float sm[FEW_W][ROWS], sl[FEW_W][ROWS];
+    __shared__ float sm[FEW_W][ROWS], slo[FEW_W][ROWS], sl[FEW_W][ROWS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.x % c.kv_heads, wg = blockIdx.x / c.kv_heads, G = work.G;
@@ -370,7 +370,7 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
             // rows of this lane: R times l16; q's fragments, 16 channels of each 64.
             // q, the first pages and their K are on their way before any is used.
             Raw8 raw[R][2 * KU];
-            float f[R], m[R], l[R], slope2[R];
+            float f[R], m[R], mlo[R], l[R], slope2[R];  // m, mlo: the weights' offset in two terms
             int pos[R], lim[R];
 #pragma unroll
             for (int r = 0; r < R; r++) {
@@ -391,6 +391,7 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
             }
             half8 qf[R][NT][2 * KU];
             f32x4 acc[R][DT];
+            bool far[R];  // some row of the sixteen has an offset of FAR and more
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 float x[2 * KU][8], top = 0.f;
@@ -416,7 +417,8 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
                     if constexpr (NT == 2) qf[r][NT - 1][i] = __builtin_bit_cast(half8, l4);
                 }
                 m[r] = M_NONE;
-                l[r] = 0.f;
+                mlo[r] = l[r] = 0.f;
+                far[r] = false;
 #pragma unroll
                 for (int d = 0; d < DT; d++) acc[r][d] = f32x4{};
             }
@@ -455,21 +457,23 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
                 half8 pf[R][NT][2];
 #pragma unroll
                 for (int r = 0; r < R; r++) {
-                    const float x = f[r] * ks, far = (float)(pos[r] - j0 - 4 * g);
+                    float x = factor(f[r] * ks);  // scores are x t, unless there is more to do
+                    const float ahead = (float)(pos[r] - j0 - 4 * g);
                     const int left = there ? lim[r] - j0 - 4 * g : 0x80000000;
-#pragma unroll
-                    for (int i = 0; i < 16; i++) t[r][i >> 2][i & 3] *= x;
                     if (sc.cap2 && sc.fine) {
 #pragma unroll
-                        for (int i = 0; i < 16; i++) t[r][i >> 2][i & 3] = capped_fine(t[r][i >> 2][i & 3], sc.cap2);
+                        for (int i = 0; i < 16; i++) t[r][i >> 2][i & 3] = capped_fine(t[r][i >> 2][i & 3] * x, sc.cap2);
+                        x = 1.f;
                     } else if (sc.cap2) {
 #pragma unroll
-                        for (int i = 0; i < 16; i++) t[r][i >> 2][i & 3] = capped(t[r][i >> 2][i & 3], sc.cap2);
+                        for (int i = 0; i < 16; i++) t[r][i >> 2][i & 3] = capped(t[r][i >> 2][i & 3] * x, sc.cap2);
+                        x = 1.f;
                     }
                     if (sc.bias) {
 #pragma unroll
                         for (int i = 0; i < 16; i++)
-                            t[r][i >> 2][i & 3] = fmaf(-slope2[r], fabsf(far - (float)(16 * (i >> 2) + (i & 3))), t[r][i >> 2][i & 3]);
+                            t[r][i >> 2][i & 3] = fmaf(-slope2[r], fabsf(ahead - (float)(16 * (i >> 2) + (i & 3))), t[r][i >> 2][i & 3] * x);
+                        x = 1.f;
                     }
                     if (cut) {
 #pragma unroll
@@ -480,14 +484,24 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
                     float mt = t[r][0][0];
 #pragma unroll
                     for (int i = 1; i < 16; i++) mt = fmaxf(mt, t[r][i >> 2][i & 3]);
-                    if (__ballot(mt > m[r] + RAISE)) {
+                    if (__ballot(fmaf(mt, x, -m[r]) - mlo[r] > RAISE)) {
                         mt = max32(max16(mt));
-                        const float now = mt > m[r] + RAISE ? mt - OFFSET : m[r];
-                        const float keep = __builtin_amdgcn_exp2f(m[r] - now);
-                        m[r] = now;
+                        const float y = mt * x, off = fmaf(mt, x, -y) - OFFSET;
+                        const bool raise = fmaf(mt, x, -m[r]) - mlo[r] > RAISE, two = fabsf(y) >= FAR;
+                        const float now = two ? y : y - OFFSET, rest = two ? off : 0.f;
+                        const float keep = raise ? __builtin_amdgcn_exp2f((m[r] - now) + (mlo[r] - rest)) : 1.f;
+                        m[r] = raise ? now : m[r];
+                        mlo[r] = raise ? rest : mlo[r];
+                        far[r] = __ballot(fabsf(m[r]) >= FAR && m[r] != M_NONE);
                         l[r] *= keep;
 #pragma unroll
                         for (int d = 0; d < DT; d++) acc[r][d] *= keep;
+                    }
+                    float nm = -m[r];
+                    if (far[r]) {
+#pragma unroll
+                        for (int i = 0; i < 16; i++) t[r][i >> 2][i & 3] = fmaf(t[r][i >> 2][i & 3], x, -m[r]) - mlo[r];
+                        x = 1.f, nm = 0.f;
                     }
                     float sum = 0.f;
 #pragma unroll
@@ -496,8 +510,8 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const int i = 8 * u + 2 * e;
-                            const float p0 = __builtin_amdgcn_exp2f(t[r][i >> 2][i & 3] - m[r]);
-                            const float p1 = __builtin_amdgcn_exp2f(t[r][i >> 2][(i & 3) + 1] - m[r]);
+                            const float p0 = __builtin_amdgcn_exp2f(fmaf(t[r][i >> 2][i & 3], x, nm));
+                            const float p1 = __builtin_amdgcn_exp2f(fmaf(t[r][i >> 2][(i & 3) + 1], x, nm));
                             uint32_t hi, lo;
                             split2(p0, p1, 1.f, hi, lo, _Float16());
                             h[e] = hi, l4[e] = lo;
@@ -530,7 +544,7 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
             for (int r = 0; r < R; r++) {
                 l[r] = sum32(sum16(l[r]));
                 const int row = 16 * r + l16;
-                if (g == 0) sm[wave][row] = m[r], sl[wave][row] = l[r];
+                if (g == 0) sm[wave][row] = m[r], slo[wave][row] = mlo[r], sl[wave][row] = l[r];
 #pragma unroll
                 for (int d = 0; d < DT; d++) *(f32x4 *)&so[wave][row][16 * d + 4 * g] = acc[r][d];
             }
@@ -541,14 +555,16 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
                 *parts.begun(kvh, wg) = {run.ends(pages, work.wgs), first, r0, rows};
             for (int e = tid; e < ROWS * HD / 4; e += 64 * FEW_W) {
                 const int row = e / (HD / 4), d = e % (HD / 4) * 4;
-                float top = sm[0][row];
+                float top = sm[0][row], rest = slo[0][row], sum = 0.f;
 #pragma unroll
-                for (int w = 1; w < FEW_W; w++) top = fmaxf(top, sm[w][row]);
-                float sum = 0.f;
+                for (int w = 1; w < FEW_W; w++) {
+                    const bool more = (sm[w][row] - top) + (slo[w][row] - rest) > 0.f;
+                    top = more ? sm[w][row] : top, rest = more ? slo[w][row] : rest;
+                }
                 f32x4 x = {};
 #pragma unroll
                 for (int w = 0; w < FEW_W; w++) {
-                    const float keep = __builtin_amdgcn_exp2f(sm[w][row] - top);
+                    const float keep = __builtin_amdgcn_exp2f((sm[w][row] - top) + (slo[w][row] - rest));
                     sum += sl[w][row] * keep;
                     const f32x4 y = *(const f32x4 *)&so[w][row][d];
 #pragma unroll
@@ -556,7 +572,7 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
                 }
                 if (!done) {
                     *(f32x4 *)(part + row * HD + d) = x;
-                    if (d == 0) part[ROWS * HD + row] = top, part[ROWS * (HD + 1) + row] = sum;
+                    if (d == 0) part[ROWS * HD + row] = sum, part[ROWS * (HD + 1) + row] = top, part[ROWS * (HD + 2) + row] = rest;
                 } else if (r0 + row < rows) {
                     const float inv = sum == 0.f ? 0.f : 1.f / sum;
                     const int tok = (r0 + row) / G, head = kvh * G + (r0 + row) % G;
@@ -581,38 +597,36 @@ __global__ __launch_bounds__(256) void k_kv_join(Fh3kAttn a, Fh3kKv c, void *__r
                                                  const float *__restrict__ ws) {
     constexpr int RB = 1024 / HD / SB;
     __shared__ __align__(16) float so[SB][RB * HD];
-    __shared__ float sm[SB][RB], sl[SB][RB];
+    __shared__ float sm[SB][RB], slo[SB][RB], sl[SB][RB];
     const int tid = threadIdx.x, wg = blockIdx.x, kvh = blockIdx.y, G = work.G, ROWS = 1 << work.shift;
     const Parts<HD> parts = {(float *)ws, ROWS, c.kv_heads, work.wgs};
     const Begun b = *parts.begun(kvh, wg);
     const int row0 = blockIdx.z * RB;
     if (b.last == 0 || b.r0 + row0 >= b.rows) return;
     const int grp = tid / (256 / SB), t = tid % (256 / SB), r = t / (HD / 4), d = t % (HD / 4) * 4, row = row0 + r;
-    float top = M_NONE, sum = 0.f;
+    float top = M_NONE, rest = 0.f, sum = 0.f;
     f32x4 x = {};
 #pragma unroll 4
     for (int w = wg + grp; w <= b.last; w += SB) {
         const float *p = parts.of(kvh, w, w == wg);
-        const float pm = p[ROWS * HD + row], pl = p[ROWS * (HD + 1) + row];
+        const float pl = p[ROWS * HD + row], pm = p[ROWS * (HD + 1) + row], plo = p[ROWS * (HD + 2) + row];
         const f32x4 y = *(const f32x4 *)(p + row * HD + d);
-        const float now = fmaxf(top, pm);
-        const float keep = __builtin_amdgcn_exp2f(top - now), add = __builtin_amdgcn_exp2f(pm - now);
-        top = now;
+        float keep, add;
+        join_offsets(top, rest, pm, plo, keep, add);
         sum = sum * keep + pl * add;
 #pragma unroll
         for (int v = 0; v < 4; v++) x[v] = x[v] * keep + y[v] * add;
     }
     if constexpr (SB > 1) {
         *(f32x4 *)&so[grp][r * HD + d] = x;
-        if (d == 0) sm[grp][r] = top, sl[grp][r] = sum;
+        if (d == 0) sm[grp][r] = top, slo[grp][r] = rest, sl[grp][r] = sum;
         __syncthreads();
         if (grp) return;
 #pragma unroll
         for (int e = 1; e < SB; e++) {
-            const float pm = sm[e][r], now = fmaxf(top, pm);
-            const float keep = __builtin_amdgcn_exp2f(top - now), add = __builtin_amdgcn_exp2f(pm - now);
+            float keep, add;
+            join_offsets(top, rest, sm[e][r], slo[e][r], keep, add);
             const f32x4 y = *(const f32x4 *)&so[e][r * HD + d];
-            top = now;
             sum = sum * keep + sl[e][r] * add;
 #pragma unroll
             for (int v = 0; v < 4; v++) x[v] = x[v] * keep + y[v] * add;
@@ -739,7 +753,9 @@ __global__ __launch_bounds__(64 * MANY_W, 2) void k_kv_many(Fh3kAttn a, Fh3kKv c
                         __builtin_amdgcn_sched_group_barrier(0x008, NT, 0);
                         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
                     }
-                    w.weights(x, w.template scores<false>(x, sc, ks_n, nullptr, j0, j0 + KV_PAGE > lo, w.lim), pf);
+                    float nm;
+                    const float c = w.template scores<false>(x, sc, ks_n, nullptr, j0, j0 + KV_PAGE > lo, w.lim, nm);
+                    w.weights(x, c, nm, pf);
                     // pages of the same scale add up in the product's accumulator
                     if (vs_n > ref) {
                         const float down = ref / vs_n;
@@ -791,7 +807,7 @@ __global__ __launch_bounds__(64 * MANY_W, 2) void k_kv_many(Fh3kAttn a, Fh3kKv c
                 const float inv = done ? (l == 0.f ? 0.f : ref / l) : ref;
                 const int64_t at_o = (int64_t)(first + tok) * ldo + head * HD;
                 const int r = WAVE_R * wave + l32;
-                if (!done && hf == 0) part[ROWS * HD + r] = w.m, part[ROWS * (HD + 1) + r] = l;
+                if (!done && hf == 0) part[ROWS * HD + r] = l, part[ROWS * (HD + 1) + r] = w.m, part[ROWS * (HD + 2) + r] = w.lo;
 #pragma unroll
                 for (int db = 0; db < R::DB; db++)
 #pragma unroll

@@ -161,7 +161,7 @@ __device__ __forceinline__ void join_halves(R &w, float &unit, float first, int 
     };
     __syncthreads();
     if (half) {
-        ml[0] = w.m, ml[256] = w.l, ml[512] = unit;
+        ml[0] = w.m, ml[256] = w.l, ml[512] = unit, ml[768] = w.lo;
 #pragma unroll
         for (int db = 0; db < R::DB; db++)
 #pragma unroll
@@ -169,13 +169,13 @@ __device__ __forceinline__ void join_halves(R &w, float &unit, float first, int 
     }
     __syncthreads();
     if (half) return;
-    const float m = ml[0], now = fmaxf(w.m, m), other = ml[512];
-    const float x = __builtin_amdgcn_exp2f(w.m - now), y = __builtin_amdgcn_exp2f(m - now);
+    const float other = ml[512];
+    float x, y;
+    join_offsets(w.m, w.lo, ml[0], ml[768], x, y);
     // (a half that saw nothing has no say in the unit)
     const float mine = unit >= 0.f ? unit : max32(w.l) > 0.f ? first : 0.f, its = other >= 0.f ? other : max32(ml[256]) > 0.f ? first : 0.f;
     const float u = fmaxf(mine, its), ox = u > 0.f ? x * (mine / u) : 0.f, oy = u > 0.f ? y * (its / u) : 0.f;
     unit = u;
-    w.m = now;
     w.l = w.l * x + ml[256] * y;
 #pragma unroll
     for (int db = 0; db < R::DB; db++)
@@ -318,9 +318,10 @@ __global__ __launch_bounds__(256, 2) void k_attn_seqs16(SeqsArgs g) {
         if (e + 1 < n_tiles) load_v(e + 1, vn);
         if (j0 < hi) {
             v8 pf[1][4];
-            const float c = w.template scores<false>(s, sc, 1.f, nullptr, j0, j0 + TILE_K > lo, w.lim);
+            float nm;
+            const float c = w.template scores<false>(s, sc, 1.f, nullptr, j0, j0 + TILE_K > lo, w.lim, nm);
             products(kn, next);  // past the last tile: what is there, not used
-            w.weights(s, c, pf);
+            w.weights(s, c, nm, pf);
             product2(ve, pf);
             constexpr int M1 = 2 * R::KS, M2 = 4 * R::DB;  // matrix instructions of the two products
             __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);  // LDS reads, four ahead
@@ -508,13 +509,16 @@ __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
     __syncthreads();
     // Keys whose V stands there by a factor: it goes to the weight, in units of the
     // largest one that a key with a weight has had (2^-25 of that one's weights is
-    // the least that fp16 holds).
-    auto units = [&](f32x16 &s, float c, float nm, const float *vs) {
+    // the least that fp16 holds).  s becomes the weights' arguments themselves.
+    auto units = [&](f32x16 &s, float &c, float &nm, const float *vs) {
         vs += 4 * (lane >> 5);
         float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; i++)
-            if (fmaf(s[i], c, nm) > -25.f) top = fmaxf(top, vs[8 * (i >> 2) + (i & 3)]);
+        for (int i = 0; i < 16; i++) {
+            s[i] = fmaf(s[i], c, nm);
+            if (s[i] > -25.f) top = fmaxf(top, vs[8 * (i >> 2) + (i & 3)]);
+        }
+        c = 1.f, nm = 0.f;
         top = max32(top);
         const float was = unit >= 0.f ? unit : max32(w.l) > 0.f ? 1.f / V_UP : 0.f;
         unit = fmaxf(was, top);
@@ -527,9 +531,9 @@ __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             const float r = fminf(vs[8 * (i >> 2) + (i & 3)] / unit, 1.f);
-            full += __builtin_amdgcn_exp2f(fmaf(s[i], c, nm));
-            s[i] = r > 0.f ? s[i] + __builtin_amdgcn_logf(r) / c : -INFINITY;  // (0: zeros, or too small beside the unit)
-            left += __builtin_amdgcn_exp2f(fmaf(s[i], c, nm));
+            full += __builtin_amdgcn_exp2f(s[i]);
+            s[i] = r > 0.f ? s[i] + __builtin_amdgcn_logf(r) : -INFINITY;  // (0: zeros, or too small beside the unit)
+            left += __builtin_amdgcn_exp2f(s[i]);
         }
         w.l += full - left;
     };
@@ -566,7 +570,7 @@ __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
         }
         if (other) again_v(rv, v_next, vs_next);
         load(g.v, g.ldv, there(tile(e + 2)), rv);
-        const float c = w.template scores<true>(s, sc, 1.f, ks, j0, j0 + TILE_32 > lo, w.lim), nm = -w.m;
+        float nm, c = w.template scores<true>(s, sc, 1.f, ks, j0, j0 + TILE_32 > lo, w.lim, nm);
         if (__builtin_amdgcn_readfirstlane(some_odd)) units(s[0], c, nm, vs);
         scales(rk, up);
         float sum[2] = {};
@@ -616,7 +620,7 @@ __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
         if (e + 1 < steps) step(e + 1, lk1[half], lk0[half], lv1[half], lv0[half], ks1[half], ks0[half], vs1[half], vs0[half]);
     }
     if constexpr (KH == 2) {
-        static_assert(sizeof lk0 >= R::DB / 2 * 16384 && sizeof lv0 >= 3 * 1024, "");
+        static_assert(sizeof lk0 >= R::DB / 2 * 16384 && sizeof lv0 >= 4 * 1024, "");
         join_halves(w, unit, 1.f / V_UP, half, wave, (char *)lk0, (char *)lk1, (char *)lv0);
         if (half) return;
     }

@@ -20,8 +20,20 @@ constexpr int WAVE_R = 32;   // rows per wavefront
 // it by more than RAISE: the weights stay within 2^-OFFSET .. 2^RAISE of what a
 // fresh maximum would give, and most tiles need no rescale of the sums.  The
 // offset keeps small weights out of fp16's subnormal range (2^14 < 65504).
-constexpr float OFFSET = 6.f, RAISE = 14.f;
-constexpr float M_NONE = -1e30f;  // no key seen yet: finite, so that masked t = -inf gives 0
+// From |t| = FAR on, m alone could not stand 6 below the largest t (half a step of fp32
+// is 8 and more from 2^27), nor is t = c s itself exact enough: there m is the rounded largest
+// t and a second term lo what the exact product is off it by, and the weights' arguments
+// (c s - m) - lo are small numbers made by one multiply-add from the products s.  Below, lo
+// is 0 and arguments are c s - m.
+constexpr float OFFSET = 6.f, RAISE = 14.f, FAR = 0x1p20f;
+constexpr float M_NONE = -3.402823466e38f;  // no key seen yet: finite, so that masked t = -inf gives 0
+// Parts of a row with offsets (m, lo) and (m2, lo2): what the larger offset leaves of each; m, lo become the larger.
+__device__ __forceinline__ void join_offsets(float &m, float &lo, float m2, float lo2, float &keep, float &add) {
+    const float d = (m2 - m) + (lo2 - lo), e = __builtin_amdgcn_exp2f(-fabsf(d));
+    keep = d > 0.f ? e : 1.f;
+    add = d > 0.f ? 1.f : e;
+    m = d > 0.f ? m2 : m, lo = d > 0.f ? lo2 : lo;
+}
 
 template <class T> struct Vec;
 template <> struct Vec<_Float16> {
@@ -67,6 +79,9 @@ __device__ __forceinline__ Score score_of(const Fh3kAttn &a) {
     sc.bias = a.slopes != nullptr;
     return sc;
 }
+// A factor of the products, kept positive and finite: a product of 0 and a masked -inf are then
+// what they should be (0 or an infinite factor would make a NaN of them).
+__device__ __forceinline__ float factor(float x) { return __builtin_amdgcn_fmed3f(x, 0x1p-149f, 3.402823466e38f); }
 // cap tanh(z), z = x / cap, from y = 2 log2(e) z: tanh = 1 - 2 / (1 + e^2z).  Its error is
 // 10^-7 of the cap, whatever x is: enough for 16-bit rows and caps to 64 (10^-5).
 __device__ __forceinline__ float capped(float y, float cap2) {
@@ -189,7 +204,8 @@ template <int HD, class TQ, class TP, int QT> struct Rows {
 
     q8 q[QT][KS];
     f32x16 o[DB];
-    float m, l;      // of the row: the weights' offset, the sum over this lane's keys
+    float m, lo, l;  // of the row: the weights' offset in two terms, the sum over this lane's keys
+    uint64_t far;    // rows of the wavefront that have an offset of FAR and more
     float f;         // Score::f over the row's own power of two
     float slope2;
     int pos, lim;    // the row sees keys 0 .. lim - 1
@@ -236,7 +252,8 @@ template <int HD, class TQ, class TP, int QT> struct Rows {
 #pragma unroll
         for (int i = 0; i < DB; i++) o[i] = f32x16{};
         m = M_NONE;
-        l = 0.f;
+        lo = l = 0.f;
+        far = 0;
     }
 
     // S^T of the 64 keys whose rows sk holds.
@@ -254,12 +271,12 @@ template <int HD, class TQ, class TP, int QT> struct Rows {
             }
     }
 
-    // From the products to scores t = c s (c is returned), their offset m raised
+    // From the products to weights exp2(c s + nm) (c is returned), the offset raised
     // where one asks for it.  The 32 NS keys are those from position j0 on; kscale: one
     // scale for the tile, or (PER_KEY) sks[key]; cut: keys from `seen` on are not seen.
     template <bool PER_KEY, int NS>
     __device__ __forceinline__ float scores(f32x16 (&s)[NS], const Score &sc, float kscale, const float *sks, int j0,
-                                            bool cut, int seen) {
+                                            bool cut, int seen, float &nm) {
         const int hf = (threadIdx.x >> 5) & 1;
         if constexpr (PER_KEY) {
 #pragma unroll
@@ -315,22 +332,36 @@ template <int HD, class TQ, class TP, int QT> struct Rows {
         float mt = fmaxf(s[0][0], s[NS - 1][15]);
 #pragma unroll
         for (int i = 1; i < 16 * NS - 1; i += 2) mt = fmaxf(fmaxf(mt, s[i >> 4][i & 15]), s[(i + 1) >> 4][(i + 1) & 15]);
-        mt *= c;
-        if (__ballot(mt > m + RAISE)) {  // wave-uniform
-            mt = max32(mt);
-            const float now = mt > m + RAISE ? mt - OFFSET : m;
-            const float keep = __builtin_amdgcn_exp2f(m - now);
-            m = now;
-            l *= keep;
+        nm = -m;
+        const uint64_t up = __ballot(fmaf(mt, c, -m) - lo > RAISE);
+        if (up | far) {  // wave-uniform
+            if (up) {
+                mt = max32(mt);
+                const float t = mt * c, off = fmaf(mt, c, -t) - OFFSET;
+                const bool raise = fmaf(mt, c, -m) - lo > RAISE, two = fabsf(t) >= FAR;
+                const float now = two ? t : t - OFFSET, rest = two ? off : 0.f;
+                const float keep = raise ? __builtin_amdgcn_exp2f((m - now) + (lo - rest)) : 1.f;
+                m = raise ? now : m;
+                lo = raise ? rest : lo;
+                nm = -m;
+                far = __ballot(fabsf(m) >= FAR && m != M_NONE);
+                l *= keep;
 #pragma unroll
-            for (int i = 0; i < DB; i++) o[i] *= keep;
+                for (int i = 0; i < DB; i++) o[i] *= keep;
+            }
+            if (far) {
+#pragma unroll
+                for (int st = 0; st < NS; st++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++) s[st][v] = fmaf(s[st][v], c, -m) - lo;
+                c = 1.f, nm = 0.f;
+            }
         }
         return c;
     }
 
-    // The weights exp2(t - m) as the second product's operand, and their sum.
-    __device__ __forceinline__ void weights(const f32x16 (&s)[2], float c, p8 (&pf)[QT][4]) {
-        const float nm = -m;
+    // The weights exp2(c s + nm) as the second product's operand, and their sum.
+    __device__ __forceinline__ void weights(const f32x16 (&s)[2], float c, float nm, p8 (&pf)[QT][4]) {
         float sum[2] = {};
 #pragma unroll
         for (int tt = 0; tt < 4; tt++) {

@@ -1,0 +1,90 @@
+"""fh3_hip_attention_seqs_dev at the ends of the operands' ranges: scores of any
+size, values near the type's largest and least, scales near fp32's least, keys
+that are infinite.  The oracle is the 64-bit plain form; scores are built so that
+both compute them exactly, or so that one key wins by far."""
+import numpy as np
+import pytest
+
+import seqs_ref as R
+from seqs_ref import BF16, F16, F32
+from test_gpu_seqs import _case, _offsets, _run
+
+pytestmark = pytest.mark.gpu
+
+
+def _near(got, want, t, what, tol=None):
+    """Relative Frobenius error within the type's (seqs_ref.FRO), nothing that is not finite."""
+    got = R.from_type(got, t)
+    big = np.abs(want).max()
+    got, want = got / big, want / big      # (squares of the largest values would overflow)
+    fro = float(np.linalg.norm(got - want) / np.linalg.norm(want))
+    print("%s %s: rel_fro %.2e" % (what, R.NAMES[t], fro), flush=True)
+    assert np.isfinite(got).all(), what
+    assert fro <= (R.FRO[t] if tol is None else tol), (what, fro)
+
+
+def exact_scores(seed, t, n, heads, kv, hd):
+    """q, k, v whose products are +-2^30 + 128 n_j, exact in every type and in fp32 sums, n_j from 0 to 20."""
+    rng = np.random.default_rng(seed)
+    q, k = np.zeros((n, heads, hd)), np.zeros((n, kv, hd))
+    q[:, :, 0] = np.where(np.arange(heads) % 2, -2.0 ** 15, 2.0 ** 15)
+    q[:, :, hd - 1] = 128
+    k[:, :, 0] = 2.0 ** 15
+    k[:, :, hd - 1] = rng.integers(0, 21, (n, kv))
+    v = rng.standard_normal((n, kv * hd))
+    return [R.to_type(x.reshape(n, -1), t) for x in (q, k, v)]
+
+
+# at 2^-7 neighbouring scores differ by 1 at 8 10^6; at 2^90 all are beyond 10^36
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("scale", [2.0 ** e for e in (-14, -7, -5, -4, -3, 0, 20, 40, 69, 90)])
+def test_scores_of_any_size(gpu, t, hd, scale):
+    heads, kv, lens = 4, 2, [300, 37]
+    first = _offsets(lens)
+    arrays = exact_scores(3, t, first[-1], heads, kv, hd)
+    for causal in (True, False):
+        got = _run(gpu, arrays, t, first, heads, kv, hd, scale=scale, causal=causal)
+        o, _, _ = R.attention(*(R.from_type(x, t) for x in arrays), first, heads, kv, hd, causal, scale)
+        _near(got, o, t, "scale %g causal %s" % (scale, causal))
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("size", [5e3, 1e4, 1.5e4, 3e4])
+def test_large_operands(gpu, t, size):
+    """Scores of 10^8 to 10^10, whose fp32 sums are off by more than 1: only that each row is a mean of what it sees can be said."""
+    heads, kv, hd, n = 4, 1, 128, 200
+    rng = np.random.default_rng(4)
+    q, k = (np.clip(rng.standard_normal((n, w * hd)) * size, -6e4, 6e4) for w in (heads, kv))
+    arrays = [R.to_type(x, t) for x in (q, k, np.ones((n, kv * hd)))]
+    got = R.from_type(_run(gpu, arrays, t, [0, n], heads, kv, hd), t)
+    assert np.isfinite(got).all()
+    # weights and their sum: half a step each (F32: two terms of the weights, 2^-21; sums of up to 200)
+    assert np.abs(got - 1).max() <= (2.0 ** -20 if t == F32 else 2 * R.UNIT[t])
+    arrays[2] = R.to_type(rng.standard_normal((n, kv * hd)), t)
+    got = R.from_type(_run(gpu, arrays, t, [0, n], heads, kv, hd), t)
+    v = R.from_type(arrays[2], t)
+    assert np.isfinite(got).all() and np.abs(got[0].reshape(heads, hd) - v[0]).max() <= 2 * R.UNIT[t] * np.abs(v[0]).max() + 2.0 ** -20
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("slope", [1e8, -1e8, 1e30, -1e30])
+def test_distance_bias_of_any_size(gpu, t, slope):
+    """The nearest token wins, or the farthest, by far."""
+    heads, kv, hd, lens = 2, 1, 64, [150, 40]
+    first = _offsets(lens)
+    arrays = _case(6, t, first[-1], heads, kv, hd)
+    slopes = np.asarray([slope, slope / 3], np.float32)
+    got = _run(gpu, arrays, t, first, heads, kv, hd, None, slopes)
+    o, _, _ = R.attention(*(R.from_type(x, t) for x in arrays), first, heads, kv, hd, True, None, 0.0, slopes)
+    _near(got, o, t, "slope %g" % slope)
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+def test_capped_scores_far_below_zero(gpu, t):
+    """Every score is -10^30, the cap: the mean of what is seen."""
+    heads, kv, hd, n = 2, 1, 64, 100
+    arrays = exact_scores(7, t, n, heads, kv, hd)
+    got = _run(gpu, arrays, t, [0, n], heads, kv, hd, scale=2.0 ** 75, softcap=1e30)
+    o, _, _ = R.attention(*(R.from_type(x, t) for x in arrays), [0, n], heads, kv, hd, True, 2.0 ** 75, 1e30)
+    _near(got, o, t, "cap")
