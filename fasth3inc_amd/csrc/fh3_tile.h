@@ -288,7 +288,7 @@ template <int HD, class TQ, class TP, int QT> struct Rows {
                     for (int v = 0; v < 4; v++) s[st][4 * g + v] *= ks[v];
                 }
         }
-        float c = f * kscale;  // t = c s, unless there is more to do
+        float c = factor(f * kscale);  // t = c s, unless there is more to do
         // (two loops and two branches: in one loop both would be computed and selected)
         if (sc.cap2) {
             if (sc.fine) {

@@ -46,3 +46,17 @@ def test_scores_of_any_size(gpu, t, hd, scale):
         q[:, :, 0] = np.where(np.arange(heads) % 2, -2.0 ** 15, 2.0 ** 15)
         q[:, :, hd - 1] = 0.25
         _against(h, t, R.to_type(q.reshape(2 * new, -1), t), first, heads, "scale %g, %d new" % (scale, new), scale=scale)
+
+
+@pytest.mark.parametrize("new", NEW)
+def test_pages_of_zeros_and_small_queries(gpu, new):
+    """Pages whose K is 0 have the least scale, 2^-100; times that of a small q it is below fp32's least number.  All
+    scores are 0: the mean of what is seen."""
+    heads, kv, hd, lens = 4, 2, 128, [200, 70]
+    h = Held(gpu, kv, hd, lens, 36)
+    h.model.q[:, :, 0] = 0
+    h.model.scale[:, :, 0] = 2.0 ** -100
+    _put(h)
+    for size in (1.0, 1e-8, 1e-13, 1e-25):
+        first = _offsets([new, new])
+        _against(h, F32, _rows(37, F32, 2 * new, heads * hd, size), first, heads, "q %g, %d new" % (size, new))

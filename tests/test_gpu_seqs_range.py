@@ -88,3 +88,15 @@ def test_capped_scores_far_below_zero(gpu, t):
     got = _run(gpu, arrays, t, [0, n], heads, kv, hd, scale=2.0 ** 75, softcap=1e30)
     o, _, _ = R.attention(*(R.from_type(x, t) for x in arrays), [0, n], heads, kv, hd, True, 2.0 ** 75, 1e30)
     _near(got, o, t, "cap")
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("scale", [1e-30, 1e-40, 1e-44])
+def test_scales_near_the_least(gpu, t, scale):
+    """All scores are 0 to within fp32: the mean of what is seen."""
+    heads, kv, hd, lens = 4, 2, 128, [100, 9]
+    first = _offsets(lens)
+    arrays = _case(8, t, first[-1], heads, kv, hd)
+    got = _run(gpu, arrays, t, first, heads, kv, hd, scale=scale)
+    o, _, _ = R.attention(*(R.from_type(x, t) for x in arrays), first, heads, kv, hd, True, scale)
+    _near(got, o, t, "scale %g" % scale)
