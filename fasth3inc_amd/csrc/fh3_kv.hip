@@ -306,6 +306,11 @@ __host__ __device__ constexpr int64_t parts_bytes(int hd, int rows, int kv_heads
     return (int64_t)kv_heads * wgs * (2 * rows * (hd + 3) * (int)sizeof(float) + (int)sizeof(Begun));
 }
 
+// Weighted sums of V, V's page scale (2^-100 to 2^121) in them, are held times DOWN: 2^17
+// keys of the largest value with weights of 2^14 each (2^25 with 2^6) stay below fp32's
+// largest number, and the least scale times 2^6 is still fp32's least normal one.
+constexpr float DOWN = 0x1p-32f, BACK = 0x1p32f;
+
 __device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
@@ -327,6 +332,7 @@ __device__ __forceinline__ half8 to_half(uint32_t a, uint32_t b) {
 // in 94 us and 102 with the join (5.0 TB/s; a device copy moves 4.8), 140 MB in 31
 // and 39.  One token of one sequence takes 8 us, launch and latencies.
 constexpr int FEW_W = 4;
+constexpr float OFFSET = Vec<_Float16>::OFFSET, RAISE = Vec<_Float16>::RAISE;
 template <int HD, int R, int NT>
 __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, const void *__restrict__ q, int64_t ldq,
                                                           void *__restrict__ o, int64_t ldo, Fh3kSeqs s, KvWork work,
@@ -428,7 +434,7 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
                 for (int i = 0; i < DT; i++) vr[i] = b[64 * (4 * KU + i)];
                 const bool there = __builtin_amdgcn_readlane(ids, n & 63) >= 0;
                 const float ks = lane_value(scs[0], n);
-                const float vs = lane_value(scs[1], n);
+                const float vs = lane_value(scs[1], n) * DOWN;
                 const int j0 = (page0 + wave + FEW_W * n) * KV_PAGE;
                 f32x4 t[R][4] = {};
 #pragma unroll
@@ -577,7 +583,7 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
                     const float inv = sum == 0.f ? 0.f : 1.f / sum;
                     const int tok = (r0 + row) / G, head = kvh * G + (r0 + row) % G;
 #pragma unroll
-                    for (int v = 0; v < 4; v++) x[v] *= inv;
+                    for (int v = 0; v < 4; v++) x[v] = x[v] * inv * BACK;
                     store4(o, a.type, (int64_t)(first + tok) * ldo + head * HD + d, x);
                 }
             }
@@ -636,7 +642,7 @@ __global__ __launch_bounds__(256) void k_kv_join(Fh3kAttn a, Fh3kKv c, void *__r
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const int tok = (b.r0 + row) / G, head = kvh * G + (b.r0 + row) % G;
 #pragma unroll
-    for (int v = 0; v < 4; v++) x[v] *= inv;
+    for (int v = 0; v < 4; v++) x[v] = x[v] * inv * BACK;
     store4(o, a.type, (int64_t)(b.first + tok) * ldo + head * HD + d, x);
 }
 
@@ -804,7 +810,7 @@ __global__ __launch_bounds__(64 * MANY_W, 2) void k_kv_many(Fh3kAttn a, Fh3kKv c
                 *parts.begun(kvh, wg) = {run.ends(pages, work.wgs), first, r0, rows};
             if (row < rows) {
                 float *part = done ? nullptr : parts.of(kvh, wg, page0 == 0);
-                const float inv = done ? (l == 0.f ? 0.f : ref / l) : ref;
+                const float inv = done ? (l == 0.f ? 0.f : 1.f / l) : 1.f, unit = done ? ref : ref * DOWN;
                 const int64_t at_o = (int64_t)(first + tok) * ldo + head * HD;
                 const int r = WAVE_R * wave + l32;
                 if (!done && hf == 0) part[ROWS * HD + r] = l, part[ROWS * (HD + 1) + r] = w.m, part[ROWS * (HD + 2) + r] = w.lo;
@@ -815,7 +821,7 @@ __global__ __launch_bounds__(64 * MANY_W, 2) void k_kv_many(Fh3kAttn a, Fh3kKv c
                         const int d = 32 * db + 8 * g + 4 * hf;
                         f32x4 x;
 #pragma unroll
-                        for (int i = 0; i < 4; i++) x[i] = w.o[db][4 * g + i] * inv;
+                        for (int i = 0; i < 4; i++) x[i] = w.o[db][4 * g + i] * inv * unit;
                         if (done) store4(o, a.type, at_o + d, x);
                         else *(f32x4 *)(part + r * HD + d) = x;
                     }

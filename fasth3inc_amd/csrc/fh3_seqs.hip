@@ -135,7 +135,7 @@ __device__ __forceinline__ void lose(R &w, const SeqsArgs &g, const Place &p, in
 template <int HD, int TYPE, class R>
 __device__ __forceinline__ void put_rows(const R &w, const SeqsArgs &g, const Place &p, int row, int head, float unit) {
     const int hf = (threadIdx.x >> 5) & 1;
-    const float l = sum32(w.l), inv = l == 0.f ? 0.f : unit / l;
+    const float l = sum32(w.l), inv = l == 0.f ? 0.f : 1.f / l;
     if (row >= p.rows) return;
     const int64_t at = (int64_t)(p.first + w.pos) * g.ldo + head * HD + 4 * hf;
 #pragma unroll
@@ -144,7 +144,7 @@ __device__ __forceinline__ void put_rows(const R &w, const SeqsArgs &g, const Pl
         for (int c = 0; c < 4; c++) {
             f32x4 x;
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = w.o[db][4 * c + i] * inv;
+            for (int i = 0; i < 4; i++) x[i] = w.o[db][4 * c + i] * inv * unit;  // (unit / l could leave fp32's range)
             store4(g.o, TYPE, at + 32 * db + 8 * c, x);
         }
 }

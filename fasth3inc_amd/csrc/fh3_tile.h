@@ -16,16 +16,18 @@ namespace {
 
 constexpr int TILE_K = 64;   // keys per tile
 constexpr int WAVE_R = 32;   // rows per wavefront
-// Weights are exp2(t - m) where m is raised only when a tile's largest t exceeds
-// it by more than RAISE: the weights stay within 2^-OFFSET .. 2^RAISE of what a
-// fresh maximum would give, and most tiles need no rescale of the sums.  The
-// offset keeps small weights out of fp16's subnormal range (2^14 < 65504).
-// From |t| = FAR on, m alone could not stand 6 below the largest t (half a step of fp32
+// Weights are exp2(t - m) where m is raised, to OFFSET below a tile's largest t, only when
+// that exceeds it by more than RAISE: the largest weight is from 2^OFFSET to 2^RAISE
+// and most tiles need no rescale of the sums.  In fp16 6 and 14 keep small weights out of
+// the subnormal range (2^14 < 65504).  bf16 weights have fp32's range, and so has V
+// then: with -18 and -10 the sums of 1024 keys stay below V's largest (at 2^14 those
+// of 10^34 passed it), and V's least normal numbers times 2^-18 are still held.
+// From |t| = FAR on, m alone could not stand OFFSET below the largest t (half a step of fp32
 // is 8 and more from 2^27), nor is t = c s itself exact enough: there m is the rounded largest
 // t and a second term lo what the exact product is off it by, and the weights' arguments
 // (c s - m) - lo are small numbers made by one multiply-add from the products s.  Below, lo
 // is 0 and arguments are c s - m.
-constexpr float OFFSET = 6.f, RAISE = 14.f, FAR = 0x1p20f;
+constexpr float FAR = 0x1p20f;
 constexpr float M_NONE = -3.402823466e38f;  // no key seen yet: finite, so that masked t = -inf gives 0
 // Parts of a row with offsets (m, lo) and (m2, lo2): what the larger offset leaves of each; m, lo become the larger.
 __device__ __forceinline__ void join_offsets(float &m, float &lo, float m2, float lo2, float &keep, float &add) {
@@ -38,6 +40,7 @@ __device__ __forceinline__ void join_offsets(float &m, float &lo, float m2, floa
 template <class T> struct Vec;
 template <> struct Vec<_Float16> {
     typedef half8 v8;
+    static constexpr float OFFSET = 6.f, RAISE = 14.f;
     static __device__ __forceinline__ uint32_t pair(float a, float b) {
         uint32_t w = __builtin_bit_cast(uint32_t, half2v{(_Float16)a, (_Float16)b});
         asm("" : "+v"(w));  // one pair, not converted once for each use
@@ -49,6 +52,7 @@ template <> struct Vec<_Float16> {
 };
 template <> struct Vec<__bf16> {
     typedef bf8 v8;
+    static constexpr float OFFSET = -18.f, RAISE = -10.f;
     static __device__ __forceinline__ uint32_t pair(float a, float b) {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf2));
     }
@@ -199,6 +203,7 @@ __device__ __forceinline__ float sum16(float x) {
 template <int HD, class TQ, class TP, int QT> struct Rows {
     static constexpr int KS = HD / 16, DB = HD / 32;
     static constexpr int KROW = HD + 8;  // LDS row of K
+    static constexpr float OFFSET = Vec<TP>::OFFSET, RAISE = Vec<TP>::RAISE;
     typedef typename Vec<TQ>::v8 q8;
     typedef typename Vec<TP>::v8 p8;
 

@@ -48,6 +48,24 @@ def test_scores_of_any_size(gpu, t, hd, scale):
         _against(h, t, R.to_type(q.reshape(2 * new, -1), t), first, heads, "scale %g, %d new" % (scale, new), scale=scale)
 
 
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("kind", ["large", "mixed", "small"])
+def test_values_near_the_ends(gpu, t, kind):
+    """V of up to 127 2^121, of 2^-100 at the least, and pages of either kind beside each other."""
+    heads, kv, hd, lens = 4, 2, 64, [3000, 70]
+    h = Held(gpu, kv, hd, lens, 33)
+    rng = np.random.default_rng(34)
+    e = {"large": np.full((h.model.pages, kv), 121), "small": np.full((h.model.pages, kv), -100),
+         "mixed": rng.choice([121, 119, 0, -100], (h.model.pages, kv))}[kind]
+    h.model.scale[:, :, 0] = 2.0 ** -6
+    h.model.scale[:, :, 1] = 2.0 ** e
+    h.model.q[:, :, 1] = rng.integers(40, 128, h.model.q[:, :, 1].shape)
+    _put(h)
+    for new in NEW:
+        first = _offsets([new, new])
+        _against(h, t, _rows(35, t, 2 * new, heads * hd, 0.5), first, heads, "%s, %d new" % (kind, new))
+
+
 @pytest.mark.parametrize("new", NEW)
 def test_pages_of_zeros_and_small_queries(gpu, new):
     """Pages whose K is 0 have the least scale, 2^-100; times that of a small q it is below fp32's least number.  All

@@ -100,3 +100,18 @@ def test_scales_near_the_least(gpu, t, scale):
     got = _run(gpu, arrays, t, first, heads, kv, hd, scale=scale)
     o, _, _ = R.attention(*(R.from_type(x, t) for x in arrays), first, heads, kv, hd, True, scale)
     _near(got, o, t, "scale %g" % scale)
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("size,n", [(3.3e38, 1000), (1e36, 3000), (1e-30, 300), (1e-34, 3000)])
+def test_values_near_the_ends(gpu, t, hd, size, n):
+    """V next to the type's largest and least normal values; the outputs are its means."""
+    heads, kv = 4, 2
+    q, k, _ = _case(9, t, n, heads, kv, hd)
+    rng = np.random.default_rng(10)
+    v = R.to_type(rng.uniform(0.5, 1.0, (n, kv * hd)) * np.where(rng.random((n, kv * hd)) < 0.25, -1, 1) * size, t)
+    assert np.isfinite(R.from_type(v, t)).all()
+    got = _run(gpu, (q, k, v), t, [0, n], heads, kv, hd)
+    o, _, _ = R.attention(*(R.from_type(x, t) for x in (q, k, v)), [0, n], heads, kv, hd)
+    _near(got, o, t, "v %g" % size)
