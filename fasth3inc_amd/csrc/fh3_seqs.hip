@@ -397,11 +397,11 @@ __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
             r[i] = *(const u32x4 *)(base + (uint32_t)((uint32_t)key * (uint32_t)ld + d0));
         }
     };
-    // 0 where each row of a piece has a value of 2^-5 at least and none of `limit` or more.
     auto largest = [&](const u32x4 &r) {
         const f32x4 x = __builtin_bit_cast(f32x4, r);
         return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
     };
+    // 0 where each row of a piece has a value of 2^-5 at least and none of `limit` or more.
     auto rows_odd = [&](float top, float limit) {
         uint64_t some = __ballot(top >= 0.03125f);  // any lane of a row
 #pragma unroll
@@ -409,19 +409,21 @@ __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
         constexpr uint64_t FIRST = CPR == 32 ? 0x0000000100000001ull : 0x0001000100010001ull;
         return (~some & FIRST) | __ballot(!(top < limit));
     };
-    // Powers of two for this thread's pieces of K: 1 for such rows (fp16's second term
-    // then reaches down to 2^-25, 2^-20 of the row's largest); otherwise the row's
-    // largest gives it.
+    // Powers of two for this thread's pieces of K: 64 for rows from 2^-5 to 512 (the
+    // largest comes to 2 at least, and the second term's rounding, 2^-25, is 2^-26 of
+    // that; with 1 in place of 64 rows of about 0.03 were 2^-20 off, and outputs 1.5e-6);
+    // otherwise the row's largest gives it.
+    constexpr float K_UP = 64.f;
     auto scales = [&](const u32x4 (&r)[CH], float (&up)[CH]) {
         float top[CH];
         uint64_t other = 0;
 #pragma unroll
-        for (int i = 0; i < CH; i++) top[i] = largest(r[i]), up[i] = 1.f, other |= rows_odd(top[i], 32768.f);
+        for (int i = 0; i < CH; i++) top[i] = largest(r[i]), up[i] = K_UP, other |= rows_odd(top[i], 512.f);
         if (other) {
 #pragma unroll
             for (int i = 0; i < CH; i++) {
                 const float m = row_max<CPR>(top[i]);  // each row for itself
-                up[i] = m >= 0.03125f && m < 32768.f ? 1.f : pow2_to_14(m);
+                up[i] = m >= 0.03125f && m < 512.f ? K_UP : pow2_to_14(m);
             }
         }
     };
