@@ -488,7 +488,10 @@ __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
     const int tok = rc / p.G, head = p.kvh * p.G + rc % p.G;
     const Score sc = score_of(g.a);
     R w;
-    w.template load_q<true>(g.q, Op::TYPE, (int64_t)(p.first + tok) * g.ldq + head * HD, sc);
+    // (q's largest to 2^2 .. 2^3, not 2^13: its products with K at its own size, 2^10 times that
+    // at most, stay in fp32's range for K up to 2^117; the second term's rounding, 2^-25, is
+    // 2^-27 of the largest)
+    w.template load_q<true>(g.q, Op::TYPE, (int64_t)(p.first + tok) * g.ldq + head * HD, sc, 0x1p-11f);
     w.clear();
     w.pos = tok;
     w.lim = p.limit(tok);

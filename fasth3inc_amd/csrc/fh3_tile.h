@@ -216,8 +216,9 @@ template <int HD, class TQ, class TP, int QT> struct Rows {
     int pos, lim;    // the row sees keys 0 .. lim - 1
 
     // q's fragments: lane holds row lane & 31, channels 16 kk + 8 (lane >> 5) ..
-    // SCALED: by the row's power of two (fp32 or the cache's fp16 products)
-    template <bool SCALED> __device__ __forceinline__ void load_q(const void *qp, int type, int64_t at, const Score &sc) {
+    // SCALED: by the row's power of two (fp32 or the cache's fp16 products), its largest to [2^13, 2^14) times `less`
+    template <bool SCALED>
+    __device__ __forceinline__ void load_q(const void *qp, int type, int64_t at, const Score &sc, float less = 1.f) {
         const int hf = (threadIdx.x >> 5) & 1;
         f = sc.f;
         if constexpr (!SCALED) {
@@ -232,7 +233,7 @@ template <int HD, class TQ, class TP, int QT> struct Rows {
                 for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[kk][i]));
             }
             top = max32(top);
-            const float up = pow2_to_14(top);
+            const float up = pow2_to_14(top) * less;
             f = sc.f / up;
 #pragma unroll
             for (int kk = 0; kk < KS; kk++) {

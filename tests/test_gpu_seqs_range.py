@@ -115,3 +115,15 @@ def test_values_near_the_ends(gpu, t, hd, size, n):
     got = _run(gpu, (q, k, v), t, [0, n], heads, kv, hd)
     o, _, _ = R.attention(*(R.from_type(x, t) for x in (q, k, v)), [0, n], heads, kv, hd)
     _near(got, o, t, "v %g" % size)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("qs,ks", [(1e-32, 1e32), (1e-33, 2e34), (1e36, 1e-36), (1e-20, 1e34)])
+def test_keys_near_the_ends(gpu, hd, qs, ks):
+    """fp32 q and k at the two ends of the range, products of ordinary size (the last: of 10^14, one key wins)."""
+    heads, kv, n = 4, 2, 300
+    rng = np.random.default_rng(11)
+    arrays = [(rng.standard_normal((n, w * hd)) * s).astype(np.float32) for w, s in ((heads, qs), (kv, ks), (kv, 1.0))]
+    got = _run(gpu, arrays, F32, [0, n], heads, kv, hd)
+    o, _, _ = R.attention(*(x.astype(np.float64) for x in arrays), [0, n], heads, kv, hd)
+    _near(got, o, F32, "q %g k %g" % (qs, ks))
