@@ -207,7 +207,10 @@ int fh3_hip_vsa_attention_qkv_dev(const Fh3VsaCfg *c, const float *d_qkv, const 
  * fp16 terms each after a power of two for each row (relative error about 4e-7;
  * beside a value of v of size V nothing below 2^-30 V counts); softmax and sums
  * are fp32, the weights are rounded to the operand type for the second product
- * (F32: two terms).  Deterministic. */
+ * (F32: two terms).  Deterministic.
+ * Operands may be of any finite size.  What passes fp32's range counts as infinite:
+ * scores and biases (also before the other is added), products with F32 keys of
+ * 2^118 and more, sums of BF16 values above 2^128 * 1024 / keys. */
 typedef struct Fh3AttnCfg {
     int heads;
     int kv_heads;
@@ -227,11 +230,14 @@ typedef struct Fh3AttnCfg {
  * last sequence are neither read nor written.  d_prefix (NULL, or device
  * [n_seq]): the first d_prefix[s] tokens are seen by every row of sequence s,
  * causal or not.  Pointers and row starts 16-byte aligned; o must not overlap
- * the inputs.  A NaN or infinity in a key or value makes the rows that see it
- * non-finite (at the least in the channels that hold it) and no other row.  No
- * workspace: calls on different streams do not disturb each other.  n_tok at most
- * 2^24, n_seq 2^20, n_tok * heads 2^30, n_tok * heads / 128 + n_seq * kv_heads
- * below 2^23; larger calls are refused. */
+ * the inputs.  A NaN in a key, and in F32 keys an infinity, makes the rows that see
+ * it NaN; in F16 and BF16 keys an infinity gives infinite scores: +infinity makes
+ * the row NaN, -infinity leaves the key out, and a softcap takes them to +-softcap.
+ * A NaN or infinity in a value makes the rows that see it non-finite, at the least
+ * in the channels that hold it.  No other row changes.  No workspace: calls on
+ * different streams do not disturb each other.  n_tok at most 2^24, n_seq 2^20,
+ * n_tok * heads 2^30, n_tok * heads / 128 + n_seq * kv_heads below 2^23; larger
+ * calls are refused. */
 int fh3_hip_attention_seqs_dev(const Fh3AttnCfg *c, const void *d_q, int64_t ldq, const void *d_k, int64_t ldk,
                                const void *d_v, int64_t ldv, void *d_o, int64_t ldo, int n_tok, int n_seq,
                                const int *d_first, const int *d_prefix, void *stream);
@@ -302,7 +308,9 @@ int fh3_hip_kv_read_dev(const Fh3KvCache *kv, int type, void *d_k, int64_t ldk, 
  * positions up to its own; otherwise all d_len[s].  The cached integers are exact in
  * the fp16 matrix products; q is scaled by a power of two for each row and
  * rounded to fp16 (F16 and BF16: exact but for values 2^-24 below the row's
- * largest; F32: two terms), the weights too (F32: two terms).  The work is split
+ * largest; F32: two terms), the weights too (F32: two terms).  Scales of V up to
+ * 2^121 add up for 2^17 tokens at least, and beside a page of scale S that a row
+ * sees values below 2^-120 S may count as 0.  The work is split
  * over the keys by the lengths on the device; d_ws (16-byte aligned,
  * fh3_hip_kv_attention_workspace_bytes, may be 0) holds the parts until a
  * second kernel joins them in order: deterministic.  Calls that may overlap need

@@ -127,3 +127,39 @@ def test_keys_near_the_ends(gpu, hd, qs, ks):
     got = _run(gpu, arrays, F32, [0, n], heads, kv, hd)
     o, _, _ = R.attention(*(x.astype(np.float64) for x in arrays), [0, n], heads, kv, hd)
     _near(got, o, F32, "q %g k %g" % (qs, ks))
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("cap", [0.0, 30.0, 1e4])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf])
+def test_infinite_keys(gpu, t, cap, bad):
+    """A key with an infinite channel.  F16 and BF16: its score is infinite as the sign of q says: +inf makes the row
+    NaN, -inf leaves the key out, and a cap takes either to +-cap.  F32: the row is NaN."""
+    heads, kv, hd, n, at, ch = 4, 2, 64, 150, 70, 21
+    arrays = _case(12, t, n, heads, kv, hd)
+    arrays[1][at, hd + ch] = R.to_type(np.full(1, bad), t)[0]
+    got = R.from_type(_run(gpu, arrays, t, [0, n], heads, kv, hd, softcap=cap), t).reshape(n, heads, hd)
+    q, k, v = (R.from_type(x, t) for x in arrays)
+    k0 = k.copy()
+    k0[at, hd + ch] = 0
+    o, _, _ = R.attention(q, k0, v, [0, n], heads, kv, hd, True, None, cap)
+    o = o.reshape(n, heads, hd)
+    _near(R.to_type(got[:at], t), o[:at], t, "before")
+    _near(R.to_type(got[:, :2], t), o[:, :2], t, "the other key head")
+    lost = 0
+    for h in (2, 3):
+        sign = np.sign(q[:, h * hd + ch]) * np.sign(bad)
+        for r in range(at, n):
+            if t == F32 or (not cap and sign[r] > 0):
+                assert np.isnan(got[r, h]).all(), (r, h)
+                lost += 1
+                continue
+            s = (k0[:r + 1, hd:] @ q[r, h * hd:(h + 1) * hd]) / np.sqrt(hd)
+            s = cap * np.tanh(s / cap) if cap else s
+            s[at] = sign[r] * cap if cap else -np.inf
+            w = np.exp(s - s.max())
+            want = w @ v[:r + 1, hd:] / w.sum()
+            # half a step of the weights and one of the output, of the weighted |v|
+            lim = 3 * R.UNIT[t] * (w @ np.abs(v[:r + 1, hd:]) / w.sum()) + 1e-5
+            assert (np.abs(got[r, h] - want) <= lim).all(), (r, h)
+    assert lost == (2 * (n - at) if t == F32 else 0 if cap else lost) and (cap or 0 < lost)
