@@ -78,3 +78,63 @@ def test_pages_of_zeros_and_small_queries(gpu, new):
     for size in (1.0, 1e-8, 1e-13, 1e-25):
         first = _offsets([new, new])
         _against(h, F32, _rows(37, F32, 2 * new, heads * hd, size), first, heads, "q %g, %d new" % (size, new))
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("new", [1, 40])
+def test_runs_of_hundreds_of_pages(gpu, t, new):
+    """256 key heads: two workgroups to a head, runs of 310 pages each, so that page numbers and scales are fetched
+    64 at a time more than once.  The table repeats seven pages in no order."""
+    F, kv, hd, pages, n_pages = gpu, 256, 64, 7, 620
+    rng = np.random.default_rng(41)
+    table = rng.integers(0, pages, (1, n_pages))
+    length = n_pages * R.PAGE - 5
+    h = Held(F, kv, hd, [length], 42, pages=pages, table=table, max_pages=n_pages)
+    first = [0, new]
+    q = _rows(43, t, new, kv * hd, 0.5)
+    got = R.from_type(h.attend(t, q, first, kv), t).reshape(new, kv, hd)
+    m, qv = h.model, R.from_type(q, t).reshape(new, kv, hd)
+    pos = length - new + np.arange(new)
+    see = np.arange(length)[None, :] <= pos[:, None]
+    for head in (0, 1, 100, 255):
+        k, v = ((m.q[table[0], head, w] * m.scale[table[0], head, w][:, None, None]).reshape(-1, hd)[:length] for w in (0, 1))
+        o, _, _ = R.head_outputs(qv[:, head], k, v, pos, 1 / np.sqrt(hd), 0.0, None, see)
+        _near(R.to_type(got[:, head], t), o, t, "head %d, %d new" % (head, new))
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_many_long_sequences(gpu, t):
+    """100 sequences of 1 to 1500 tokens, one new token each: divided tiles behind the first 64 sequences."""
+    kv, hd, heads, n = 2, 64, 4, 100
+    lens = [int(x) for x in np.random.default_rng(44).integers(1, 1500, n)]
+    lens[70], lens[99] = 1500, 1400
+    h = Held(gpu, kv, hd, lens, 45)
+    _against(h, t, _rows(46, t, n, heads * hd), list(range(n + 1)), heads, "100 sequences")
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("singles", [30, 150])
+def test_a_chunk_beside_single_tokens(gpu, t, singles):
+    """One sequence's chunk in a call with single tokens of others: 128-row tiles for all, or 32-row ones."""
+    kv, hd, heads = 2, 64, 16
+    rng = np.random.default_rng(47)
+    new = [1] * (singles // 2) + [300] + [1] * (singles - singles // 2)
+    lens = [int(x) for x in rng.integers(1, 700, len(new))]
+    lens[singles // 2] = 900
+    h = Held(gpu, kv, hd, lens, 48)
+    first = _offsets(new)
+    _against(h, t, _rows(49, t, first[-1], heads * hd), first, heads, "chunk and %d tokens" % singles)
+
+
+def test_read_back_between_each_other(gpu):
+    """K and V read to the two halves of one buffer's rows."""
+    F, kv, hd, lens = gpu, 2, 64, [70, 3]
+    h = Held(F, kv, hd, lens, 50)
+    first = _offsets(lens)
+    want = h.model.read(first, lens)
+    w = kv * hd
+    out, df = F.DeviceBuffer(first[-1] * 2 * w * 4), F.DeviceBuffer.from_array(np.asarray(first, np.int32))
+    F.kv_read_dev(h.kv, F32, out.ptr, out.ptr + w * 4, first[-1], 2, df, ldk=2 * w, ldv=2 * w)
+    F.synchronize()
+    got = out.download(np.float32, (first[-1], 2, w))
+    assert np.array_equal(got[:, 0], want[0]) and np.array_equal(got[:, 1], want[1])
