@@ -518,10 +518,15 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
                             const int i = 8 * u + 2 * e;
                             const float p0 = __builtin_amdgcn_exp2f(fmaf(t[r][i >> 2][i & 3], x, nm));
                             const float p1 = __builtin_amdgcn_exp2f(fmaf(t[r][i >> 2][(i & 3) + 1], x, nm));
-                            uint32_t hi, lo;
-                            split2(p0, p1, 1.f, hi, lo, _Float16());
-                            h[e] = hi, l4[e] = lo;
-                            sum += p0 + p1;
+                            if constexpr (NT == 2) {
+                                uint32_t hi, lo;
+                                split2(p0, p1, 1.f, hi, lo, _Float16());
+                                h[e] = hi, l4[e] = lo;
+                                sum += p0 + p1;
+                            } else {  // the sum is of the rounded weights, which the product takes
+                                h[e] = Vec<_Float16>::pair(p0, p1);
+                                sum = Vec<_Float16>::sum(h[e], sum);
+                            }
                         }
                         pf[r][0][u] = __builtin_bit_cast(half8, h);
                         if constexpr (NT == 2) pf[r][NT - 1][u] = __builtin_bit_cast(half8, l4);

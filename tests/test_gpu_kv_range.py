@@ -80,6 +80,30 @@ def test_pages_of_zeros_and_small_queries(gpu, new):
         _against(h, F32, _rows(37, F32, 2 * new, heads * hd, size), first, heads, "q %g, %d new" % (size, new))
 
 
+@pytest.mark.parametrize("t", [F16, BF16])
+def test_equal_values_come_back_exactly(gpu, t):
+    """V the same in every token, whole numbers of seven bits: the weights as they enter the product are what is summed,
+    so the output is V.  The last token's key is the only one that is not 0, by 0 to 10 in scores above the others
+    that came before it, so that a weight which is no power of two decides the sum."""
+    heads, kv, hd = 64, 2, 64
+    lens = [300, 261, 40, 3, 2]
+    h = Held(gpu, kv, hd, lens, 38)
+    h.model.scale[:, :, 1] = 2.0 ** -4
+    h.model.q[:, :, 1] = np.random.default_rng(39).integers(96, 128, (1, kv, 1, hd))
+    h.model.q[:, :, 0] = 0
+    h.model.scale[:, :, 0] = 2.0 ** -6
+    for s, n in enumerate(lens):
+        h.model.q[h.model.page(s, (n - 1) // R.PAGE), :, 0, (n - 1) % R.PAGE, 0] = 64
+    _put(h)
+    want = np.repeat(h.model.q[0, :, 1, 0] / 16, heads // kv, 0).ravel()
+    for new in (1, 2):
+        first = _offsets([new] * len(lens))
+        q = np.zeros((first[-1], heads, hd))
+        q[:, :, 0] = np.random.default_rng(40).uniform(0, 80, q.shape[:2])
+        got = R.from_type(h.attend(t, R.to_type(q.reshape(first[-1], -1), t), first, heads), t)
+        assert np.array_equal(got, np.broadcast_to(want, got.shape)), new
+
+
 @pytest.mark.parametrize("t", [F32, BF16])
 @pytest.mark.parametrize("new", [1, 40])
 def test_runs_of_hundreds_of_pages(gpu, t, new):
