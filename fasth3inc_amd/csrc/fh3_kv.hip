@@ -416,7 +416,7 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         uint32_t hi, lo;
-                        split2(x[i][2 * e], x[i][2 * e + 1], up, hi, lo, _Float16());
+                        split2(x[i][2 * e], x[i][2 * e + 1], up, hi, lo);
                         h[e] = hi, l4[e] = lo;
                     }
                     qf[r][0][i] = __builtin_bit_cast(half8, h);
@@ -520,7 +520,7 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
                             const float p1 = __builtin_amdgcn_exp2f(fmaf(t[r][i >> 2][(i & 3) + 1], x, nm));
                             if constexpr (NT == 2) {
                                 uint32_t hi, lo;
-                                split2(p0, p1, 1.f, hi, lo, _Float16());
+                                split2(p0, p1, 1.f, hi, lo);
                                 h[e] = hi, l4[e] = lo;
                                 sum += p0 + p1;
                             } else {  // the sum is of the rounded weights, which the product takes

@@ -31,11 +31,6 @@ __device__ __forceinline__ float value_at(const void *p, int type, int64_t i) {
     if (type == FH3K_F16) return (float)((const _Float16 *)p)[i];
     return __builtin_bit_cast(float, (uint32_t)((const uint16_t *)p)[i] << 16);
 }
-__device__ __forceinline__ void put_value(void *p, int type, int64_t i, float x) {
-    if (type == FH3K_F32) ((float *)p)[i] = x;
-    else if (type == FH3K_F16) ((_Float16 *)p)[i] = (_Float16)x;
-    else ((__bf16 *)p)[i] = (__bf16)x;
-}
 
 // Rows a .. a + cnt - 1 of sequence s.  Whatever first holds, they lie within n_tok.
 __device__ __forceinline__ void seq_rows(const Fh3kSeqs &s, int i, int &a, int &cnt) {

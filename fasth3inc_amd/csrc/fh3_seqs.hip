@@ -432,8 +432,8 @@ __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
         const int key = key0 + i * (NT / CPR);
         const f32x4 x = __builtin_bit_cast(f32x4, r);
         uint32_t h0, h1, l0, l1;
-        split2(x[0], x[1], up, h0, l0, TQ());
-        split2(x[2], x[3], up, h1, l1, TQ());
+        split2(x[0], x[1], up, h0, l0);
+        split2(x[2], x[3], up, h1, l1);
         *(u32x2 *)&to.x[0][key][d0] = u32x2{h0, h1};
         *(u32x2 *)&to.x[1][key][d0] = u32x2{l0, l1};
         ks[d0 ? TILE_32 + key : key] = __builtin_bit_cast(float, 0x7F000000u - __builtin_bit_cast(uint32_t, up));  // 1 / up
@@ -450,8 +450,8 @@ __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
         const int key = key0 + i * (NT / CPR);
         const f32x4 x = __builtin_bit_cast(f32x4, r);
         uint32_t h0, h1, l0, l1;
-        split2(x[0], x[1], up, h0, l0, TP());
-        split2(x[2], x[3], up, h1, l1, TP());
+        split2(x[0], x[1], up, h0, l0);
+        split2(x[2], x[3], up, h1, l1);
         *(u32x2 *)&to.x[0][key][d0] = u32x2{h0, h1};
         *(u32x2 *)&to.x[1][key][d0] = u32x2{l0, l1};
         vs[d0 ? TILE_32 + key : key] = back;
@@ -584,7 +584,7 @@ __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
             const float p0 = __builtin_amdgcn_exp2f(fmaf(s[0][8 * tt + 2 * x], c, nm));
             const float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][8 * tt + 2 * x + 1], c, nm));
             uint32_t hi, lw;
-            split2(p0, p1, 1.f, hi, lw, TP());
+            split2(p0, p1, 1.f, hi, lw);
             ph[tt][x] = hi, pl[tt][x] = lw;
             sum[0] += p0, sum[1] += p1;
         };

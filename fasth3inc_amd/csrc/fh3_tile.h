@@ -154,21 +154,13 @@ __device__ __forceinline__ void store4(void *p, int type, int64_t at, f32x4 x) {
     }
 }
 
-// two terms of 16 bits: x ~ hi + lo, both rounded to nearest
-// Two values as two terms of 16 bits each, x ~ hi + lo, all rounded to nearest; x
-// is x * scale for fp16 (a power of two).
-__device__ __forceinline__ void split2(float a, float b, float scale, uint32_t &hi, uint32_t &lo, _Float16) {
+// Two values times a power of two as two fp16 terms each, x ~ hi + lo, all rounded to nearest.
+__device__ __forceinline__ void split2(float a, float b, float scale, uint32_t &hi, uint32_t &lo) {
     const half2v h = __builtin_convertvector(f32x2{a * scale, b * scale}, half2v);
     const f32x2 l = {fmaf(a, scale, -(float)h[0]), fmaf(b, scale, -(float)h[1])};
     hi = __builtin_bit_cast(uint32_t, h);
     lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(l, half2v));
 }
-__device__ __forceinline__ void split2(float a, float b, float, uint32_t &hi, uint32_t &lo, __bf16) {
-    hi = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf2));
-    const float ha = __builtin_bit_cast(float, hi << 16), hb = __builtin_bit_cast(float, hi & 0xFFFF0000u);
-    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a - ha, b - hb}, bf2));
-}
-
 // The lanes 32 (16) apart: the larger value, the sum, in both.
 __device__ __forceinline__ f32x2 swap32(float x) {
     const uint32_t b = __builtin_bit_cast(uint32_t, x);
@@ -242,7 +234,7 @@ template <int HD, class TQ, class TP, int QT> struct Rows {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         uint32_t hi, lo;
-                        split2(x[kk][2 * i], x[kk][2 * i + 1], up, hi, lo, TQ());
+                        split2(x[kk][2 * i], x[kk][2 * i + 1], up, hi, lo);
                         h[i] = hi, l4[i] = lo;
                     }
                     q[0][kk] = __builtin_bit_cast(q8, h), q[QT - 1][kk] = __builtin_bit_cast(q8, l4);
@@ -379,7 +371,7 @@ template <int HD, class TQ, class TP, int QT> struct Rows {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     uint32_t hi, lo;
-                    split2(p[2 * e], p[2 * e + 1], 1.f, hi, lo, TP());
+                    split2(p[2 * e], p[2 * e + 1], 1.f, hi, lo);
                     h[e] = hi, l4[e] = lo;
                     sum[0] += p[2 * e], sum[1] += p[2 * e + 1];
                 }
