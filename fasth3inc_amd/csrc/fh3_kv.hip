@@ -866,10 +866,18 @@ extern "C" hipError_t fh3k_kv_read(const Fh3kKv *c, int type, void *k, int64_t l
 }
 
 // How the rows of a call are tiled: by the average sequence, which is what the
-// host knows (any tiling is right for any sequence).  fp16, 8 key heads of 128, 16
-// sequences of 4000 tokens, us with tiles of 16 / 32 / 128 rows: 8 rows each 31 / 37
-// / 48, 16 rows 33 / 38 / 49, 18 rows - / 38 / 50, 32 rows - / 42 / 52; 40 rows in 128
-// 58.  Two sequences of 16000: 8 rows 21 / 23 / 33, 16 rows 22 / 27 / 33, 32 rows - / 31 / 34.
+// host knows (any tiling is right for any sequence).  8 key heads of 128, us with tiles of 16
+// / 32 / 128 rows.  fp16, 16 sequences of 4000 tokens: 8 rows each 31.5 / 40 / 49, 16 rows
+// 33.6 / 42 / 50, 18 rows 37 / 43 / 52, 32 rows 37 / 46 / 54, 40 rows 69 / 56 / 60; two of 16000:
+// 16 rows 24 / 30 / 35, 32 rows 31 / 35 / 36; 64 of 2000: 32 rows 45 / 30 / 48; 200 of 1000: 32
+// rows 72 / 58 / 85; 32 of 2000: 64 rows 53 / 44 / 56, 96 rows 78 / 77 / 62, 128 rows 101 / 78 /
+// 69.  fp32, whose 32-row tiles spill 58 registers at hd 128 and 128-row ones 46: 16 of 4000, 8
+// rows 33 / 58 / 83, 32 rows 44 / 67 / 87, 64 of 2000, 32 rows 46 / 36 / 64, 32 of 2000, 64 rows 64
+// / 67 / 88, 128 rows 124 / 121 / 109.  From 17 to 32 rows either of the first two may be the
+// faster, as the tiles' number fits the card.
+// One chunk in a call with single tokens (bf16, all of 4000 tokens, 8 rows to a token): 512
+// tokens alone 114, 127 single tokens alone 188, together 350 (in 128-row tiles); 255 single
+// tokens alone 369, with the chunk 445 (in 32-row tiles).
 struct KvForm {
     KvWork work;
     int64_t tiles;  // of all sequences at most

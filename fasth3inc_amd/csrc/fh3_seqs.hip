@@ -634,12 +634,17 @@ __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
 }
 
 // F32 with every other tile of keys to four more wavefronts, against four wavefronts
-// alone, us: one sequence at 64 heads over 8, hd 128, 37 tokens 15.5 / 11.0, 300
-// tokens 32 / 36, 600 tokens 53 / 66, 900 tokens 89 / 95, 1200 tokens (608
-// workgroups) 134 / 127; 16 heads over 16, hd 64, 500 tokens 22 / 28, 2000 tokens
-// 65 / 92, 4000 tokens (512 workgroups) 150 / 182, 5060 tokens (672) 101 / 100.
+// alone, us.  64 heads over 8, hd 128 (one workgroup of eight to a CU, two of four): one
+// sequence of 37 tokens 16.8 / 12.1, 100 20.5 / 17.2, 150 23.5 / 22.3, 200 25.0 / 25.8, 300
+// 31.1 / 34.7, 600 50.0 / 61.9, 1000 (504 workgroups) 90.2 / 100, 1200 (600) 128 / 122;
+// several sequences, which leave no short tiles for the second round: 2 x 250 (256 workgroups)
+// 30.3 / 32.5, 2 x 300 (304) 42.0 / 39.8, 3 x 200 (312) 40.7 / 32.0, 4 x 200 (416) 48.6 / 36.5.
+// 16 heads over 16, hd 64: 150 tokens 12.0 / 12.0, 250 15.2 / 17.1, 500 21.8 / 27.6, 2000 63 /
+// 90, 4000 (512) 137 / 174, 4600 (576) 181 / 207; 2 x 1000 (256) 37.1 / 49.7, 4 x 1000 (512)
+// 64.1 / 65.2, 2 x 3000 (768) 164 / 165.
 // (16 bits: 0.7 to 0.9 as fast at hd 128, 0.8 to 1.1 at hd 64, so not there.)
-constexpr int SPLIT_TO = 512, SPLIT_FROM = 128;
+constexpr int SPLIT_FROM = 192;
+constexpr int split_to(int hd, int n_seq) { return hd == 128 && n_seq > 1 ? 256 : 512; }
 
 // Tiles of all sequences at most: each may have one that is not full.
 int64_t most_tiles(const Fh3kAttn &a, const Fh3kSeqs &s) {
@@ -658,7 +663,7 @@ hipError_t launch_seqs(const Fh3kAttn &a, const void *q, int64_t ldq, const void
     if constexpr (TY == 2) {
         // Few workgroups with more than a few tiles of keys: eight wavefronts each, so
         // that a SIMD has two and a row half as many steps.
-        if (tiles * a.kv_heads <= SPLIT_TO && (int64_t)s.n_tok >= (int64_t)SPLIT_FROM * s.n_seq)
+        if (tiles * a.kv_heads <= split_to(HD, s.n_seq) && (int64_t)s.n_tok >= (int64_t)SPLIT_FROM * s.n_seq)
             hipLaunchKernelGGL((k_attn_seqs32<HD, 2>), grid, dim3(512), 0, st, g);
         else
             hipLaunchKernelGGL((k_attn_seqs32<HD, 1>), grid, dim3(256), 0, st, g);
