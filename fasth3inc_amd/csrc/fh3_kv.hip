@@ -376,7 +376,7 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
             // rows of this lane: R times l16; q's fragments, 16 channels of each 64.
             // q, the first pages and their K are on their way before any is used.
             Raw8 raw[R][2 * KU];
-            float f[R], m[R], mlo[R], l[R], slope2[R];  // m, mlo: the weights' offset in two terms
+            float f[R], m[R], l[R], slope2[R];  // m: the weights' offset, its second term in slo
             int pos[R], lim[R];
 #pragma unroll
             for (int r = 0; r < R; r++) {
@@ -397,7 +397,7 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
             }
             half8 qf[R][NT][2 * KU];
             f32x4 acc[R][DT];
-            bool far[R];  // some row of the sixteen has an offset of FAR and more
+            int far = 0;  // bit r: some row of sixteen r has an offset of FAR and more; otherwise slo is 0 and is not read
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 float x[2 * KU][8], top = 0.f;
@@ -423,8 +423,8 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
                     if constexpr (NT == 2) qf[r][NT - 1][i] = __builtin_bit_cast(half8, l4);
                 }
                 m[r] = M_NONE;
-                mlo[r] = l[r] = 0.f;
-                far[r] = false;
+                l[r] = 0.f;
+                slo[wave][16 * r + l16] = 0.f;
 #pragma unroll
                 for (int d = 0; d < DT; d++) acc[r][d] = f32x4{};
             }
@@ -490,24 +490,31 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
                     float mt = t[r][0][0];
 #pragma unroll
                     for (int i = 1; i < 16; i++) mt = fmaxf(mt, t[r][i >> 2][i & 3]);
-                    if (__ballot(fmaf(mt, x, -m[r]) - mlo[r] > RAISE)) {
+                    float nm = -m[r];
+                    const bool was = far >> r & 1;
+                    if (was || __ballot(fmaf(mt, x, nm) > RAISE)) {
+                        float lo2 = was ? slo[wave][16 * r + l16] : 0.f;
                         mt = max32(max16(mt));
                         const float y = mt * x, off = fmaf(mt, x, -y) - OFFSET;
-                        const bool raise = fmaf(mt, x, -m[r]) - mlo[r] > RAISE, two = fabsf(y) >= FAR;
+                        const bool raise = fmaf(mt, x, nm) - lo2 > RAISE, two = fabsf(y) >= FAR;
                         const float now = two ? y : y - OFFSET, rest = two ? off : 0.f;
-                        const float keep = raise ? __builtin_amdgcn_exp2f((m[r] - now) + (mlo[r] - rest)) : 1.f;
+                        const float keep = raise ? __builtin_amdgcn_exp2f((m[r] - now) + (lo2 - rest)) : 1.f;
                         m[r] = raise ? now : m[r];
-                        mlo[r] = raise ? rest : mlo[r];
-                        far[r] = __ballot(fabsf(m[r]) >= FAR && m[r] != M_NONE);
+                        lo2 = raise ? rest : lo2;
+                        nm = -m[r];
                         l[r] *= keep;
 #pragma unroll
                         for (int d = 0; d < DT; d++) acc[r][d] *= keep;
-                    }
-                    float nm = -m[r];
-                    if (far[r]) {
+                        const bool is = __ballot(fabsf(m[r]) >= FAR && m[r] != M_NONE);
+                        if (was || is) {
+                            far = is ? far | 1 << r : far & ~(1 << r);
+                            slo[wave][16 * r + l16] = lo2;
+                        }
+                        if (is) {
 #pragma unroll
-                        for (int i = 0; i < 16; i++) t[r][i >> 2][i & 3] = fmaf(t[r][i >> 2][i & 3], x, -m[r]) - mlo[r];
-                        x = 1.f, nm = 0.f;
+                            for (int i = 0; i < 16; i++) t[r][i >> 2][i & 3] = fmaf(t[r][i >> 2][i & 3], x, nm) - lo2;
+                            x = 1.f, nm = 0.f;
+                        }
                     }
                     float sum = 0.f;
 #pragma unroll
@@ -555,7 +562,7 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
             for (int r = 0; r < R; r++) {
                 l[r] = sum32(sum16(l[r]));
                 const int row = 16 * r + l16;
-                if (g == 0) sm[wave][row] = m[r], slo[wave][row] = mlo[r], sl[wave][row] = l[r];
+                if (g == 0) sm[wave][row] = m[r], sl[wave][row] = l[r];
 #pragma unroll
                 for (int d = 0; d < DT; d++) *(f32x4 *)&so[wave][row][16 * d + 4 * g] = acc[r][d];
             }
