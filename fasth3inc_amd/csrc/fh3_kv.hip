@@ -873,18 +873,26 @@ extern "C" hipError_t fh3k_kv_read(const Fh3kKv *c, int type, void *k, int64_t l
 }
 
 // How the rows of a call are tiled: by the average sequence, which is what the
-// host knows (any tiling is right for any sequence).  8 key heads of 128, us with tiles of 16
-// / 32 / 128 rows.  fp16, 16 sequences of 4000 tokens: 8 rows each 31.5 / 40 / 49, 16 rows
-// 33.6 / 42 / 50, 18 rows 37 / 43 / 52, 32 rows 37 / 46 / 54, 40 rows 69 / 56 / 60; two of 16000:
-// 16 rows 24 / 30 / 35, 32 rows 31 / 35 / 36; 64 of 2000: 32 rows 45 / 30 / 48; 200 of 1000: 32
-// rows 72 / 58 / 85; 32 of 2000: 64 rows 53 / 44 / 56, 96 rows 78 / 77 / 62, 128 rows 101 / 78 /
-// 69.  fp32, whose 32-row tiles spill 58 registers at hd 128 and 128-row ones 46: 16 of 4000, 8
-// rows 33 / 58 / 83, 32 rows 44 / 67 / 87, 64 of 2000, 32 rows 46 / 36 / 64, 32 of 2000, 64 rows 64
-// / 67 / 88, 128 rows 124 / 121 / 109.  From 17 to 32 rows either of the first two may be the
-// faster, as the tiles' number fits the card.
-// One chunk in a call with single tokens (bf16, all of 4000 tokens, 8 rows to a token): 512
-// tokens alone 114, 127 single tokens alone 188, together 350 (in 128-row tiles); 255 single
-// tokens alone 369, with the chunk 445 (in 32-row tiles).
+// host knows (any tiling is right for any sequence).  8 key heads, us with tiles of 16 / 32 /
+// 128 rows, one to some tokens of each sequence:
+//                           fp16, hd 128      fp32, hd 128      fp16, hd 64       fp32, hd 64
+//   16 x 4000,   8 rows   31.5/37.5/49.6    33.3/57.6/83.2    20.7/25.4/33.0    22.1/29.3/41.0
+//                16       33.7/40.1/50.9    36.0/61.0/85.0    22.3/27.1/33.5    23.5/31.1/41.4
+//                32       37.2/43.8/53.9    44.2/65.6/88.8    25.3/29.1/34.9    29.1/34.2/43.3
+//                40       68.5/54.3/60.1    70.8/81.1/98.5    36.7/35.9/41.3    37.9/42.8/53.0
+//    1 x 300,    32       14.1/12.3/16.7    16.0/16.8/22.3    10.6/ 9.0/11.3    11.7/10.3/13.6
+//    4 x 300,    32       14.8/22.2/30.5    16.5/30.5/41.8    11.0/15.6/20.1    12.2/18.0/24.6
+//    1 x 120000, 32       69.1/63.4/98.7    73.5/88.8/ 152    35.6/37.2/61.4    40.0/42.8/75.0
+//   64 x 2000,   32       85.6/52.8/79.8    86.4/86.8/ 140    44.9/30.3/48.2    46.7/35.8/63.0
+//  200 x 1000,   32        138/ 109/ 142     149/ 163/ 251    71.6/58.1/85.0    81.7/71.2/ 108
+//   32 x 2000,   64       52.6/42.6/55.2    64.3/67.8/90.2    34.0/28.8/37.2    40.3/35.6/49.4
+//               128        101/76.7/70.5     120/ 121/ 109    62.4/49.8/44.5    76.7/62.5/60.1
+// fp32 at hd 128 has no 32-row form: its 53 spilled registers leave it behind 16 rows (the 46 of
+// its 128-row form do not leave that behind where a sequence has that many).  Otherwise
+// 32 rows win by more than they lose by from 17 to 32, as the number of tiles fits the card.
+// One chunk in a call with single tokens (bf16, hd 128, all of 4000 tokens, 8 rows to a token):
+// 512 tokens alone 114, 127 single tokens alone 188, together 350 (in 128-row tiles); 255
+// single tokens alone 369, with the chunk 445 (in 32-row tiles).
 struct KvForm {
     KvWork work;
     int64_t tiles;  // of all sequences at most
@@ -895,7 +903,7 @@ static KvForm kv_form(const Fh3kAttn &a, const Fh3kKv &c, const Fh3kSeqs &s) {
     const int64_t G = a.heads / a.kv_heads, rows = s.n_tok * G, avg = (rows + s.n_seq - 1) / s.n_seq;
     f.few = avg <= 32;
     static_assert(WAVE_R * MANY_W == 1 << 7, "");
-    const int shift = avg <= 16 ? 4 : avg <= 32 ? 5 : 7;
+    const int shift = avg <= (a.type == FH3K_F32 && a.hd == 128 ? 32 : 16) ? 4 : avg <= 32 ? 5 : 7;
     f.tiles = (rows >> shift) + (s.n_seq < s.n_tok ? s.n_seq : s.n_tok);
     const int64_t runs = (f.tiles * c.max_pages + WHOLE - 1) / WHOLE, most = (512 + a.kv_heads - 1) / a.kv_heads;
     f.work = {(int)G, shift, (int)(runs < most ? runs : most)};
@@ -923,8 +931,10 @@ static hipError_t kv_attn(const Fh3kAttn &a, const Fh3kKv &c, const void *q, int
         if (two) FH3K_KV((k_kv_few<HD, 1, 2>), FEW_W);
         else FH3K_KV((k_kv_few<HD, 1, 1>), FEW_W);
     } else if (f.few) {
-        if (two) FH3K_KV((k_kv_few<HD, 2, 2>), FEW_W);
-        else FH3K_KV((k_kv_few<HD, 2, 1>), FEW_W);
+        if constexpr (HD == 64) {
+            if (two) FH3K_KV((k_kv_few<HD, 2, 2>), FEW_W);
+        }
+        if (!two) FH3K_KV((k_kv_few<HD, 2, 1>), FEW_W);
     } else {
         if (two) FH3K_KV((k_kv_many<HD, 2>), MANY_W);
         else FH3K_KV((k_kv_many<HD, 1>), MANY_W);

@@ -316,8 +316,8 @@ int fh3_hip_kv_read_dev(const Fh3KvCache *kv, int type, void *d_k, int64_t ldk, 
  * second kernel joins them in order: deterministic.  Calls that may overlap need
  * a workspace each.  Sizes as in fh3_hip_attention_seqs_dev; (rows / T + n_seq) *
  * max_pages below 2^31, where rows is n_tok * heads / kv_heads and a tile has T = 16
- * of them up to 16 to an average sequence, 32 up to 32, otherwise 128.  Larger
- * calls are refused (a workspace size of 0). */
+ * of them up to 16 to an average sequence (F32 at head_dim 128: up to 32), 32 up to
+ * 32, otherwise 128.  Larger calls are refused (a workspace size of 0). */
 size_t fh3_hip_kv_attention_workspace_bytes(const Fh3AttnCfg *c, const Fh3KvCache *kv, int n_tok, int n_seq);
 int fh3_hip_kv_attention_dev(const Fh3AttnCfg *c, const Fh3KvCache *kv, const void *d_q, int64_t ldq, void *d_o,
                              int64_t ldo, int n_tok, int n_seq, const int *d_first, void *d_ws, size_t ws_bytes,
