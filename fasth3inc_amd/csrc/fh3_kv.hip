@@ -72,10 +72,10 @@ __device__ __forceinline__ bool row_page(const Fh3kKv &c, const Fh3kSeqs &s, Row
 
 // The rows go through LDS as fp32: their largest finite value gives the scale, then
 // a whole page is made in 16-byte pieces, part of one in the smallest that its
-// rows fill (K: 16 channels of a slot; V: four slots of a channel).  Prompts are bound
-// by memory (with the read-back 88 MB in 26 us, 3.4 TB/s), one token of 64 sequences by
-// the loads that wait for each other: length, page, rows (4-5 us of 14 with the
-// read-back).
+// rows fill (K: 16 channels of a slot; V: four slots of a channel).  Prompts: 55 MB in 15 us,
+// 3.6 TB/s where a copy reaches 4.8; wavefronts wait half of their time (rows, then the
+// barrier before the scale) and half of the LDS cycles are V's bank conflicts.  One token of
+// 64 sequences is bound by the loads that wait for each other: length, page, rows (4 us).
 template <int HD>
 __global__ __launch_bounds__(ROW_T) void k_kv_append(Fh3kKv c, int type, const void *__restrict__ k, int64_t ldk,
                                                      const void *__restrict__ v, int64_t ldv, Fh3kSeqs s) {
@@ -164,7 +164,9 @@ __global__ __launch_bounds__(ROW_T) void k_kv_append(Fh3kKv c, int type, const v
 }
 
 // The same pages read back as rows; rows that no page holds become zeros.  A thread
-// takes four slots x four channels, so that rows are written in order.
+// takes four slots x four channels, so that rows are written in order.  4-byte loads 16
+// bytes apart and none ahead: 10 us for the pages that one token of 64 sequences touches,
+// 14 for 5400 fp32 tokens (55 MB).
 template <int HD>
 __global__ __launch_bounds__(ROW_T) void k_kv_read(Fh3kKv c, int type, void *__restrict__ k, int64_t ldk,
                                                    void *__restrict__ v, int64_t ldv, Fh3kSeqs s) {
@@ -329,8 +331,9 @@ __device__ __forceinline__ half8 to_half(uint32_t a, uint32_t b) {
 // operands of 16x16x32 products (S^T = K Q^T, O^T = V^T P^T), and the four are
 // joined in LDS.  NT: 16-bit terms of q and of the weights (fp32: two).  16 KB are on
 // their way to each wavefront, 128 KB to a CU, so that memory bounds it: 0.5 GB of cache
-// in 94 us and 102 with the join (5.0 TB/s; a device copy moves 4.8), 140 MB in 31
-// and 39.  One token of one sequence takes 8 us, launch and latencies.
+// in 96 us and 103 with the join (5.0 TB/s; a device copy moves 4.8), 140 MB in 40 with the
+// join.  One token of one sequence takes 8.5 us, launch and latencies.  The form of 32 16-bit
+// rows at hd 128 spills one register.
 constexpr int FEW_W = 4;
 constexpr float OFFSET = Vec<_Float16>::OFFSET, RAISE = Vec<_Float16>::RAISE;
 template <int HD, int R, int NT>
@@ -607,7 +610,7 @@ __global__ __launch_bounds__(64 * FEW_W, 2) void k_kv_few(Fh3kAttn a, Fh3kKv c, 
     } while (run.u < run.end && kv_next(c, s, work, run));
 }
 
-// Joins the parts of a divided tile in order, 4-5 us.  A workgroup takes RB rows of the tile
+// Joins the parts of a divided tile in order, 4-7 us (many rows 13).  A workgroup takes RB rows of the tile
 // that workgroup blockIdx.x of key head blockIdx.y began; SB groups of threads take
 // every SB-th part each.
 template <int HD, int SB>
@@ -662,8 +665,10 @@ __global__ __launch_bounds__(256) void k_kv_join(Fh3kAttn a, Fh3kKv c, void *__r
 // into fp16 once for all of them, through double-buffered LDS: K as rows, V
 // transposed with the keys of each 16 in the order of the first product's
 // accumulator (0-3, 8-11, 4-7, 12-15).  Bound by the vector instructions of the softmax and
-// the conversion beside the matrix ones: 1000 tokens of 64 heads behind 31000 in
-// 550 us, 0.82 PFLOP/s.
+// the conversion (8 to a matrix instruction; each tile of rows converts its pages anew) beside
+// the matrix ones: 1000 tokens of 64 heads behind 31000 in 550 us, 0.82 PFLOP/s, the matrix
+// pipe busy 37 %.  fp32 (two terms of q and of the weights): 500 tokens behind 31500 in 505
+// us, busy 46 %; at hd 128 46 registers spill.
 constexpr int MANY_W = 4;
 template <int HD, int NT>
 __global__ __launch_bounds__(64 * MANY_W, 2) void k_kv_many(Fh3kAttn a, Fh3kKv c, const void *__restrict__ q,

@@ -194,7 +194,10 @@ __device__ __forceinline__ void join_halves(R &w, float &unit, float first, int 
 // is a tile ahead of V.  Bound by the matrix cores at the clock that the power
 // limit leaves: 8192 tokens x 64 heads bf16 1.03-1.11 ms, 1.0 PFLOP/s, where the
 // library's large product reaches 1.2 (through registers and one product after
-// the other 1.28 ms); capped scores by the tanh's vector instructions.
+// the other 1.28 ms); capped scores and hd 64 by vector instructions: 5.8 to a matrix
+// instruction there, 14 with the tanh (a fifth of them exponentials and reciprocals; 24
+// documents 109 us), 21 at hd 64 with the distance bias (half the matrix work for the same
+// softmax; 48 us).
 template <int HD, int TY>
 __global__ __launch_bounds__(256, 2) void k_attn_seqs16(SeqsArgs g) {
     typedef Operand<TY> Op;
@@ -353,11 +356,14 @@ __global__ __launch_bounds__(256, 2) void k_attn_seqs16(SeqsArgs g) {
 
 // F32: every operand is two fp16 terms, made on the way to LDS: the terms of the
 // next V beside the first product, the weights and the terms of the next K beside
-// the second.  (V and weights as two bf16 terms, which need no power of two: 600
-// tokens 46 us for 53, but 4e-6 off for 4e-7.)  Tiles of 32 keys, so that two workgroups fit a CU and nothing has
-// to be moved to accumulation registers (64 keys, one workgroup: 600 tokens x 64
-// heads 52.6 us; a third of the instructions were such moves).  KH = 2: eight
-// wavefronts, two to a SIMD, each four with every other tile of keys.
+// the second.  (V and weights as two bf16 terms, which need no power of two, took 46 us at
+// 600 tokens where fp16 took 49-51, but are 4e-6 off for 3e-7.)  Tiles of 32 keys, so that two
+// workgroups fit a CU and nothing has to be moved to accumulation registers (64 keys,
+// one workgroup: 600 tokens x 64 heads 52.6 us; a third of the instructions were such
+// moves).  KH = 2: eight wavefronts, two to a SIMD, each four with every other tile of keys.
+// 600 tokens x 64 heads 48.5 us: 12 vector instructions to a matrix instruction, the terms
+// for the most part, made anew for each of 38 tiles of rows; matrix pipe busy 14 %.  At hd
+// 128 24 to 26 registers spill (LDS addresses, read back once a step).
 template <int HD, int KH>
 __global__ __launch_bounds__(256 * KH, 2) void k_attn_seqs32(SeqsArgs g) {
     typedef Operand<2> Op;

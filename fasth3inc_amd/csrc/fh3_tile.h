@@ -358,7 +358,10 @@ template <int HD, class TQ, class TP, int QT> struct Rows {
         return c;
     }
 
-    // The weights exp2(c s + nm) as the second product's operand, and their sum.
+    // The weights exp2(c s + nm) as the second product's operand, and their sum.  16-bit V takes
+    // weights of its own type, one term: a second one would double that product, and the
+    // rounding (half a step of the type, r.m.s. a tenth to a third more error than fp32 weights
+    // leave after the output's own rounding) is the caller's choice of type.
     __device__ __forceinline__ void weights(const f32x16 (&s)[2], float c, float nm, p8 (&pf)[QT][4]) {
         float sum[2] = {};
 #pragma unroll

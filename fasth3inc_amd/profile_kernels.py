@@ -45,6 +45,20 @@ Workloads (each launch sequence is preceded by one untimed warmup launch):
          shape (6 text + 244 audio tokens, video grid 22x18x32, n = 12922),
          56 heads of 128, sparsity 0.8, with q/k rmsnorm, rope3 and the gate:
          fh3_hip_vsa_attention_qkv_dev -> every VSA kernel
+  seqs   attention within packed sequences: fp32 prompts of 37 and 600 tokens
+         (64 heads over 8, hd 128), 24 bf16 documents of 17 to 1500 tokens with
+         capped scores (40 over 8), 3 fp16 sequences of 1021 to 2047 tokens with
+         prefix and distance bias (16 heads of 64), 8192 bf16 tokens (64 over 8):
+         fh3_hip_attention_seqs_dev -> k_attn_seqs32, k_attn_seqs16
+  cache  the 8-bit cache at 8 key heads of 128: 16 fp32 prompts written and
+         read, one bf16 token of 64 sequences likewise, then attention of one
+         fp32 token over 300, one bf16 token of 32 sequences of 200 to 8192, one
+         fp16 token over 2 x 125000 with distance bias, 2 to 6 fp32 tokens over
+         24 x 500 to 5000 with capped scores (16 heads over 4, hd 64), chunks of
+         500 bf16 tokens over 2 x 14000 and of 250 fp32 tokens over 2 x 16000:
+         fh3_hip_kv_append_dev, _read_dev, _attention_dev -> k_kv_*
+
+seqs and cache take --only NAME,NAME of their cases.
 """
 import argparse
 import sys
@@ -252,13 +266,111 @@ def vsa(reps, heads=56, hd=128, rot=96):
         b.close()
 
 
+_TYPES = {"F32": F.FH3_QUANT_F32, "F16": F.FH3_QUANT_F16, "BF16": F.FH3_QUANT_BF16}
+
+
+def _typed(rng, n, width, t, scale=1.0):
+    x = rng.standard_normal((n, width), dtype=np.float32) * np.float32(scale)
+    x = x if t == "F32" else x.astype(np.float16) if t == "F16" else (x.view(np.uint32) >> 16).astype(np.uint16)
+    return F.DeviceBuffer.from_array(x)
+
+
+def _spread(rng, n, lo, hi):
+    return [int(x) for x in np.exp(rng.uniform(np.log(lo), np.log(hi), n)).round()]
+
+
+def _first(lens):
+    return F.DeviceBuffer.from_array(np.concatenate([[0], np.cumsum(lens)]).astype(np.int32))
+
+
+def _slopes(heads):
+    return F.DeviceBuffer.from_array((2.0 ** (-8.0 * (np.arange(heads) + 1) / heads)).astype(np.float32))
+
+
+def seqs(reps, only=None):
+    rng = np.random.default_rng(3)
+    cases = [("prompt_37", "F32", 64, 8, 128, [37], 0.0, False, 0.0), ("prompt_600", "F32", 64, 8, 128, [600], 0.0, False, 0.0),
+             ("documents", "BF16", 40, 8, 128, _spread(rng, 24, 17, 1500), 50.0, False, 0.0),
+             ("prefix", "F16", 16, 16, 64, _spread(rng, 3, 1021, 2047), 0.0, True, 0.25),
+             ("long", "BF16", 64, 8, 128, [8192], 0.0, False, 0.0)]
+    for name, t, heads, kv, hd, lens, cap, bias, prefix in cases:
+        if only and name not in only:
+            continue
+        n = sum(lens)
+        q, k, v = (_typed(rng, n, w * hd, t, s) for w, s in ((heads, 1.5), (kv, 1.0), (kv, 1.0)))
+        o, first = F.DeviceBuffer(q.nbytes), _first(lens)
+        pre = F.DeviceBuffer.from_array(np.asarray([int(x * prefix) for x in lens], np.int32)) if prefix else None
+        slopes = _slopes(heads) if bias else None
+        cfg = F.attn_cfg(heads, kv, hd, _TYPES[t], softcap=cap, d_slopes=slopes)
+        for _ in range(reps + 1):
+            F.attention_seqs_dev(cfg, q, k, v, o, n, len(lens), first, pre)
+        F.synchronize()
+        print("seqs %s: %s, %d tokens, %d launches" % (name, t, n, reps), flush=True)
+        for b in (q, k, v, o, first, pre, slopes):
+            if b is not None:
+                b.close()
+
+
+def cache(reps, only=None):
+    rng = np.random.default_rng(4)
+    cases = [("fill", "F32", 0, 8, 128, [0] * 16, _spread(rng, 16, 100, 600), 0.0, False),
+             ("append", "BF16", 0, 8, 128, _spread(rng, 64, 100, 4000), [1] * 64, 0.0, False),
+             ("token", "F32", 64, 8, 128, [299], [1], 0.0, False),
+             ("batch", "BF16", 64, 8, 128, _spread(rng, 32, 200, 8192), [1] * 32, 0.0, False),
+             ("far", "F16", 40, 8, 128, [125000] * 2, [1] * 2, 0.0, True),
+             ("few", "F32", 16, 4, 64, _spread(rng, 24, 500, 5000), [2 + i % 5 for i in range(24)], 30.0, False),
+             ("chunk", "BF16", 64, 8, 128, [13500] * 2, [500] * 2, 0.0, False),
+             ("chunk_fp32", "F32", 64, 8, 128, [15750] * 2, [250] * 2, 0.0, False)]
+    for name, t, heads, kv, hd, held, new, cap, bias in cases:
+        if only and name not in only:
+            continue
+        lens = [a + b for a, b in zip(held, new)]
+        need = [-(-x // F.KV_PAGE) for x in lens]
+        pages, n, n_seq = sum(need), sum(new), len(new)
+        raw = np.empty(F.kv_pool_bytes(kv, hd, pages), np.uint8)
+        split = raw.nbytes - pages * kv * 2 * 4
+        raw[:split] = rng.integers(1, 256, split, dtype=np.uint8)
+        raw[split:] = np.full(pages * kv * 2, 2.0 ** -6, np.float32).view(np.uint8)
+        table, order = np.full((n_seq, max(need)), -1, np.int32), rng.permutation(pages)
+        for i, (a, b) in enumerate(zip(np.cumsum([0] + need), need)):
+            table[i, :b] = order[a:a + b]
+        pool, table, length = (F.DeviceBuffer.from_array(x) for x in (raw, table, np.asarray(lens, np.int32)))
+        first = _first(new)
+        c, used = F.kv_cache(kv, hd, pages, max(need), pool, table, length), [pool, table, length, first]
+        if heads:
+            q, slopes = _typed(rng, n, heads * hd, t, 0.3), _slopes(heads) if bias else None
+            o = F.DeviceBuffer(q.nbytes)
+            cfg = F.attn_cfg(heads, kv, hd, _TYPES[t], softcap=cap, d_slopes=slopes)
+            size = F.kv_attention_workspace_bytes(cfg, c, n, n_seq)
+            ws = F.DeviceBuffer(max(1, size))
+            used += [q, o, ws] + ([slopes] if bias else [])
+            for _ in range(reps + 1):
+                F.kv_attention_dev(cfg, c, q, o, n, n_seq, ws, size, first)
+        else:
+            back = [x - (x - a) // F.KV_PAGE * F.KV_PAGE for x, a in zip(lens, new)]   # all of the touched pages
+            k, v, ko, vo = (_typed(rng, m, kv * hd, t) for m in (n, n, sum(back), sum(back)))
+            bf = _first(back)
+            used += [k, v, ko, vo, bf]
+            for _ in range(reps + 1):
+                F.kv_append_dev(c, _TYPES[t], k, v, n, n_seq, first)
+                F.kv_read_dev(c, _TYPES[t], ko, vo, sum(back), n_seq, bf)
+        F.synchronize()
+        print("cache %s: %s, %d tokens held, %d new, %d launches" % (name, t, sum(lens), n, reps), flush=True)
+        for b in used:
+            b.close()
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser()
     ap.add_argument("workload", choices=("gemv", "te", "prompt", "mid", "single", "q56", "gemm", "mlp", "copy", "attn", "vsa",
-                                         "all"))
+                                         "seqs", "cache", "all"))
     ap.add_argument("--reps", type=int, default=20)
+    ap.add_argument("--only", help="seqs, cache: these cases")
     args = ap.parse_args(argv)
     F.init(0)
+    if args.workload in ("seqs", "cache"):
+        globals()[args.workload](args.reps, args.only.split(",") if args.only else None)
+        return 0
     for name in (("gemv", "gemm", "copy") if args.workload == "all" else (args.workload,)):
         globals()[name](args.reps)
     return 0
