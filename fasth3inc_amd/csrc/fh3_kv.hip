@@ -154,7 +154,10 @@ __global__ __launch_bounds__(ROW_T) void k_kv_append(Fh3kKv c, int type, const v
             const int slot = 4 * (from + e / HD), d = e % HD;
             uint32_t *at = (uint32_t *)(page + v_byte<HD>(slot, d)), w = 0;
             if (slot < lo || slot + 4 > hi) w = *at;
-            if (redo && slot < lo) w = again4(w, ratio);  // (of slots from lo on too: they are replaced)
+            if (redo && slot < lo) {  // (bytes from lo on are new, or behind the length: those stay, as K's do)
+                const uint32_t held = slot + 4 <= lo ? ~0u : (1u << 8 * (lo - slot)) - 1;
+                w = (again4(w, ratio) & held) | (w & ~held);
+            }
             for (int i = 0; i < 4; i++)
                 if (slot + i >= lo && slot + i < hi)
                     w = (w & ~(255u << 8 * i)) | (to_byte(sx[(slot + i) * LD + d], inv) & 255) << 8 * i;
