@@ -1103,6 +1103,15 @@ static size_t span(int64_t n, int64_t ld, int64_t width, int type) {
     return (size_t)((n - 1) * ld + width) * value_bytes(type);
 }
 
+// Whether an output lies over what a call reads beside its rows: offsets, prefixes and slopes, a cache's table and lengths.
+static bool over_plan(const void *out, size_t bytes, const Fh3kSeqs &s, const int *prefix, const Fh3kAttn *a, const Fh3kKv *k) {
+    const size_t n = (size_t)s.n_seq;
+    return (s.first && overlap(out, bytes, s.first, (n + 1) * sizeof(int))) ||
+           (prefix && overlap(out, bytes, prefix, n * sizeof(int))) ||
+           (a && a->slopes && overlap(out, bytes, a->slopes, a->heads * sizeof(float))) ||
+           (k && (overlap(out, bytes, k->table, n * k->max_pages * sizeof(int)) || overlap(out, bytes, k->len, n * sizeof(int))));
+}
+
 // Whether rows of a and of b, n each, meet (rows of one pitch may stand between each other).
 static bool rows_meet(const void *a, int64_t lda, const void *b, int64_t ldb, int64_t n, int64_t width, int type) {
     if (!overlap(a, span(n, lda, width, type), b, span(n, ldb, width, type))) return false;
@@ -1130,7 +1139,7 @@ extern "C" int fh3_hip_attention_seqs_dev(const Fh3AttnCfg *c, const void *d_q, 
     if (!fh3k_attn_seqs_fits(&a, s)) return set_err(FH3_E_INVALID, "%s: too many tiles of rows for one launch", fn);
     const size_t on = span(n_tok, ldo, wq, a.type);
     if (overlap(d_o, on, d_q, span(n_tok, ldq, wq, a.type)) || overlap(d_o, on, d_k, span(n_tok, ldk, wk, a.type)) ||
-        overlap(d_o, on, d_v, span(n_tok, ldv, wk, a.type)))
+        overlap(d_o, on, d_v, span(n_tok, ldv, wk, a.type)) || over_plan(d_o, on, s, d_prefix, &a, nullptr))
         return set_err(FH3_E_INVALID, "%s: o overlaps an input", fn);
     if ((rc = ensure_init()) != FH3_OK) return rc;
     FragRt::On on_device(g.device);
@@ -1145,8 +1154,10 @@ extern "C" int fh3_hip_kv_extend_dev(const Fh3KvCache *kv, int n_tok, int n_seq,
     const Fh3kSeqs s = {d_first, n_tok, n_seq};
     int rc = check_kv(kv, &k, fn);
     if (rc == FH3_OK) rc = check_seqs(s, fn);
-    if (rc == FH3_OK) rc = ensure_init();
     if (rc != FH3_OK) return rc;
+    if (over_plan(kv->d_len, (size_t)n_seq * sizeof(int), s, nullptr, nullptr, nullptr))
+        return set_err(FH3_E_INVALID, "%s: the lengths overlap d_first", fn);
+    if ((rc = ensure_init()) != FH3_OK) return rc;
     FragRt::On on_device(g.device);
     FH3_HIPCALL(fh3k_kv_extend(kv->d_len, s, stream ? (hipStream_t)stream : g.stream));
     return FH3_OK;
@@ -1178,6 +1189,8 @@ extern "C" int fh3_hip_kv_append_dev(const Fh3KvCache *kv, int type, const void 
     int rc = kv_rows(kv, type, d_k, &ldk, d_v, &ldv, s, &k, fn);
     if (rc != FH3_OK) return rc;
     if (!d_k || !d_v) return set_err(FH3_E_INVALID, "%s: NULL k or v", fn);
+    if (over_plan(k.pool, fh3_hip_kv_pool_bytes(k.kv_heads, k.hd, k.pages), s, nullptr, nullptr, &k))
+        return set_err(FH3_E_INVALID, "%s: the pool overlaps d_first, the table or the lengths", fn);
     if ((rc = ensure_init()) != FH3_OK) return rc;
     FragRt::On on_device(g.device);
     FH3_HIPCALL(fh3k_kv_append(&k, type, d_k, ldk, d_v, ldv, s, stream ? (hipStream_t)stream : g.stream));
@@ -1194,6 +1207,10 @@ extern "C" int fh3_hip_kv_read_dev(const Fh3KvCache *kv, int type, void *d_k, in
     if (!d_k && !d_v) return set_err(FH3_E_INVALID, "%s: NULL k and v", fn);
     if (d_k && d_v && rows_meet(d_k, ldk, d_v, ldv, n_tok, (int64_t)k.kv_heads * k.hd, type))
         return set_err(FH3_E_INVALID, "%s: the rows of k and v overlap", fn);
+    const int64_t w = (int64_t)k.kv_heads * k.hd;
+    if ((d_k && over_plan(d_k, span(n_tok, ldk, w, type), s, nullptr, nullptr, &k)) ||
+        (d_v && over_plan(d_v, span(n_tok, ldv, w, type), s, nullptr, nullptr, &k)))
+        return set_err(FH3_E_INVALID, "%s: the rows overlap d_first, the table or the lengths", fn);
     if ((rc = ensure_init()) != FH3_OK) return rc;
     FragRt::On on_device(g.device);
     FH3_HIPCALL(fh3k_kv_read(&k, type, d_k, ldk, d_v, ldv, s, stream ? (hipStream_t)stream : g.stream));
@@ -1244,7 +1261,8 @@ extern "C" int fh3_hip_kv_attention_dev(const Fh3AttnCfg *c, const Fh3KvCache *k
                        ws_bytes);
     const size_t pool = fh3_hip_kv_pool_bytes(k.kv_heads, k.hd, k.pages);
     if (overlap(d_o, on, d_q, span(n_tok, ldq, w, a.type)) || overlap(d_o, on, kv->d_pool, pool) ||
-        (need && (overlap(d_ws, need, d_q, span(n_tok, ldq, w, a.type)) || overlap(d_ws, need, d_o, on) ||
+        over_plan(d_o, on, s, nullptr, &a, &k) ||
+        (need && (over_plan(d_ws, need, s, nullptr, &a, &k) || overlap(d_ws, need, d_q, span(n_tok, ldq, w, a.type)) || overlap(d_ws, need, d_o, on) ||
                   overlap(d_ws, need, kv->d_pool, pool))))
         return set_err(FH3_E_INVALID, "%s: o or the workspace overlaps another array", fn);
     if ((rc = ensure_init()) != FH3_OK) return rc;

@@ -279,7 +279,8 @@ size_t fh3_hip_kv_pool_bytes(int kv_heads, int head_dim, int pages);
  * its last tokens, at positions d_len[s] - count .. d_len[s] - 1.  Tokens whose
  * position is negative or past the table's end are not held.  All are enqueued
  * on `stream` without synchronising, allocate nothing and may be captured; a
- * captured call reads the lengths and the table anew at each replay.
+ * captured call reads the lengths and the table anew at each replay.  What a call
+ * writes must not lie over anything that it reads.
  *
  * fh3_hip_kv_extend_dev: d_len[s] += count (once a step, before the layers).
  *

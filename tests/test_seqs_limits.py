@@ -57,6 +57,29 @@ def test_read_back_onto_itself(F):
     _refused(F, F.kv_read_dev, kv, 0, at(0), at(0, w * 4), dict(n_tok=3, n_seq=3, ldk=2 * w, ldv=3 * w))
 
 
+def test_outputs_over_what_the_call_reads(F):
+    """Outputs that lie over offsets, prefixes, slopes, the page table or the lengths."""
+    cfg = F.attn_cfg(8, 2, 64, d_slopes=at(8))
+    rows, w = 12 * 8 * 64 * 4, 2 * 64 * 4
+    for d_o in (at(4), at(4, 16 - rows), at(9), at(9, 16 - rows), at(8), at(8, 16 - rows)):
+        assert "overlaps" in _refused(F, F.attention_seqs_dev, cfg, {**SEQS, "d_prefix": at(9), "d_o": d_o})
+    pool = F.kv_pool_bytes(2, 64, 40)
+    kv = F.kv_cache(2, 64, 40, 30, at(5), at(6), at(7))
+    need = F.kv_attention_workspace_bytes(cfg, kv, 3, 3)
+    good = dict(d_q=at(0), d_o=at(1), n_tok=3, n_seq=3, d_ws=at(2), ws_bytes=need, d_first=at(4))
+    for i, n in ((4, 16), (6, 3 * 30 * 4), (7, 12), (8, 32)):
+        end = (n - 1) // 16 * 16
+        for change in (dict(d_o=at(i)), dict(d_o=at(i, end)), dict(d_ws=at(i)), dict(d_ws=at(i, end)), dict(d_ws=at(i, 16 - need))):
+            assert "overlaps" in _refused(F, F.kv_attention_dev, cfg, kv, {**good, **change})
+        if i == 8:
+            continue
+        for d_k, d_v in ((at(i), at(1)), (at(0), at(i, end)), (None, at(i)), (at(i, 16 - 3 * w), None)):
+            _refused(F, F.kv_read_dev, kv, 0, d_k, d_v, dict(n_tok=3, n_seq=3, d_first=at(4)))
+    for table, length, first in ((at(5), at(7), None), (at(6), at(5, pool - 16), None), (at(6), at(7), at(5, 16))):
+        _refused(F, F.kv_append_dev, F.kv_cache(2, 64, 40, 30, at(5), table, length), 0, at(0), at(1), dict(n_tok=3, n_seq=3, d_first=first))
+    _refused(F, F.kv_extend_dev, kv, 3, 3, at(7, 4))
+
+
 @pytest.mark.parametrize("scale,softcap", [(1e-20, 1e30), (1e-44, 1e-3), (1e30, 1e-3), (1.0, 1e-44), (0.0, 1e-38)])
 def test_caps_too_far_from_the_scale(F, scale, softcap):
     """scale / softcap is one fp32 factor of the product: past its range every score would be 0, or the cap."""
