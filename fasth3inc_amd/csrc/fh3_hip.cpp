@@ -1071,8 +1071,8 @@ static int check_attn(const Fh3AttnCfg *c, int n_tok, Fh3kAttn *a, const char *f
         return set_err(FH3_E_INVALID, "%s: n_tok * heads too large", fn);
     const float scale = c->scale > 0.f ? c->scale : 1.0f / sqrtf((float)c->head_dim);
     // one fp32 factor takes a product to its part of the cap: 2 log2(e) scale / softcap, over q's power of two
-    if (c->softcap > 0.f && !((double)c->softcap <= scale * 0x1p106 && (double)c->softcap >= scale * 0x1p-100))
-        return set_err(FH3_E_INVALID, "%s: softcap must be from 2^-100 to 2^106 times the scale", fn);
+    if (c->softcap > 0.f && !((double)c->softcap <= scale * 0x1p120 && (double)c->softcap >= scale * 0x1p-120))
+        return set_err(FH3_E_INVALID, "%s: softcap must be from 2^-120 to 2^120 times the scale", fn);
     *a = {c->heads, c->kv_heads, c->head_dim, c->type, c->causal != 0, scale, c->softcap, c->d_slopes};
     return FH3_OK;
 }

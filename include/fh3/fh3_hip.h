@@ -201,7 +201,7 @@ int fh3_hip_vsa_attention_qkv_dev(const Fh3VsaCfg *c, const float *d_qkv, const 
  *   type             of q, k, v and o: FH3_QUANT_F32, _F16 or _BF16
  *   causal           non-zero: row i sees keys j <= i (and the prefix); zero: all
  *   scale            0 means 1 / sqrt(head_dim)
- *   softcap          0 means none; otherwise from 2^-100 to 2^106 times the scale
+ *   softcap          0 means none; otherwise from 2^-120 to 2^120 times the scale
  *   d_slopes         NULL, or device [heads]
  * F16 and BF16 operands enter the matrix products as they are, F32 ones as two
  * fp16 terms each after a power of two for each row (relative error about 4e-7;

@@ -91,6 +91,18 @@ def test_capped_scores_far_below_zero(gpu, t):
 
 
 @pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("scale,cap", [(1e-5, 1e30), (1e30, 1e-3), (1e-36, 1e-3), (1e25, 1e-8)])
+def test_caps_far_from_the_scale(gpu, t, scale, cap):
+    """Scores that are 0 beside the cap, or at the cap by far."""
+    heads, kv, hd, lens = 4, 2, 64, [100, 30]
+    first = _offsets(lens)
+    arrays = _case(13, t, first[-1], heads, kv, hd)
+    got = _run(gpu, arrays, t, first, heads, kv, hd, scale=scale, softcap=cap)
+    o, _, _ = R.attention(*(R.from_type(x, t) for x in arrays), first, heads, kv, hd, True, scale, cap)
+    _near(got, o, t, "scale %g cap %g" % (scale, cap))
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
 @pytest.mark.parametrize("scale", [1e-30, 1e-40, 1e-44])
 def test_scales_near_the_least(gpu, t, scale):
     """All scores are 0 to within fp32: the mean of what is seen."""

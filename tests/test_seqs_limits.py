@@ -80,7 +80,7 @@ def test_outputs_over_what_the_call_reads(F):
     _refused(F, F.kv_extend_dev, kv, 3, 3, at(7, 4))
 
 
-@pytest.mark.parametrize("scale,softcap", [(1e-20, 1e30), (1e-44, 1e-3), (1e30, 1e-3), (1.0, 1e-44), (0.0, 1e-38)])
+@pytest.mark.parametrize("scale,softcap", [(1e-20, 1e30), (1e-44, 1e-3), (1e30, 1e-7), (1.0, 1e-44), (0.0, 1e-38)])
 def test_caps_too_far_from_the_scale(F, scale, softcap):
     """scale / softcap is one fp32 factor of the product: past its range every score would be 0, or the cap."""
     cfg = F.attn_cfg(8, 2, 64, scale=scale, softcap=softcap)
