@@ -7,9 +7,10 @@ low half) or FP8 (e4m3) codes, and for each 32 of them one byte s that stands fo
   quantize  rows rounded to MX: the scale of a block is the least 2^e, e >= -127,
             with amax <= 6 * 2^e (FP4) or 448 * 2^e (FP8); FP4 rows are read back too;
   norm      h = x + add, then rmsnorm of h (modulated where asked) rounded to FP8;
-  product   y = x w^T + bias, or res + gate * (x w^T + bias), of MX rows and weights;
-  swiglu    val * silu(gate) of a product whose weight's rows are [val | gate], rounded
-            to FP8 for the product that follows.
+  product   y = x w^T + bias, or res + gate * (x w^T + bias), of FP8 or FP4 rows and
+            FP4 weights;
+  swiglu    val * silu(gate) of such a product whose weight's rows are [val | gate],
+            rounded to FP8 for the product that follows.
 """
 import math
 
@@ -28,27 +29,26 @@ FORMATS = {"FP4": (2, 0x3FFFFF, 2), "FP8": (8, 0x1FFFFF, 1)}
 def listed():
     return [
         # one token through the fused projection of a block: weights from memory, latency
-        {"name": "token_qkv", "kind": "product", "w": "FP4", "x": "FP8", "rows": 1, "in": 5120, "out": 15360, "type": "F32", "bias": False,
+        {"name": "token_qkv", "kind": "product", "x": "FP8", "rows": 1, "in": 5120, "out": 15360, "type": "F32", "bias": False,
          "gate": False},
         # a batch of sixteen tokens through a text encoder's long rows
-        {"name": "tokens_down", "kind": "product", "w": "FP4", "x": "FP8", "rows": 16, "in": 25600, "out": 5120, "type": "BF16",
+        {"name": "tokens_down", "kind": "product", "x": "FP8", "rows": 16, "in": 25600, "out": 5120, "type": "BF16",
          "bias": False, "gate": False},
         # a long prompt, with bias
-        {"name": "prompt_600", "kind": "product", "w": "FP4", "x": "FP8", "rows": 600, "in": 5120, "out": 17408, "type": "BF16",
+        {"name": "prompt_600", "kind": "product", "x": "FP8", "rows": 600, "in": 5120, "out": 17408, "type": "BF16",
          "bias": True, "gate": False},
         # a clip's tokens, both operands in four bits
-        {"name": "clip_qkv", "kind": "product", "w": "FP4", "x": "FP4", "rows": 8192, "in": 5120, "out": 15360, "type": "BF16", "bias": False,
+        {"name": "clip_qkv", "kind": "product", "x": "FP4", "rows": 8192, "in": 5120, "out": 15360, "type": "BF16", "bias": False,
          "gate": False},
-        # the projection behind attention added to the residual stream, both operands in eight bits
-        {"name": "clip_out", "kind": "product", "w": "FP8", "x": "FP8", "rows": 3016, "in": 7168, "out": 5376, "type": "F32", "bias": False,
-         "gate": True},
+        # the projection behind attention, gated and added to an fp32 residual stream
+        {"name": "clip_out", "kind": "product", "x": "FP8", "rows": 3016, "in": 7168, "out": 5376, "type": "F32", "bias": False, "gate": True},
         # the longest clip's second feed-forward product: the largest
-        {"name": "long_clip_down", "kind": "product", "w": "FP4", "x": "FP8", "rows": 32768, "in": 13824, "out": 5120, "type": "F32",
-         "bias": False, "gate": True},
+        {"name": "long_clip_down", "kind": "product", "x": "FP8", "rows": 32768, "in": 13824, "out": 5120, "type": "BF16", "bias": False,
+         "gate": True},
         # the first feed-forward product of a clip with its activation, on to the second
-        {"name": "clip_swiglu", "kind": "swiglu", "w": "FP4", "x": "FP8", "rows": 3016, "in": 5376, "out": 28672, "bias": False},
+        {"name": "clip_swiglu", "kind": "swiglu", "x": "FP8", "rows": 3016, "in": 5376, "out": 28672, "bias": False},
         # the same for a short prompt in a text encoder
-        {"name": "prompt_swiglu", "kind": "swiglu", "w": "FP4", "x": "FP8", "rows": 20, "in": 5120, "out": 51200, "bias": False},
+        {"name": "prompt_swiglu", "kind": "swiglu", "x": "FP8", "rows": 20, "in": 5120, "out": 51200, "bias": False},
         # weights made four bits wide once they are loaded, and what they then stand for
         {"name": "weights", "kind": "quantize", "to": "FP4", "rows": 13824, "in": 5120, "type": "F32"},
         # a short prompt's activations before a product
@@ -78,9 +78,8 @@ def draw(rng):
         n = _row_length(rng, 14336)
         return {"kind": kind, "rows": _log_int(rng, 1, 80_000_000 // n), "in": n, "type": qt, "add": rng.random() < 0.7,
                 "modulate": rng.random() < 0.5}
-    w, x = rng.choice([("FP4", "FP8"), ("FP4", "FP8"), ("FP4", "FP4"), ("FP8", "FP8")])
     n = max(512, _row_length(rng, 25600)) if rng.random() < 0.8 else _row_length(rng, 2000)
-    c = {"kind": kind, "w": w, "x": x, "rows": 1, "in": n, "bias": rng.random() < 0.4}
+    c = {"kind": kind, "x": rng.choice(["FP8", "FP8", "FP4"]), "rows": 1, "in": n, "bias": rng.random() < 0.4}
     if kind == "swiglu":
         c["out"] = 128 * _log_int(rng, 2, 400)
     else:
@@ -194,7 +193,7 @@ def prepare(case, seed):
     s = {"case": c}
     if c["kind"] in ("product", "swiglu"):
         s["xc"], s["xs"] = _mx_rows(g, m, n, c["x"], "x")
-        s["wc"], s["ws"] = _mx_rows(g, c["out"], n, c["w"], "w")
+        s["wc"], s["ws"] = _mx_rows(g, c["out"], n, "FP4", "w")
         if c["bias"]:
             s["bias"] = torch.randn(c["out"], generator=g, device=DEV) * 0.1
         if c.get("gate"):
@@ -240,7 +239,7 @@ def _handles(s):
         h["type"] = {"F32": F.FH3_QUANT_F32, "F16": F.FH3_QUANT_F16, "BF16": F.FH3_QUANT_BF16}[c["type"]]
     if "wc" in s:
         h["x"] = F.mx(kinds[c["x"]], c["rows"], c["in"], _at(s, "xc"), _at(s, "xs"))
-        h["w"] = F.mx(kinds[c["w"]], c["out"], c["in"], _at(s, "wc"), _at(s, "ws"))
+        h["w"] = F.mx(F.FH3_MX_FP4, c["out"], c["in"], _at(s, "wc"), _at(s, "ws"))
         h["bytes"] = F.mx_matmul_workspace_bytes(h["w"], h["x"], c["kind"] == "swiglu")
         h["ws"] = torch.empty(max(1, h["bytes"]), dtype=torch.uint8, device=DEV)
     if "yc" in s:
@@ -274,7 +273,7 @@ def _run_own(s):
 # ---------------------------------------------------------------------------
 def _plain_product(s):
     c = s["case"]
-    y = torch.matmul(_values(s["xc"], s["xs"], c["x"]), _values(s["wc"], s["ws"], c["w"]).t())
+    y = torch.matmul(_values(s["xc"], s["xs"], c["x"]), _values(s["wc"], s["ws"], "FP4").t())
     if c["bias"]:
         y = y + s["bias"]
     return y
@@ -326,7 +325,7 @@ def work(case):
         return {"bytes": m * n * size + _mx_bytes(m, n, c["to"]) + (_mx_bytes(m, n, "FP4") + 2 * m * n if c["to"] == "FP4" else 0), "flops": 0}
     if c["kind"] == "norm":
         return {"bytes": m * n * (size * (3 if c["add"] else 1) + (8 if c["modulate"] else 0)) + _mx_bytes(m, n, "FP8"), "flops": 0}
-    b = _mx_bytes(m, n, c["x"]) + _mx_bytes(c["out"], n, c["w"])
+    b = _mx_bytes(m, n, c["x"]) + _mx_bytes(c["out"], n, "FP4")
     b += _mx_bytes(m, c["out"] // 2, "FP8") if c["kind"] == "swiglu" else m * c["out"] * (size + (size + 4 if c["gate"] else 0))
     return {"bytes": b, "flops": 2 * m * n * c["out"]}
 
@@ -386,7 +385,7 @@ def exact(case, seed):
             n = n + n * s["scale"].double() + s["shift"].double()
         codes, scales = _exact_quantized(n, "FP8")
         return {"codes": codes, "scales": scales, "sum": out}
-    y = _exact_values(s["xc"], s["xs"], c["x"]) @ _exact_values(s["wc"], s["ws"], c["w"]).t()
+    y = _exact_values(s["xc"], s["xs"], c["x"]) @ _exact_values(s["wc"], s["ws"], "FP4").t()
     if c["bias"]:
         y += s["bias"].double()
     if c["kind"] == "swiglu":
