@@ -1272,6 +1272,183 @@ extern "C" int fh3_hip_kv_attention_dev(const Fh3AttnCfg *c, const Fh3KvCache *k
 }
 
 // ---------------------------------------------------------------------------
+// Microscaled operands (fh3_mx.hip)
+// ---------------------------------------------------------------------------
+static int64_t mx_row_bytes(const Fh3kMx &m) { return m.type == FH3_MX_FP4 ? m.in / 2 : m.in; }
+static size_t mx_codes_span(const Fh3kMx &m) { return (size_t)((m.rows - 1) * m.ld + mx_row_bytes(m)); }
+static size_t mx_scales_span(const Fh3kMx &m) { return (size_t)((m.rows - 1) * m.lds + m.in / 32); }
+
+// Sizes, and with `arrays` set the pointers too.
+static int check_mx(const Fh3Mx *m, bool arrays, Fh3kMx *o, const char *what, const char *fn) {
+    if (!m || (m->type != FH3_MX_FP4 && m->type != FH3_MX_FP8))
+        return set_err(FH3_E_INVALID, "%s: %s is no FP4 or FP8 operand", fn, what);
+    if (m->rows <= 0 || m->rows > (1 << 24) || m->in <= 0 || m->in > (1 << 20) || m->in % 32)
+        return set_err(FH3_E_INVALID, "%s: rows of %s must be 1 to 2^24, in a multiple of 32 up to 2^20", fn, what);
+    *o = {m->type, m->rows, m->in, (uint8_t *)m->d_codes, m->ld, m->d_scales, m->ld_scales};
+    if (o->ld == 0) o->ld = mx_row_bytes(*o);
+    if (o->lds == 0) o->lds = round_up(o->in / 32, 4);
+    if (o->ld < mx_row_bytes(*o) || o->ld > (1 << 23) || o->ld % 16 || o->lds < o->in / 32 || o->lds > (1 << 23) || o->lds % 4)
+        return set_err(FH3_E_INVALID, "%s: strides of %s: codes a multiple of 16, scales of 4, no less than a row, at most 2^23", fn, what);
+    if (!arrays) return FH3_OK;
+    if (!o->codes || !o->scales || (uintptr_t)o->codes & 15u || (uintptr_t)o->scales & 3u)
+        return set_err(FH3_E_INVALID, "%s: codes of %s must be 16-byte, scales 4-byte aligned", fn, what);
+    return FH3_OK;
+}
+
+// Whether [p, p + bytes) meets the codes or the scales of m.
+static bool over_mx(const void *p, size_t bytes, const Fh3kMx &m) {
+    return overlap(p, bytes, m.codes, mx_codes_span(m)) || overlap(p, bytes, m.scales, mx_scales_span(m));
+}
+
+// Whether MX rows that a call writes meet [p, p + bytes) or each other.
+static bool mx_over(const Fh3kMx &m, const void *p, size_t bytes) { return p && over_mx(p, bytes, m); }
+static bool mx_meets_itself(const Fh3kMx &m) { return overlap(m.codes, mx_codes_span(m), m.scales, mx_scales_span(m)); }
+static bool mx_meets(const Fh3kMx &a, const Fh3kMx &b) {
+    return over_mx(a.codes, mx_codes_span(a), b) || over_mx(a.scales, mx_scales_span(a), b);
+}
+
+extern "C" int fh3_hip_mx_quantize_dev(int type, const void *d_x, int64_t ldx, const Fh3Mx *y, void *stream) {
+    const char *fn = "fh3_hip_mx_quantize_dev";
+    Fh3kMx m;
+    int rc = check_mx(y, true, &m, "y", fn);
+    if (rc != FH3_OK) return rc;
+    if (!value_bytes(type)) return set_err(FH3_E_INVALID, "%s: type %d is not F32, F16 or BF16", fn, type);
+    if ((rc = check_rows(d_x, &ldx, m.in, type, "x", fn)) != FH3_OK) return rc;
+    if (mx_meets_itself(m) || mx_over(m, d_x, span(m.rows, ldx, m.in, type)))
+        return set_err(FH3_E_INVALID, "%s: x, y's codes and y's scales overlap", fn);
+    if ((rc = ensure_init()) != FH3_OK) return rc;
+    FragRt::On on_device(g.device);
+    FH3_HIPCALL(fh3k_mx_quantize(type, d_x, ldx, &m, stream ? (hipStream_t)stream : g.stream));
+    return FH3_OK;
+}
+
+extern "C" int fh3_hip_mx_dequant_dev(const Fh3Mx *x, int type, void *d_y, int64_t ldy, void *stream) {
+    const char *fn = "fh3_hip_mx_dequant_dev";
+    Fh3kMx m;
+    int rc = check_mx(x, true, &m, "x", fn);
+    if (rc != FH3_OK) return rc;
+    if (!value_bytes(type)) return set_err(FH3_E_INVALID, "%s: type %d is not F32, F16 or BF16", fn, type);
+    if ((rc = check_rows(d_y, &ldy, m.in, type, "y", fn)) != FH3_OK) return rc;
+    if (over_mx(d_y, span(m.rows, ldy, m.in, type), m)) return set_err(FH3_E_INVALID, "%s: y overlaps x", fn);
+    if ((rc = ensure_init()) != FH3_OK) return rc;
+    FragRt::On on_device(g.device);
+    FH3_HIPCALL(fh3k_mx_dequant(&m, type, d_y, ldy, stream ? (hipStream_t)stream : g.stream));
+    return FH3_OK;
+}
+
+extern "C" int fh3_hip_mx_norm_dev(int type, const void *d_x, int64_t ldx, const void *d_add, int64_t ldadd, void *d_sum,
+                                   int64_t ldsum, const float *d_norm_w, float eps, const float *d_shift,
+                                   const float *d_scale, const Fh3Mx *y, void *stream) {
+    const char *fn = "fh3_hip_mx_norm_dev";
+    Fh3kMx m;
+    int rc = check_mx(y, true, &m, "y", fn);
+    if (rc != FH3_OK) return rc;
+    if (m.in > fh3k_max_in())
+        return set_err(FH3_E_INVALID, "%s: in=%lld is above %d", fn, (long long)m.in, fh3k_max_in());
+    if (!value_bytes(type)) return set_err(FH3_E_INVALID, "%s: type %d is not F32, F16 or BF16", fn, type);
+    if (!d_norm_w || (d_shift == nullptr) != (d_scale == nullptr) || (d_add && !d_sum) || !(eps >= 0.f && eps <= 1e30f))
+        return set_err(FH3_E_INVALID, "%s: bad arguments", fn);
+    if (((uintptr_t)d_norm_w & 15u) || ((uintptr_t)d_shift & 15u) || ((uintptr_t)d_scale & 15u))
+        return set_err(FH3_E_INVALID, "%s: pointers must be 16-byte aligned", fn);
+    if ((rc = check_rows(d_x, &ldx, m.in, type, "x", fn)) != FH3_OK) return rc;
+    if (d_add && (rc = check_rows(d_add, &ldadd, m.in, type, "add", fn)) != FH3_OK) return rc;
+    if (d_sum && (rc = check_rows(d_sum, &ldsum, m.in, type, "sum", fn)) != FH3_OK) return rc;
+    const size_t nx = span(m.rows, ldx, m.in, type), na = d_add ? span(m.rows, ldadd, m.in, type) : 0;
+    const size_t ns = d_sum ? span(m.rows, ldsum, m.in, type) : 0, nf = (size_t)m.in * sizeof(float), nm = nf * (size_t)m.rows;
+    if (mx_meets_itself(m) || mx_over(m, d_x, nx) || mx_over(m, d_add, na) || mx_over(m, d_sum, ns) ||
+        mx_over(m, d_norm_w, nf) || mx_over(m, d_shift, nm) || mx_over(m, d_scale, nm))
+        return set_err(FH3_E_INVALID, "%s: y overlaps another array", fn);
+    if (d_sum && ((overlap(d_sum, ns, d_x, nx) && !(d_sum == d_x && ldsum == ldx)) ||
+                  (d_add && overlap(d_sum, ns, d_add, na) && !(d_sum == d_add && ldsum == ldadd)) ||
+                  overlap(d_sum, ns, d_norm_w, nf) || (d_shift && (overlap(d_sum, ns, d_shift, nm) || overlap(d_sum, ns, d_scale, nm)))))
+        return set_err(FH3_E_INVALID, "%s: sum overlaps another array and is not x or add itself", fn);
+    if ((rc = ensure_init()) != FH3_OK) return rc;
+    FragRt::On on_device(g.device);
+    FH3_HIPCALL(fh3k_mx_norm(type, d_x, ldx, d_add, ldadd, d_sum, ldsum, d_norm_w, eps, d_shift, d_scale, &m,
+                             stream ? (hipStream_t)stream : g.stream));
+    return FH3_OK;
+}
+
+static int check_mx_product(const Fh3Mx *w, const Fh3Mx *x, bool arrays, bool swiglu, Fh3kMx *kw, Fh3kMx *kx, const char *fn) {
+    int rc = check_mx(w, arrays, kw, "w", fn);
+    if (rc == FH3_OK) rc = check_mx(x, arrays, kx, "x", fn);
+    if (rc != FH3_OK) return rc;
+    if (w->type != FH3_MX_FP4) return set_err(FH3_E_INVALID, "%s: weights must be FP4", fn);
+    if (w->in != x->in) return set_err(FH3_E_INVALID, "%s: rows of w and x differ in length", fn);
+    if (swiglu && w->rows % 128) return set_err(FH3_E_INVALID, "%s: w's rows must be a multiple of 128", fn);
+    if (!fh3k_mx_matmul_fits(kw, kx)) return set_err(FH3_E_INVALID, "%s: too many tiles for one launch", fn);
+    return FH3_OK;
+}
+
+extern "C" size_t fh3_hip_mx_matmul_workspace_bytes(const Fh3Mx *w, const Fh3Mx *x, int swiglu) {
+    Fh3kMx kw, kx;
+    if (check_mx_product(w, x, false, swiglu != 0, &kw, &kx, "fh3_hip_mx_matmul_workspace_bytes") != FH3_OK) return 0;
+    return fh3k_mx_matmul_ws_bytes(&kw, &kx, swiglu != 0);
+}
+
+// The inputs, the bias and the workspace of a product; `out` is tested against all of them.
+static int check_mx_ws(const Fh3kMx &w, const Fh3kMx &x, const float *bias, void *ws, size_t ws_bytes, size_t need,
+                       const char *fn) {
+    if ((uintptr_t)bias & 3u) return set_err(FH3_E_INVALID, "%s: bias misaligned", fn);
+    if (ws_bytes < need || (need && (!ws || (uintptr_t)ws & 15u)))
+        return set_err(FH3_E_INVALID, "%s: a 16-byte aligned workspace of %zu bytes is needed (%zu given)", fn, need, ws_bytes);
+    if (need && (over_mx(ws, need, w) || over_mx(ws, need, x) || (bias && overlap(ws, need, bias, (size_t)w.rows * sizeof(float)))))
+        return set_err(FH3_E_INVALID, "%s: the workspace overlaps an input", fn);
+    return FH3_OK;
+}
+
+extern "C" int fh3_hip_mx_matmul_dev(const Fh3Mx *w, const Fh3Mx *x, const float *d_bias, const float *d_gate,
+                                     const void *d_res, int64_t ldres, int type, void *d_y, int64_t ldy, void *d_ws,
+                                     size_t ws_bytes, void *stream) {
+    const char *fn = "fh3_hip_mx_matmul_dev";
+    Fh3kMx kw, kx;
+    int rc = check_mx_product(w, x, true, false, &kw, &kx, fn);
+    if (rc != FH3_OK) return rc;
+    const size_t size = value_bytes(type);
+    if (!size) return set_err(FH3_E_INVALID, "%s: type %d is not F32, F16 or BF16", fn, type);
+    const int64_t n = kw.rows;
+    if (ldy == 0) ldy = n;
+    if (ldres == 0) ldres = n;
+    if (!d_y || (uintptr_t)d_y % size || ldy < n || ldy > (1 << 25) || (d_gate && !d_res) || (uintptr_t)d_gate & 3u ||
+        (d_res && ((uintptr_t)d_res % size || ldres < n || ldres > (1 << 25))))
+        return set_err(FH3_E_INVALID, "%s: y, res and gate must be aligned to their type, with strides from w's rows to "
+                                      "2^25; gate needs res", fn);
+    const size_t need = fh3k_mx_matmul_ws_bytes(&kw, &kx, 0), ny = span(kx.rows, ldy, n, type);
+    if ((rc = check_mx_ws(kw, kx, d_bias, d_ws, ws_bytes, need, fn)) != FH3_OK) return rc;
+    const size_t nr = d_res ? span(kx.rows, ldres, n, type) : 0, ng = (size_t)kx.rows * n * sizeof(float);
+    if (over_mx(d_y, ny, kw) || over_mx(d_y, ny, kx) || (d_bias && overlap(d_y, ny, d_bias, n * sizeof(float))) ||
+        (d_gate && overlap(d_y, ny, d_gate, ng)) || (d_res && overlap(d_y, ny, d_res, nr) && !(d_res == d_y && ldres == ldy)) ||
+        (need && (overlap(d_ws, need, d_y, ny) || (d_gate && overlap(d_ws, need, d_gate, ng)) || (d_res && overlap(d_ws, need, d_res, nr)))))
+        return set_err(FH3_E_INVALID, "%s: y or the workspace overlaps another array", fn);
+    if ((rc = ensure_init()) != FH3_OK) return rc;
+    FragRt::On on_device(g.device);
+    const Fh3kMxOut o = {d_bias, d_gate, d_res, ldres, type, d_y, ldy, nullptr};
+    FH3_HIPCALL(fh3k_mx_matmul(&kw, &kx, &o, d_ws, stream ? (hipStream_t)stream : g.stream));
+    return FH3_OK;
+}
+
+extern "C" int fh3_hip_mx_matmul_swiglu_dev(const Fh3Mx *w, const Fh3Mx *x, const float *d_bias, const Fh3Mx *y, void *d_ws,
+                                            size_t ws_bytes, void *stream) {
+    const char *fn = "fh3_hip_mx_matmul_swiglu_dev";
+    Fh3kMx kw, kx, ky;
+    int rc = check_mx_product(w, x, true, true, &kw, &kx, fn);
+    if (rc == FH3_OK) rc = check_mx(y, true, &ky, "y", fn);
+    if (rc != FH3_OK) return rc;
+    if (ky.rows != kx.rows || 2 * ky.in != kw.rows)
+        return set_err(FH3_E_INVALID, "%s: y must have x's rows of half as many values as w has rows", fn);
+    const size_t need = fh3k_mx_matmul_ws_bytes(&kw, &kx, 1);
+    if ((rc = check_mx_ws(kw, kx, d_bias, d_ws, ws_bytes, need, fn)) != FH3_OK) return rc;
+    if (mx_meets_itself(ky) || mx_meets(ky, kw) || mx_meets(ky, kx) || mx_over(ky, d_bias, (size_t)kw.rows * sizeof(float)) ||
+        (need && over_mx(d_ws, need, ky)))
+        return set_err(FH3_E_INVALID, "%s: y overlaps another array", fn);
+    if ((rc = ensure_init()) != FH3_OK) return rc;
+    FragRt::On on_device(g.device);
+    const Fh3kMxOut o = {d_bias, nullptr, nullptr, 0, FH3_QUANT_F32, nullptr, 0, &ky};
+    FH3_HIPCALL(fh3k_mx_matmul(&kw, &kx, &o, d_ws, stream ? (hipStream_t)stream : g.stream));
+    return FH3_OK;
+}
+
+// ---------------------------------------------------------------------------
 // Weight registration: a host range uploaded once, kept on the device and
 // found by the host-pointer wrappers, which then copy only x in and y out
 // ---------------------------------------------------------------------------

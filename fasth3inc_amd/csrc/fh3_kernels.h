@@ -202,6 +202,37 @@ size_t fh3k_kv_attn_ws_bytes(const Fh3kAttn *a, const Fh3kKv *c, Fh3kSeqs s);
 hipError_t fh3k_kv_attn(const Fh3kAttn *a, const Fh3kKv *c, const void *q, int64_t ldq, void *o, int64_t ldo,
                         Fh3kSeqs s, void *ws, hipStream_t st);
 
+// Microscaled operands (fh3_mx.hip), with strides filled in; arguments are
+// checked by the callers.
+enum { FH3K_MX_FP4 = 1, FH3K_MX_FP8 = 2 };
+typedef struct Fh3kMx {
+    int type;
+    int64_t rows, in;
+    uint8_t *codes;
+    int64_t ld;
+    uint8_t *scales;
+    int64_t lds;
+} Fh3kMx;
+// What is done with a product's sums: rows of `type`, or (y set) SwiGLU to MX rows.
+typedef struct Fh3kMxOut {
+    const float *bias, *gate;
+    const void *res;
+    int64_t ldres;
+    int type;
+    void *out;
+    int64_t ldo;
+    const Fh3kMx *y;
+} Fh3kMxOut;
+hipError_t fh3k_mx_quantize(int type, const void *x, int64_t ldx, const Fh3kMx *y, hipStream_t st);
+hipError_t fh3k_mx_dequant(const Fh3kMx *x, int type, void *y, int64_t ldy, hipStream_t st);
+hipError_t fh3k_mx_norm(int type, const void *x, int64_t ldx, const void *add, int64_t lda, void *sum, int64_t lds,
+                        const float *w, float eps, const float *shift, const float *scale, const Fh3kMx *y,
+                        hipStream_t st);
+// Whether launches can number the product's tiles.
+int fh3k_mx_matmul_fits(const Fh3kMx *w, const Fh3kMx *x);
+size_t fh3k_mx_matmul_ws_bytes(const Fh3kMx *w, const Fh3kMx *x, int swiglu);
+hipError_t fh3k_mx_matmul(const Fh3kMx *w, const Fh3kMx *x, const Fh3kMxOut *o, void *ws, hipStream_t st);
+
 // Largest in-dimension (K) the activation preparation handles.
 int fh3k_max_in(void);
 

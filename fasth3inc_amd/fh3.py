@@ -27,6 +27,9 @@ FH3_QUANT_Q5_K = 13
 FH3_QUANT_Q6_K = 14
 FH3_QUANT_BF16 = 30
 
+FH3_MX_FP4 = 1
+FH3_MX_FP8 = 2
+
 FH3_OK = 0
 FH3_ERR = -1
 FH3_E_IO = -2
@@ -84,6 +87,11 @@ class Fh3KvCache(ctypes.Structure):      # include/fh3/fh3_hip.h
     _fields_ = [("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("pages", ctypes.c_int),
                 ("max_pages", ctypes.c_int), ("d_pool", ctypes.c_void_p), ("d_table", ctypes.c_void_p),
                 ("d_len", ctypes.c_void_p)]
+
+
+class Fh3Mx(ctypes.Structure):           # include/fh3/fh3_hip.h
+    _fields_ = [("type", ctypes.c_int), ("rows", ctypes.c_int64), ("in_", ctypes.c_int64), ("d_codes", ctypes.c_void_p),
+                ("ld", ctypes.c_int64), ("d_scales", ctypes.c_void_p), ("ld_scales", ctypes.c_int64)]
 
 
 class Fh3LayerView(ctypes.Structure):
@@ -211,6 +219,15 @@ SIGNATURES = {
     "fh3_hip_vsa_attention_qkv_dev": (_c_int, [ctypes.POINTER(Fh3VsaCfg), _c_void_p, _c_void_p, _c_void_p,
                                                ctypes.c_float, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p,
                                                ctypes.POINTER(Fh3Seq), _c_int, _c_int, _c_void_p]),
+    "fh3_hip_mx_quantize_dev": (_c_int, [_c_int, _c_void_p, _c_i64, ctypes.POINTER(Fh3Mx), _c_void_p]),
+    "fh3_hip_mx_dequant_dev": (_c_int, [ctypes.POINTER(Fh3Mx), _c_int, _c_void_p, _c_i64, _c_void_p]),
+    "fh3_hip_mx_norm_dev": (_c_int, [_c_int, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p,
+                                     ctypes.c_float, _c_void_p, _c_void_p, ctypes.POINTER(Fh3Mx), _c_void_p]),
+    "fh3_hip_mx_matmul_workspace_bytes": (_c_size, [ctypes.POINTER(Fh3Mx), ctypes.POINTER(Fh3Mx), _c_int]),
+    "fh3_hip_mx_matmul_dev": (_c_int, [ctypes.POINTER(Fh3Mx), ctypes.POINTER(Fh3Mx), _c_void_p, _c_void_p, _c_void_p,
+                                       _c_i64, _c_int, _c_void_p, _c_i64, _c_void_p, _c_size, _c_void_p]),
+    "fh3_hip_mx_matmul_swiglu_dev": (_c_int, [ctypes.POINTER(Fh3Mx), ctypes.POINTER(Fh3Mx), _c_void_p,
+                                              ctypes.POINTER(Fh3Mx), _c_void_p, _c_size, _c_void_p]),
     "fh3_hip_register_weights": (_c_int, [_c_void_p, _c_size, ctypes.POINTER(_c_void_p)]),
     "fh3_hip_unregister_weights": (_c_int, [_c_void_p]),
     "fh3_hip_registered_ptr": (_c_void_p, [_c_void_p, _c_size]),
@@ -539,6 +556,52 @@ def kv_attention_dev(cfg, kv, d_q, d_o, n_tok, n_seq, d_ws, ws_bytes, d_first=No
     _check(lib().fh3_hip_kv_attention_dev(ctypes.byref(cfg), ctypes.byref(kv), _ptr_of(d_q), ldq, _ptr_of(d_o), ldo,
                                           n_tok, n_seq, _ptr_of(d_first), _ptr_of(d_ws), ws_bytes, stream_ptr),
            "fh3_hip_kv_attention_dev")
+
+
+def mx(mx_type, rows, n, d_codes, d_scales, ld=0, ld_scales=0):
+    """An Fh3Mx over device buffers that the caller keeps alive."""
+    return Fh3Mx(mx_type, rows, n, _ptr_of(d_codes), ld, _ptr_of(d_scales), ld_scales)
+
+
+def mx_bytes(mx_type, rows, n):
+    """Bytes of the codes and of the scales of dense rows."""
+    return rows * (n // 2 if mx_type == FH3_MX_FP4 else n), rows * ((n // 32 + 3) // 4 * 4)
+
+
+def mx_quantize_dev(qtype, d_x, y, ldx=0, stream_ptr=None):
+    """fh3_hip_mx_quantize_dev: rows to microscaled codes."""
+    _check(lib().fh3_hip_mx_quantize_dev(qtype, _ptr_of(d_x), ldx, ctypes.byref(y), stream_ptr), "fh3_hip_mx_quantize_dev")
+
+
+def mx_dequant_dev(x, qtype, d_y, ldy=0, stream_ptr=None):
+    """fh3_hip_mx_dequant_dev: the values of microscaled rows."""
+    _check(lib().fh3_hip_mx_dequant_dev(ctypes.byref(x), qtype, _ptr_of(d_y), ldy, stream_ptr), "fh3_hip_mx_dequant_dev")
+
+
+def mx_norm_dev(qtype, d_x, d_norm_w, eps, y, d_add=None, d_sum=None, d_shift=None, d_scale=None, ldx=0, ldadd=0,
+                ldsum=0, stream_ptr=None):
+    """fh3_hip_mx_norm_dev: residual addition, rmsnorm (and modulation), microscaled output."""
+    _check(lib().fh3_hip_mx_norm_dev(qtype, _ptr_of(d_x), ldx, _ptr_of(d_add), ldadd, _ptr_of(d_sum), ldsum,
+                                     _ptr_of(d_norm_w), eps, _ptr_of(d_shift), _ptr_of(d_scale), ctypes.byref(y),
+                                     stream_ptr), "fh3_hip_mx_norm_dev")
+
+
+def mx_matmul_workspace_bytes(w, x, swiglu=False):
+    return lib().fh3_hip_mx_matmul_workspace_bytes(ctypes.byref(w), ctypes.byref(x), int(swiglu))
+
+
+def mx_matmul_dev(w, x, qtype, d_y, d_ws=None, ws_bytes=0, d_bias=None, d_gate=None, d_res=None, ldres=0, ldy=0,
+                  stream_ptr=None):
+    """fh3_hip_mx_matmul_dev: y = x W^T (+ bias), or res + gate * that."""
+    _check(lib().fh3_hip_mx_matmul_dev(ctypes.byref(w), ctypes.byref(x), _ptr_of(d_bias), _ptr_of(d_gate),
+                                       _ptr_of(d_res), ldres, qtype, _ptr_of(d_y), ldy, _ptr_of(d_ws), ws_bytes,
+                                       stream_ptr), "fh3_hip_mx_matmul_dev")
+
+
+def mx_matmul_swiglu_dev(w, x, y, d_ws=None, ws_bytes=0, d_bias=None, stream_ptr=None):
+    """fh3_hip_mx_matmul_swiglu_dev: val * silu(gate) of the product, microscaled."""
+    _check(lib().fh3_hip_mx_matmul_swiglu_dev(ctypes.byref(w), ctypes.byref(x), _ptr_of(d_bias), ctypes.byref(y),
+                                              _ptr_of(d_ws), ws_bytes, stream_ptr), "fh3_hip_mx_matmul_swiglu_dev")
 
 
 def seq_of(n, num_text=0, num_audio=0, num_video=None, grid=(0, 0, 0)):

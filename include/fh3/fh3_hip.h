@@ -324,6 +324,85 @@ int fh3_hip_kv_attention_dev(const Fh3AttnCfg *c, const Fh3KvCache *kv, const vo
                              int64_t ldo, int n_tok, int n_seq, const int *d_first, void *d_ws, size_t ws_bytes,
                              void *stream);
 
+/* A linear layer on microscaled (MX) operands: rows of 4-bit or 8-bit codes
+ * with one power of two for each 32 of them, as the block-scaled matrix
+ * instructions take them, four and two times the rate of fp16's.  Beside
+ * fh3_hip_matmul_dev and its prologue and epilogues: weights quantised once
+ * (from fh3_hip_dequant_dev's rows or any others), activations by the norm
+ * before a product, by the product before it, or by themselves.
+ *   type       FH3_MX_FP4: e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign), two to
+ *              a byte, the first in the low half; FH3_MX_FP8: e4m3 codes (up to 448)
+ *   rows       up to 2^24
+ *   in         values of a row, a multiple of 32 up to 2^20
+ *   d_codes    device, 16-byte aligned; rows ld bytes apart (0 = dense, in / 2 or in
+ *              bytes; a multiple of 16, at most 2^23)
+ *   d_scales   device, 4-byte aligned; in / 32 bytes for each row, ld_scales bytes
+ *              apart (0 = in / 32 rounded up to a multiple of 4, which it has to be; at
+ *              most 2^23): byte s stands for 2^(s - 127), 255 for NaN
+ * A value is code * scale.  Where rows are written, the bytes between in / 32 and
+ * ld_scales stay as they were; where they are read, those do not matter. */
+#define FH3_MX_FP4 1
+#define FH3_MX_FP8 2
+typedef struct Fh3Mx {
+    int type;
+    int64_t rows;
+    int64_t in;
+    void *d_codes;
+    int64_t ld;
+    uint8_t *d_scales;
+    int64_t ld_scales;
+} Fh3Mx;
+
+/* All of the calls below are enqueued on `stream` without synchronising, allocate
+ * nothing and may be captured.  `type` is FH3_QUANT_F32, _F16 or _BF16; row
+ * strides (ldx, ...) are in values, 0 = dense.  What a call writes must not lie
+ * over what it reads, but for the places named.  Deterministic.
+ *
+ * fh3_hip_mx_quantize_dev: rows d_x [y->rows][y->in] of `type` to y.  The scale of
+ * a block is the least 2^e, e >= -127, with amax <= 6 * 2^e (FP4) or 448 * 2^e
+ * (FP8), so no code saturates; code = value / scale to the nearest, ties to even.
+ * A block that holds a NaN or an infinity gets the scale 255 and codes 0.
+ * fh3_hip_mx_dequant_dev: the values of x as `type` (rounded once; exact but where
+ * they leave its range).  Rows 16-byte aligned, ldx and ldy at most 2^23. */
+int fh3_hip_mx_quantize_dev(int type, const void *d_x, int64_t ldx, const Fh3Mx *y, void *stream);
+int fh3_hip_mx_dequant_dev(const Fh3Mx *x, int type, void *d_y, int64_t ldy, void *stream);
+
+/* The norm before a product: h = x + add, rounded to `type` and stored in d_sum;
+ * rmsnorm of the stored h with weight d_norm_w [in] and eps; with d_shift and d_scale
+ * ([rows][in] fp32, both or neither) n * (1 + scale) + shift, as
+ * fh3_hip_rownorm_dev; quantised to y as above.  d_add NULL: h = x, and d_sum may be
+ * NULL (else it gets a copy).  d_sum may be d_x or d_add itself (with its row stride).
+ * y->in at most 32768.  Sums of squares are in 64 bits: rows of any finite size. */
+int fh3_hip_mx_norm_dev(int type, const void *d_x, int64_t ldx, const void *d_add, int64_t ldadd, void *d_sum,
+                        int64_t ldsum, const float *d_norm_w, float eps, const float *d_shift, const float *d_scale,
+                        const Fh3Mx *y, void *stream);
+
+/* The product y [x->rows][w->rows] = x * W^T of `type`; w is FH3_MX_FP4, x
+ * FH3_MX_FP4 or _FP8, w->in == x->in.
+ *   d_bias    NULL or [w->rows]: added
+ *   d_res     NULL or [x->rows][w->rows] of `type`, ldres values a row: the result is
+ *             res + that, or with d_gate ([x->rows][w->rows] fp32) res + gate * that
+ *             (fh3_gate_residual).  d_res may be d_y itself (with its row stride).
+ * d_y, d_res, d_gate and d_bias need only be aligned to their type (16-byte aligned
+ * rows are faster).  Products are exact, sums fp32.  FP8 rows to F16 or BF16 outputs:
+ * the matrix instruction sums eight products at a time with 13 bits below the
+ * largest, about 1e-5 of the result; to F32 outputs the codes are split into two
+ * products for which that is exact (half the rate).  A NaN in a row of x or W
+ * makes the outputs of that row NaN and no other.
+ * d_ws: fh3_hip_mx_matmul_workspace_bytes(w, x, 0) bytes, 16-byte aligned (may be 0);
+ * calls that may overlap need one each.
+ *
+ * fh3_hip_mx_matmul_swiglu_dev: W's rows are [val (F) | gate (F)], 2 F == w->rows a
+ * multiple of 128, as FH3_EPI_SWIGLU; y [x->rows][F] = val * silu(gate), bias
+ * included, quantised as above for the product that follows.  The workspace is that
+ * of (w, x, 1).  Only the sizes and types in w and x are read for its size; 0 is
+ * also the answer for sizes that are refused. */
+size_t fh3_hip_mx_matmul_workspace_bytes(const Fh3Mx *w, const Fh3Mx *x, int swiglu);
+int fh3_hip_mx_matmul_dev(const Fh3Mx *w, const Fh3Mx *x, const float *d_bias, const float *d_gate, const void *d_res,
+                          int64_t ldres, int type, void *d_y, int64_t ldy, void *d_ws, size_t ws_bytes, void *stream);
+int fh3_hip_mx_matmul_swiglu_dev(const Fh3Mx *w, const Fh3Mx *x, const float *d_bias, const Fh3Mx *y, void *d_ws,
+                                 size_t ws_bytes, void *stream);
+
 /* Weight registration (the boundary's "host data -> device pointer" hook).
  * fh3_hip_register_weights uploads [host, host + bytes) once and keeps the
  * copy on the device; the host-pointer wrappers fh3_matmul / fh3_dequant then
