@@ -1422,7 +1422,7 @@ extern "C" int fh3_hip_mx_matmul_dev(const Fh3Mx *w, const Fh3Mx *x, const float
         return set_err(FH3_E_INVALID, "%s: y or the workspace overlaps another array", fn);
     if ((rc = ensure_init()) != FH3_OK) return rc;
     FragRt::On on_device(g.device);
-    const Fh3kMxOut o = {d_bias, d_gate, d_res, ldres, type, d_y, ldy, nullptr};
+    const Fh3kMxOut o = {d_bias, d_gate, d_res, ldres, type, d_y, ldy, {}};
     FH3_HIPCALL(fh3k_mx_matmul(&kw, &kx, &o, d_ws, stream ? (hipStream_t)stream : g.stream));
     return FH3_OK;
 }
@@ -1443,7 +1443,7 @@ extern "C" int fh3_hip_mx_matmul_swiglu_dev(const Fh3Mx *w, const Fh3Mx *x, cons
         return set_err(FH3_E_INVALID, "%s: y overlaps another array", fn);
     if ((rc = ensure_init()) != FH3_OK) return rc;
     FragRt::On on_device(g.device);
-    const Fh3kMxOut o = {d_bias, nullptr, nullptr, 0, FH3_QUANT_F32, nullptr, 0, &ky};
+    const Fh3kMxOut o = {d_bias, nullptr, nullptr, 0, FH3_QUANT_F32, nullptr, 0, ky};
     FH3_HIPCALL(fh3k_mx_matmul(&kw, &kx, &o, d_ws, stream ? (hipStream_t)stream : g.stream));
     return FH3_OK;
 }

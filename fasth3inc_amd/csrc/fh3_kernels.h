@@ -213,7 +213,7 @@ typedef struct Fh3kMx {
     uint8_t *scales;
     int64_t lds;
 } Fh3kMx;
-// What is done with a product's sums: rows of `type`, or (y set) SwiGLU to MX rows.
+// What is done with a product's sums: rows of `type`, or (y.codes set) SwiGLU to MX rows.
 typedef struct Fh3kMxOut {
     const float *bias, *gate;
     const void *res;
@@ -221,7 +221,7 @@ typedef struct Fh3kMxOut {
     int type;
     void *out;
     int64_t ldo;
-    const Fh3kMx *y;
+    Fh3kMx y;
 } Fh3kMxOut;
 hipError_t fh3k_mx_quantize(int type, const void *x, int64_t ldx, const Fh3kMx *y, hipStream_t st);
 hipError_t fh3k_mx_dequant(const Fh3kMx *x, int type, void *y, int64_t ldy, hipStream_t st);

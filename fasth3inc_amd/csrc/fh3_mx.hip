@@ -234,10 +234,7 @@ template <int T, bool F8, int C> __global__ __launch_bounds__(1024) void k_mx_no
 }
 
 // ---------------------------------------------------------------------------
-// Product.  One wavefront: 16 weight rows (A) x 16 tokens (B), 128 values of a
-// row at a step.  v_mfma_scale_f32_16x16x128: lane (r, g) holds of row r the FP4
-// codes 32 g .. 32 g + 31, or the FP8 codes 16 g .. + 15 and 64 + 16 g .. + 15, and
-// the scale of block g in either case.
+// Products
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ void set4(i32x8 &v, int at, const u32x4 &a) {
 #pragma unroll
@@ -252,75 +249,488 @@ __device__ __forceinline__ uint32_t fp8_large(uint32_t c) {
 }
 
 
-template <bool F8> __global__ __launch_bounds__(256) void k_mx_simple(Fh3kMx w, Fh3kMx x, float *__restrict__ y) {
-    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const int64_t n0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16, m0 = (int64_t)blockIdx.y * 16;
-    if (n0 >= w.rows) return;
-    const int64_t n = n0 + r < w.rows ? n0 + r : w.rows - 1, m = m0 + r < x.rows ? m0 + r : x.rows - 1;
-    const uint8_t *wc = w.codes + n * w.ld, *xc = x.codes + m * x.ld, *ws = w.scales + n * w.lds, *xs = x.scales + m * x.lds;
-    const int nb = (int)(w.in / MX_BLOCK);
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int b = 0; b < nb; b += 4) {
-        i32x8 a = {}, c = {};
-        int sa = 0, sb = 0;
-        if (b + g < nb) {
-            set4(a, 0, *(const u32x4 *)(wc + (b + g) * 16));
-            sa = ws[b + g];
-            sb = xs[b + g];
-            if (!F8) set4(c, 0, *(const u32x4 *)(xc + (b + g) * 16));
+// ---------------------------------------------------------------------------
+// Many rows: tiles of BW weight rows x BX tokens, four wavefronts of TW x TX
+// products of 32 x 32.  v_mfma_scale_f32_32x32x64: lane (r, g), g = 0 or 1, holds of
+// row r the FP4 codes 32 g .. + 31, or the FP8 codes 16 g .. + 15 and 32 + 16 g .. + 15,
+// and the scale of block g.  A stage is 256 values of a row (128 with FP8 rows), its
+// blocks taken so that a lane's scales lie side by side: block g of step t is the
+// stage's block g * T + t, so one read brings a row's scales for all T steps and
+// the instruction picks the byte.
+// Rows come to LDS by DMA in 16-byte pieces (a line of 128 bytes to eight lanes), piece
+// p of row r at place p ^ r % 8, so that eight rows' pieces p lie in different banks.
+// ---------------------------------------------------------------------------
+typedef __attribute__((address_space(3))) void lds_void;
+
+template <int TW_, int TX_, bool F8_> struct Gemm {
+    static constexpr int TW = TW_, TX = TX_;
+    static constexpr bool F8 = F8_;
+    static constexpr int KS = F8 ? 128 : 256, NB = KS / MX_BLOCK, T = NB / 2;
+    static constexpr int WROW = KS / 2, XROW = 128;      // bytes of a stage's row
+    static constexpr int BW = TW * 64, BX = TX * 64;
+    static constexpr int NBUF = F8 ? 3 : 2;
+    static constexpr int WI = BW * WROW / 4096, XI = BX * XROW / 4096;                   // DMA instructions of a wavefront
+    static constexpr int WSD = BW * NB / 16, XSD = BX * NB / 16;                         // dwords of scales, likewise
+    static constexpr int LOADS = WI + XI + (WSD + 63) / 64 + (XSD + 63) / 64;
+    struct Buf {
+        u32x4 x[BX * XROW / 16], w[BW * WROW / 16];
+        uint32_t xs[BX * NB / 4], ws[BW * NB / 4];
+    };
+};
+
+// What a wavefront loads of one operand: a quarter of the tile's rows.
+template <int N, int SD> struct Rows {
+    __amdgpu_buffer_rsrc_t code, scale;
+    uint32_t off[N];                    // of this lane's piece, for each instruction
+    uint32_t soff[(SD + 63) / 64];
+};
+constexpr uint32_t MX_OUTSIDE = 0xC0000000u;   // past every buffer here: reads as zero
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rsrc(const void *p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, (int)bytes, 0x00020000);
+}
+
+// rows base .. base + count - 1 of m (those past its end: its last row), ROW bytes a stage
+template <int ROW, int NB, int N, int SD> __device__ __forceinline__ void mx_rows(Rows<N, SD> &o, const Fh3kMx &m, int64_t base, int lane) {
+    constexpr int P = ROW / 16, RPI = 64 / P;
+    if (base >= m.rows) base = m.rows - 1;
+    const int64_t left = m.rows - base;
+    const int last = left < N * RPI ? (int)left - 1 : N * RPI - 1;
+    o.code = mx_rsrc(m.codes + base * m.ld, (uint32_t)(last * m.ld + (m.type == FH3K_MX_FP8 ? m.in : m.in / 2)));
+    o.scale = mx_rsrc(m.scales + base * m.lds, (uint32_t)(last * m.lds + (m.in / MX_BLOCK + 3) / 4 * 4));
+    const int sub = lane / P, slot = lane % P;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        const int r = j * RPI + sub, piece = slot ^ (P == 8 ? r & 7 : (r >> 1) & 3);
+        o.off[j] = (uint32_t)((r < last ? r : last) * m.ld) + piece * 16;
+    }
+#pragma unroll
+    for (int j = 0; j < (SD + 63) / 64; j++) {
+        const int d = j * 64 + lane, r = d / (NB / 4);
+        o.soff[j] = (uint32_t)((r < last ? r : last) * m.lds) + d % (NB / 4) * 4;
+    }
+}
+
+template <int ROW, int N, int SD> __device__ __forceinline__ void mx_dma(const Rows<N, SD> &o, u32x4 *code, uint32_t *scale, int lane, int wave,
+                                                                         int st, int sb, int pieces) {
+    constexpr int P = ROW / 16;
+    if (pieces >= P) {
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(o.code, (lds_void *)(code + (wave * N + j) * 64), 16, o.off[j], st * ROW, 0, 0);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const int sub = j * (64 / P) + lane / P, piece = lane % P ^ (P == 8 ? sub & 7 : (sub >> 1) & 3);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(o.code, (lds_void *)(code + (wave * N + j) * 64), 16,
+                                                     piece < pieces ? o.off[j] : MX_OUTSIDE, st * ROW, 0, 0);
         }
-        if constexpr (F8) {
-            if (b + (g >> 1) < nb) set4(c, 0, *(const u32x4 *)(xc + b * 32 + g * 16));
-            if (b + 2 + (g >> 1) < nb) set4(c, 4, *(const u32x4 *)(xc + b * 32 + 64 + g * 16));
-            i32x8 h;
+    }
+#pragma unroll
+    for (int j = 0; j < (SD + 63) / 64; j++) {
+        if (SD % 64 == 0 || lane < SD % 64)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(o.scale, (lds_void *)(scale + wave * SD + j * 64), 4, o.soff[j], st * sb, 0, 0);
+    }
+}
+
+// Stage st of both operands; left: blocks of the rows from there on (none: no memory is read, but as many loads issued).
+template <class G> __device__ __forceinline__ void mx_load(const Rows<G::WI, G::WSD> &lw, const Rows<G::XI, G::XSD> &lx, typename G::Buf &b,
+                                                          int lane, int wave, int st, int left) {
+    left = left < G::NB ? left : G::NB;
+    mx_dma<G::WROW, G::WI, G::WSD>(lw, b.w, b.ws, lane, wave, st, G::NB, left);
+    mx_dma<G::XROW, G::XI, G::XSD>(lx, b.x, b.xs, lane, wave, st, G::NB, G::F8 ? 2 * left : left);
+}
+
+template <class G> struct Frags {
+    u32x4 w[G::TW];
+    typename std::conditional<G::F8, i32x8, u32x4>::type x[G::TX];
+};
+template <class G> struct Scales {
+    int w[G::TW], x[G::TX];
+};
+
+// piece p of row r of a stage's rows
+template <int ROW> __device__ __forceinline__ u32x4 mx_piece(const u32x4 *b, int r, int p) {
+    constexpr int P = ROW / 16;
+    return b[r * P + (p ^ (P == 8 ? r & 7 : (r >> 1) & 3))];
+}
+
+// Operand n (0 .. TW - 1: weights, then tokens) of step t.
+template <class G, int t, int n> __device__ __forceinline__ void mx_read(Frags<G> &f, const typename G::Buf &b, int wr, int xr, int g) {
+    if constexpr (n < G::TW) {
+        f.w[n] = mx_piece<G::WROW>(b.w, wr + 32 * n, g * G::T + t);
+    } else if constexpr (n < G::TW + G::TX) {
+        constexpr int i = n - G::TW;
+        if constexpr (G::F8) {
+            set4(f.x[i], 0, mx_piece<G::XROW>(b.x, xr + 32 * i, 2 * t + g));
+            set4(f.x[i], 4, mx_piece<G::XROW>(b.x, xr + 32 * i, 2 * (G::T + t) + g));
+        } else {
+            f.x[i] = mx_piece<G::XROW>(b.x, xr + 32 * i, g * G::T + t);
+        }
+    }
+}
+// The scales of a row for all steps; keep: zeros where the row has ended.
+template <class G, int n> __device__ __forceinline__ void mx_read_scale(Scales<G> &s, const typename G::Buf &b, int wr, int xr, int g, int keep) {
+    const uint32_t *p = n < G::TW ? b.ws : b.xs;
+    const int r = n < G::TW ? wr + 32 * n : xr + 32 * (n - G::TW);
+    int v;
+    if constexpr (G::NB == 8) v = (int)p[r * 2 + g];
+    else v = (int)((const uint16_t *)p)[r * 2 + g];
+    v &= keep;
+    if constexpr (n < G::TW) s.w[n] = v;
+    else s.x[n - G::TW] = v;
+}
+
+// The products of TW tiles of weights with one of tokens, sums in accumulation
+// registers.  The nops stand between an operand made by the VALU (scales, split codes)
+// and the matrix instruction that reads it, which the compiler does not see here.
+#define MX_MFMA(C, W, S, FMT, SEL) "v_mfma_scale_f32_32x32x64_f8f6f4 " C ", " W ", %[x], " C ", " S ", %[xs] " SEL " cbsz:4" FMT "\n\t"
+#define MX_MFMA4(FMT, SEL)                                                                                           \
+    asm volatile("s_nop 1\n\t" MX_MFMA("%0", "%[w0]", "%[s0]", FMT, SEL) MX_MFMA("%1", "%[w1]", "%[s1]", FMT, SEL)   \
+                     MX_MFMA("%2", "%[w2]", "%[s2]", FMT, SEL) MX_MFMA("%3", "%[w3]", "%[s3]", FMT, SEL)              \
+                 : "+a"(acc[0]), "+a"(acc[1]), "+a"(acc[2]), "+a"(acc[3])                                            \
+                 : [w0] "v"(w[0]), [w1] "v"(w[1]), [w2] "v"(w[2]), [w3] "v"(w[3]), [x] "v"(x), [s0] "v"(s[0]),        \
+                   [s1] "v"(s[1]), [s2] "v"(s[2]), [s3] "v"(s[3]), [xs] "v"(xs))
+#define MX_MFMA2(FMT, SEL)                                                                                           \
+    asm volatile("s_nop 1\n\t" MX_MFMA("%0", "%[w0]", "%[s0]", FMT, SEL) MX_MFMA("%1", "%[w1]", "%[s1]", FMT, SEL)   \
+                 : "+a"(acc[0]), "+a"(acc[1])                                                                        \
+                 : [w0] "v"(w[0]), [w1] "v"(w[1]), [x] "v"(x), [s0] "v"(s[0]), [s1] "v"(s[1]), [xs] "v"(xs))
+#define MX_SEL0 "op_sel:[0,0,0] op_sel_hi:[0,0,0]"
+#define MX_SEL1 "op_sel:[1,1,0] op_sel_hi:[0,0,0]"
+#define MX_SEL2 "op_sel:[0,0,0] op_sel_hi:[1,1,0]"
+#define MX_SEL3 "op_sel:[1,1,0] op_sel_hi:[1,1,0]"
+template <int t> __device__ __forceinline__ void mx_mfma(f32x16 (&acc)[4], const u32x4 (&w)[4], const int (&s)[4], const u32x4 &x, int xs) {
+    if constexpr (t == 0) MX_MFMA4(" blgp:4", MX_SEL0);
+    else if constexpr (t == 1) MX_MFMA4(" blgp:4", MX_SEL1);
+    else if constexpr (t == 2) MX_MFMA4(" blgp:4", MX_SEL2);
+    else MX_MFMA4(" blgp:4", MX_SEL3);
+}
+template <int t> __device__ __forceinline__ void mx_mfma(f32x16 (&acc)[4], const u32x4 (&w)[4], const int (&s)[4], const i32x8 &x, int xs) {
+    if constexpr (t == 0) MX_MFMA4("", MX_SEL0);
+    else MX_MFMA4("", MX_SEL1);
+}
+template <int t> __device__ __forceinline__ void mx_mfma(f32x16 (&acc)[2], const u32x4 (&w)[2], const int (&s)[2], const u32x4 &x, int xs) {
+    if constexpr (t == 0) MX_MFMA2(" blgp:4", MX_SEL0);
+    else if constexpr (t == 1) MX_MFMA2(" blgp:4", MX_SEL1);
+    else if constexpr (t == 2) MX_MFMA2(" blgp:4", MX_SEL2);
+    else MX_MFMA2(" blgp:4", MX_SEL3);
+}
+template <int t> __device__ __forceinline__ void mx_mfma(f32x16 (&acc)[2], const u32x4 (&w)[2], const int (&s)[2], const i32x8 &x, int xs) {
+    if constexpr (t == 0) MX_MFMA2("", MX_SEL0);
+    else MX_MFMA2("", MX_SEL1);
+}
+
+// Operands n .. of step t that fall to the gap behind products j of TX.
+template <class G, int t, bool SC, int n, int end> __device__ __forceinline__ void mx_reads(Frags<G> &f, Scales<G> &s, const typename G::Buf &b, int wr,
+                                                                                           int xr, int g, int keep) {
+    if constexpr (n < end) {
+        mx_read<G, t, n>(f, b, wr, xr, g);
+        if constexpr (SC) mx_read_scale<G, n>(s, b, wr, xr, g, keep);
+        mx_reads<G, t, SC, n + 1, end>(f, s, b, wr, xr, g, keep);
+    }
+}
+
+// One step's products; between them operand reads of step tn from nb, and (SC) the scales that go with them.
+template <class G, bool SPLIT, int t, int tn, bool SC, int j = 0> __device__ __forceinline__ void mx_step(
+    f32x16 (&acc)[G::TX][G::TW], const Frags<G> &f, const Scales<G> &s, Frags<G> &nf, Scales<G> &ns, const typename G::Buf &nb, int wr, int xr,
+    int g, int keep) {
+    if constexpr (j < G::TX) {
+        constexpr int per = (G::TW + G::TX) / G::TX;
+        if constexpr (SPLIT) {
+            i32x8 h, l;
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                h[k] = (int)fp8_large((uint32_t)c[k]);
-                c[k] ^= h[k];
+                h[k] = (int)fp8_large((uint32_t)f.x[j][k]);
+                l[k] = f.x[j][k] ^ h[k];
             }
-            acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, h, acc, 4, 0, 0, sa, 0, sb);
+            mx_mfma<t>(acc[j], f.w, s.w, h, s.x[j]);
+            mx_reads<G, tn, SC, j * per, (j + 1) * per>(nf, ns, nb, wr, xr, g, keep);
+            __builtin_amdgcn_sched_barrier(0);
+            mx_mfma<t>(acc[j], f.w, s.w, l, s.x[j]);
+        } else {
+            mx_mfma<t>(acc[j], f.w, s.w, f.x[j], s.x[j]);
+            mx_reads<G, tn, SC, j * per, (j + 1) * per>(nf, ns, nb, wr, xr, g, keep);
         }
-        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, c, acc, 4, F8 ? 0 : 4, 0, sa, 0, sb);
+        __builtin_amdgcn_sched_barrier(0);
+        mx_step<G, SPLIT, t, tn, SC, j + 1>(acc, f, s, nf, ns, nb, wr, xr, g, keep);
     }
-    if (m0 + r < x.rows)
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (n0 + 4 * g + k < w.rows) y[(m0 + r) * w.rows + n0 + 4 * g + k] = acc[k];
 }
 
-// Sums to outputs, a value to a thread.
+// Wait states between matrix instructions and others that touch their sums.
+template <int TX, int TW> __device__ __forceinline__ void mx_settle(f32x16 (&acc)[TX][TW]) {
+#pragma unroll
+    for (int i = 0; i < TX; i++)
+#pragma unroll
+        for (int j = 0; j < TW; j++) asm volatile("" : "+a"(acc[i][j]));
+    asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[TX - 1][TW - 1]));
+#pragma unroll
+    for (int i = 0; i < TX; i++)
+#pragma unroll
+        for (int j = 0; j < TW; j++) asm volatile("" : "+a"(acc[i][j]));
+}
+
+template <class G, int n = 0> __device__ __forceinline__ void mx_read_all(Frags<G> &f, Scales<G> &s, const typename G::Buf &b, int wr, int xr, int g,
+                                                                          int keep) {
+    if constexpr (n < G::TW + G::TX) {
+        mx_read<G, 0, n>(f, b, wr, xr, g);
+        mx_read_scale<G, n>(s, b, wr, xr, g, keep);
+        mx_read_all<G, n + 1>(f, s, b, wr, xr, g, keep);
+    }
+}
+
+constexpr int waits(int vm, int lgkm) { return (vm & 15) | 7 << 4 | lgkm << 8 | (vm >> 4) << 14; }
+
 __device__ __forceinline__ float silu(float g) { return g / (1.f + __builtin_amdgcn_exp2f(-LOG2E * g)); }
 
-template <int T> __global__ __launch_bounds__(256) void k_mx_finish(const float *__restrict__ p, int64_t rows, int64_t n, Fh3kMxOut o) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t t = i / n, c = i - t * n;
-    if (t >= rows) return;
-    float v = p[i];
-    if (o.bias) v += o.bias[c];
+// Four values of a row to where they go.
+template <int T> __device__ __forceinline__ void mx_put4(const Fh3kMxOut &o, int64_t t, int n, int64_t cols, f32x4 v) {
+    if (o.bias)
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] += o.bias[n + k];
     if (o.res) {
-        const float h = value_at(o.res, T, t * o.ldres + c);
-        v = o.gate ? __builtin_fmaf(o.gate[i], v, h) : h + v;
+        f32x4 h;
+        if constexpr (T == FH3K_F32) {
+            h = *(const f32x4 *)((const float *)o.res + t * o.ldres + n);
+        } else {
+            const u32x2 a = *(const u32x2 *)((const uint16_t *)o.res + t * o.ldres + n);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint32_t b = a[k >> 1] >> (16 * (k & 1)) & 0xFFFFu;
+                h[k] = T == FH3K_F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)b) : __builtin_bit_cast(float, b << 16);
+            }
+        }
+        if (o.gate) {
+            const f32x4 q = *(const f32x4 *)(o.gate + t * cols + n);
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] = __builtin_fmaf(q[k], v[k], h[k]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] += h[k];
+        }
     }
-    if constexpr (T == FH3K_F32) ((float *)o.out)[t * o.ldo + c] = v;
-    else ((uint16_t *)o.out)[t * o.ldo + c] = to_half<T>(v);
+    if constexpr (T == FH3K_F32) {
+        *(f32x4 *)((float *)o.out + t * o.ldo + n) = v;
+    } else {
+        u32x2 a;
+#pragma unroll
+        for (int k = 0; k < 2; k++) a[k] = to_half<T>(v[2 * k]) | (uint32_t)to_half<T>(v[2 * k + 1]) << 16;
+        *(u32x2 *)((uint16_t *)o.out + t * o.ldo + n) = a;
+    }
+}
+template <int T> __device__ __forceinline__ void mx_put1(const Fh3kMxOut &o, int64_t t, int n, int64_t cols, float v) {
+    if (o.bias) v += o.bias[n];
+    if (o.res) {
+        const float h = value_at(o.res, T, t * o.ldres + n);
+        v = o.gate ? __builtin_fmaf(o.gate[t * cols + n], v, h) : h + v;
+    }
+    if constexpr (T == FH3K_F32) ((float *)o.out)[t * o.ldo + n] = v;
+    else ((uint16_t *)o.out)[t * o.ldo + n] = to_half<T>(v);
 }
 
-template <bool F8> __global__ __launch_bounds__(256) void k_mx_swiglu(const float *__restrict__ p, const float *__restrict__ bias, Fh3kMx y) {
-    const int64_t row = blockIdx.x, f = y.in;
+// A wavefront's 32 tokens x COLS values, staged as [32][COLS / 4] pieces of four with piece c of token t at c ^ t % 16, to rows of the output.
+template <int T, int COLS> __device__ __forceinline__ void mx_rows_out(const Fh3kMxOut &o, const f32x4 *stg, int lane, int64_t t0, int64_t rows,
+                                                                       int n0, int64_t cols, bool vec) {
+    constexpr int C = COLS / 4, TPI = 64 / C;
+    if (vec) {
+        const int c = lane % C, n = n0 + 4 * c;
+        if (n >= cols) return;
+#pragma unroll 4
+        for (int it = 0; it < 32; it += TPI) {
+            const int t = it + lane / C;
+            if (t0 + t < rows) mx_put4<T>(o, t0 + t, n, cols, stg[t * C + (c ^ (t & 15))]);
+        }
+    } else {
+        const float *p = (const float *)stg;
+        for (int k = 0; k < COLS; k += 64) {
+            const int n = k + lane, c = n >> 2;
+            if (n0 + n >= cols) return;
+#pragma unroll 4
+            for (int t = 0; t < 32; t++)
+                if (t0 + t < rows) mx_put1<T>(o, t0 + t, n0 + n, cols, p[(t * C + (c ^ (t & 15))) * 4 + (n & 3)]);
+        }
+    }
+}
+// The same where the first half of the columns are values and the second their gates: SwiGLU to codes.
+template <bool F8, int COLS> __device__ __forceinline__ void mx_swiglu_out(const Fh3kMxOut &o, const f32x4 *stg, int lane, int64_t t0, int64_t rows,
+                                                                           int f0) {
+    constexpr int C = COLS / 4, L = COLS / 16, TPI = 64 / L;   // eight outputs to a lane
+    const int64_t f = o.y.in;
+    const int e = lane % L, col = f0 + 8 * e;
+    if (col >= f) return;
+#pragma unroll 2
+    for (int it = 0; it < 32; it += TPI) {
+        const int t = it + lane / L;
+        float a[8];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const f32x4 v = stg[t * C + ((2 * e + h) ^ (t & 15))], q = stg[t * C + ((C / 2 + 2 * e + h) ^ (t & 15))];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float bv = o.bias ? o.bias[col + 4 * h + k] : 0.f, bg = o.bias ? o.bias[f + col + 4 * h + k] : 0.f;
+                a[4 * h + k] = (v[k] + bv) * silu(q[k] + bg);
+            }
+        }
+        if (t0 + t < rows) mx_store<F8>(o.y, t0 + t, col, a);   // a token's lanes go together
+    }
+}
+
+template <int TW, int TX, bool F8, bool SPLIT> __global__ __launch_bounds__(256, TW == 4 ? 1 : 2) void k_mx_gemm(
+    Fh3kMx w, Fh3kMx x, Fh3kMxOut o, float *part, int64_t ldp, int m_tiles, int n_tiles, int per, bool vec) {
+    using G = Gemm<TW, TX, F8>;
+    __shared__ typename G::Buf b0, b1;
+    __shared__ typename std::conditional<G::NBUF == 3, typename G::Buf, int>::type b2;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wn = wave & 1, wm = wave >> 1, g = lane >> 5;
+    // the tiles of a band of four token tiles, column by column, on one XCD
+    constexpr int GB = 4;
+    const int total = m_tiles * n_tiles, id = blockIdx.x, share = total >> 3;
+    const int L = id < share * 8 ? (id & 7) * share + (id >> 3) : id;
+    const int band = L / (GB * n_tiles), gs = min(GB, m_tiles - band * GB), in = L - band * GB * n_tiles;
+    const int nt = in / gs, mt = band * GB + in - nt * gs;
+    const int64_t m0 = (int64_t)mt * G::BX;
+    const bool swiglu = o.y.codes != nullptr && !part;
+
+    Rows<G::WI, G::WSD> lw;
+    Rows<G::XI, G::XSD> lx;
+    const int64_t f = w.rows >> 1;
+    mx_rows<G::WROW, G::NB>(lw, w, swiglu ? (wave & 1 ? f : 0) + (int64_t)nt * (G::BW / 2) + (wave >> 1) * (G::BW / 4)
+                                         : (int64_t)nt * G::BW + wave * (G::BW / 4), lane);
+    mx_rows<G::XROW, G::NB>(lx, x, m0 + wave * (G::BX / 4), lane);
+    const int blocks = (int)(w.in / MX_BLOCK), stages = (blocks + G::NB - 1) / G::NB;
+    const int s0 = blockIdx.y * per, s1 = min(s0 + per, stages);
+
+    auto keep = [&](int st) {                        // scale bytes that stand for blocks of the row
+        const int left = blocks - st * G::NB - g * G::T;
+        return left >= G::T ? -1 : left <= 0 ? 0 : (int)((1u << (8 * left)) - 1);
+    };
+
+    f32x16 acc[TX][TW];
+#pragma unroll
+    for (int i = 0; i < TX; i++)
+#pragma unroll
+        for (int j = 0; j < TW; j++) acc[i][j] = f32x16{};
+    Frags<G> fr[2] = {};
+    Scales<G> sc, sn;
+    const int wr = wn * (G::BW / 2) + (lane & 31), xr = wm * (G::BX / 2) + (lane & 31);
+
+    mx_load<G>(lw, lx, b0, lane, wave, s0, s0 < s1 ? blocks - (s0) * G::NB : 0);
+    mx_load<G>(lw, lx, b1, lane, wave, s0 + 1, s0 + 1 < s1 ? blocks - (s0 + 1) * G::NB : 0);
+    if constexpr (G::NBUF == 3) mx_load<G>(lw, lx, b2, lane, wave, s0 + 2, s0 + 2 < s1 ? blocks - (s0 + 2) * G::NB : 0);
+    __builtin_amdgcn_s_waitcnt(waits((G::NBUF - 1) * G::LOADS, 0));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    mx_read_all<G>(fr[0], sc, b0, wr, xr, g, keep(s0));
+
+    auto stage = [&](int s, typename G::Buf &cur, const typename G::Buf &nxt) {
+        mx_step<G, SPLIT, 0, 1, false>(acc, fr[0], sc, fr[1], sn, cur, wr, xr, g, 0);
+        if constexpr (G::T == 4) {
+            mx_step<G, SPLIT, 1, 2, false>(acc, fr[1], sc, fr[0], sn, cur, wr, xr, g, 0);
+            mx_step<G, SPLIT, 2, 3, false>(acc, fr[0], sc, fr[1], sn, cur, wr, xr, g, 0);
+        }
+        // this stage's operands are all read, the next one's have landed
+        __builtin_amdgcn_s_waitcnt(waits((G::NBUF - 2) * G::LOADS, 0));
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        mx_load<G>(lw, lx, cur, lane, wave, s + G::NBUF, s + G::NBUF < s1 ? blocks - (s + G::NBUF) * G::NB : 0);
+        __builtin_amdgcn_sched_barrier(0);
+        mx_step<G, SPLIT, G::T - 1, 0, true>(acc, fr[1], sc, fr[0], sn, nxt, wr, xr, g, keep(s + 1));
+        sc = sn;
+    };
+    mx_settle(acc);
+    for (int s = s0;;) {
+        stage(s, b0, b1);
+        if (++s >= s1) break;
+        if constexpr (G::NBUF == 3) {
+            stage(s, b1, b2);
+            if (++s >= s1) break;
+            stage(s, b2, b0);
+            if (++s >= s1) break;
+        } else {
+            stage(s, b1, b0);
+            if (++s >= s1) break;
+        }
+    }
+    mx_settle(acc);
+    __builtin_amdgcn_s_waitcnt(waits(0, 0));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+
+    constexpr int COLS = TW * 32, C = COLS / 4;
+    f32x4 *stg = (f32x4 *)(wm ? b1.x : b0.x) + wn * (32 * C);
+    const int tl = lane & 31;
+    if (part) {
+        o = Fh3kMxOut{};
+        o.out = part + blockIdx.y * (x.rows * ldp);
+        o.ldo = ldp;
+    }
+    auto put = [&](const f32x16(&a)[TW]) {
+#pragma unroll
+        for (int j = 0; j < TW; j++)
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                stg[tl * C + ((8 * j + 2 * q + g) ^ (tl & 15))] = f32x4{a[j][4 * q], a[j][4 * q + 1], a[j][4 * q + 2], a[j][4 * q + 3]};
+    };
+#pragma unroll 1
+    for (int i = 0; i < TX; i++) {   // rolled: unrolled, the code of the stores runs once for each and is fetched each time
+        if (i == 0) put(acc[0]);
+        else if (i == 1) put(acc[1]);
+        if constexpr (TX == 4) {
+            if (i == 2) put(acc[2]);
+            else if (i == 3) put(acc[3]);
+        }
+        __builtin_amdgcn_wave_barrier();
+        const int64_t t0 = m0 + wm * (G::BX / 2) + 32 * i;
+        const int n0 = nt * G::BW + wn * (G::BW / 2);
+        if (swiglu) {
+            if (o.y.type == FH3K_MX_FP8) mx_swiglu_out<true, COLS>(o, stg, lane, t0, x.rows, n0 / 2);
+            else mx_swiglu_out<false, COLS>(o, stg, lane, t0, x.rows, n0 / 2);
+        } else if (o.type == FH3K_F32) mx_rows_out<FH3K_F32, COLS>(o, stg, lane, t0, x.rows, n0, w.rows, vec);
+        else if (o.type == FH3K_F16) mx_rows_out<FH3K_F16, COLS>(o, stg, lane, t0, x.rows, n0, w.rows, vec);
+        else mx_rows_out<FH3K_BF16, COLS>(o, stg, lane, t0, x.rows, n0, w.rows, vec);
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// The parts of a split product, added in their order, to rows of the output: four values to a thread.
+template <int T> __global__ __launch_bounds__(256) void k_mx_join(const float *__restrict__ part, int S, int64_t ldp, int64_t rows, int64_t cols,
+                                                                  Fh3kMxOut o, bool vec) {
+    const int64_t t = blockIdx.x;
+    const int n = 4 * (blockIdx.y * 256 + threadIdx.x);
+    if (n >= cols) return;
+    f32x4 v = *(const f32x4 *)(part + t * ldp + n);
+    for (int s = 1; s < S; s++) {
+        const f32x4 a = *(const f32x4 *)(part + (s * rows + t) * ldp + n);
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] += a[k];
+    }
+    if (vec) {
+        mx_put4<T>(o, t, n, cols, v);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (n + k < cols) mx_put1<T>(o, t, n + k, cols, v[k]);
+    }
+}
+
+template <bool F8> __global__ __launch_bounds__(256) void k_mx_join_swiglu(const float *__restrict__ part, int S, int64_t ldp, int64_t rows,
+                                                                           Fh3kMxOut o) {
+    const int64_t t = blockIdx.x, f = o.y.in;
     const int col = 8 * (blockIdx.y * 256 + threadIdx.x);
     if (col >= f) return;
-    float v[8], g[8], a[8];
-    load8<FH3K_F32>(p, row * 2 * f + col, v);
-    load8<FH3K_F32>(p, row * 2 * f + f + col, g);
+    float v[8] = {}, q[8] = {}, a[8];
+    for (int s = 0; s < S; s++) {
+        float c[8], d[8];
+        load8<FH3K_F32>(part, (s * rows + t) * ldp + col, c);
+        load8<FH3K_F32>(part, (s * rows + t) * ldp + f + col, d);
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
-        if (bias) {
-            v[k] += bias[col + k];
-            g[k] += bias[f + col + k];
+        for (int k = 0; k < 8; k++) {
+            v[k] += c[k];
+            q[k] += d[k];
         }
-        a[k] = v[k] * silu(g[k]);
     }
-    mx_store<F8>(y, row, col, a);
+#pragma unroll
+    for (int k = 0; k < 8; k++) a[k] = (v[k] + (o.bias ? o.bias[col + k] : 0.f)) * silu(q[k] + (o.bias ? o.bias[f + col + k] : 0.f));
+    mx_store<F8>(o.y, t, col, a);
 }
 
 // lanes to a row: a power of two, eight values each
@@ -377,27 +787,74 @@ extern "C" hipError_t fh3k_mx_norm(int type, const void *x, int64_t ldx, const v
     });
 }
 
+namespace {
+
+// How a product is cut: tiles, and parts of the rows' length.
+struct Plan {
+    int bw, bx, parts, per;       // per: stages of a part
+    int64_t m_tiles, n_tiles, ldp;
+};
+Plan plan_of(const Fh3kMx *w, const Fh3kMx *x) {
+    Plan p;
+    auto tiles = [&](int b) { return ((w->rows + b - 1) / b) * ((x->rows + b - 1) / b); };
+    p.bw = p.bx = tiles(256) >= 192 ? 256 : 128;
+    p.m_tiles = (x->rows + p.bx - 1) / p.bx;
+    p.n_tiles = (w->rows + p.bw - 1) / p.bw;
+    const int ks = x->type == FH3K_MX_FP8 ? 128 : 256;
+    const int stages = (int)((w->in + ks - 1) / ks);
+    const int64_t t = p.m_tiles * p.n_tiles;
+    int parts = 1;
+    if (p.bw == 128 && t < 384) parts = (int)(512 / t);
+    if (parts > stages / 4) parts = stages / 4;
+    if (parts < 1) parts = 1;
+    p.per = (stages + parts - 1) / parts;
+    p.parts = (stages + p.per - 1) / p.per;
+    p.ldp = (w->rows + 3) / 4 * 4;
+    return p;
+}
+
+template <int TW, int TX, bool F8, bool SPLIT> void launch_gemm(const Fh3kMx *w, const Fh3kMx *x, const Fh3kMxOut *o, const Plan &p, float *part,
+                                                                bool vec, hipStream_t st) {
+    const dim3 grid((unsigned)(p.m_tiles * p.n_tiles), (unsigned)p.parts);
+    k_mx_gemm<TW, TX, F8, SPLIT><<<grid, 256, 0, st>>>(*w, *x, *o, part, p.ldp, (int)p.m_tiles, (int)p.n_tiles, p.per, vec || part);
+}
+
+// Whether rows of an array, ld values apart, can be taken four at a time.
+bool fours(const void *p, int64_t ld, int size) { return !p || ((uintptr_t)p % (4 * size) == 0 && ld % 4 == 0); }
+
+}  // namespace
+
 extern "C" int fh3k_mx_matmul_fits(const Fh3kMx *w, const Fh3kMx *x) {
-    return (w->rows + 63) / 64 < ((int64_t)1 << 31) && (x->rows + 15) / 16 < 65536 &&
-           w->rows * x->rows <= ((int64_t)1 << 38);
+    const Plan p = plan_of(w, x);
+    return p.m_tiles * p.n_tiles < ((int64_t)1 << 23) && p.ldp * x->rows <= ((int64_t)1 << 40);
 }
 
 extern "C" size_t fh3k_mx_matmul_ws_bytes(const Fh3kMx *w, const Fh3kMx *x, int) {
-    return (size_t)w->rows * x->rows * sizeof(float);
+    const Plan p = plan_of(w, x);
+    return p.parts > 1 ? (size_t)p.parts * p.ldp * x->rows * sizeof(float) : 0;
 }
 
 extern "C" hipError_t fh3k_mx_matmul(const Fh3kMx *w, const Fh3kMx *x, const Fh3kMxOut *o, void *ws, hipStream_t st) {
-    const dim3 grid((unsigned)((w->rows + 63) / 64), (unsigned)((x->rows + 15) / 16));
-    float *p = (float *)ws;
-    if (x->type == FH3K_MX_FP8) k_mx_simple<true><<<grid, 256, 0, st>>>(*w, *x, p);
-    else k_mx_simple<false><<<grid, 256, 0, st>>>(*w, *x, p);
-    if (o->y) {
-        const dim3 g2((unsigned)x->rows, (unsigned)((o->y->in + 2047) / 2048));
-        if (o->y->type == FH3K_MX_FP8) k_mx_swiglu<true><<<g2, 256, 0, st>>>(p, o->bias, *o->y);
-        else k_mx_swiglu<false><<<g2, 256, 0, st>>>(p, o->bias, *o->y);
+    const Plan p = plan_of(w, x);
+    float *part = p.parts > 1 ? (float *)ws : nullptr;
+    const int size = o->type == FH3K_F32 ? 4 : 2;
+    const bool vec = w->rows % 4 == 0 && fours(o->out, o->ldo, size) && fours(o->res, o->ldres, size) && fours(o->gate, 0, 4);
+    const bool f8 = x->type == FH3K_MX_FP8, split = f8 && o->type == FH3K_F32 && !o->y.codes;
+    auto go = [&](auto tile) {
+        constexpr int N = tile();
+        if (!f8) launch_gemm<N, N, false, false>(w, x, o, p, part, vec, st);
+        else if (!split) launch_gemm<N, N, true, false>(w, x, o, p, part, vec, st);
+        else launch_gemm<N, N, true, true>(w, x, o, p, part, vec, st);
+    };
+    if (p.bw == 256) go(std::integral_constant<int, 4>{});
+    else go(std::integral_constant<int, 2>{});
+    if (!part) return hipGetLastError();
+    if (o->y.codes) {
+        const dim3 grid((unsigned)x->rows, (unsigned)((o->y.in + 2047) / 2048));
+        if (o->y.type == FH3K_MX_FP8) k_mx_join_swiglu<true><<<grid, 256, 0, st>>>(part, p.parts, p.ldp, x->rows, *o);
+        else k_mx_join_swiglu<false><<<grid, 256, 0, st>>>(part, p.parts, p.ldp, x->rows, *o);
         return hipGetLastError();
     }
-    return by_type(o->type, [&](auto t) {
-        k_mx_finish<t()><<<(unsigned)((x->rows * w->rows + 255) / 256), 256, 0, st>>>(p, x->rows, w->rows, *o);
-    });
+    const dim3 grid((unsigned)x->rows, (unsigned)((w->rows + 1023) / 1024));
+    return by_type(o->type, [&](auto t) { k_mx_join<t()><<<grid, 256, 0, st>>>(part, p.parts, p.ldp, x->rows, w->rows, *o, vec); });
 }
