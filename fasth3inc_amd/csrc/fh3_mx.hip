@@ -255,10 +255,12 @@ __device__ __forceinline__ uint32_t fp8_large(uint32_t c) {
 // row r the FP4 codes 32 g .. + 31, or the FP8 codes 16 g .. + 15 and 32 + 16 g .. + 15,
 // and the scale of block g.  A stage is 256 values of a row (128 with FP8 rows), its
 // blocks taken so that a lane's scales lie side by side: block g of step t is the
-// stage's block g * T + t, so one read brings a row's scales for all T steps and
-// the instruction picks the byte.
+// stage's block g * T + t, and the instruction picks byte t.
 // Rows come to LDS by DMA in 16-byte pieces (a line of 128 bytes to eight lanes), piece
-// p of row r at place p ^ r % 8, so that eight rows' pieces p lie in different banks.
+// p of row r at place p ^ r / 2 % 8 (rows of 64 bytes: p ^ r / 4 % 4), so that the pieces
+// p of sixteen rows lie in different banks.  Scales come for NBUF * 2 or NBUF stages at a
+// time (a request to L2 for each row's 8 or 4 bytes of a stage took as many requests
+// as the codes) and are held in registers.
 // ---------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) void lds_void;
 
@@ -268,98 +270,113 @@ template <int TW_, int TX_, bool F8_> struct Gemm {
     static constexpr int KS = F8 ? 128 : 256, NB = KS / MX_BLOCK, T = NB / 2;
     static constexpr int WROW = KS / 2, XROW = 128;      // bytes of a stage's row
     static constexpr int BW = TW * 64, BX = TX * 64;
-    static constexpr int NBUF = F8 ? 3 : 2;
-    static constexpr int WI = BW * WROW / 4096, XI = BX * XROW / 4096;                   // DMA instructions of a wavefront
-    static constexpr int WSD = BW * NB / 16, XSD = BX * NB / 16;                         // dwords of scales, likewise
-    static constexpr int LOADS = WI + XI + (WSD + 63) / 64 + (XSD + 63) / 64;
+    static constexpr int NBUF = F8 ? 3 : 2, CH = F8 ? 3 : 4;   // stages in LDS, stages of a chunk of scales
+    static constexpr int SD = F8 ? 4 : 8;                // dwords of a row's chunk in LDS
+    static constexpr int WI = BW * WROW / 4096, XI = BX * XROW / 4096, D = WI + XI;   // a wavefront's DMA instructions: a stage's codes
+    static constexpr int WS = BW * SD / 256, XS = BX * SD / 256;                       // and a chunk's scales
     struct Buf {
         u32x4 x[BX * XROW / 16], w[BW * WROW / 16];
-        uint32_t xs[BX * NB / 4], ws[BW * NB / 4];
+    };
+    struct ScaleBuf {
+        uint32_t x[BX * SD], w[BW * SD];
     };
 };
 
-// What a wavefront loads of one operand: a quarter of the tile's rows.
-template <int N, int SD> struct Rows {
-    __amdgpu_buffer_rsrc_t code, scale;
-    uint32_t off[N];                    // of this lane's piece, for each instruction
-    uint32_t soff[(SD + 63) / 64];
-};
+// place of piece p of row r among its row's P pieces, or the piece at place p
+template <int P> __device__ __forceinline__ int mx_place(int r, int p) { return p ^ (P == 8 ? (r >> 1) & 7 : (r >> 2) & 3); }
+
 constexpr uint32_t MX_OUTSIDE = 0xC0000000u;   // past every buffer here: reads as zero
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rsrc(const void *p, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, (int)bytes, 0x00020000);
 }
 
-// rows base .. base + count - 1 of m (those past its end: its last row), ROW bytes a stage
-template <int ROW, int NB, int N, int SD> __device__ __forceinline__ void mx_rows(Rows<N, SD> &o, const Fh3kMx &m, int64_t base, int lane) {
-    constexpr int P = ROW / 16, RPI = 64 / P;
-    if (base >= m.rows) base = m.rows - 1;
-    const int64_t left = m.rows - base;
-    const int last = left < N * RPI ? (int)left - 1 : N * RPI - 1;
-    o.code = mx_rsrc(m.codes + base * m.ld, (uint32_t)(last * m.ld + (m.type == FH3K_MX_FP8 ? m.in : m.in / 2)));
-    o.scale = mx_rsrc(m.scales + base * m.lds, (uint32_t)(last * m.lds + (m.in / MX_BLOCK + 3) / 4 * 4));
-    const int sub = lane / P, slot = lane % P;
-#pragma unroll
-    for (int j = 0; j < N; j++) {
-        const int r = j * RPI + sub, piece = slot ^ (P == 8 ? r & 7 : (r >> 1) & 3);
-        o.off[j] = (uint32_t)((r < last ? r : last) * m.ld) + piece * 16;
-    }
-#pragma unroll
-    for (int j = 0; j < (SD + 63) / 64; j++) {
-        const int d = j * 64 + lane, r = d / (NB / 4);
-        o.soff[j] = (uint32_t)((r < last ? r : last) * m.lds) + d % (NB / 4) * 4;
-    }
+// `at` is uniform, which the compiler loses sight of where it runs short of scalar registers
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, u32x4 *to, uint32_t off, int at) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)to, 16, off, __builtin_amdgcn_readfirstlane(at), 0, 0);
+}
+__device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t r, uint32_t *to, uint32_t off, int at) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)to, 4, off, __builtin_amdgcn_readfirstlane(at), 0, 0);
 }
 
-template <int ROW, int N, int SD> __device__ __forceinline__ void mx_dma(const Rows<N, SD> &o, u32x4 *code, uint32_t *scale, int lane, int wave,
-                                                                         int st, int sb, int pieces) {
-    constexpr int P = ROW / 16;
-    if (pieces >= P) {
+// What a wavefront loads of one operand: a quarter of the tile's rows.
+template <class G, int ROW, int N, int NS> struct Rows {
+    static constexpr int P = ROW / 16, RPI = 64 / P;   // pieces of a row, rows to an instruction
+    __amdgpu_buffer_rsrc_t code, scale;
+    uint32_t off[N], soff[NS];                         // of this lane, for each instruction
+    int piece[2];                                      // of its row, in even and odd instructions
+
+    // rows base .. of m; those past its end: its last row
+    __device__ __forceinline__ void init(const Fh3kMx &m, int64_t base, int lane) {
+        if (base >= m.rows) base = m.rows - 1;
+        const int64_t left = m.rows - base;
+        const int last = left < N * RPI ? (int)left - 1 : N * RPI - 1;
+        code = mx_rsrc(m.codes + base * m.ld, (uint32_t)(last * m.ld + (m.type == FH3K_MX_FP8 ? m.in : m.in / 2)));
+        scale = mx_rsrc(m.scales + base * m.lds, (uint32_t)(last * m.lds + (m.in / MX_BLOCK + 3) / 4 * 4));
 #pragma unroll
-        for (int j = 0; j < N; j++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(o.code, (lds_void *)(code + (wave * N + j) * 64), 16, o.off[j], st * ROW, 0, 0);
-    } else {
+        for (int j = 0; j < 2; j++) piece[j] = mx_place<P>(j * RPI + lane / P, lane % P);
 #pragma unroll
         for (int j = 0; j < N; j++) {
-            const int sub = j * (64 / P) + lane / P, piece = lane % P ^ (P == 8 ? sub & 7 : (sub >> 1) & 3);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(o.code, (lds_void *)(code + (wave * N + j) * 64), 16,
-                                                     piece < pieces ? o.off[j] : MX_OUTSIDE, st * ROW, 0, 0);
+            const int r = j * RPI + lane / P;
+            off[j] = (uint32_t)((r < last ? r : last) * m.ld) + piece[j & 1] * 16;
+        }
+        // FP4 stages have two dwords of scales to a row, here in the order [g][stage]; FP8 stages one
+#pragma unroll
+        for (int j = 0; j < NS; j++) {
+            const int d = j * 64 + lane, r = d / G::SD, k = d % G::SD;
+            soff[j] = (uint32_t)((r < last ? r : last) * m.lds) + 4 * (G::F8 ? k : (k & 3) * 2 + (k >> 2));
+            if (G::F8 && k == 3) soff[j] = MX_OUTSIDE;
         }
     }
-#pragma unroll
-    for (int j = 0; j < (SD + 63) / 64; j++) {
-        if (SD % 64 == 0 || lane < SD % 64)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(o.scale, (lds_void *)(scale + wave * SD + j * 64), 4, o.soff[j], st * sb, 0, 0);
+    // instruction j of stage st, of whose row `pieces` pieces are there
+    template <int j> __device__ __forceinline__ void dma(u32x4 *to, int wave, int st, int pieces) const {
+        dma16(code, to + (wave * N + j) * 64, piece[j & 1] < pieces ? off[j] : MX_OUTSIDE, st * ROW);
     }
-}
+    __device__ __forceinline__ void dma_scales(uint32_t *to, int wave, int st) const {
+#pragma unroll
+        for (int j = 0; j < NS; j++) dma4(scale, to + (wave * NS + j) * 64, soff[j], st * G::NB);
+    }
+};
+template <class G> struct Load {
+    Rows<G, G::WROW, G::WI, G::WS> w;
+    Rows<G, G::XROW, G::XI, G::XS> x;
+    int wave, blocks, end;              // blocks of a row; stages past the end load nothing, with as many instructions
 
-// Stage st of both operands; left: blocks of the rows from there on (none: no memory is read, but as many loads issued).
-template <class G> __device__ __forceinline__ void mx_load(const Rows<G::WI, G::WSD> &lw, const Rows<G::XI, G::XSD> &lx, typename G::Buf &b,
-                                                          int lane, int wave, int st, int left) {
-    left = left < G::NB ? left : G::NB;
-    mx_dma<G::WROW, G::WI, G::WSD>(lw, b.w, b.ws, lane, wave, st, G::NB, left);
-    mx_dma<G::XROW, G::XI, G::XSD>(lx, b.x, b.xs, lane, wave, st, G::NB, G::F8 ? 2 * left : left);
-}
+    template <int d, int to> __device__ __forceinline__ void codes(typename G::Buf &b, int st) const {
+        if constexpr (d < to) {
+            const int left = st < end ? blocks - st * G::NB : 0;
+            if constexpr (d < G::WI) w.template dma<d>(b.w, wave, st, left);
+            else x.template dma<d - G::WI>(b.x, wave, st, G::F8 ? 2 * left : left);
+            codes<d + 1, to>(b, st);
+        }
+    }
+    __device__ __forceinline__ void scales(typename G::ScaleBuf &b, int st) const {
+        w.dma_scales(b.w, wave, st);
+        x.dma_scales(b.x, wave, st);
+    }
+};
 
 template <class G> struct Frags {
     u32x4 w[G::TW];
     typename std::conditional<G::F8, i32x8, u32x4>::type x[G::TX];
 };
-template <class G> struct Scales {
+template <class G> struct Scales {       // of a chunk: a dword (FP8: both lanes' halves of one) for each stage
+    u32x4 w[G::TW], x[G::TX];
+};
+template <class G> struct StageScales {
     int w[G::TW], x[G::TX];
 };
 
 // piece p of row r of a stage's rows
 template <int ROW> __device__ __forceinline__ u32x4 mx_piece(const u32x4 *b, int r, int p) {
-    constexpr int P = ROW / 16;
-    return b[r * P + (p ^ (P == 8 ? r & 7 : (r >> 1) & 3))];
+    return b[r * (ROW / 16) + mx_place<ROW / 16>(r, p)];
 }
 
 // Operand n (0 .. TW - 1: weights, then tokens) of step t.
 template <class G, int t, int n> __device__ __forceinline__ void mx_read(Frags<G> &f, const typename G::Buf &b, int wr, int xr, int g) {
     if constexpr (n < G::TW) {
         f.w[n] = mx_piece<G::WROW>(b.w, wr + 32 * n, g * G::T + t);
-    } else if constexpr (n < G::TW + G::TX) {
+    } else {
         constexpr int i = n - G::TW;
         if constexpr (G::F8) {
             set4(f.x[i], 0, mx_piece<G::XROW>(b.x, xr + 32 * i, 2 * t + g));
@@ -369,16 +386,18 @@ template <class G, int t, int n> __device__ __forceinline__ void mx_read(Frags<G
         }
     }
 }
-// The scales of a row for all steps; keep: zeros where the row has ended.
-template <class G, int n> __device__ __forceinline__ void mx_read_scale(Scales<G> &s, const typename G::Buf &b, int wr, int xr, int g, int keep) {
-    const uint32_t *p = n < G::TW ? b.ws : b.xs;
-    const int r = n < G::TW ? wr + 32 * n : xr + 32 * (n - G::TW);
-    int v;
-    if constexpr (G::NB == 8) v = (int)p[r * 2 + g];
-    else v = (int)((const uint16_t *)p)[r * 2 + g];
-    v &= keep;
+template <class G, int n> __device__ __forceinline__ void mx_read_scale(Scales<G> &s, const typename G::ScaleBuf &b, int wr, int xr, int g) {
+    const uint32_t *p = n < G::TW ? b.w + (wr + 32 * n) * G::SD : b.x + (xr + 32 * (n - G::TW)) * G::SD;
+    const u32x4 v = *(const u32x4 *)(p + (G::F8 ? 0 : 4 * g));
     if constexpr (n < G::TW) s.w[n] = v;
     else s.x[n - G::TW] = v;
+}
+// The scales of the chunk's stage c; keep: zeros where the row has ended.
+template <class G, int c> __device__ __forceinline__ void mx_stage_scales(StageScales<G> &o, const Scales<G> &s, int g, int keep) {
+#pragma unroll
+    for (int i = 0; i < G::TW; i++) o.w[i] = (int)(G::F8 ? s.w[i][c] >> (16 * g) : s.w[i][c]) & keep;
+#pragma unroll
+    for (int i = 0; i < G::TX; i++) o.x[i] = (int)(G::F8 ? s.x[i][c] >> (16 * g) : s.x[i][c]) & keep;
 }
 
 // The products of TW tiles of weights with one of tokens, sums in accumulation
@@ -420,22 +439,29 @@ template <int t> __device__ __forceinline__ void mx_mfma(f32x16 (&acc)[2], const
     else MX_MFMA2("", MX_SEL1);
 }
 
-// Operands n .. of step t that fall to the gap behind products j of TX.
-template <class G, int t, bool SC, int n, int end> __device__ __forceinline__ void mx_reads(Frags<G> &f, Scales<G> &s, const typename G::Buf &b, int wr,
-                                                                                           int xr, int g, int keep) {
+// Operands n .. end - 1 of step t, and (SC) the chunk of scales that goes with them.
+template <class G, int t, bool SC, int n, int end> __device__ __forceinline__ void mx_reads(Frags<G> &f, Scales<G> &s, const typename G::Buf &b,
+                                                                                           const typename G::ScaleBuf &sb, int wr, int xr, int g) {
     if constexpr (n < end) {
         mx_read<G, t, n>(f, b, wr, xr, g);
-        if constexpr (SC) mx_read_scale<G, n>(s, b, wr, xr, g, keep);
-        mx_reads<G, t, SC, n + 1, end>(f, s, b, wr, xr, g, keep);
+        if constexpr (SC) mx_read_scale<G, n>(s, sb, wr, xr, g);
+        mx_reads<G, t, SC, n + 1, end>(f, s, b, sb, wr, xr, g);
     }
 }
 
-// One step's products; between them operand reads of step tn from nb, and (SC) the scales that go with them.
-template <class G, bool SPLIT, int t, int tn, bool SC, int j = 0> __device__ __forceinline__ void mx_step(
-    f32x16 (&acc)[G::TX][G::TW], const Frags<G> &f, const Scales<G> &s, Frags<G> &nf, Scales<G> &ns, const typename G::Buf &nb, int wr, int xr,
-    int g, int keep) {
+// One step's products; between them operand reads of step tn from nb (SC: and the
+// next chunk's scales), and where Q is 0 or 1 that half of stage `to`'s loads into lb.
+// Loads are issued a few at a time: all at once they kept the matrix instructions behind
+// them waiting for the address unit (8192 x 5120 -> 15360 FP4 515 us).
+template <class G, bool SPLIT, int t, int tn, bool SC, int Q, int j = 0> __device__ __forceinline__ void mx_step(
+    f32x16 (&acc)[G::TX][G::TW], const Frags<G> &f, const StageScales<G> &s, Frags<G> &nf, Scales<G> &ns, const typename G::Buf &nb,
+    const typename G::ScaleBuf &sb, const Load<G> &ld, typename G::Buf &lb, int to, int wr, int xr, int g) {
     if constexpr (j < G::TX) {
-        constexpr int per = (G::TW + G::TX) / G::TX;
+        constexpr int per = (G::TW + G::TX) / G::TX, gap = Q * G::TX + j, gaps = 2 * G::TX;
+        auto between = [&]() {
+            mx_reads<G, tn, SC, j * per, (j + 1) * per>(nf, ns, nb, sb, wr, xr, g);
+            if constexpr (Q >= 0) ld.template codes<gap * G::D / gaps, (gap + 1) * G::D / gaps>(lb, to);
+        };
         if constexpr (SPLIT) {
             i32x8 h, l;
 #pragma unroll
@@ -444,15 +470,15 @@ template <class G, bool SPLIT, int t, int tn, bool SC, int j = 0> __device__ __f
                 l[k] = f.x[j][k] ^ h[k];
             }
             mx_mfma<t>(acc[j], f.w, s.w, h, s.x[j]);
-            mx_reads<G, tn, SC, j * per, (j + 1) * per>(nf, ns, nb, wr, xr, g, keep);
+            between();
             __builtin_amdgcn_sched_barrier(0);
             mx_mfma<t>(acc[j], f.w, s.w, l, s.x[j]);
         } else {
             mx_mfma<t>(acc[j], f.w, s.w, f.x[j], s.x[j]);
-            mx_reads<G, tn, SC, j * per, (j + 1) * per>(nf, ns, nb, wr, xr, g, keep);
+            between();
         }
         __builtin_amdgcn_sched_barrier(0);
-        mx_step<G, SPLIT, t, tn, SC, j + 1>(acc, f, s, nf, ns, nb, wr, xr, g, keep);
+        mx_step<G, SPLIT, t, tn, SC, Q, j + 1>(acc, f, s, nf, ns, nb, sb, ld, lb, to, wr, xr, g);
     }
 }
 
@@ -467,15 +493,6 @@ template <int TX, int TW> __device__ __forceinline__ void mx_settle(f32x16 (&acc
     for (int i = 0; i < TX; i++)
 #pragma unroll
         for (int j = 0; j < TW; j++) asm volatile("" : "+a"(acc[i][j]));
-}
-
-template <class G, int n = 0> __device__ __forceinline__ void mx_read_all(Frags<G> &f, Scales<G> &s, const typename G::Buf &b, int wr, int xr, int g,
-                                                                          int keep) {
-    if constexpr (n < G::TW + G::TX) {
-        mx_read<G, 0, n>(f, b, wr, xr, g);
-        mx_read_scale<G, n>(s, b, wr, xr, g, keep);
-        mx_read_all<G, n + 1>(f, s, b, wr, xr, g, keep);
-    }
 }
 
 constexpr int waits(int vm, int lgkm) { return (vm & 15) | 7 << 4 | lgkm << 8 | (vm >> 4) << 14; }
@@ -579,6 +596,7 @@ template <int TW, int TX, bool F8, bool SPLIT> __global__ __launch_bounds__(256,
     using G = Gemm<TW, TX, F8>;
     __shared__ typename G::Buf b0, b1;
     __shared__ typename std::conditional<G::NBUF == 3, typename G::Buf, int>::type b2;
+    __shared__ typename G::ScaleBuf sb;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wn = wave & 1, wm = wave >> 1, g = lane >> 5;
     // the tiles of a band of four token tiles, column by column, on one XCD
@@ -590,19 +608,15 @@ template <int TW, int TX, bool F8, bool SPLIT> __global__ __launch_bounds__(256,
     const int64_t m0 = (int64_t)mt * G::BX;
     const bool swiglu = o.y.codes != nullptr && !part;
 
-    Rows<G::WI, G::WSD> lw;
-    Rows<G::XI, G::XSD> lx;
+    Load<G> ld;
     const int64_t f = w.rows >> 1;
-    mx_rows<G::WROW, G::NB>(lw, w, swiglu ? (wave & 1 ? f : 0) + (int64_t)nt * (G::BW / 2) + (wave >> 1) * (G::BW / 4)
-                                         : (int64_t)nt * G::BW + wave * (G::BW / 4), lane);
-    mx_rows<G::XROW, G::NB>(lx, x, m0 + wave * (G::BX / 4), lane);
-    const int blocks = (int)(w.in / MX_BLOCK), stages = (blocks + G::NB - 1) / G::NB;
-    const int s0 = blockIdx.y * per, s1 = min(s0 + per, stages);
-
-    auto keep = [&](int st) {                        // scale bytes that stand for blocks of the row
-        const int left = blocks - st * G::NB - g * G::T;
-        return left >= G::T ? -1 : left <= 0 ? 0 : (int)((1u << (8 * left)) - 1);
-    };
+    ld.w.init(w, swiglu ? (wave & 1 ? f : 0) + (int64_t)nt * (G::BW / 2) + (wave >> 1) * (G::BW / 4)
+                        : (int64_t)nt * G::BW + wave * (G::BW / 4), lane);
+    ld.x.init(x, m0 + wave * (G::BX / 4), lane);
+    ld.wave = wave;
+    ld.blocks = (int)(w.in / MX_BLOCK);
+    const int s0 = blockIdx.y * per;
+    ld.end = min(s0 + per, (ld.blocks + G::NB - 1) / G::NB);
 
     f32x16 acc[TX][TW];
 #pragma unroll
@@ -611,43 +625,63 @@ template <int TW, int TX, bool F8, bool SPLIT> __global__ __launch_bounds__(256,
         for (int j = 0; j < TW; j++) acc[i][j] = f32x16{};
     Frags<G> fr[2] = {};
     Scales<G> sc, sn;
+    StageScales<G> ss;
     const int wr = wn * (G::BW / 2) + (lane & 31), xr = wm * (G::BX / 2) + (lane & 31);
 
-    mx_load<G>(lw, lx, b0, lane, wave, s0, s0 < s1 ? blocks - (s0) * G::NB : 0);
-    mx_load<G>(lw, lx, b1, lane, wave, s0 + 1, s0 + 1 < s1 ? blocks - (s0 + 1) * G::NB : 0);
-    if constexpr (G::NBUF == 3) mx_load<G>(lw, lx, b2, lane, wave, s0 + 2, s0 + 2 < s1 ? blocks - (s0 + 2) * G::NB : 0);
-    __builtin_amdgcn_s_waitcnt(waits((G::NBUF - 1) * G::LOADS, 0));
+    // the first stages, the last of them to half: the other half is loaded in the first stage's first step
+    ld.scales(sb, s0);
+    ld.template codes<0, G::D>(b0, s0);
+    if constexpr (G::NBUF == 3) {
+        ld.template codes<0, G::D>(b1, s0 + 1);
+        ld.template codes<0, G::TX * G::D / (2 * G::TX)>(b2, s0 + 2);
+    } else {
+        ld.template codes<0, G::TX * G::D / (2 * G::TX)>(b1, s0 + 1);
+    }
+    __builtin_amdgcn_s_waitcnt(waits((G::NBUF - 2) * G::D + G::D / 2, 0));
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    mx_read_all<G>(fr[0], sc, b0, wr, xr, g, keep(s0));
+    mx_reads<G, 0, true, 0, G::TW + G::TX>(fr[0], sc, b0, sb, wr, xr, g);
 
-    auto stage = [&](int s, typename G::Buf &cur, const typename G::Buf &nxt) {
-        mx_step<G, SPLIT, 0, 1, false>(acc, fr[0], sc, fr[1], sn, cur, wr, xr, g, 0);
+    // Stage s, the chunk's c-th.
+    auto stage = [&](int s, auto ci, typename G::Buf &cur, const typename G::Buf &nxt, typename G::Buf &prev) {
+        constexpr int c = ci();
+        const int left = ld.blocks - s * G::NB - g * G::T;   // blocks of the row for this lane's scale bytes
+        mx_stage_scales<G, c>(ss, sc, g, left >= G::T ? -1 : left <= 0 ? 0 : (int)((1u << (8 * left)) - 1));
+        mx_step<G, SPLIT, 0, 1, false, 1>(acc, fr[0], ss, fr[1], sn, cur, sb, ld, prev, s + G::NBUF - 1, wr, xr, g);
         if constexpr (G::T == 4) {
-            mx_step<G, SPLIT, 1, 2, false>(acc, fr[1], sc, fr[0], sn, cur, wr, xr, g, 0);
-            mx_step<G, SPLIT, 2, 3, false>(acc, fr[0], sc, fr[1], sn, cur, wr, xr, g, 0);
+            mx_step<G, SPLIT, 1, 2, false, -1>(acc, fr[1], ss, fr[0], sn, cur, sb, ld, prev, 0, wr, xr, g);
+            mx_step<G, SPLIT, 2, 3, false, -1>(acc, fr[0], ss, fr[1], sn, cur, sb, ld, prev, 0, wr, xr, g);
         }
         // this stage's operands are all read, the next one's have landed
-        __builtin_amdgcn_s_waitcnt(waits((G::NBUF - 2) * G::LOADS, 0));
+        __builtin_amdgcn_s_waitcnt(waits((G::NBUF - 2) * G::D, 0));
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        mx_load<G>(lw, lx, cur, lane, wave, s + G::NBUF, s + G::NBUF < s1 ? blocks - (s + G::NBUF) * G::NB : 0);
-        __builtin_amdgcn_sched_barrier(0);
-        mx_step<G, SPLIT, G::T - 1, 0, true>(acc, fr[1], sc, fr[0], sn, nxt, wr, xr, g, keep(s + 1));
-        sc = sn;
+        if constexpr (c == 0) ld.scales(sb, s + G::CH);   // this chunk's are all in registers
+        mx_step<G, SPLIT, G::T - 1, 0, c == G::CH - 1, 0>(acc, fr[1], ss, fr[0], sn, nxt, sb, ld, cur, s + G::NBUF, wr, xr, g);
+        if constexpr (c == G::CH - 1) sc = sn;
     };
     mx_settle(acc);
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    using I3 = std::integral_constant<int, 3>;
     for (int s = s0;;) {
-        stage(s, b0, b1);
-        if (++s >= s1) break;
         if constexpr (G::NBUF == 3) {
-            stage(s, b1, b2);
-            if (++s >= s1) break;
-            stage(s, b2, b0);
-            if (++s >= s1) break;
+            stage(s, I0{}, b0, b1, b2);
+            if (++s >= ld.end) break;
+            stage(s, I1{}, b1, b2, b0);
+            if (++s >= ld.end) break;
+            stage(s, I2{}, b2, b0, b1);
+            if (++s >= ld.end) break;
         } else {
-            stage(s, b1, b0);
-            if (++s >= s1) break;
+            stage(s, I0{}, b0, b1, b1);
+            if (++s >= ld.end) break;
+            stage(s, I1{}, b1, b0, b0);
+            if (++s >= ld.end) break;
+            stage(s, I2{}, b0, b1, b1);
+            if (++s >= ld.end) break;
+            stage(s, I3{}, b1, b0, b0);
+            if (++s >= ld.end) break;
         }
     }
     mx_settle(acc);
