@@ -80,17 +80,10 @@ template <bool F8> __device__ __forceinline__ uint32_t mx_scale(uint32_t u) {
 // 2^(s - 127); the conversions take its exponent alone, so zero bits serve for s = 0
 __device__ __forceinline__ float mx_unit(uint32_t s) { return __builtin_bit_cast(float, s << 23); }
 
-// A quad's block to codes (eight of each lane: 4 or 8 bytes) and its scale byte.  The
-// conversions divide by the scale and round to the nearest, ties to even, in one.
-template <bool F8> __device__ __forceinline__ void mx_codes(const float (&in)[8], u32x2 &code, uint32_t &s) {
+// Eight values to codes of a block with scale byte s: 4 or 8 bytes.  The conversions
+// divide by the scale and round to the nearest, ties to even, in one.
+template <bool F8> __device__ __forceinline__ u32x2 mx_encode(const float (&in)[8], uint32_t s) {
     float v[8];
-    uint32_t u = 0;
-#pragma unroll
-    for (int k = 0; k < 8; k++) {
-        const uint32_t b = __builtin_bit_cast(uint32_t, in[k]) & 0x7FFFFFFFu;
-        u = u > b ? u : b;
-    }
-    s = mx_scale<F8>(quad_max(u));
 #pragma unroll
     for (int k = 0; k < 8; k++) v[k] = s == 255u ? 0.f : in[k];
     const float unit = mx_unit(s == 255u ? 127u : s);
@@ -100,21 +93,26 @@ template <bool F8> __device__ __forceinline__ void mx_codes(const float (&in)[8]
         a = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(a, v[2], v[3], unit, true);
         b = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(b, v[4], v[5], unit, false);
         b = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(b, v[6], v[7], unit, true);
-        code = u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+        return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
     } else {
         uint32_t a = 0;
         a = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(a, v[0], v[1], unit, 0);
         a = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(a, v[2], v[3], unit, 1);
         a = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(a, v[4], v[5], unit, 2);
         a = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(a, v[6], v[7], unit, 3);
-        code = u32x2{a, 0};
+        return u32x2{a, 0};
     }
 }
 // Values col .. col + 7 of a row; every lane of the quad calls it.
 template <bool F8> __device__ __forceinline__ void mx_store(const Fh3kMx &y, int64_t row, int col, const float (&v)[8]) {
-    u32x2 code;
-    uint32_t s;
-    mx_codes<F8>(v, code, s);
+    uint32_t u = 0;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const uint32_t b = __builtin_bit_cast(uint32_t, v[k]) & 0x7FFFFFFFu;
+        u = u > b ? u : b;
+    }
+    const uint32_t s = mx_scale<F8>(quad_max(u));
+    const u32x2 code = mx_encode<F8>(v, s);
     if constexpr (F8) *(u32x2 *)(y.codes + row * y.ld + col) = code;
     else *(uint32_t *)(y.codes + row * y.ld + col / 2) = code.x;
     if ((col & (MX_BLOCK - 1)) == 0) y.scales[row * y.lds + col / MX_BLOCK] = (uint8_t)s;
@@ -264,16 +262,16 @@ __device__ __forceinline__ uint32_t fp8_large(uint32_t c) {
 // ---------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) void lds_void;
 
-template <int TW_, int TX_, bool F8_> struct Gemm {
-    static constexpr int TW = TW_, TX = TX_;
+template <int TW_, int TX_, int NW_, int NX_, bool F8_, int KS_, int NBUF_> struct Gemm {
+    static constexpr int TW = TW_, TX = TX_, NW = NW_, NX = NX_, WAVES = NW * NX;
     static constexpr bool F8 = F8_;
-    static constexpr int KS = F8 ? 128 : 256, NB = KS / MX_BLOCK, T = NB / 2;
-    static constexpr int WROW = KS / 2, XROW = 128;      // bytes of a stage's row
-    static constexpr int BW = TW * 64, BX = TX * 64;
-    static constexpr int NBUF = F8 ? 3 : 2, CH = F8 ? 3 : 4;   // stages in LDS, stages of a chunk of scales
-    static constexpr int SD = F8 ? 4 : 8;                // dwords of a row's chunk in LDS
-    static constexpr int WI = BW * WROW / 4096, XI = BX * XROW / 4096, D = WI + XI;   // a wavefront's DMA instructions: a stage's codes
-    static constexpr int WS = BW * SD / 256, XS = BX * SD / 256;                       // and a chunk's scales
+    static constexpr int KS = KS_, NB = KS / MX_BLOCK, T = NB / 2;
+    static constexpr int WROW = KS / 2, XROW = F8 ? KS : KS / 2;   // bytes of a stage's row
+    static constexpr int BW = NW * TW * 32, BX = NX * TX * 32;
+    static constexpr int NBUF = NBUF_, CH = NBUF == 3 ? 3 : 4;     // stages in LDS, stages of a chunk of scales
+    static constexpr int SD = NB == 8 ? 8 : 4;                     // dwords of a row's chunk in LDS
+    static constexpr int WI = BW * WROW / 1024 / WAVES, XI = BX * XROW / 1024 / WAVES, D = WI + XI;   // a wavefront's DMA instructions: a stage's codes
+    static constexpr int WS = BW * SD / 64 / WAVES, XS = BX * SD / 64 / WAVES;                         // and a chunk's scales
     struct Buf {
         u32x4 x[BX * XROW / 16], w[BW * WROW / 16];
     };
@@ -320,12 +318,12 @@ template <class G, int ROW, int N, int NS> struct Rows {
             const int r = j * RPI + lane / P;
             off[j] = (uint32_t)((r < last ? r : last) * m.ld) + piece[j & 1] * 16;
         }
-        // FP4 stages have two dwords of scales to a row, here in the order [g][stage]; FP8 stages one
+        // stages of eight blocks have two dwords of scales to a row, here in the order [g][stage]; those of four one
 #pragma unroll
         for (int j = 0; j < NS; j++) {
             const int d = j * 64 + lane, r = d / G::SD, k = d % G::SD;
-            soff[j] = (uint32_t)((r < last ? r : last) * m.lds) + 4 * (G::F8 ? k : (k & 3) * 2 + (k >> 2));
-            if (G::F8 && k == 3) soff[j] = MX_OUTSIDE;
+            soff[j] = (uint32_t)((r < last ? r : last) * m.lds) + 4 * (G::NB == 4 ? k : (k & 3) * 2 + (k >> 2));
+            if (k >= (G::NB == 4 ? G::CH : 8)) soff[j] = MX_OUTSIDE;
         }
     }
     // instruction j of stage st, of whose row `pieces` pieces are there
@@ -360,7 +358,7 @@ template <class G> struct Frags {
     u32x4 w[G::TW];
     typename std::conditional<G::F8, i32x8, u32x4>::type x[G::TX];
 };
-template <class G> struct Scales {       // of a chunk: a dword (FP8: both lanes' halves of one) for each stage
+template <class G> struct Scales {       // of a chunk: a dword (of four blocks: both lanes' halves) for each stage
     u32x4 w[G::TW], x[G::TX];
 };
 template <class G> struct StageScales {
@@ -388,16 +386,16 @@ template <class G, int t, int n> __device__ __forceinline__ void mx_read(Frags<G
 }
 template <class G, int n> __device__ __forceinline__ void mx_read_scale(Scales<G> &s, const typename G::ScaleBuf &b, int wr, int xr, int g) {
     const uint32_t *p = n < G::TW ? b.w + (wr + 32 * n) * G::SD : b.x + (xr + 32 * (n - G::TW)) * G::SD;
-    const u32x4 v = *(const u32x4 *)(p + (G::F8 ? 0 : 4 * g));
+    const u32x4 v = *(const u32x4 *)(p + (G::NB == 4 ? 0 : 4 * g));
     if constexpr (n < G::TW) s.w[n] = v;
     else s.x[n - G::TW] = v;
 }
 // The scales of the chunk's stage c; keep: zeros where the row has ended.
 template <class G, int c> __device__ __forceinline__ void mx_stage_scales(StageScales<G> &o, const Scales<G> &s, int g, int keep) {
 #pragma unroll
-    for (int i = 0; i < G::TW; i++) o.w[i] = (int)(G::F8 ? s.w[i][c] >> (16 * g) : s.w[i][c]) & keep;
+    for (int i = 0; i < G::TW; i++) o.w[i] = (int)(G::NB == 4 ? s.w[i][c] >> (16 * g) : s.w[i][c]) & keep;
 #pragma unroll
-    for (int i = 0; i < G::TX; i++) o.x[i] = (int)(G::F8 ? s.x[i][c] >> (16 * g) : s.x[i][c]) & keep;
+    for (int i = 0; i < G::TX; i++) o.x[i] = (int)(G::NB == 4 ? s.x[i][c] >> (16 * g) : s.x[i][c]) & keep;
 }
 
 // The products of TW tiles of weights with one of tokens, sums in accumulation
@@ -499,40 +497,42 @@ constexpr int waits(int vm, int lgkm) { return (vm & 15) | 7 << 4 | lgkm << 8 | 
 
 __device__ __forceinline__ float silu(float g) { return g / (1.f + __builtin_amdgcn_exp2f(-LOG2E * g)); }
 
-// Four values of a row to where they go.
-template <int T> __device__ __forceinline__ void mx_put4(const Fh3kMxOut &o, int64_t t, int n, int64_t cols, f32x4 v) {
+// Eight values of a row, or one, to where they go; Beside: what is read for them.
+struct Beside {
+    f32x4 gate[2], res[2];     // 16-bit residuals: as stored, in res[0]
+};
+template <int T> __device__ __forceinline__ void mx_beside(Beside &b, const Fh3kMxOut &o, int64_t t, int n, int64_t cols) {
+    if (o.res) {
+        const f32x4 *p = (const f32x4 *)((const uint8_t *)o.res + (t * o.ldres + n) * (T == FH3K_F32 ? 4 : 2));
+        b.res[0] = p[0];
+        if constexpr (T == FH3K_F32) b.res[1] = p[1];
+        if (o.gate) {
+            b.gate[0] = *(const f32x4 *)(o.gate + t * cols + n);
+            b.gate[1] = *(const f32x4 *)(o.gate + t * cols + n + 4);
+        }
+    }
+}
+template <int T> __device__ __forceinline__ float half_value(uint32_t b) {
+    return T == FH3K_F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)b) : __builtin_bit_cast(float, b << 16);
+}
+template <int T> __device__ __forceinline__ void mx_put(const Fh3kMxOut &o, int64_t t, int n, float (&v)[8], const Beside &b) {
     if (o.bias)
 #pragma unroll
-        for (int k = 0; k < 4; k++) v[k] += o.bias[n + k];
+        for (int k = 0; k < 8; k++) v[k] += o.bias[n + k];
     if (o.res) {
-        f32x4 h;
-        if constexpr (T == FH3K_F32) {
-            h = *(const f32x4 *)((const float *)o.res + t * o.ldres + n);
-        } else {
-            const u32x2 a = *(const u32x2 *)((const uint16_t *)o.res + t * o.ldres + n);
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const uint32_t b = a[k >> 1] >> (16 * (k & 1)) & 0xFFFFu;
-                h[k] = T == FH3K_F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)b) : __builtin_bit_cast(float, b << 16);
+        for (int k = 0; k < 8; k++) {
+            float h;
+            if constexpr (T == FH3K_F32) {
+                h = b.res[k / 4][k % 4];
+            } else {
+                const float pair = b.res[0][k >> 1];
+                h = half_value<T>(__builtin_bit_cast(uint32_t, pair) >> (16 * (k & 1)) & 0xFFFFu);
             }
-        }
-        if (o.gate) {
-            const f32x4 q = *(const f32x4 *)(o.gate + t * cols + n);
-#pragma unroll
-            for (int k = 0; k < 4; k++) v[k] = __builtin_fmaf(q[k], v[k], h[k]);
-        } else {
-#pragma unroll
-            for (int k = 0; k < 4; k++) v[k] += h[k];
+            v[k] = o.gate ? __builtin_fmaf(b.gate[k / 4][k % 4], v[k], h) : v[k] + h;
         }
     }
-    if constexpr (T == FH3K_F32) {
-        *(f32x4 *)((float *)o.out + t * o.ldo + n) = v;
-    } else {
-        u32x2 a;
-#pragma unroll
-        for (int k = 0; k < 2; k++) a[k] = to_half<T>(v[2 * k]) | (uint32_t)to_half<T>(v[2 * k + 1]) << 16;
-        *(u32x2 *)((uint16_t *)o.out + t * o.ldo + n) = a;
-    }
+    store8<T>(o.out, t * o.ldo + n, v);
 }
 template <int T> __device__ __forceinline__ void mx_put1(const Fh3kMxOut &o, int64_t t, int n, int64_t cols, float v) {
     if (o.bias) v += o.bias[n];
@@ -544,61 +544,139 @@ template <int T> __device__ __forceinline__ void mx_put1(const Fh3kMxOut &o, int
     else ((uint16_t *)o.out)[t * o.ldo + n] = to_half<T>(v);
 }
 
-// A wavefront's 32 tokens x COLS values, staged as [32][COLS / 4] pieces of four with piece c of token t at c ^ t % 16, to rows of the output.
-template <int T, int COLS> __device__ __forceinline__ void mx_rows_out(const Fh3kMxOut &o, const f32x4 *stg, int lane, int64_t t0, int64_t rows,
-                                                                       int n0, int64_t cols, bool vec) {
-    constexpr int C = COLS / 4, TPI = 64 / C;
-    if (vec) {
-        const int c = lane % C, n = n0 + 4 * c;
-        if (n >= cols) return;
-#pragma unroll 4
-        for (int it = 0; it < 32; it += TPI) {
-            const int t = it + lane / C;
-            if (t0 + t < rows) mx_put4<T>(o, t0 + t, n, cols, stg[t * C + (c ^ (t & 15))]);
+// A tile's 32 columns of a token lie in lanes l and l + 32, four by four; after the
+// exchange lane l has columns 0 .. 7 and 16 .. 23, l + 32 the others.
+__device__ __forceinline__ void mx_columns(const f32x16 &a, float (&v)[2][8]) {
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float x = a[8 * m + k], y = a[8 * m + 4 + k];
+            const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y), false, false);
+            const uint32_t p = r[0], q = r[1];
+            v[m][k] = __builtin_bit_cast(float, p);
+            v[m][4 + k] = __builtin_bit_cast(float, q);
         }
-    } else {
-        const float *p = (const float *)stg;
-        for (int k = 0; k < COLS; k += 64) {
-            const int n = k + lane, c = n >> 2;
-            if (n0 + n >= cols) return;
-#pragma unroll 4
-            for (int t = 0; t < 32; t++)
-                if (t0 + t < rows) mx_put1<T>(o, t0 + t, n0 + n, cols, p[(t * C + (c ^ (t & 15))) * 4 + (n & 3)]);
-        }
-    }
 }
-// The same where the first half of the columns are values and the second their gates: SwiGLU to codes.
-template <bool F8, int COLS> __device__ __forceinline__ void mx_swiglu_out(const Fh3kMxOut &o, const f32x4 *stg, int lane, int64_t t0, int64_t rows,
-                                                                           int f0) {
-    constexpr int C = COLS / 4, L = COLS / 16, TPI = 64 / L;   // eight outputs to a lane
-    const int64_t f = o.y.in;
-    const int e = lane % L, col = f0 + 8 * e;
-    if (col >= f) return;
-#pragma unroll 2
-    for (int it = 0; it < 32; it += TPI) {
-        const int t = it + lane / L;
-        float a[8];
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const f32x4 v = stg[t * C + ((2 * e + h) ^ (t & 15))], q = stg[t * C + ((C / 2 + 2 * e + h) ^ (t & 15))];
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const float bv = o.bias ? o.bias[col + 4 * h + k] : 0.f, bg = o.bias ? o.bias[f + col + 4 * h + k] : 0.f;
-                a[4 * h + k] = (v[k] + bv) * silu(q[k] + bg);
-            }
-        }
-        if (t0 + t < rows) mx_store<F8>(o.y, t0 + t, col, a);   // a token's lanes go together
+
+// acc[idx / TW][idx % TW], of a rolled loop: unrolled over the sums, the code of the stores ran once for each and was fetched each time.
+template <int TX, int TW, int i = 0> __device__ __forceinline__ void mx_pick(f32x16 &v, const f32x16 (&acc)[TX][TW], int idx) {
+    if constexpr (i < TX * TW) {
+        if (idx == i) v = acc[i / TW][i % TW];
+        else mx_pick<TX, TW, i + 1>(v, acc, idx);
     }
 }
 
-template <int TW, int TX, bool F8, bool SPLIT> __global__ __launch_bounds__(256, TW == 4 ? 1 : 2) void k_mx_gemm(
+// A wavefront's sums to rows of the output, straight from the registers: a store
+// covers 32 bytes (64 in fp32) of 32 rows, which L2 puts together.  What is read
+// beside a tile comes while the one before is stored.
+template <int T, int TX, int TW> __device__ __forceinline__ void mx_rows_out(const Fh3kMxOut &o, const f32x16 (&acc)[TX][TW], int lane, int64_t t0,
+                                                                             int64_t rows, int n0, int64_t cols, bool vec) {
+    const int g = lane >> 5, l = lane & 31;
+    auto at = [&](int idx, int64_t &t, int &n) {
+        t = t0 + 32 * (idx / TW) + l;
+        n = n0 + 32 * (idx % TW) + 8 * g;
+    };
+    if (vec) {
+        Beside b[2], c[2];
+        auto read = [&](int idx) {
+            int64_t t;
+            int n;
+            at(idx, t, n);
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+                if (t < rows && n + 16 * m + 8 <= cols) mx_beside<T>(c[m], o, t, n + 16 * m, cols);
+        };
+        read(0);
+#pragma unroll 1
+        for (int idx = 0; idx < TX * TW; idx++) {
+            f32x16 a;
+            float v[2][8];
+            int64_t t;
+            int n;
+            mx_pick<TX, TW>(a, acc, idx);
+            mx_columns(a, v);
+            b[0] = c[0];
+            b[1] = c[1];
+            if (idx + 1 < TX * TW) read(idx + 1);
+            at(idx, t, n);
+#pragma unroll
+            for (int m = 0; m < 2; m++, n += 16) {
+                if (t >= rows) continue;
+                if (n + 8 <= cols) mx_put<T>(o, t, n, v[m], b[m]);
+                else
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        if (n + k < cols) mx_put1<T>(o, t, n + k, cols, v[m][k]);
+            }
+        }
+    } else {
+#pragma unroll 1
+        for (int idx = 0; idx < TX * TW; idx++) {
+            f32x16 a;
+            float v[2][8];
+            int64_t t;
+            int n;
+            mx_pick<TX, TW>(a, acc, idx);
+            mx_columns(a, v);
+            at(idx, t, n);
+            if (t >= rows) continue;
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (n + 16 * m + k < cols) mx_put1<T>(o, t, n + 16 * m + k, cols, v[m][k]);
+        }
+    }
+}
+// The same where the wavefront's first tiles are values and the others their gates: SwiGLU to codes.  A block is a tile's 32 columns.
+template <bool F8, int TX, int TW> __device__ __forceinline__ void mx_swiglu_out(const Fh3kMxOut &o, const f32x16 (&acc)[TX][TW], int lane,
+                                                                                 int64_t t0, int64_t rows, int f0) {
+    const int64_t f = o.y.in;
+    const int g = lane >> 5;
+#pragma unroll 1
+    for (int idx = 0; idx < TX * TW / 2; idx++) {
+        const int i = idx / (TW / 2), j = idx % (TW / 2), col = f0 + 32 * j;
+        const int64_t t = t0 + 32 * i + (lane & 31);
+        f32x16 a, b;
+        float v[2][8], q[2][8];
+        mx_pick<TX, TW>(a, acc, i * TW + j);
+        mx_pick<TX, TW>(b, acc, i * TW + j + TW / 2);
+        mx_columns(a, v);
+        mx_columns(b, q);
+        if (col >= f) continue;               // the whole wavefront
+        uint32_t u = 0;
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int n = col + 16 * m + 8 * g + k;
+                const float bv = o.bias ? o.bias[n] : 0.f, bg = o.bias ? o.bias[f + n] : 0.f;
+                v[m][k] = (v[m][k] + bv) * silu(q[m][k] + bg);
+                const uint32_t w = __builtin_bit_cast(uint32_t, v[m][k]) & 0x7FFFFFFFu;
+                u = u > w ? u : w;
+            }
+        const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        const uint32_t r0 = r[0], r1 = r[1], s = mx_scale<F8>(r0 > r1 ? r0 : r1);
+        if (t >= rows) continue;
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            const u32x2 c = mx_encode<F8>(v[m], s);
+            if constexpr (F8) *(u32x2 *)(o.y.codes + t * o.y.ld + col + 16 * m + 8 * g) = c;
+            else *(uint32_t *)(o.y.codes + t * o.y.ld + (col + 16 * m + 8 * g) / 2) = c.x;
+        }
+        if (!g) o.y.scales[t * o.y.lds + col / MX_BLOCK] = (uint8_t)s;
+    }
+}
+
+template <class G, bool SPLIT> __global__ __launch_bounds__(64 * G::WAVES, 8 / G::WAVES) void k_mx_gemm(
     Fh3kMx w, Fh3kMx x, Fh3kMxOut o, float *part, int64_t ldp, int m_tiles, int n_tiles, int per, bool vec) {
-    using G = Gemm<TW, TX, F8>;
+    constexpr int TW = G::TW, TX = G::TX;
     __shared__ typename G::Buf b0, b1;
     __shared__ typename std::conditional<G::NBUF == 3, typename G::Buf, int>::type b2;
     __shared__ typename G::ScaleBuf sb;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wn = wave & 1, wm = wave >> 1, g = lane >> 5;
+    const int wn = wave % G::NW, wm = wave / G::NW, g = lane >> 5;
     // the tiles of a band of four token tiles, column by column, on one XCD
     constexpr int GB = 4;
     const int total = m_tiles * n_tiles, id = blockIdx.x, share = total >> 3;
@@ -610,9 +688,12 @@ template <int TW, int TX, bool F8, bool SPLIT> __global__ __launch_bounds__(256,
 
     Load<G> ld;
     const int64_t f = w.rows >> 1;
-    ld.w.init(w, swiglu ? (wave & 1 ? f : 0) + (int64_t)nt * (G::BW / 2) + (wave >> 1) * (G::BW / 4)
-                        : (int64_t)nt * G::BW + wave * (G::BW / 4), lane);
-    ld.x.init(x, m0 + wave * (G::BX / 4), lane);
+    // SwiGLU: each wavefront column's rows are the values' and then their gates'
+    constexpr int RW = G::BW / G::WAVES, CW = G::BW / G::NW;
+    const int wc = wave * RW / CW, wa = wave * RW % CW;
+    ld.w.init(w, swiglu ? (wa >= CW / 2 ? f : 0) + (int64_t)nt * (G::BW / 2) + wc * (CW / 2) + wa % (CW / 2)
+                        : (int64_t)nt * G::BW + wave * RW, lane);
+    ld.x.init(x, m0 + wave * (G::BX / G::WAVES), lane);
     ld.wave = wave;
     ld.blocks = (int)(w.in / MX_BLOCK);
     const int s0 = blockIdx.y * per;
@@ -624,18 +705,18 @@ template <int TW, int TX, bool F8, bool SPLIT> __global__ __launch_bounds__(256,
 #pragma unroll
         for (int j = 0; j < TW; j++) acc[i][j] = f32x16{};
     Frags<G> fr[2] = {};
-    Scales<G> sc, sn;
+    Scales<G> sc;
     StageScales<G> ss;
-    const int wr = wn * (G::BW / 2) + (lane & 31), xr = wm * (G::BX / 2) + (lane & 31);
+    const int wr = wn * CW + (lane & 31), xr = wm * (G::BX / G::NX) + (lane & 31);
 
     // the first stages, the last of them to half: the other half is loaded in the first stage's first step
     ld.scales(sb, s0);
     ld.template codes<0, G::D>(b0, s0);
     if constexpr (G::NBUF == 3) {
         ld.template codes<0, G::D>(b1, s0 + 1);
-        ld.template codes<0, G::TX * G::D / (2 * G::TX)>(b2, s0 + 2);
+        ld.template codes<0, G::D / 2>(b2, s0 + 2);
     } else {
-        ld.template codes<0, G::TX * G::D / (2 * G::TX)>(b1, s0 + 1);
+        ld.template codes<0, G::D / 2>(b1, s0 + 1);
     }
     __builtin_amdgcn_s_waitcnt(waits((G::NBUF - 2) * G::D + G::D / 2, 0));
     __builtin_amdgcn_s_barrier();
@@ -647,18 +728,17 @@ template <int TW, int TX, bool F8, bool SPLIT> __global__ __launch_bounds__(256,
         constexpr int c = ci();
         const int left = ld.blocks - s * G::NB - g * G::T;   // blocks of the row for this lane's scale bytes
         mx_stage_scales<G, c>(ss, sc, g, left >= G::T ? -1 : left <= 0 ? 0 : (int)((1u << (8 * left)) - 1));
-        mx_step<G, SPLIT, 0, 1, false, 1>(acc, fr[0], ss, fr[1], sn, cur, sb, ld, prev, s + G::NBUF - 1, wr, xr, g);
+        mx_step<G, SPLIT, 0, 1, false, 1>(acc, fr[0], ss, fr[1], sc, cur, sb, ld, prev, s + G::NBUF - 1, wr, xr, g);
         if constexpr (G::T == 4) {
-            mx_step<G, SPLIT, 1, 2, false, -1>(acc, fr[1], ss, fr[0], sn, cur, sb, ld, prev, 0, wr, xr, g);
-            mx_step<G, SPLIT, 2, 3, false, -1>(acc, fr[0], ss, fr[1], sn, cur, sb, ld, prev, 0, wr, xr, g);
+            mx_step<G, SPLIT, 1, 2, false, -1>(acc, fr[1], ss, fr[0], sc, cur, sb, ld, prev, 0, wr, xr, g);
+            mx_step<G, SPLIT, 2, 3, false, -1>(acc, fr[0], ss, fr[1], sc, cur, sb, ld, prev, 0, wr, xr, g);
         }
         // this stage's operands are all read, the next one's have landed
         __builtin_amdgcn_s_waitcnt(waits((G::NBUF - 2) * G::D, 0));
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (c == 0) ld.scales(sb, s + G::CH);   // this chunk's are all in registers
-        mx_step<G, SPLIT, G::T - 1, 0, c == G::CH - 1, 0>(acc, fr[1], ss, fr[0], sn, nxt, sb, ld, cur, s + G::NBUF, wr, xr, g);
-        if constexpr (c == G::CH - 1) sc = sn;
+        mx_step<G, SPLIT, G::T - 1, 0, c == G::CH - 1, 0>(acc, fr[1], ss, fr[0], sc, nxt, sb, ld, cur, s + G::NBUF, wr, xr, g);
     };
     mx_settle(acc);
     using I0 = std::integral_constant<int, 0>;
@@ -685,63 +765,42 @@ template <int TW, int TX, bool F8, bool SPLIT> __global__ __launch_bounds__(256,
         }
     }
     mx_settle(acc);
-    __builtin_amdgcn_s_waitcnt(waits(0, 0));
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-
-    constexpr int COLS = TW * 32, C = COLS / 4;
-    f32x4 *stg = (f32x4 *)(wm ? b1.x : b0.x) + wn * (32 * C);
-    const int tl = lane & 31;
+    __builtin_amdgcn_s_waitcnt(waits(0, 0));   // nothing more comes to LDS, which may be another workgroup's soon
     if (part) {
         o = Fh3kMxOut{};
         o.out = part + blockIdx.y * (x.rows * ldp);
         o.ldo = ldp;
     }
-    auto put = [&](const f32x16(&a)[TW]) {
-#pragma unroll
-        for (int j = 0; j < TW; j++)
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-                stg[tl * C + ((8 * j + 2 * q + g) ^ (tl & 15))] = f32x4{a[j][4 * q], a[j][4 * q + 1], a[j][4 * q + 2], a[j][4 * q + 3]};
-    };
-#pragma unroll 1
-    for (int i = 0; i < TX; i++) {   // rolled: unrolled, the code of the stores runs once for each and is fetched each time
-        if (i == 0) put(acc[0]);
-        else if (i == 1) put(acc[1]);
-        if constexpr (TX == 4) {
-            if (i == 2) put(acc[2]);
-            else if (i == 3) put(acc[3]);
-        }
-        __builtin_amdgcn_wave_barrier();
-        const int64_t t0 = m0 + wm * (G::BX / 2) + 32 * i;
-        const int n0 = nt * G::BW + wn * (G::BW / 2);
-        if (swiglu) {
-            if (o.y.type == FH3K_MX_FP8) mx_swiglu_out<true, COLS>(o, stg, lane, t0, x.rows, n0 / 2);
-            else mx_swiglu_out<false, COLS>(o, stg, lane, t0, x.rows, n0 / 2);
-        } else if (o.type == FH3K_F32) mx_rows_out<FH3K_F32, COLS>(o, stg, lane, t0, x.rows, n0, w.rows, vec);
-        else if (o.type == FH3K_F16) mx_rows_out<FH3K_F16, COLS>(o, stg, lane, t0, x.rows, n0, w.rows, vec);
-        else mx_rows_out<FH3K_BF16, COLS>(o, stg, lane, t0, x.rows, n0, w.rows, vec);
-        __builtin_amdgcn_wave_barrier();
-    }
+    const int64_t t0 = m0 + wm * (G::BX / G::NX);
+    const int n0 = nt * G::BW + wn * CW;
+    if (swiglu) {
+        if (o.y.type == FH3K_MX_FP8) mx_swiglu_out<true>(o, acc, lane, t0, x.rows, n0 / 2);
+        else mx_swiglu_out<false>(o, acc, lane, t0, x.rows, n0 / 2);
+    } else if (o.type == FH3K_F32) mx_rows_out<FH3K_F32>(o, acc, lane, t0, x.rows, n0, part ? ldp : w.rows, vec);
+    else if (o.type == FH3K_F16) mx_rows_out<FH3K_F16>(o, acc, lane, t0, x.rows, n0, w.rows, vec);
+    else mx_rows_out<FH3K_BF16>(o, acc, lane, t0, x.rows, n0, w.rows, vec);
 }
 
-// The parts of a split product, added in their order, to rows of the output: four values to a thread.
+// The parts of a split product, added in their order, to rows of the output: eight values to a thread.
 template <int T> __global__ __launch_bounds__(256) void k_mx_join(const float *__restrict__ part, int S, int64_t ldp, int64_t rows, int64_t cols,
                                                                   Fh3kMxOut o, bool vec) {
     const int64_t t = blockIdx.x;
-    const int n = 4 * (blockIdx.y * 256 + threadIdx.x);
+    const int n = 8 * (blockIdx.y * 256 + threadIdx.x);
     if (n >= cols) return;
-    f32x4 v = *(const f32x4 *)(part + t * ldp + n);
-    for (int s = 1; s < S; s++) {
-        const f32x4 a = *(const f32x4 *)(part + (s * rows + t) * ldp + n);
+    float v[8] = {};
+    for (int s = 0; s < S; s++) {
+        float a[8];
+        load8<FH3K_F32>(part, (s * rows + t) * ldp + n, a);
 #pragma unroll
-        for (int k = 0; k < 4; k++) v[k] += a[k];
+        for (int k = 0; k < 8; k++) v[k] += a[k];
     }
-    if (vec) {
-        mx_put4<T>(o, t, n, cols, v);
+    if (vec && n + 8 <= cols) {
+        Beside b;
+        mx_beside<T>(b, o, t, n, cols);
+        mx_put<T>(o, t, n, v, b);
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; k++)
+        for (int k = 0; k < 8; k++)
             if (n + k < cols) mx_put1<T>(o, t, n + k, cols, v[k]);
     }
 }
@@ -832,9 +891,16 @@ Plan plan_of(const Fh3kMx *w, const Fh3kMx *x) {
     Plan p;
     auto tiles = [&](int b) { return ((w->rows + b - 1) / b) * ((x->rows + b - 1) / b); };
     p.bw = p.bx = tiles(256) >= 192 ? 256 : 128;
+#ifdef CFG2
+    if (p.bw == 256) p.bx = 128;
+#endif
     p.m_tiles = (x->rows + p.bx - 1) / p.bx;
     p.n_tiles = (w->rows + p.bw - 1) / p.bw;
+    #ifdef CFG2
+    const int ks = x->type == FH3K_MX_FP8 || p.bw == 256 ? 128 : 256;
+#else
     const int ks = x->type == FH3K_MX_FP8 ? 128 : 256;
+#endif
     const int stages = (int)((w->in + ks - 1) / ks);
     const int64_t t = p.m_tiles * p.n_tiles;
     int parts = 1;
@@ -843,18 +909,18 @@ Plan plan_of(const Fh3kMx *w, const Fh3kMx *x) {
     if (parts < 1) parts = 1;
     p.per = (stages + parts - 1) / parts;
     p.parts = (stages + p.per - 1) / p.per;
-    p.ldp = (w->rows + 3) / 4 * 4;
+    p.ldp = (w->rows + 7) / 8 * 8;
     return p;
 }
 
-template <int TW, int TX, bool F8, bool SPLIT> void launch_gemm(const Fh3kMx *w, const Fh3kMx *x, const Fh3kMxOut *o, const Plan &p, float *part,
-                                                                bool vec, hipStream_t st) {
+template <class G, bool SPLIT = false> void launch_gemm(const Fh3kMx *w, const Fh3kMx *x, const Fh3kMxOut *o, const Plan &p, float *part, bool vec,
+                                                       hipStream_t st) {
     const dim3 grid((unsigned)(p.m_tiles * p.n_tiles), (unsigned)p.parts);
-    k_mx_gemm<TW, TX, F8, SPLIT><<<grid, 256, 0, st>>>(*w, *x, *o, part, p.ldp, (int)p.m_tiles, (int)p.n_tiles, p.per, vec || part);
+    k_mx_gemm<G, SPLIT><<<grid, 64 * G::WAVES, 0, st>>>(*w, *x, *o, part, p.ldp, (int)p.m_tiles, (int)p.n_tiles, p.per, vec || part);
 }
 
-// Whether rows of an array, ld values apart, can be taken four at a time.
-bool fours(const void *p, int64_t ld, int size) { return !p || ((uintptr_t)p % (4 * size) == 0 && ld % 4 == 0); }
+// Whether rows of an array, ld values apart, can be taken 16 bytes at a time.
+bool sixteens(const void *p, int64_t ld, int size) { return !p || ((uintptr_t)p % 16 == 0 && ld * size % 16 == 0); }
 
 }  // namespace
 
@@ -872,16 +938,26 @@ extern "C" hipError_t fh3k_mx_matmul(const Fh3kMx *w, const Fh3kMx *x, const Fh3
     const Plan p = plan_of(w, x);
     float *part = p.parts > 1 ? (float *)ws : nullptr;
     const int size = o->type == FH3K_F32 ? 4 : 2;
-    const bool vec = w->rows % 4 == 0 && fours(o->out, o->ldo, size) && fours(o->res, o->ldres, size) && fours(o->gate, 0, 4);
+    const bool vec = sixteens(o->out, o->ldo, size) && sixteens(o->res, o->ldres, size) && sixteens(o->gate, w->rows, 4);
     const bool f8 = x->type == FH3K_MX_FP8, split = f8 && o->type == FH3K_F32 && !o->y.codes;
-    auto go = [&](auto tile) {
-        constexpr int N = tile();
-        if (!f8) launch_gemm<N, N, false, false>(w, x, o, p, part, vec, st);
-        else if (!split) launch_gemm<N, N, true, false>(w, x, o, p, part, vec, st);
-        else launch_gemm<N, N, true, true>(w, x, o, p, part, vec, st);
-    };
-    if (p.bw == 256) go(std::integral_constant<int, 4>{});
-    else go(std::integral_constant<int, 2>{});
+#ifdef CFG2
+    using Big4 = Gemm<4, 2, 2, 2, false, 128, 3>;
+    using Big8 = Gemm<4, 2, 2, 2, true, 128, 2>;
+#else
+    using Big4 = Gemm<4, 2, 2, 4, false, 256, 2>;
+    using Big8 = Gemm<4, 2, 2, 4, true, 128, 3>;
+#endif
+    using Small4 = Gemm<2, 2, 2, 2, false, 256, 2>;
+    using Small8 = Gemm<2, 2, 2, 2, true, 128, 3>;
+    if (p.bw == 256) {
+        if (!f8) launch_gemm<Big4>(w, x, o, p, part, vec, st);
+        else if (!split) launch_gemm<Big8>(w, x, o, p, part, vec, st);
+        else launch_gemm<Big8, true>(w, x, o, p, part, vec, st);
+    } else {
+        if (!f8) launch_gemm<Small4>(w, x, o, p, part, vec, st);
+        else if (!split) launch_gemm<Small8>(w, x, o, p, part, vec, st);
+        else launch_gemm<Small8, true>(w, x, o, p, part, vec, st);
+    }
     if (!part) return hipGetLastError();
     if (o->y.codes) {
         const dim3 grid((unsigned)x->rows, (unsigned)((o->y.in + 2047) / 2048));
@@ -889,6 +965,6 @@ extern "C" hipError_t fh3k_mx_matmul(const Fh3kMx *w, const Fh3kMx *x, const Fh3
         else k_mx_join_swiglu<false><<<grid, 256, 0, st>>>(part, p.parts, p.ldp, x->rows, *o);
         return hipGetLastError();
     }
-    const dim3 grid((unsigned)x->rows, (unsigned)((w->rows + 1023) / 1024));
+    const dim3 grid((unsigned)x->rows, (unsigned)((w->rows + 2047) / 2048));
     return by_type(o->type, [&](auto t) { k_mx_join<t()><<<grid, 256, 0, st>>>(part, p.parts, p.ldp, x->rows, w->rows, *o, vec); });
 }
