@@ -495,7 +495,8 @@ template <int TX, int TW> __device__ __forceinline__ void mx_settle(f32x16 (&acc
 
 constexpr int waits(int vm, int lgkm) { return (vm & 15) | 7 << 4 | lgkm << 8 | (vm >> 4) << 14; }
 
-__device__ __forceinline__ float silu(float g) { return g / (1.f + __builtin_amdgcn_exp2f(-LOG2E * g)); }
+// g / (1 + exp(-g)), to two units in the last place and those of exp2's argument
+__device__ __forceinline__ float silu(float g) { return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-LOG2E * g)); }
 
 // Eight values of a row, or one, to where they go; Beside: what is read for them.
 struct Beside {
@@ -567,66 +568,56 @@ template <int TX, int TW, int i = 0> __device__ __forceinline__ void mx_pick(f32
     }
 }
 
-// A wavefront's sums to rows of the output, straight from the registers: a store
-// covers 32 bytes (64 in fp32) of 32 rows, which L2 puts together.  What is read
-// beside a tile comes while the one before is stored.
-template <int T, int TX, int TW> __device__ __forceinline__ void mx_rows_out(const Fh3kMxOut &o, const f32x16 (&acc)[TX][TW], int lane, int64_t t0,
-                                                                             int64_t rows, int n0, int64_t cols, bool vec) {
-    const int g = lane >> 5, l = lane & 31;
-    auto at = [&](int idx, int64_t &t, int &n) {
-        t = t0 + 32 * (idx / TW) + l;
-        n = n0 + 32 * (idx % TW) + 8 * g;
-    };
-    if (vec) {
-        Beside b[2], c[2];
-        auto read = [&](int idx) {
-            int64_t t;
-            int n;
-            at(idx, t, n);
+// A wavefront's sums to rows of the output through its own piece of LDS, 32 tokens at
+// a time, [32][COLS / 4] pieces of four values with piece c of token t at c ^ t % 16:
+// whole rows of COLS values to a store.  Straight from the registers a store covers 32
+// bytes of 32 rows, and 252 MB took 110 us in place of .
+// What is read beside them and the pieces come for several stores at once: one by one,
+// each waited for its own.
+template <int T, int TX, int TW> __device__ __forceinline__ void mx_rows_out(const Fh3kMxOut &o, const f32x16 (&acc)[TX][TW], f32x4 *stg, int lane,
+                                                                             int64_t t0, int64_t rows, int n0, int64_t cols, bool vec) {
+    constexpr int COLS = TW * 32, C = COLS / 4, L = COLS / 8, TPI = 64 / L, U = 4;   // eight values to a lane
+    const int g = lane >> 5, l = lane & 31, e = lane % L, n = n0 + 8 * e;
 #pragma unroll
-            for (int m = 0; m < 2; m++)
-                if (t < rows && n + 16 * m + 8 <= cols) mx_beside<T>(c[m], o, t, n + 16 * m, cols);
-        };
-        read(0);
+    for (int i = 0; i < TX; i++) {
+        const int64_t ti = t0 + 32 * i;
+#pragma unroll
+        for (int j = 0; j < TW; j++)
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                stg[l * C + ((8 * j + 2 * q + g) ^ (l & 15))] = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        __builtin_amdgcn_wave_barrier();
+        const bool whole = vec && n + 8 <= cols;
 #pragma unroll 1
-        for (int idx = 0; idx < TX * TW; idx++) {
-            f32x16 a;
-            float v[2][8];
-            int64_t t;
-            int n;
-            mx_pick<TX, TW>(a, acc, idx);
-            mx_columns(a, v);
-            b[0] = c[0];
-            b[1] = c[1];
-            if (idx + 1 < TX * TW) read(idx + 1);
-            at(idx, t, n);
+        for (int it = 0; it < 32; it += TPI * U) {
+            const int tl = it + lane / L;
+            if (whole) {
+                Beside b[U];
+                f32x4 a[U][2];
 #pragma unroll
-            for (int m = 0; m < 2; m++, n += 16) {
-                if (t >= rows) continue;
-                if (n + 8 <= cols) mx_put<T>(o, t, n, v[m], b[m]);
-                else
+                for (int u = 0; u < U; u++) {
+                    const int t = tl + u * TPI;
+                    mx_beside<T>(b[u], o, ti + t < rows ? ti + t : rows - 1, n, cols);   // past the end: the last row's
 #pragma unroll
-                    for (int k = 0; k < 8; k++)
-                        if (n + k < cols) mx_put1<T>(o, t, n + k, cols, v[m][k]);
+                    for (int h = 0; h < 2; h++) a[u][h] = stg[t * C + ((2 * e + h) ^ (t & 15))];
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    float v[8] = {a[u][0][0], a[u][0][1], a[u][0][2], a[u][0][3], a[u][1][0], a[u][1][1], a[u][1][2], a[u][1][3]};
+                    if (ti + tl + u * TPI < rows) mx_put<T>(o, ti + tl + u * TPI, n, v, b[u]);
+                }
+            } else {
+                for (int t = tl; t < tl + TPI * U; t += TPI)
+                    if (ti + t < rows)
+#pragma unroll
+                        for (int k = 0; k < 8; k++)
+                            if (n + k < cols) {
+                                const f32x4 a = stg[t * C + ((2 * e + (k >> 2)) ^ (t & 15))];
+                                mx_put1<T>(o, ti + t, n + k, cols, a[k & 3]);
+                            }
             }
         }
-    } else {
-#pragma unroll 1
-        for (int idx = 0; idx < TX * TW; idx++) {
-            f32x16 a;
-            float v[2][8];
-            int64_t t;
-            int n;
-            mx_pick<TX, TW>(a, acc, idx);
-            mx_columns(a, v);
-            at(idx, t, n);
-            if (t >= rows) continue;
-#pragma unroll
-            for (int m = 0; m < 2; m++)
-#pragma unroll
-                for (int k = 0; k < 8; k++)
-                    if (n + 16 * m + k < cols) mx_put1<T>(o, t, n + 16 * m + k, cols, v[m][k]);
-        }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 // The same where the wavefront's first tiles are values and the others their gates: SwiGLU to codes.  A block is a tile's 32 columns.
@@ -765,7 +756,13 @@ template <class G, bool SPLIT> __global__ __launch_bounds__(64 * G::WAVES, 8 / G
         }
     }
     mx_settle(acc);
-    __builtin_amdgcn_s_waitcnt(waits(0, 0));   // nothing more comes to LDS, which may be another workgroup's soon
+    // nothing more comes to LDS, and nobody reads it
+    __builtin_amdgcn_s_waitcnt(waits(0, 0));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    constexpr int PIECE = TW * 32 * 32 / 4, PER = sizeof(typename G::Buf) / 16 / PIECE;   // 16-byte words of a wavefront, wavefronts to a buffer
+    static_assert(G::NBUF * PER >= G::WAVES, "the sums' room");
+    f32x4 *stg = (f32x4 *)(wave < PER ? b0.x : wave < 2 * PER || G::NBUF == 2 ? b1.x : (u32x4 *)&b2) + wave % PER * PIECE;
     if (part) {
         o = Fh3kMxOut{};
         o.out = part + blockIdx.y * (x.rows * ldp);
@@ -776,9 +773,9 @@ template <class G, bool SPLIT> __global__ __launch_bounds__(64 * G::WAVES, 8 / G
     if (swiglu) {
         if (o.y.type == FH3K_MX_FP8) mx_swiglu_out<true>(o, acc, lane, t0, x.rows, n0 / 2);
         else mx_swiglu_out<false>(o, acc, lane, t0, x.rows, n0 / 2);
-    } else if (o.type == FH3K_F32) mx_rows_out<FH3K_F32>(o, acc, lane, t0, x.rows, n0, part ? ldp : w.rows, vec);
-    else if (o.type == FH3K_F16) mx_rows_out<FH3K_F16>(o, acc, lane, t0, x.rows, n0, w.rows, vec);
-    else mx_rows_out<FH3K_BF16>(o, acc, lane, t0, x.rows, n0, w.rows, vec);
+    } else if (o.type == FH3K_F32) mx_rows_out<FH3K_F32>(o, acc, stg, lane, t0, x.rows, n0, part ? ldp : w.rows, vec);
+    else if (o.type == FH3K_F16) mx_rows_out<FH3K_F16>(o, acc, stg, lane, t0, x.rows, n0, w.rows, vec);
+    else mx_rows_out<FH3K_BF16>(o, acc, stg, lane, t0, x.rows, n0, w.rows, vec);
 }
 
 // The parts of a split product, added in their order, to rows of the output: eight values to a thread.
