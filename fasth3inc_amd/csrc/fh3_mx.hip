@@ -285,22 +285,35 @@ template <int P> __device__ __forceinline__ int mx_place(int r, int p) { return 
 
 constexpr uint32_t MX_OUTSIDE = 0xC0000000u;   // past every buffer here: reads as zero
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rsrc(const void *p, uint32_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, (int)bytes, 0x00020000);
+__device__ __forceinline__ u32x4 mx_rsrc(const void *p, uint32_t bytes) {
+    const uint64_t a = (uint64_t)(uintptr_t)p;
+    return u32x4{(uint32_t)a, (uint32_t)(a >> 32) & 0xFFFFu, bytes, 0x00020000u};
 }
-
-// `at` is uniform, which the compiler loses sight of where it runs short of scalar registers
-__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, u32x4 *to, uint32_t off, int at) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)to, 16, off, __builtin_amdgcn_readfirstlane(at), 0, 0);
+// DMA to LDS, 16 or 4 bytes of each lane to consecutive places.  As builtins they made
+// the compiler wait for all of them (vmcnt(0)) before reads of other buffers here and
+// there; as asm, which has no outputs, the waits are the kernel's own.  The nops stand
+// between a scalar that the VALU may have written and the load that reads it.  m0 is
+// used for nothing else here.
+template <int BYTES> __device__ __forceinline__ void mx_dma(const u32x4 &r, void *to, uint32_t off, int at) {
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_void *)to;
+    at = __builtin_amdgcn_readfirstlane(at);   // uniform, which the compiler loses sight of where it runs short of scalars
+    if constexpr (BYTES == 16)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(lds), "v"(off), "s"(r), "s"(at) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, %3 offen lds" : : "s"(lds), "v"(off), "s"(r), "s"(at) : "memory");
 }
-__device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t r, uint32_t *to, uint32_t off, int at) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)to, 4, off, __builtin_amdgcn_readfirstlane(at), 0, 0);
+// All but the last VM loads have landed and all operands are read, in every wavefront.
+template <int VM> __device__ __forceinline__ void mx_barrier() {
+    static_assert(VM < 64, "the counter's range");
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(VM) : "memory");
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // What a wavefront loads of one operand: a quarter of the tile's rows.
 template <class G, int ROW, int N, int NS> struct Rows {
     static constexpr int P = ROW / 16, RPI = 64 / P;   // pieces of a row, rows to an instruction
-    __amdgpu_buffer_rsrc_t code, scale;
+    u32x4 code, scale;
     uint32_t off[N], soff[NS];                         // of this lane, for each instruction
     int piece[2];                                      // of its row, in even and odd instructions
 
@@ -328,11 +341,11 @@ template <class G, int ROW, int N, int NS> struct Rows {
     }
     // instruction j of stage st, of whose row `pieces` pieces are there
     template <int j> __device__ __forceinline__ void dma(u32x4 *to, int wave, int st, int pieces) const {
-        dma16(code, to + (wave * N + j) * 64, piece[j & 1] < pieces ? off[j] : MX_OUTSIDE, st * ROW);
+        mx_dma<16>(code, to + (wave * N + j) * 64, piece[j & 1] < pieces ? off[j] : MX_OUTSIDE, st * ROW);
     }
     __device__ __forceinline__ void dma_scales(uint32_t *to, int wave, int st) const {
 #pragma unroll
-        for (int j = 0; j < NS; j++) dma4(scale, to + (wave * NS + j) * 64, soff[j], st * G::NB);
+        for (int j = 0; j < NS; j++) mx_dma<4>(scale, to + (wave * NS + j) * 64, soff[j], st * G::NB);
     }
 };
 template <class G> struct Load {
@@ -455,9 +468,11 @@ template <class G, bool SPLIT, int t, int tn, bool SC, int Q, int j = 0> __devic
     f32x16 (&acc)[G::TX][G::TW], const Frags<G> &f, const StageScales<G> &s, Frags<G> &nf, Scales<G> &ns, const typename G::Buf &nb,
     const typename G::ScaleBuf &sb, const Load<G> &ld, typename G::Buf &lb, int to, int wr, int xr, int g) {
     if constexpr (j < G::TX) {
-        constexpr int per = (G::TW + G::TX) / G::TX, gap = Q * G::TX + j, gaps = 2 * G::TX;
+        constexpr int gap = Q * G::TX + j, gaps = 2 * G::TX;
         auto between = [&]() {
-            mx_reads<G, tn, SC, j * per, (j + 1) * per>(nf, ns, nb, sb, wr, xr, g);
+            // (FP8 codes split in two leave registers for half of them)
+            constexpr int N = G::TW + G::TX, n0 = SPLIT ? j * N / G::TX : j ? N : 0, n1 = SPLIT ? (j + 1) * N / G::TX : N;
+            mx_reads<G, tn, SC, n0, n1>(nf, ns, nb, sb, wr, xr, g);
             if constexpr (Q >= 0) ld.template codes<gap * G::D / gaps, (gap + 1) * G::D / gaps>(lb, to);
         };
         if constexpr (SPLIT) {
@@ -493,8 +508,6 @@ template <int TX, int TW> __device__ __forceinline__ void mx_settle(f32x16 (&acc
         for (int j = 0; j < TW; j++) asm volatile("" : "+a"(acc[i][j]));
 }
 
-constexpr int waits(int vm, int lgkm) { return (vm & 15) | 7 << 4 | lgkm << 8 | (vm >> 4) << 14; }
-
 // g / (1 + exp(-g)), to two units in the last place and those of exp2's argument
 __device__ __forceinline__ float silu(float g) { return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-LOG2E * g)); }
 
@@ -502,8 +515,8 @@ __device__ __forceinline__ float silu(float g) { return g * __builtin_amdgcn_rcp
 struct Beside {
     f32x4 gate[2], res[2];     // 16-bit residuals: as stored, in res[0]
 };
-template <int T> __device__ __forceinline__ void mx_beside(Beside &b, const Fh3kMxOut &o, int64_t t, int n, int64_t cols) {
-    if (o.res) {
+template <int T, bool RES> __device__ __forceinline__ void mx_beside(Beside &b, const Fh3kMxOut &o, int64_t t, int n, int64_t cols) {
+    if constexpr (RES) {
         const f32x4 *p = (const f32x4 *)((const uint8_t *)o.res + (t * o.ldres + n) * (T == FH3K_F32 ? 4 : 2));
         b.res[0] = p[0];
         if constexpr (T == FH3K_F32) b.res[1] = p[1];
@@ -516,11 +529,11 @@ template <int T> __device__ __forceinline__ void mx_beside(Beside &b, const Fh3k
 template <int T> __device__ __forceinline__ float half_value(uint32_t b) {
     return T == FH3K_F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)b) : __builtin_bit_cast(float, b << 16);
 }
-template <int T> __device__ __forceinline__ void mx_put(const Fh3kMxOut &o, int64_t t, int n, float (&v)[8], const Beside &b) {
+template <int T, bool RES> __device__ __forceinline__ void mx_put(const Fh3kMxOut &o, int64_t t, int n, float (&v)[8], const Beside &b) {
     if (o.bias)
 #pragma unroll
         for (int k = 0; k < 8; k++) v[k] += o.bias[n + k];
-    if (o.res) {
+    if constexpr (RES) {
 #pragma unroll
         for (int k = 0; k < 8; k++) {
             float h;
@@ -571,13 +584,15 @@ template <int TX, int TW, int i = 0> __device__ __forceinline__ void mx_pick(f32
 // A wavefront's sums to rows of the output through its own piece of LDS, 32 tokens at
 // a time, [32][COLS / 4] pieces of four values with piece c of token t at c ^ t % 16:
 // whole rows of COLS values to a store.  Straight from the registers a store covers 32
-// bytes of 32 rows, and 252 MB took 110 us in place of .
-// What is read beside them and the pieces come for several stores at once: one by one,
-// each waited for its own.
-template <int T, int TX, int TW> __device__ __forceinline__ void mx_rows_out(const Fh3kMxOut &o, const f32x16 (&acc)[TX][TW], f32x4 *stg, int lane,
-                                                                             int64_t t0, int64_t rows, int n0, int64_t cols, bool vec) {
-    constexpr int COLS = TW * 32, C = COLS / 4, L = COLS / 8, TPI = 64 / L, U = 4;   // eight values to a lane
+// bytes of 32 rows: 8192 x 5120 -> 15360 in FP4 398 against 387 us.
+// What is read beside them and the pieces come for U stores at once: one by one, each
+// waited for its own.
+template <int T, bool RES, int TX, int TW> __device__ __forceinline__ void mx_rows_out(const Fh3kMxOut &o, const f32x16 (&acc)[TX][TW], f32x4 *stg,
+                                                                                       int lane, int64_t t0, int64_t rows, int n0, int64_t cols,
+                                                                                       bool vec) {
+    constexpr int COLS = TW * 32, C = COLS / 4, L = COLS / 8, TPI = 64 / L, U = RES ? 2 : 4;   // eight values to a lane
     const int g = lane >> 5, l = lane & 31, e = lane % L, n = n0 + 8 * e;
+    const bool whole = vec && n + 8 <= cols;
 #pragma unroll
     for (int i = 0; i < TX; i++) {
         const int64_t ti = t0 + 32 * i;
@@ -587,7 +602,6 @@ template <int T, int TX, int TW> __device__ __forceinline__ void mx_rows_out(con
             for (int q = 0; q < 4; q++)
                 stg[l * C + ((8 * j + 2 * q + g) ^ (l & 15))] = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
         __builtin_amdgcn_wave_barrier();
-        const bool whole = vec && n + 8 <= cols;
 #pragma unroll 1
         for (int it = 0; it < 32; it += TPI * U) {
             const int tl = it + lane / L;
@@ -597,28 +611,31 @@ template <int T, int TX, int TW> __device__ __forceinline__ void mx_rows_out(con
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     const int t = tl + u * TPI;
-                    mx_beside<T>(b[u], o, ti + t < rows ? ti + t : rows - 1, n, cols);   // past the end: the last row's
+                    mx_beside<T, RES>(b[u], o, ti + t < rows ? ti + t : rows - 1, n, cols);   // past the end: the last row's
 #pragma unroll
                     for (int h = 0; h < 2; h++) a[u][h] = stg[t * C + ((2 * e + h) ^ (t & 15))];
                 }
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     float v[8] = {a[u][0][0], a[u][0][1], a[u][0][2], a[u][0][3], a[u][1][0], a[u][1][1], a[u][1][2], a[u][1][3]};
-                    if (ti + tl + u * TPI < rows) mx_put<T>(o, ti + tl + u * TPI, n, v, b[u]);
+                    if (ti + tl + u * TPI < rows) mx_put<T, RES>(o, ti + tl + u * TPI, n, v, b[u]);
                 }
             } else {
+#pragma unroll 1
                 for (int t = tl; t < tl + TPI * U; t += TPI)
-                    if (ti + t < rows)
-#pragma unroll
-                        for (int k = 0; k < 8; k++)
-                            if (n + k < cols) {
-                                const f32x4 a = stg[t * C + ((2 * e + (k >> 2)) ^ (t & 15))];
-                                mx_put1<T>(o, ti + t, n + k, cols, a[k & 3]);
-                            }
+#pragma unroll 1
+                    for (int k = 0; k < 8; k++)
+                        if (ti + t < rows && n + k < cols)
+                            mx_put1<T>(o, ti + t, n + k, cols, ((const float *)(stg + t * C + ((2 * e + (k >> 2)) ^ (t & 15))))[k & 3]);
             }
         }
         __builtin_amdgcn_wave_barrier();
     }
+}
+template <int T, int TX, int TW> __device__ __forceinline__ void mx_rows_out(const Fh3kMxOut &o, const f32x16 (&acc)[TX][TW], f32x4 *stg, int lane,
+                                                                             int64_t t0, int64_t rows, int n0, int64_t cols, bool vec) {
+    if (o.res) mx_rows_out<T, true>(o, acc, stg, lane, t0, rows, n0, cols, vec);
+    else mx_rows_out<T, false>(o, acc, stg, lane, t0, rows, n0, cols, vec);
 }
 // The same where the wavefront's first tiles are values and the others their gates: SwiGLU to codes.  A block is a tile's 32 columns.
 template <bool F8, int TX, int TW> __device__ __forceinline__ void mx_swiglu_out(const Fh3kMxOut &o, const f32x16 (&acc)[TX][TW], int lane,
@@ -709,9 +726,7 @@ template <class G, bool SPLIT> __global__ __launch_bounds__(64 * G::WAVES, 8 / G
     } else {
         ld.template codes<0, G::D / 2>(b1, s0 + 1);
     }
-    __builtin_amdgcn_s_waitcnt(waits((G::NBUF - 2) * G::D + G::D / 2, 0));
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
+    mx_barrier<(G::NBUF - 2) * G::D + G::D / 2>();
     mx_reads<G, 0, true, 0, G::TW + G::TX>(fr[0], sc, b0, sb, wr, xr, g);
 
     // Stage s, the chunk's c-th.
@@ -725,9 +740,7 @@ template <class G, bool SPLIT> __global__ __launch_bounds__(64 * G::WAVES, 8 / G
             mx_step<G, SPLIT, 2, 3, false, -1>(acc, fr[0], ss, fr[1], sc, cur, sb, ld, prev, 0, wr, xr, g);
         }
         // this stage's operands are all read, the next one's have landed
-        __builtin_amdgcn_s_waitcnt(waits((G::NBUF - 2) * G::D, 0));
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
+        mx_barrier<(G::NBUF - 2) * G::D>();
         if constexpr (c == 0) ld.scales(sb, s + G::CH);   // this chunk's are all in registers
         mx_step<G, SPLIT, G::T - 1, 0, c == G::CH - 1, 0>(acc, fr[1], ss, fr[0], sc, nxt, sb, ld, cur, s + G::NBUF, wr, xr, g);
     };
@@ -757,9 +770,7 @@ template <class G, bool SPLIT> __global__ __launch_bounds__(64 * G::WAVES, 8 / G
     }
     mx_settle(acc);
     // nothing more comes to LDS, and nobody reads it
-    __builtin_amdgcn_s_waitcnt(waits(0, 0));
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
+    mx_barrier<0>();
     constexpr int PIECE = TW * 32 * 32 / 4, PER = sizeof(typename G::Buf) / 16 / PIECE;   // 16-byte words of a wavefront, wavefronts to a buffer
     static_assert(G::NBUF * PER >= G::WAVES, "the sums' room");
     f32x4 *stg = (f32x4 *)(wave < PER ? b0.x : wave < 2 * PER || G::NBUF == 2 ? b1.x : (u32x4 *)&b2) + wave % PER * PIECE;
@@ -793,8 +804,12 @@ template <int T> __global__ __launch_bounds__(256) void k_mx_join(const float *_
     }
     if (vec && n + 8 <= cols) {
         Beside b;
-        mx_beside<T>(b, o, t, n, cols);
-        mx_put<T>(o, t, n, v, b);
+        if (o.res) {
+            mx_beside<T, true>(b, o, t, n, cols);
+            mx_put<T, true>(o, t, n, v, b);
+        } else {
+            mx_put<T, false>(o, t, n, v, b);
+        }
     } else {
 #pragma unroll
         for (int k = 0; k < 8; k++)
