@@ -838,6 +838,215 @@ template <bool F8> __global__ __launch_bounds__(256) void k_mx_join_swiglu(const
     mx_store<F8>(o.y, t, col, a);
 }
 
+// ---------------------------------------------------------------------------
+// Few rows (up to 16 TT): bound by the weights' way from memory.  A workgroup
+// takes 16 R weight rows, its wavefronts a share each of the rows' windows of 128 S
+// values, straight from memory into 16x16x128 products, and their sums meet in LDS.
+// Lane (r, g), g = 0 .. 3, holds of row r the FP4 codes 32 g .. + 31 of a step's 128, or
+// the FP8 codes 16 g .. + 15 and 64 + 16 g .. + 15, and the scale of block g.
+// FP8 rows to fp32 enter as two products (fp8_large).
+// SwiGLU: half of the R tiles are values' rows, half their gates'.
+// ---------------------------------------------------------------------------
+constexpr int MX_WAVES = 12, MX_WAVES_AHEAD = 8;   // the most wavefronts to a workgroup
+
+__device__ __forceinline__ u32x4 mx_load16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
+}
+__device__ __forceinline__ u32x2 mx_load8(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, 0));
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_buffer(const void *p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, (int)bytes, 0x00020000);
+}
+
+// Sixteen rows of an operand: those past the end are the last one.
+struct Few {
+    __amdgpu_buffer_rsrc_t code, scale;
+    uint32_t off, soff;                  // of this lane's row
+    __device__ __forceinline__ void init(const Fh3kMx &m, int64_t base, int r) {
+        if (base >= m.rows) base = m.rows - 1;
+        const int last = m.rows - base < 16 ? (int)(m.rows - base) - 1 : 15;
+        code = mx_buffer(m.codes + base * m.ld, (uint32_t)(last * m.ld + (m.type == FH3K_MX_FP8 ? m.in : m.in / 2)));
+        scale = mx_buffer(m.scales + base * m.lds, (uint32_t)(last * m.lds + (m.in / MX_BLOCK + 3) / 4 * 4));
+        r = r < last ? r : last;
+        off = (uint32_t)(r * m.ld);
+        soff = (uint32_t)(r * m.lds);
+    }
+};
+
+__device__ __forceinline__ f32x4 mx_mfma16(const u32x4 &w, const i32x8 &x, f32x4 acc, int ws, int xs, bool f8) {
+    const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+    if (f8) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, x, acc, 4, 0, 0, ws, 0, xs);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, x, acc, 4, 4, 0, ws, 0, xs);
+}
+
+template <bool F8, int TT, int R> struct Window {
+    static constexpr int S = TT == 1 ? 4 : 2;                              // steps
+    static constexpr int WB = 64 * S, XB = F8 ? 128 * S : 64 * S;          // bytes of a row
+    typedef typename std::conditional<S == 4, u32x4, u32x2>::type Dwords;  // of scales, one for each step's four blocks
+    u32x4 w[R][S];
+    u32x4 x[TT][S][F8 ? 2 : 1];
+    Dwords ws[R], xs[TT];
+
+    __device__ __forceinline__ static void scales(Dwords &d, __amdgpu_buffer_rsrc_t r, uint32_t off) {
+        if constexpr (S == 4) d = mx_load16(r, off);
+        else d = mx_load8(r, off);
+    }
+    // window `at`, `left` blocks from its start to the rows' end
+    __device__ __forceinline__ void load(const Few (&fw)[R], const Few (&fx)[TT], int at, int left, int g) {
+#pragma unroll
+        for (int i = 0; i < R; i++) scales(ws[i], fw[i].scale, fw[i].soff + at * (4 * S));
+#pragma unroll
+        for (int j = 0; j < TT; j++) scales(xs[j], fx[j].scale, fx[j].soff + at * (4 * S));
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            const bool in = 4 * s + g < left;
+#pragma unroll
+            for (int i = 0; i < R; i++) w[i][s] = mx_load16(fw[i].code, in ? fw[i].off + at * WB + s * 64 + g * 16 : MX_OUTSIDE);
+#pragma unroll
+            for (int j = 0; j < TT; j++) {
+                if constexpr (F8) {
+                    const int b = 4 * s + (g >> 1);
+                    const uint32_t off = fx[j].off + at * XB + s * 128 + g * 16;
+                    x[j][s][0] = mx_load16(fx[j].code, b < left ? off : MX_OUTSIDE);
+                    x[j][s][1] = mx_load16(fx[j].code, b + 2 < left ? off + 64 : MX_OUTSIDE);
+                } else {
+                    x[j][s][0] = mx_load16(fx[j].code, in ? fx[j].off + at * XB + s * 64 + g * 16 : MX_OUTSIDE);
+                }
+            }
+        }
+    }
+    // the scale of step s's block g; past the row's end 0, whatever stands there
+    __device__ __forceinline__ static int scale(uint32_t d, int s, int left, int g) { return 4 * s + g < left ? (int)(d >> (8 * g)) : 0; }
+
+    template <bool SPLIT> __device__ __forceinline__ void products(f32x4 (&acc)[R][TT], int left, int g) const {
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            int sw[R];
+#pragma unroll
+            for (int i = 0; i < R; i++) sw[i] = scale(ws[i][s], s, left, g);
+#pragma unroll
+            for (int j = 0; j < TT; j++) {
+                const int sx = scale(xs[j][s], s, left, g);
+                i32x8 v = {}, h;
+                set4(v, 0, x[j][s][0]);
+                if constexpr (F8) set4(v, 4, x[j][s][1]);
+                if constexpr (SPLIT) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        h[k] = (int)fp8_large((uint32_t)v[k]);
+                        v[k] ^= h[k];
+                    }
+#pragma unroll
+                    for (int i = 0; i < R; i++) acc[i][j] = mx_mfma16(w[i][s], h, acc[i][j], sw[i], sx, true);
+                }
+#pragma unroll
+                for (int i = 0; i < R; i++) acc[i][j] = mx_mfma16(w[i][s], v, acc[i][j], sw[i], sx, F8);
+            }
+        }
+    }
+};
+
+template <bool F8, bool SPLIT, int TT, int R, bool AHEAD> __global__ __launch_bounds__(64 * (AHEAD || TT == 4 || R * TT == 8 ? MX_WAVES_AHEAD : MX_WAVES)) void k_mx_few(Fh3kMx w, Fh3kMx x, Fh3kMxOut o) {
+    extern __shared__ f32x4 parts[];         // [wavefront][R][TT][64]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int r = lane & 15, g = lane >> 4;
+    const bool swiglu = o.y.codes != nullptr;
+    const int64_t f = w.rows >> 1, n0 = (int64_t)blockIdx.x * (swiglu ? 8 * R : 16 * R);
+    Few fw[R], fx[TT];
+#pragma unroll
+    for (int i = 0; i < R; i++) fw[i].init(w, swiglu ? (i < R / 2 ? 0 : f) + n0 + 16 * (i % (R / 2 > 0 ? R / 2 : 1)) : n0 + 16 * i, r);
+#pragma unroll
+    for (int j = 0; j < TT; j++) fx[j].init(x, 16 * j, r);
+    typedef Window<F8, TT, R> Win;
+    constexpr int WBL = 4 * Win::S;          // blocks of a window
+    const int blocks = (int)(w.in / MX_BLOCK), windows = (blocks + WBL - 1) / WBL;
+    f32x4 acc[R][TT] = {};
+    // AHEAD: the next window's loads before this one's products
+    Win v[AHEAD ? 2 : 1];
+    if (AHEAD && wave < windows) v[0].load(fw, fx, wave, blocks - WBL * wave, g);
+    for (int at = wave; at < windows; at += 2 * waves) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int a = at + h * waves, b = a + waves;
+            if (a >= windows) break;
+            if (!AHEAD) v[0].load(fw, fx, a, blocks - WBL * a, g);
+            else if (b < windows) v[AHEAD ? 1 - h : 0].load(fw, fx, b, blocks - WBL * b, g);
+            v[AHEAD ? h : 0].template products<SPLIT>(acc, blocks - WBL * a, g);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < R; i++)
+#pragma unroll
+        for (int j = 0; j < TT; j++) parts[((wave * R + i) * TT + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    // a wavefront to a tile of 16 x 16 (SwiGLU: to one of values and its gates)
+    auto sum = [&](int i, int j) {
+        f32x4 v = parts[(i * TT + j) * 64 + lane];
+        for (int k = 1; k < waves; k++) {
+            const f32x4 a = parts[((k * R + i) * TT + j) * 64 + lane];
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] += a[e];
+        }
+        return v;
+    };
+    if (swiglu) {
+        if constexpr (R == 4) {
+            // both tiles of a block of 32 outputs: lane (t, g) has its outputs 4 g .. and 16 + 4 g .. of token t
+            for (int j = wave; j < TT; j += waves) {
+                const int64_t t = 16 * j + r;
+                float a[2][4];
+                uint32_t u = 0;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const f32x4 v = sum(i, j), q = sum(2 + i, j);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int64_t n = n0 + 16 * i + 4 * g + e;
+                        a[i][e] = (v[e] + (o.bias ? o.bias[n] : 0.f)) * silu(q[e] + (o.bias ? o.bias[f + n] : 0.f));
+                        const float c = a[i][e];
+                        const uint32_t b = __builtin_bit_cast(uint32_t, c) & 0x7FFFFFFFu;
+                        u = u > b ? u : b;
+                    }
+                }
+                u = max(u, (uint32_t)__shfl_xor((int)u, 16));
+                u = max(u, (uint32_t)__shfl_xor((int)u, 32));
+                const bool to8 = o.y.type == FH3K_MX_FP8;
+                const uint32_t s = to8 ? mx_scale<true>(u) : mx_scale<false>(u);
+                float v[8] = {a[0][0], a[0][1], a[0][2], a[0][3], a[1][0], a[1][1], a[1][2], a[1][3]};
+                if (t >= x.rows) continue;
+                if (to8) {
+                    const u32x2 c = mx_encode<true>(v, s);
+                    uint8_t *p = o.y.codes + t * o.y.ld + n0 + 4 * g;
+                    *(uint32_t *)p = c.x;
+                    *(uint32_t *)(p + 16) = c.y;
+                } else {
+                    const uint32_t c = mx_encode<false>(v, s).x;
+                    uint8_t *p = o.y.codes + t * o.y.ld + n0 / 2 + 2 * g;
+                    *(uint16_t *)p = (uint16_t)c;
+                    *(uint16_t *)(p + 8) = (uint16_t)(c >> 16);
+                }
+                if (g == 0) o.y.scales[t * o.y.lds + n0 / MX_BLOCK] = (uint8_t)s;
+            }
+        }
+        return;
+    }
+    for (int tile = wave; tile < R * TT; tile += waves) {
+        const int i = tile / TT, j = tile % TT;
+        const int64_t t = 16 * j + r;
+        const f32x4 v = sum(i, j);
+        if (t >= x.rows) continue;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int64_t n = n0 + 16 * i + 4 * g + e;
+            if (n >= w.rows) continue;
+            if (o.type == FH3K_F32) mx_put1<FH3K_F32>(o, t, (int)n, w.rows, v[e]);
+            else if (o.type == FH3K_F16) mx_put1<FH3K_F16>(o, t, (int)n, w.rows, v[e]);
+            else mx_put1<FH3K_BF16>(o, t, (int)n, w.rows, v[e]);
+        }
+    }
+}
+
 // lanes to a row: a power of two, eight values each
 int row_lanes(int64_t in) {
     int n = 4;
@@ -896,23 +1105,34 @@ namespace {
 
 // How a product is cut: tiles, and parts of the rows' length.
 struct Plan {
+    bool few;                     // k_mx_few
     int bw, bx, parts, per;       // per: stages of a part
     int64_t m_tiles, n_tiles, ldp;
 };
-Plan plan_of(const Fh3kMx *w, const Fh3kMx *x) {
-    Plan p;
+// Tiles of 16 weight rows to a workgroup of k_mx_few: the most that leave 150
+// workgroups, since each reads all rows of x.  SwiGLU: a block of 32 outputs.
+int few_tiles(const Fh3kMx *w, const Fh3kMx *x, bool swiglu) {
+    const int64_t n16 = (w->rows + 15) / 16;
+    return swiglu || (n16 >= 600 && x->rows <= 16) ? 4 : n16 >= 300 ? 2 : 1;
+}
+
+Plan plan_of(const Fh3kMx *w, const Fh3kMx *x, bool swiglu) {
+    Plan p = {};
+    // k_mx_few where what its workgroups read of x stays below 2^26 values, SwiGLU
+    // 2^27; fp32 / bf16 outputs, FP8 rows, us, it and the tiles: 5120 -> 5120, 64 rows 21.2 / 16.8,
+    // 22.8 / 20.2; 8192 -> 5120, 64 rows 30.9 / 27.2, 25.2 / 21.2; 25600 -> 5120, 16 rows 30.6 / 30.7, 43.6 / 32.5,
+    // 32 rows 46.1 / 44.4, 43.6 / 32.5; 5120 -> 51200 SwiGLU, 32 rows 57, 60, 64 rows 76, 60
+    const int64_t rows = 16 * few_tiles(w, x, swiglu), groups = (w->rows + rows - 1) / rows;
+    if (x->rows <= 64 && groups * x->rows * w->in <= ((int64_t)1 << (swiglu ? 27 : 26))) {
+        p.few = true;
+        p.parts = 1;
+        return p;
+    }
     auto tiles = [&](int b) { return ((w->rows + b - 1) / b) * ((x->rows + b - 1) / b); };
     p.bw = p.bx = tiles(256) >= 192 ? 256 : 128;
-#ifdef CFG2
-    if (p.bw == 256) p.bx = 128;
-#endif
     p.m_tiles = (x->rows + p.bx - 1) / p.bx;
     p.n_tiles = (w->rows + p.bw - 1) / p.bw;
-    #ifdef CFG2
-    const int ks = x->type == FH3K_MX_FP8 || p.bw == 256 ? 128 : 256;
-#else
-    const int ks = x->type == FH3K_MX_FP8 ? 128 : 256;
-#endif
+        const int ks = x->type == FH3K_MX_FP8 ? 128 : 256;
     const int stages = (int)((w->in + ks - 1) / ks);
     const int64_t t = p.m_tiles * p.n_tiles;
     int parts = 1;
@@ -931,34 +1151,64 @@ template <class G, bool SPLIT = false> void launch_gemm(const Fh3kMx *w, const F
     k_mx_gemm<G, SPLIT><<<grid, 64 * G::WAVES, 0, st>>>(*w, *x, *o, part, p.ldp, (int)p.m_tiles, (int)p.n_tiles, p.per, vec || part);
 }
 
+template <bool F8, bool SPLIT, int TT, int R> void launch_few(const Fh3kMx *w, const Fh3kMx *x, const Fh3kMxOut *o, hipStream_t st) {
+    const int64_t n = o->y.codes ? w->rows / 2 : w->rows, per = o->y.codes ? 8 * R : 16 * R;
+    // as many wavefronts as share the windows evenly, and whose sums fit 64 KiB; where
+    // that leaves each more than one, eight that load ahead
+    constexpr int WIN = 128 * Window<F8, TT, R>::S;
+    const int room = 64 / (R * TT), windows = (int)((w->in + WIN - 1) / WIN);
+    auto go = [&](auto ahead, int most) {
+        if (most > room) most = room;
+        const int each = (windows + most - 1) / most, waves = (windows + each - 1) / each;
+        k_mx_few<F8, SPLIT, TT, R, ahead()><<<(unsigned)((n + per - 1) / per), 64 * waves, waves * R * TT * 1024, st>>>(*w, *x, *o);
+    };
+    // (registers for two windows)
+    if constexpr (Window<F8, TT, R>::S * (R + TT * (F8 ? 2 : 1)) <= 20) {
+        if (windows > MX_WAVES) return go(std::true_type{}, MX_WAVES_AHEAD);
+    }
+    go(std::false_type{}, TT == 4 || R * TT == 8 ? MX_WAVES_AHEAD : MX_WAVES);
+}
+
 // Whether rows of an array, ld values apart, can be taken 16 bytes at a time.
 bool sixteens(const void *p, int64_t ld, int size) { return !p || ((uintptr_t)p % 16 == 0 && ld * size % 16 == 0); }
 
 }  // namespace
 
 extern "C" int fh3k_mx_matmul_fits(const Fh3kMx *w, const Fh3kMx *x) {
-    const Plan p = plan_of(w, x);
+    const Plan p = plan_of(w, x, false);
     return p.m_tiles * p.n_tiles < ((int64_t)1 << 23) && p.ldp * x->rows <= ((int64_t)1 << 40);
 }
 
-extern "C" size_t fh3k_mx_matmul_ws_bytes(const Fh3kMx *w, const Fh3kMx *x, int) {
-    const Plan p = plan_of(w, x);
+extern "C" size_t fh3k_mx_matmul_ws_bytes(const Fh3kMx *w, const Fh3kMx *x, int swiglu) {
+    const Plan p = plan_of(w, x, swiglu);
     return p.parts > 1 ? (size_t)p.parts * p.ldp * x->rows * sizeof(float) : 0;
 }
 
 extern "C" hipError_t fh3k_mx_matmul(const Fh3kMx *w, const Fh3kMx *x, const Fh3kMxOut *o, void *ws, hipStream_t st) {
-    const Plan p = plan_of(w, x);
+    const Plan p = plan_of(w, x, o->y.codes);
     float *part = p.parts > 1 ? (float *)ws : nullptr;
     const int size = o->type == FH3K_F32 ? 4 : 2;
     const bool vec = sixteens(o->out, o->ldo, size) && sixteens(o->res, o->ldres, size) && sixteens(o->gate, w->rows, 4);
     const bool f8 = x->type == FH3K_MX_FP8, split = f8 && o->type == FH3K_F32 && !o->y.codes;
-#ifdef CFG2
-    using Big4 = Gemm<4, 2, 2, 2, false, 128, 3>;
-    using Big8 = Gemm<4, 2, 2, 2, true, 128, 2>;
-#else
+    if (p.few) {
+        auto go = [&](auto f, auto sp, auto tt) {
+            const int r = few_tiles(w, x, o->y.codes);
+            if (r == 4) launch_few<f(), sp(), tt(), 4>(w, x, o, st);
+            else if (r == 2) launch_few<f(), sp(), tt(), 2>(w, x, o, st);
+            else launch_few<f(), sp(), tt(), 1>(w, x, o, st);
+        };
+        auto by_rows = [&](auto f, auto sp) {
+            if (x->rows <= 16) go(f, sp, std::integral_constant<int, 1>{});
+            else if (x->rows <= 32) go(f, sp, std::integral_constant<int, 2>{});
+            else go(f, sp, std::integral_constant<int, 4>{});
+        };
+        if (!f8) by_rows(std::false_type{}, std::false_type{});
+        else if (!split) by_rows(std::true_type{}, std::false_type{});
+        else by_rows(std::true_type{}, std::true_type{});
+        return hipGetLastError();
+    }
     using Big4 = Gemm<4, 2, 2, 4, false, 256, 2>;
     using Big8 = Gemm<4, 2, 2, 4, true, 128, 3>;
-#endif
     using Small4 = Gemm<2, 2, 2, 2, false, 256, 2>;
     using Small8 = Gemm<2, 2, 2, 2, true, 128, 3>;
     if (p.bw == 256) {
