@@ -1118,29 +1118,42 @@ int few_tiles(const Fh3kMx *w, const Fh3kMx *x, bool swiglu) {
 
 Plan plan_of(const Fh3kMx *w, const Fh3kMx *x, bool swiglu) {
     Plan p = {};
-    // k_mx_few where what its workgroups read of x stays below 2^26 values, SwiGLU
-    // 2^27; fp32 / bf16 outputs, FP8 rows, us, it and the tiles: 5120 -> 5120, 64 rows 21.2 / 16.8,
-    // 22.8 / 20.2; 8192 -> 5120, 64 rows 30.9 / 27.2, 25.2 / 21.2; 25600 -> 5120, 16 rows 30.6 / 30.7, 43.6 / 32.5,
-    // 32 rows 46.1 / 44.4, 43.6 / 32.5; 5120 -> 51200 SwiGLU, 32 rows 57, 60, 64 rows 76, 60
+    // k_mx_few where what its workgroups read of x stays below 3 * 2^24 values; FP8 rows
+    // to bf16, us, it and the tiles: 4096 -> 4096, 64 rows (2^26) 13.7, 15.4; 5120 -> 5120, 64 rows (50 M) 16.8, 15.8;
+    // 5120 -> 15360, 17 rows (42 M) 18.6, 21.9, 32 rows (79 M) 22.4, 21.9; 8192 -> 5120, 33 rows (43 M) 21.0, 18.2;
+    // 5120 -> 51200 SwiGLU, 16 rows (66 M) 42, 47, 32 rows 57, 47
     const int64_t rows = 16 * few_tiles(w, x, swiglu), groups = (w->rows + rows - 1) / rows;
-    if (x->rows <= 64 && groups * x->rows * w->in <= ((int64_t)1 << (swiglu ? 27 : 26))) {
+    if (x->rows <= 64 && groups * x->rows * w->in <= 3 << 24) {
         p.few = true;
         p.parts = 1;
         return p;
     }
-    auto tiles = [&](int b) { return ((w->rows + b - 1) / b) * ((x->rows + b - 1) / b); };
-    p.bw = p.bx = tiles(256) >= 192 ? 256 : 128;
-    p.m_tiles = (x->rows + p.bx - 1) / p.bx;
-    p.n_tiles = (w->rows + p.bw - 1) / p.bw;
-        const int ks = x->type == FH3K_MX_FP8 ? 128 : 256;
-    const int stages = (int)((w->in + ks - 1) / ks);
-    const int64_t t = p.m_tiles * p.n_tiles;
-    int parts = 1;
-    if (p.bw == 128 && t < 384) parts = (int)(512 / t);
-    if (parts > stages / 4) parts = stages / 4;
-    if (parts < 1) parts = 1;
-    p.per = (stages + parts - 1) / parts;
-    p.parts = (stages + p.per - 1) / p.per;
+    // Otherwise the tile size and the number of parts with the least time by what was
+    // measured: us for a stage on a CU that has one workgroup of 128 x 128, two, or one of 256 x 256, and for a round's
+    // beginning and end; parts are written and read at 4 MB a us and joined by a launch of 3.5 us.
+    const bool f8 = x->type == FH3K_MX_FP8;
+    const int ks = f8 ? 128 : 256, stages = (int)((w->in + ks - 1) / ks);
+    const double one = f8 ? 0.65 : 1.05, two = f8 ? 1.0 : 1.42, big = f8 ? 1.45 : 2.1;
+    double least = 0;
+    for (int b = 128; b <= 256; b += 128) {
+        const int64_t m = (x->rows + b - 1) / b, n = (w->rows + b - 1) / b;
+        for (int parts = 1; parts <= 32 && (parts == 1 || parts * 4 <= stages); parts++) {
+            const int per = (stages + parts - 1) / parts;
+            if (parts > 1 && (stages + per - 1) / per != parts) continue;
+            const int64_t groups = m * n * parts, slots = b == 128 ? 512 : 256, rest = groups % slots;
+            const double round = b == 256 ? per * big + 9 : per * two + 4, last = b == 256 || rest > 256 ? round : per * one + 3;
+            double t = (double)(groups / slots) * round + (rest ? last : 0);
+            if (parts > 1) t += 3.5 + (double)parts * x->rows * w->rows * 8 / 4e6;
+            if (least == 0 || t < least) {
+                least = t;
+                p.bw = p.bx = b;
+                p.parts = parts;
+                p.per = per;
+                p.m_tiles = m;
+                p.n_tiles = n;
+            }
+        }
+    }
     p.ldp = (w->rows + 7) / 8 * 8;
     return p;
 }
