@@ -269,6 +269,7 @@ template <int TW_, int TX_, int NW_, int NX_, bool F8_, int KS_, int NBUF_> stru
     static constexpr int WROW = KS / 2, XROW = F8 ? KS : KS / 2;   // bytes of a stage's row
     static constexpr int BW = NW * TW * 32, BX = NX * TX * 32;
     static constexpr int NBUF = NBUF_, CH = NBUF == 3 ? 3 : 4;     // stages in LDS, stages of a chunk of scales
+    static constexpr int HALVES = F8 ? 1 : 2;                      // steps over which a stage's loads are spread
     static constexpr int SD = NB == 8 ? 8 : 4;                     // dwords of a row's chunk in LDS
     static constexpr int WI = BW * WROW / 1024 / WAVES, XI = BX * XROW / 1024 / WAVES, D = WI + XI;   // a wavefront's DMA instructions: a stage's codes
     static constexpr int WS = BW * SD / 64 / WAVES, XS = BX * SD / 64 / WAVES;                         // and a chunk's scales
@@ -463,17 +464,18 @@ template <class G, int t, bool SC, int n, int end> __device__ __forceinline__ vo
 // One step's products; between them operand reads of step tn from nb (SC: and the
 // next chunk's scales), and where Q is 0 or 1 that half of stage `to`'s loads into lb.
 // Loads are issued a few at a time: all at once they kept the matrix instructions behind
-// them waiting for the address unit (8192 x 5120 -> 15360 FP4 515 us).
+// them waiting for the address unit.  Over one step or two: 8192 x 5120 -> 15360 FP4 362,
+// 353 us; 32768 x 13824 -> 5120 FP8 1826, 1850.
 template <class G, bool SPLIT, int t, int tn, bool SC, int Q, int j = 0> __device__ __forceinline__ void mx_step(
     f32x16 (&acc)[G::TX][G::TW], const Frags<G> &f, const StageScales<G> &s, Frags<G> &nf, Scales<G> &ns, const typename G::Buf &nb,
     const typename G::ScaleBuf &sb, const Load<G> &ld, typename G::Buf &lb, int to, int wr, int xr, int g) {
     if constexpr (j < G::TX) {
-        constexpr int gap = Q * G::TX + j, gaps = 2 * G::TX;
+        constexpr int gap = Q * G::TX + j, gaps = G::HALVES * G::TX;
         auto between = [&]() {
             // (FP8 codes split in two leave registers for half of them)
             constexpr int N = G::TW + G::TX, n0 = SPLIT ? j * N / G::TX : j ? N : 0, n1 = SPLIT ? (j + 1) * N / G::TX : N;
             mx_reads<G, tn, SC, n0, n1>(nf, ns, nb, sb, wr, xr, g);
-            if constexpr (Q >= 0) ld.template codes<gap * G::D / gaps, (gap + 1) * G::D / gaps>(lb, to);
+            if constexpr (Q >= 0 && Q < G::HALVES) ld.template codes<gap * G::D / gaps, (gap + 1) * G::D / gaps>(lb, to);
         };
         if constexpr (SPLIT) {
             i32x8 h, l;
@@ -717,16 +719,16 @@ template <class G, bool SPLIT> __global__ __launch_bounds__(64 * G::WAVES, 8 / G
     StageScales<G> ss;
     const int wr = wn * CW + (lane & 31), xr = wm * (G::BX / G::NX) + (lane & 31);
 
-    // the first stages, the last of them to half: the other half is loaded in the first stage's first step
+    // the first stages (the last of them to half, where loads are spread: the other half is loaded in the first stage's first step)
     ld.scales(sb, s0);
     ld.template codes<0, G::D>(b0, s0);
     if constexpr (G::NBUF == 3) {
         ld.template codes<0, G::D>(b1, s0 + 1);
-        ld.template codes<0, G::D / 2>(b2, s0 + 2);
+        ld.template codes<0, G::D / G::HALVES>(b2, s0 + 2);
     } else {
-        ld.template codes<0, G::D / 2>(b1, s0 + 1);
+        ld.template codes<0, G::D / G::HALVES>(b1, s0 + 1);
     }
-    mx_barrier<(G::NBUF - 2) * G::D + G::D / 2>();
+    mx_barrier<(G::NBUF - 2) * G::D + G::D / G::HALVES>();
     mx_reads<G, 0, true, 0, G::TW + G::TX>(fr[0], sc, b0, sb, wr, xr, g);
 
     // Stage s, the chunk's c-th.
