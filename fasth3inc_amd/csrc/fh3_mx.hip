@@ -118,49 +118,66 @@ template <bool F8> __device__ __forceinline__ void mx_store(const Fh3kMx &y, int
     if ((col & (MX_BLOCK - 1)) == 0) y.scales[row * y.lds + col / MX_BLOCK] = (uint8_t)s;
 }
 
-__device__ __forceinline__ float fp4_value(uint32_t c) {
-    const uint32_t m = c & 7;
-    const float a = m < 2 ? 0.5f * (float)m : __builtin_bit_cast(float, (126u + (m >> 1)) << 23 | (m & 1) << 22);
-    return c & 8 ? -a : a;
-}
-__device__ __forceinline__ float fp8_value(uint32_t c) {
-    const uint32_t e = c >> 3 & 15, f = c & 7;
-    float a = e ? __builtin_bit_cast(float, (e + 120) << 23 | f << 20) : (float)f * 0x1p-9f;
-    if ((c & 127) == 127) a = __builtin_bit_cast(float, 0x7FC00000u);
-    return c & 128 ? -a : a;
-}
-// 2^(s - 127) as a factor: 2^-127 lies below fp32's normal numbers, 255 is NaN
-__device__ __forceinline__ float mx_factor(uint32_t s) {
-    return __builtin_bit_cast(float, s == 255u ? 0x7FC00000u : s ? s << 23 : 0x00400000u);
+// Eight codes' values under scale byte s; exact in fp32 (checked for every code and scale).
+template <bool F8> __device__ __forceinline__ void mx_decode(const u32x2 &c, uint32_t s, float (&v)[8]) {
+    const float unit = mx_unit(s);
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        f32x2 p;
+        if constexpr (F8) {
+            if (k & 1) p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[k >> 1], unit, true);
+            else p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[k >> 1], unit, false);
+        } else {
+            if (k == 0) p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[0], unit, 0);
+            else if (k == 1) p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[0], unit, 1);
+            else if (k == 2) p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[0], unit, 2);
+            else p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[0], unit, 3);
+        }
+        const float nan = __builtin_bit_cast(float, 0x7FC00000u);
+        v[2 * k] = s == 255u ? nan : p[0];
+        v[2 * k + 1] = s == 255u ? nan : p[1];
+    }
 }
 
-// Rows to codes.  rpw rows to a workgroup, eight values to a lane.  Bound by memory.
+// Rows to codes and back: a wavefront's lanes on neighbouring eights of values, MX_EACH
+// of them to a lane a workgroup's width apart, loaded before the first is used.  Bound by memory.
+constexpr int MX_EACH = 4;
 template <int T, bool F8> __global__ __launch_bounds__(256) void k_mx_quantize(const void *__restrict__ x, int64_t ldx,
                                                                                Fh3kMx y, int lanes) {
     const int64_t row = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
-    const int col = 8 * (blockIdx.y * lanes + threadIdx.x % lanes);
-    if (row >= y.rows || col >= y.in) return;  // whole quads: in is a multiple of 32
-    float v[8];
-    load8<T>(x, row * ldx + col, v);
-    mx_store<F8>(y, row, col, v);
+    const int col = 8 * (blockIdx.y * lanes * MX_EACH + threadIdx.x % lanes);
+    if (row >= y.rows) return;
+    float v[MX_EACH][8];
+#pragma unroll
+    for (int i = 0; i < MX_EACH; i++)
+        if (col + 8 * lanes * i < y.in) load8<T>(x, row * ldx + col + 8 * lanes * i, v[i]);
+#pragma unroll
+    for (int i = 0; i < MX_EACH; i++)   // whole quads: in is a multiple of 32
+        if (col + 8 * lanes * i < y.in) mx_store<F8>(y, row, col + 8 * lanes * i, v[i]);
 }
 
-template <int T> __global__ __launch_bounds__(256) void k_mx_dequant(Fh3kMx x, void *__restrict__ y, int64_t ldy, int lanes) {
+template <int T, bool F8> __global__ __launch_bounds__(256) void k_mx_dequant(Fh3kMx x, void *__restrict__ y, int64_t ldy, int lanes) {
     const int64_t row = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
-    const int col = 8 * (blockIdx.y * lanes + threadIdx.x % lanes);
-    if (row >= x.rows || col >= x.in) return;
-    const float f = mx_factor(x.scales[row * x.lds + col / MX_BLOCK]);
-    float v[8];
-    if (x.type == FH3K_MX_FP8) {
-        const u32x2 c = *(const u32x2 *)(x.codes + row * x.ld + col);
+    const int col = 8 * (blockIdx.y * lanes * MX_EACH + threadIdx.x % lanes);
+    if (row >= x.rows) return;
+    u32x2 c[MX_EACH];
+    uint32_t s[MX_EACH];
 #pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = fp8_value(c[k >> 2] >> (8 * (k & 3)) & 255) * f;
-    } else {
-        const uint32_t c = *(const uint32_t *)(x.codes + row * x.ld + col / 2);
-#pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = fp4_value(c >> (4 * k) & 15) * f;
+    for (int i = 0; i < MX_EACH; i++) {
+        const int n = col + 8 * lanes * i;
+        if (n >= x.in) continue;
+        s[i] = x.scales[row * x.lds + n / MX_BLOCK];
+        if constexpr (F8) c[i] = *(const u32x2 *)(x.codes + row * x.ld + n);
+        else c[i].x = *(const uint32_t *)(x.codes + row * x.ld + n / 2);
     }
-    store8<T>(y, row * ldy + col, v);
+#pragma unroll
+    for (int i = 0; i < MX_EACH; i++) {
+        const int n = col + 8 * lanes * i;
+        if (n >= x.in) continue;
+        float v[8];
+        mx_decode<F8>(c[i], s[i], v);
+        store8<T>(y, row * ldy + n, v);
+    }
 }
 
 // A 64-bit value cut to fp32, the last bit set where anything was cut off: rounding
@@ -1069,7 +1086,7 @@ template <class F> hipError_t by_type(int type, F f) {
 
 extern "C" hipError_t fh3k_mx_quantize(int type, const void *x, int64_t ldx, const Fh3kMx *y, hipStream_t st) {
     const int lanes = row_lanes(y->in), rpw = 256 / lanes;
-    const dim3 grid((unsigned)((y->rows + rpw - 1) / rpw), (unsigned)((y->in + 8 * lanes - 1) / (8 * lanes)));
+    const dim3 grid((unsigned)((y->rows + rpw - 1) / rpw), (unsigned)((y->in + 8 * MX_EACH * lanes - 1) / (8 * MX_EACH * lanes)));
     return by_type(type, [&](auto t) {
         if (y->type == FH3K_MX_FP8) k_mx_quantize<t(), true><<<grid, 256, 0, st>>>(x, ldx, *y, lanes);
         else k_mx_quantize<t(), false><<<grid, 256, 0, st>>>(x, ldx, *y, lanes);
@@ -1078,8 +1095,11 @@ extern "C" hipError_t fh3k_mx_quantize(int type, const void *x, int64_t ldx, con
 
 extern "C" hipError_t fh3k_mx_dequant(const Fh3kMx *x, int type, void *y, int64_t ldy, hipStream_t st) {
     const int lanes = row_lanes(x->in), rpw = 256 / lanes;
-    const dim3 grid((unsigned)((x->rows + rpw - 1) / rpw), (unsigned)((x->in + 8 * lanes - 1) / (8 * lanes)));
-    return by_type(type, [&](auto t) { k_mx_dequant<t()><<<grid, 256, 0, st>>>(*x, y, ldy, lanes); });
+    const dim3 grid((unsigned)((x->rows + rpw - 1) / rpw), (unsigned)((x->in + 8 * MX_EACH * lanes - 1) / (8 * MX_EACH * lanes)));
+    return by_type(type, [&](auto t) {
+        if (x->type == FH3K_MX_FP8) k_mx_dequant<t(), true><<<grid, 256, 0, st>>>(*x, y, ldy, lanes);
+        else k_mx_dequant<t(), false><<<grid, 256, 0, st>>>(*x, y, ldy, lanes);
+    });
 }
 
 extern "C" hipError_t fh3k_mx_norm(int type, const void *x, int64_t ldx, const void *add, int64_t lda, void *sum, int64_t lds,
