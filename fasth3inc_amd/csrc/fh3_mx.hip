@@ -196,7 +196,7 @@ __device__ __forceinline__ float cut(double d) {
 // finite size, and codes that are the formula's.  Bound by memory.
 // ---------------------------------------------------------------------------
 template <int T, bool F8, int C> __global__ __launch_bounds__(1024) void k_mx_norm(
-    const void *__restrict__ x, int64_t ldx, const void *add, int64_t lda, void *sum, int64_t lds,
+    const void *x, int64_t ldx, const void *add, int64_t lda, void *sum, int64_t lds,
     const float *__restrict__ w, float eps, const float *__restrict__ shift, const float *__restrict__ scale, Fh3kMx y) {
     __shared__ double part[16];
     const int64_t row = blockIdx.x;
