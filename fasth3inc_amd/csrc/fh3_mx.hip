@@ -142,9 +142,15 @@ template <bool F8> __device__ __forceinline__ void mx_decode(const u32x2 &c, uin
 // Rows to codes and back: a wavefront's lanes on neighbouring eights of values, MX_EACH
 // of them to a lane a workgroup's width apart, loaded before the first is used.  Bound by memory.
 constexpr int MX_EACH = 4;
+// Workgroups by rows: a launch's x has fewer than 2^32 lanes, so 2^21 workgroups there, the rest by z.
+constexpr int64_t MX_GRID = 1 << 21;
+__device__ __forceinline__ int64_t first_row() { return blockIdx.x + MX_GRID * blockIdx.z; }
+dim3 row_grid(int64_t groups, int64_t y) {
+    return dim3((unsigned)(groups < MX_GRID ? groups : MX_GRID), (unsigned)y, (unsigned)((groups + MX_GRID - 1) / MX_GRID));
+}
 template <int T, bool F8> __global__ __launch_bounds__(256) void k_mx_quantize(const void *__restrict__ x, int64_t ldx,
                                                                                Fh3kMx y, int lanes) {
-    const int64_t row = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+    const int64_t row = first_row() * (256 / lanes) + threadIdx.x / lanes;
     const int col = 8 * (blockIdx.y * lanes * MX_EACH + threadIdx.x % lanes);
     if (row >= y.rows) return;
     float v[MX_EACH][8];
@@ -157,7 +163,7 @@ template <int T, bool F8> __global__ __launch_bounds__(256) void k_mx_quantize(c
 }
 
 template <int T, bool F8> __global__ __launch_bounds__(256) void k_mx_dequant(Fh3kMx x, void *__restrict__ y, int64_t ldy, int lanes) {
-    const int64_t row = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+    const int64_t row = first_row() * (256 / lanes) + threadIdx.x / lanes;
     const int col = 8 * (blockIdx.y * lanes * MX_EACH + threadIdx.x % lanes);
     if (row >= x.rows) return;
     u32x2 c[MX_EACH];
@@ -199,7 +205,8 @@ template <int T, bool F8, int C> __global__ __launch_bounds__(1024) void k_mx_no
     const void *x, int64_t ldx, const void *add, int64_t lda, void *sum, int64_t lds,
     const float *__restrict__ w, float eps, const float *__restrict__ shift, const float *__restrict__ scale, Fh3kMx y) {
     __shared__ double part[16];
-    const int64_t row = blockIdx.x;
+    const int64_t row = first_row();
+    if (row >= y.rows) return;
     const int tid = threadIdx.x, nt = blockDim.x, n = (int)y.in;
     float v[C][8];
     double ss = 0;
@@ -374,14 +381,16 @@ template <class G> struct Load {
     template <int d, int to> __device__ __forceinline__ void codes(typename G::Buf &b, int st) const {
         if constexpr (d < to) {
             const int left = st < end ? blocks - st * G::NB : 0;
-            if constexpr (d < G::WI) w.template dma<d>(b.w, wave, st, left);
-            else x.template dma<d - G::WI>(b.x, wave, st, G::F8 ? 2 * left : left);
+            const int at = st < end ? st : 0;   // no offset past the rows, whose range it is subtracted from
+            if constexpr (d < G::WI) w.template dma<d>(b.w, wave, at, left);
+            else x.template dma<d - G::WI>(b.x, wave, at, G::F8 ? 2 * left : left);
             codes<d + 1, to>(b, st);
         }
     }
     __device__ __forceinline__ void scales(typename G::ScaleBuf &b, int st) const {
-        w.dma_scales(b.w, wave, st);
-        x.dma_scales(b.x, wave, st);
+        const int at = st < end ? st : 0;
+        w.dma_scales(b.w, wave, at);
+        x.dma_scales(b.x, wave, at);
     }
 };
 
@@ -1086,7 +1095,7 @@ template <class F> hipError_t by_type(int type, F f) {
 
 extern "C" hipError_t fh3k_mx_quantize(int type, const void *x, int64_t ldx, const Fh3kMx *y, hipStream_t st) {
     const int lanes = row_lanes(y->in), rpw = 256 / lanes;
-    const dim3 grid((unsigned)((y->rows + rpw - 1) / rpw), (unsigned)((y->in + 8 * MX_EACH * lanes - 1) / (8 * MX_EACH * lanes)));
+    const dim3 grid = row_grid((y->rows + rpw - 1) / rpw, (y->in + 8 * MX_EACH * lanes - 1) / (8 * MX_EACH * lanes));
     return by_type(type, [&](auto t) {
         if (y->type == FH3K_MX_FP8) k_mx_quantize<t(), true><<<grid, 256, 0, st>>>(x, ldx, *y, lanes);
         else k_mx_quantize<t(), false><<<grid, 256, 0, st>>>(x, ldx, *y, lanes);
@@ -1095,7 +1104,7 @@ extern "C" hipError_t fh3k_mx_quantize(int type, const void *x, int64_t ldx, con
 
 extern "C" hipError_t fh3k_mx_dequant(const Fh3kMx *x, int type, void *y, int64_t ldy, hipStream_t st) {
     const int lanes = row_lanes(x->in), rpw = 256 / lanes;
-    const dim3 grid((unsigned)((x->rows + rpw - 1) / rpw), (unsigned)((x->in + 8 * MX_EACH * lanes - 1) / (8 * MX_EACH * lanes)));
+    const dim3 grid = row_grid((x->rows + rpw - 1) / rpw, (x->in + 8 * MX_EACH * lanes - 1) / (8 * MX_EACH * lanes));
     return by_type(type, [&](auto t) {
         if (x->type == FH3K_MX_FP8) k_mx_dequant<t(), true><<<grid, 256, 0, st>>>(*x, y, ldy, lanes);
         else k_mx_dequant<t(), false><<<grid, 256, 0, st>>>(*x, y, ldy, lanes);
@@ -1111,7 +1120,7 @@ extern "C" hipError_t fh3k_mx_norm(int type, const void *x, int64_t ldx, const v
     const int c = (int)((y->in + 8 * nt - 1) / (8 * nt));
     return by_type(type, [&](auto t) {
         auto go = [&](auto f8, auto cc) {
-            k_mx_norm<t(), f8(), cc()><<<(unsigned)y->rows, nt, 0, st>>>(x, ldx, add, lda, sum, lds, w, eps, shift, scale, *y);
+            k_mx_norm<t(), f8(), cc()><<<row_grid(y->rows, 1), nt, 0, st>>>(x, ldx, add, lda, sum, lds, w, eps, shift, scale, *y);
         };
         auto pick = [&](auto f8) {
             if (c <= 1) go(f8, std::integral_constant<int, 1>{});

@@ -5,7 +5,7 @@ import threading
 import numpy as np
 import pytest
 
-from mx_ref import BF16, F16, F32, FP4, FP8, Mx, buf, from_type, quantize, random_rows, strides, to_type, unpack, values
+from mx_ref import BF16, F16, F32, FP4, FP8, HALF, Mx, buf, from_type, quantize, random_rows, scale_bytes, strides, to_type, unit, unpack, values
 from test_gpu_mx import Case, _check_quantized, _norm_exact, _product_bound, NORM_REL
 from test_gpu_seqs_calls import _streams
 
@@ -266,3 +266,155 @@ def test_the_same_bits_each_time(gpu, rows):
     for t in (F32, F16, BF16):
         y = c.run(gpu, t)
         assert all(np.array_equal(c.run(gpu, t), y) for _ in range(3))
+
+
+@pytest.mark.parametrize("call", ["quantize", "norm"])
+def test_more_rows_than_a_launch_dimension_has_lanes_for(gpu, call):
+    """Rows of bf16 values (64 GiB) with 1024 lanes to each row of the norm, 256 of the quantisation: 2^32 lanes and more."""
+    F, n, rows, last = gpu, 8192, (1 << 22) + 3, 5
+    if call == "quantize":
+        n, rows = 2048, (1 << 24)
+    x = to_type(np.random.default_rng(6).standard_normal((last, n)).astype(np.float32), BF16)
+    big = F.DeviceBuffer(rows * n * 2)
+    big.fill(0)
+    _tail(F, big, (rows - last) * n * 2, x)
+    lc, ls = strides(FP4, n)
+    dc, ds = F.DeviceBuffer(rows * lc), F.DeviceBuffer(rows * ls)
+    dc.fill(0xEE)
+    m = F.mx(FP4, rows, n, dc, ds)
+    if call == "norm":
+        F.mx_norm_dev(BF16, big, buf(F, np.ones(n, np.float32)), 1e-6, m)
+    else:
+        F.mx_quantize_dev(BF16, big, m)
+    F.synchronize()
+
+    def read(b, at, shape):
+        a = np.empty(shape, np.uint8)
+        assert F.lib().fh3_hip_memcpy_dtoh(a.ctypes.data, b.ptr + at, a.nbytes) == 0
+        return a
+
+    for r in (0, rows // 2, 1 << 21, rows - last - 1):
+        assert not read(dc, r * lc, (1, lc)).any()
+    got = unpack(read(dc, (rows - last) * lc, (last, lc)), FP4), read(ds, (rows - last) * ls, (last, ls))
+    if call == "norm":
+        _check_quantized(got, _norm_exact(from_type(x, BF16), np.ones(n), 1e-6), FP4, NORM_REL)
+    else:
+        want = quantize(from_type(x, BF16), FP4)
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+        big.fill(0x77)
+        F.mx_dequant_dev(m, BF16, big)
+        F.synchronize()
+        a = np.empty((last, n), np.uint16)
+        assert F.lib().fh3_hip_memcpy_dtoh(a.ctypes.data, big.ptr + (rows - last) * n * 2, a.nbytes) == 0
+        assert np.array_equal(a, to_type(values(*want, FP4).astype(np.float32), BF16))
+
+
+class Repeated:
+    """Many rows made of few: copy k of the base rows has 2^(k % 5) times their scales (weights: % 7), so that the
+    outputs of all follow from the products of the base rows."""
+
+    def __init__(self, seed, rows, n, out, fmt, base_x=90, base_w=130):
+        rng = np.random.default_rng(seed)
+        self.rows, self.n, self.out, self.fmt = rows, n, out, fmt
+        self.x, self.w = random_rows(rng, base_x, n, fmt, 0.3), random_rows(rng, base_w, n, FP4, 0.3)
+        self.ix, self.iw = np.arange(rows) % base_x, np.arange(out) % base_w
+        self.px, self.pw = np.arange(rows) // base_x % 5, np.arange(out) // base_w % 7
+
+    def arrays(self, F):
+        def of(part, i, p, fmt):
+            return Mx(F, fmt, len(i), self.n, part[0][i], (part[1][i] - 6 + p[:, None]).astype(np.uint8))
+        return of(self.x, self.ix, self.px, self.fmt), of(self.w, self.iw, self.pw, FP4)
+
+    def exact(self, t):
+        """The products and the bound on their sums."""
+        y = self.x[2] @ self.w[2].T * 2.0 ** -12
+        b, _ = _product_bound(self.x[2], self.w[2], t, self.fmt == FP8, y)
+        k = np.exp2(self.px[:, None] + self.pw[None])
+        at = np.ix_(self.ix, self.iw)
+        return y[at] * k, b[at] * k * 2.0 ** -12
+
+
+# many tiles, whole and in parts of the rows' length: the larger tiles
+LARGE = [(1930, 1824, 4401), (422, 16480, 5532)]
+
+
+@pytest.mark.parametrize("fmt", [FP8, FP4])
+@pytest.mark.parametrize("t,off,more,extra", [(F32, 0, 7, False), (BF16, 0, 7, True), (F16, 1, 4, True), (F32, 0, 3, True)])
+@pytest.mark.parametrize("rows,n,out", LARGE)
+def test_large_products(gpu, rows, n, out, t, off, more, extra, fmt):
+    F, c = gpu, Repeated(rows, rows, n, out, fmt)
+    x, w = c.arrays(F)
+    want, b = c.exact(t)
+    rng = np.random.default_rng(1)
+    kind, ld = to_type(np.zeros(1, np.float32), t).dtype, out + more
+    full = np.full(off + rows * ld, 77, kind)
+    kw = {}
+    size = np.abs(want)
+    if extra:
+        bias, gate = rng.standard_normal(out).astype(np.float32), rng.standard_normal((rows, out)).astype(np.float32)
+        res = to_type(4 * rng.standard_normal((rows, out)).astype(np.float32), t)
+        r = from_type(res, t).astype(np.float64)
+        want, b, size = r + gate * (want + bias), b * np.abs(gate), np.abs(r) + np.abs(gate) * (size + np.abs(bias))
+        kw = dict(d_bias=buf(F, bias), d_gate=buf(F, gate), d_res=buf(F, res))
+    y = buf(F, full)
+    need = F.mx_matmul_workspace_bytes(w.mx, x.mx)
+    assert (need > 0) == (rows == 422)
+    ws = F.DeviceBuffer(max(1, need))
+    ws.fill(0xFF)
+    F.mx_matmul_dev(w.mx, x.mx, t, y.ptr + off * kind.itemsize, ws, need, ldy=ld, **kw)
+    F.synchronize()
+    got = y.download(kind, full.shape)
+    rest = got[off:].reshape(rows, ld)
+    assert (got[:off] == 77).all() and (rest[:, out:] == 77).all()
+    bad = np.abs(from_type(rest[:, :out], t).astype(np.float64) - want) - (b + 2.0 ** -22 * size + HALF[t] * np.abs(want))
+    assert (bad <= 0).all(), (float(bad.max()), np.argwhere(~(bad <= 0))[:3])
+
+
+@pytest.mark.parametrize("fmt", [FP8, FP4])
+@pytest.mark.parametrize("to", [FP8, FP4])
+@pytest.mark.parametrize("rows,n,out", [(1930, 1824, 4480), (422, 16480, 5504)])
+def test_large_swiglu(gpu, rows, n, out, to, fmt):
+    F, c, f = gpu, Repeated(rows + 1, rows, n, out, fmt), out // 2
+    x, w = c.arrays(F)
+    y, b = c.exact(BF16)
+    o = Mx(F, to, rows, f)
+    need = F.mx_matmul_workspace_bytes(w.mx, x.mx, True)
+    assert (need > 0) == (rows == 422)
+    ws = F.DeviceBuffer(max(1, need))
+    ws.fill(0xFF)
+    F.mx_matmul_swiglu_dev(w.mx, x.mx, o.mx, ws, need)
+    F.synchronize()
+    codes, s = o.read()
+    val, gate = y[:, :f], y[:, f:]
+    with np.errstate(over="ignore"):
+        act = val * gate / (1 + np.exp(-gate))
+    # as in the small cases: through silu (slope at most 1.1) and val, and six roundings
+    b = b + 2.0 ** -23 * np.abs(y)
+    tol = np.abs(gate) * b[:, :f] + 1.1 * np.abs(val) * b[:, f:] + 1.1 * b[:, :f] * b[:, f:] + np.abs(act) * (8 + np.abs(gate)) * 2.0 ** -23
+    amax, blocks = np.abs(act).reshape(rows, -1, 32), tol.reshape(rows, -1, 32)
+    lo, hi = scale_bytes(np.maximum(amax - blocks, 0).max(-1), to), scale_bytes((amax + blocks).max(-1), to)
+    assert ((s >= lo) & (s <= hi)).all()
+    half = np.maximum(np.abs(act) * (2.0 ** -2 if to == FP4 else 2.0 ** -4), (0.25 if to == FP4 else 2.0 ** -10) * np.repeat(unit(s), 32, 1))
+    off = np.abs(values(codes, s, to) - act)
+    assert (off <= half + 1.25 * tol).all(), float((off - half - 1.25 * tol).max())
+
+
+@pytest.mark.parametrize("fmt", [FP8, FP4])
+def test_large_products_nan_rows(gpu, fmt):
+    F, c = gpu, Repeated(3, 1930, 1824, 4401, fmt)
+    x, w = c.arrays(F)
+    y = F.DeviceBuffer(1930 * 4401 * 4)
+
+    def run():
+        y.fill(0)
+        F.mx_matmul_dev(w.mx, x.mx, F32, y, None, 0)
+        F.synchronize()
+        return y.download(np.float32, (1930, 4401))
+
+    clean = run()
+    _tail(F, x.ds, 1000 * strides(fmt, 1824)[1] + 56, np.array([255], np.uint8))
+    _tail(F, w.ds, 4400 * strides(FP4, 1824)[1], np.array([255], np.uint8))
+    bad = run()
+    nan = np.zeros(clean.shape, bool)
+    nan[1000], nan[:, 4400] = True, True
+    assert np.array_equal(np.isnan(bad), nan) and np.array_equal(bad[~nan], clean[~nan])
