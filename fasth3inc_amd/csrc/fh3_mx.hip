@@ -817,6 +817,19 @@ template <class G, bool SPLIT> __global__ __launch_bounds__(64 * G::WAVES, 8 / G
     else mx_rows_out<FH3K_BF16>(o, acc, stg, lane, t0, x.rows, n0, w.rows, vec);
 }
 
+// Eight sums' parts, n values apart, added in their order; four are loaded at once, since one by one each
+// waited for its own.
+__device__ __forceinline__ void mx_add_parts(const float *part, int S, int64_t n, int64_t at, float (&v)[8]) {
+    for (int s = 0; s < S; s += 4) {
+        float a[4][8];
+#pragma unroll
+        for (int i = 0; i < 4; i++) load8<FH3K_F32>(part, min(s + i, S - 1) * n + at, a[i]);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = s + i < S ? v[k] + a[i][k] : v[k];
+    }
+}
 // The parts of a split product, added in their order, to rows of the output: eight values to a thread.
 template <int T> __global__ __launch_bounds__(256) void k_mx_join(const float *__restrict__ part, int S, int64_t ldp, int64_t rows, int64_t cols,
                                                                   Fh3kMxOut o, bool vec) {
@@ -824,12 +837,7 @@ template <int T> __global__ __launch_bounds__(256) void k_mx_join(const float *_
     const int n = 8 * (blockIdx.y * 256 + threadIdx.x);
     if (n >= cols) return;
     float v[8] = {};
-    for (int s = 0; s < S; s++) {
-        float a[8];
-        load8<FH3K_F32>(part, (s * rows + t) * ldp + n, a);
-#pragma unroll
-        for (int k = 0; k < 8; k++) v[k] += a[k];
-    }
+    mx_add_parts(part, S, rows * ldp, t * ldp + n, v);
     if (vec && n + 8 <= cols) {
         Beside b;
         if (o.res) {
@@ -851,16 +859,8 @@ template <bool F8> __global__ __launch_bounds__(256) void k_mx_join_swiglu(const
     const int col = 8 * (blockIdx.y * 256 + threadIdx.x);
     if (col >= f) return;
     float v[8] = {}, q[8] = {}, a[8];
-    for (int s = 0; s < S; s++) {
-        float c[8], d[8];
-        load8<FH3K_F32>(part, (s * rows + t) * ldp + col, c);
-        load8<FH3K_F32>(part, (s * rows + t) * ldp + f + col, d);
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-            v[k] += c[k];
-            q[k] += d[k];
-        }
-    }
+    mx_add_parts(part, S, rows * ldp, t * ldp + col, v);
+    mx_add_parts(part, S, rows * ldp, t * ldp + f + col, q);
 #pragma unroll
     for (int k = 0; k < 8; k++) a[k] = (v[k] + (o.bias ? o.bias[col + k] : 0.f)) * silu(q[k] + (o.bias ? o.bias[f + col + k] : 0.f));
     mx_store<F8>(o.y, t, col, a);
@@ -975,6 +975,50 @@ template <bool F8, int TT, int R> struct Window {
     }
 };
 
+// Both 16 x 16 tiles of a block of 32 outputs, values and gates: lane (t, g) has the block's outputs 4 g .. and 16 + 4 g .. of token t.
+__device__ __forceinline__ void mx_swiglu16(const Fh3kMxOut &o, const f32x4 &v0, const f32x4 &q0, const f32x4 &v1, const f32x4 &q1, int64_t t,
+                                            int64_t rows, int64_t n0, int g) {
+    const int64_t f = o.y.in;
+    float a[8];
+    uint32_t u = 0;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const int64_t n = n0 + 16 * (k >> 2) + 4 * g + (k & 3);
+        const float v = k < 4 ? v0[k & 3] : v1[k & 3], q = k < 4 ? q0[k & 3] : q1[k & 3];
+        a[k] = (v + (o.bias ? o.bias[n] : 0.f)) * silu(q + (o.bias ? o.bias[f + n] : 0.f));
+        const float c = a[k];
+        const uint32_t b = __builtin_bit_cast(uint32_t, c) & 0x7FFFFFFFu;
+        u = u > b ? u : b;
+    }
+    u = max(u, (uint32_t)__shfl_xor((int)u, 16));
+    u = max(u, (uint32_t)__shfl_xor((int)u, 32));
+    const bool to8 = o.y.type == FH3K_MX_FP8;
+    const uint32_t s = to8 ? mx_scale<true>(u) : mx_scale<false>(u);
+    if (t >= rows) return;
+    if (to8) {
+        const u32x2 c = mx_encode<true>(a, s);
+        uint8_t *p = o.y.codes + t * o.y.ld + n0 + 4 * g;
+        *(uint32_t *)p = c.x;
+        *(uint32_t *)(p + 16) = c.y;
+    } else {
+        const uint32_t c = mx_encode<false>(a, s).x;
+        uint8_t *p = o.y.codes + t * o.y.ld + n0 / 2 + 2 * g;
+        *(uint16_t *)p = (uint16_t)c;
+        *(uint16_t *)(p + 8) = (uint16_t)(c >> 16);
+    }
+    if (g == 0) o.y.scales[t * o.y.lds + n0 / MX_BLOCK] = (uint8_t)s;
+}
+// Four outputs n .. n + 3 of token t, those of them that are there.
+__device__ __forceinline__ void mx_put4(const Fh3kMxOut &o, int64_t t, int64_t n, int64_t cols, const f32x4 &v) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        if (n + e >= cols) continue;
+        if (o.type == FH3K_F32) mx_put1<FH3K_F32>(o, t, (int)n + e, cols, v[e]);
+        else if (o.type == FH3K_F16) mx_put1<FH3K_F16>(o, t, (int)n + e, cols, v[e]);
+        else mx_put1<FH3K_BF16>(o, t, (int)n + e, cols, v[e]);
+    }
+}
+
 template <bool F8, bool SPLIT, int TT, int R, bool AHEAD> __global__ __launch_bounds__(64 * (AHEAD || TT == 4 || R * TT == 8 ? MX_WAVES_AHEAD : MX_WAVES)) void k_mx_few(Fh3kMx w, Fh3kMx x, Fh3kMxOut o) {
     extern __shared__ f32x4 parts[];         // [wavefront][R][TT][64]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
@@ -1020,42 +1064,7 @@ template <bool F8, bool SPLIT, int TT, int R, bool AHEAD> __global__ __launch_bo
     };
     if (swiglu) {
         if constexpr (R == 4) {
-            // both tiles of a block of 32 outputs: lane (t, g) has its outputs 4 g .. and 16 + 4 g .. of token t
-            for (int j = wave; j < TT; j += waves) {
-                const int64_t t = 16 * j + r;
-                float a[2][4];
-                uint32_t u = 0;
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const f32x4 v = sum(i, j), q = sum(2 + i, j);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int64_t n = n0 + 16 * i + 4 * g + e;
-                        a[i][e] = (v[e] + (o.bias ? o.bias[n] : 0.f)) * silu(q[e] + (o.bias ? o.bias[f + n] : 0.f));
-                        const float c = a[i][e];
-                        const uint32_t b = __builtin_bit_cast(uint32_t, c) & 0x7FFFFFFFu;
-                        u = u > b ? u : b;
-                    }
-                }
-                u = max(u, (uint32_t)__shfl_xor((int)u, 16));
-                u = max(u, (uint32_t)__shfl_xor((int)u, 32));
-                const bool to8 = o.y.type == FH3K_MX_FP8;
-                const uint32_t s = to8 ? mx_scale<true>(u) : mx_scale<false>(u);
-                float v[8] = {a[0][0], a[0][1], a[0][2], a[0][3], a[1][0], a[1][1], a[1][2], a[1][3]};
-                if (t >= x.rows) continue;
-                if (to8) {
-                    const u32x2 c = mx_encode<true>(v, s);
-                    uint8_t *p = o.y.codes + t * o.y.ld + n0 + 4 * g;
-                    *(uint32_t *)p = c.x;
-                    *(uint32_t *)(p + 16) = c.y;
-                } else {
-                    const uint32_t c = mx_encode<false>(v, s).x;
-                    uint8_t *p = o.y.codes + t * o.y.ld + n0 / 2 + 2 * g;
-                    *(uint16_t *)p = (uint16_t)c;
-                    *(uint16_t *)(p + 8) = (uint16_t)(c >> 16);
-                }
-                if (g == 0) o.y.scales[t * o.y.lds + n0 / MX_BLOCK] = (uint8_t)s;
-            }
+            for (int j = wave; j < TT; j += waves) mx_swiglu16(o, sum(0, j), sum(2, j), sum(1, j), sum(3, j), 16 * j + r, x.rows, n0, g);
         }
         return;
     }
@@ -1063,14 +1072,185 @@ template <bool F8, bool SPLIT, int TT, int R, bool AHEAD> __global__ __launch_bo
         const int i = tile / TT, j = tile % TT;
         const int64_t t = 16 * j + r;
         const f32x4 v = sum(i, j);
-        if (t >= x.rows) continue;
+        if (t < x.rows) mx_put4(o, t, n0 + 16 * i + 4 * g, w.rows, v);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Up to 64 rows (16 TT) against many weight rows: as k_mx_few, but a workgroup, one to a
+// CU, keeps its part of the rows' length of x in registers (each wavefront NS steps of
+// 128 values) and takes tile after tile of 16 weight rows, straight from memory, two of
+// them while the next two are on their way; the wavefronts' sums meet in LDS four tiles at a time.
+// k_mx_few reads all of x for each 16 R weight rows: 20 rows x 5120 -> 51200 SwiGLU, 139 MB
+// of weights, took it 57 us, the tiles 43, this 32 (27.5 with one row: 5.1 TB/s).
+// Where x is longer than 40 steps (24), each part of it has its own workgroups, and the
+// parts' sums are joined: 16 rows x 25600 -> 5120 29 us, tiles 24, this 19.
+// Two tiles to each splitting of FP8 codes (fp32 outputs): with one, that took longer than the loads.
+// Nothing that is known before the loop is kept over it (the asm statements): the
+// registers are full of loads, and a reload from scratch waits for all loads before it.
+// ---------------------------------------------------------------------------
+// byte xb of xs; a constant once unrolled
+__device__ __forceinline__ f32x4 mx_mfma16(const u32x4 &w, const i32x8 &x, f32x4 acc, int ws, int xs, int xb, bool f8) {
+    const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+#define MX_M16(B) (f8 ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, x, acc, 4, 0, 0, ws, B, xs) : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, x, acc, 4, 4, 0, ws, B, xs))
+    switch (xb) {
+        case 0: return MX_M16(0);
+        case 1: return MX_M16(1);
+        case 2: return MX_M16(2);
+        default: return MX_M16(3);
+    }
+}
+constexpr int MX_STREAM = 8;    // wavefronts of a workgroup
+// NS steps' scales of a row, one dword each
+template <int NS> __device__ __forceinline__ void mx_step_scales(uint32_t (&s)[NS], __amdgpu_buffer_rsrc_t r, uint32_t off) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int64_t n = n0 + 16 * i + 4 * g + e;
-            if (n >= w.rows) continue;
-            if (o.type == FH3K_F32) mx_put1<FH3K_F32>(o, t, (int)n, w.rows, v[e]);
-            else if (o.type == FH3K_F16) mx_put1<FH3K_F16>(o, t, (int)n, w.rows, v[e]);
-            else mx_put1<FH3K_BF16>(o, t, (int)n, w.rows, v[e]);
+    for (int i = 0; i + 4 <= NS; i += 4) {
+        const u32x4 v = mx_load16(r, off + 4 * i);
+#pragma unroll
+        for (int k = 0; k < 4; k++) s[i + k] = v[k];
+    }
+#pragma unroll
+    for (int i = NS & ~3; i < NS; i++) s[i] = __builtin_amdgcn_raw_buffer_load_b32(r, (int)(off + 4 * i), 0, 0);
+}
+template <int NS> struct Streamed {
+    u32x4 w[NS];
+    uint32_t s[NS];
+    // rows n0 .. of w (rows: how many are there), for this wavefront's steps from `first` on, n of them
+    __device__ __forceinline__ void load(const Fh3kMx &m, int64_t n0, bool any, int r, int g, int first, int blocks) {
+        if (n0 >= m.rows) n0 = m.rows - 1;
+        const int last = m.rows - n0 < 16 ? (int)(m.rows - n0) - 1 : 15;
+        const __amdgpu_buffer_rsrc_t code = mx_buffer(m.codes + n0 * m.ld, any ? (uint32_t)(last * m.ld + m.in / 2) : 0u);
+        const __amdgpu_buffer_rsrc_t scale = mx_buffer(m.scales + n0 * m.lds, any ? (uint32_t)(last * m.lds + (m.in / MX_BLOCK + 3) / 4 * 4) : 0u);
+        r = r < last ? r : last;
+        const uint32_t off = (uint32_t)(r * m.ld) + first * 64 + g * 16;
+        mx_step_scales<NS>(s, scale, (uint32_t)(r * m.lds) + first * 4);
+#pragma unroll
+        for (int i = 0; i < NS; i++) w[i] = mx_load16(code, 4 * i + g < blocks ? off + i * 64 : MX_OUTSIDE);
+    }
+};
+
+template <bool F8, bool SPLIT, int TT, int NS> __global__ __launch_bounds__(64 * MX_STREAM, 2) void k_mx_stream(
+    Fh3kMx w, Fh3kMx x, Fh3kMxOut o, float *part, int64_t ldp, int units, int per) {
+    __shared__ f32x4 sums[4][TT][MX_STREAM][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    const bool swiglu = o.y.codes != nullptr && !part;
+    const int64_t f = w.rows >> 1;
+    const int G = gridDim.x;
+    // this wavefront's steps
+    const int steps = (int)((w.in + 127) / 128), end = min((int)(blockIdx.y + 1) * per, steps);
+    const int share = (per + MX_STREAM - 1) / MX_STREAM, first = blockIdx.y * per + wave * share;
+    int blocks = min(min(first + share, end) * 4, (int)(w.in / MX_BLOCK)) - first * 4;   // of it, 0 or less: none
+    const int count = swiglu ? (units - (int)blockIdx.x + G - 1) / G * 4 : (units - (int)blockIdx.x + G - 1) / G;
+    auto row = [&](int k, int q) -> int64_t {
+        if (swiglu) return ((q & 1) ? f : 0) + (int64_t)(blockIdx.x + (k >> 2) * G) * 32 + (q >> 1) * 16;
+        return (int64_t)(blockIdx.x + (k + q) * G) * 16;
+    };
+    u32x4 xc[TT][NS][F8 ? 2 : 1];
+    uint32_t xs[TT][(NS + 3) / 4] = {}, xd[TT][NS];
+#pragma unroll
+    for (int j = 0; j < TT; j++) {
+        Few fx;
+        fx.init(x, 16 * j, r);
+        mx_step_scales<NS>(xd[j], fx.scale, fx.soff + first * 4);
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+            if constexpr (F8) {
+                const int b = 4 * i + (g >> 1);
+                const uint32_t off = fx.off + (first + i) * 128 + g * 16;
+                xc[j][i][0] = mx_load16(fx.code, b < blocks ? off : MX_OUTSIDE);
+                xc[j][i][1] = mx_load16(fx.code, b + 2 < blocks ? off + 64 : MX_OUTSIDE);
+            } else {
+                xc[j][i][0] = mx_load16(fx.code, 4 * i + g < blocks ? fx.off + (first + i) * 64 + g * 16 : MX_OUTSIDE);
+            }
+        }
+    }
+    // two tiles at a time, the next two on their way
+    Streamed<NS> v[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) v[0][i].load(w, row(0, i), i < count, r, g, first, blocks);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < TT; j++)
+#pragma unroll
+        for (int i = 0; i < NS; i++) xs[j][i >> 2] |= (4 * i + g < blocks ? xd[j][i] >> (8 * g) & 0xFFu : 0u) << (8 * (i & 3));
+    for (int k = 0; k < count; k += 4) {
+#pragma unroll
+        for (int d = 0; d < 2; d++) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int a = 2 * d + 2 + i;
+                v[1 - d][i].load(w, row(k + (a & ~3), a & 3), k + a < count, r, g, first, blocks);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            f32x4 acc[2][TT] = {};
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                int sw[2];
+#pragma unroll
+                for (int i = 0; i < 2; i++) sw[i] = 4 * s + g < blocks ? (int)(v[d][i].s[s] >> (8 * g)) : 0;
+#pragma unroll
+                for (int j = 0; j < TT; j++) {
+                    i32x8 c = {}, h;
+                    // split here each time: kept, the halves take twice the registers (one tile of rows: there is room for them)
+                    if constexpr (SPLIT && TT > 1) asm volatile("" : "+v"(xc[j][s][0]), "+v"(xc[j][s][1]));
+                    set4(c, 0, xc[j][s][0]);
+                    if constexpr (F8) set4(c, 4, xc[j][s][1]);
+                    if constexpr (SPLIT) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            h[e] = (int)fp8_large((uint32_t)c[e]);
+                            c[e] ^= h[e];
+                        }
+#pragma unroll
+                        for (int i = 0; i < 2; i++) acc[i][j] = mx_mfma16(v[d][i].w[s], h, acc[i][j], sw[i], (int)xs[j][s >> 2], s & 3, true);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; i++) acc[i][j] = mx_mfma16(v[d][i].w[s], c, acc[i][j], sw[i], (int)xs[j][s >> 2], s & 3, F8);
+                }
+            }
+            // the sums of the last trip are read
+            if (d == 0) asm volatile("s_barrier" : : : "memory");
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < TT; j++) sums[2 * d + i][j][wave][lane] = acc[i][j];
+            asm volatile("" : : : "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
+        int to = lane;
+        asm volatile("" : "+v"(to));   // addresses made from it are not kept over the loads
+        auto sum = [&](int d, int j) {
+            f32x4 v = sums[d][j][0][to];
+#pragma unroll
+            for (int i = 1; i < MX_STREAM; i++) {
+                const f32x4 a = sums[d][j][i][to];
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] += a[e];
+                if (i & 1) asm volatile("" : "+v"(v) : : "memory");   // the registers are full of loads
+            }
+            return v;
+        };
+        if (swiglu) {
+            if (wave < TT) {
+                const f32x4 v0 = sum(0, wave), q0 = sum(1, wave), v1 = sum(2, wave), q1 = sum(3, wave);
+                mx_swiglu16(o, v0, q0, v1, q1, 16 * wave + (to & 15), x.rows, row(k, 0), to >> 4);
+            }
+        } else {
+#pragma unroll 1
+            for (int i = wave; i < 4 * TT; i += MX_STREAM) {
+                const int d = i / TT, j = i % TT;
+                if (k + d >= count) break;
+                const f32x4 v = sum(d, j);
+                const int64_t t = 16 * j + (to & 15), n = row(k, d) + 4 * (to >> 4);
+                if (t >= x.rows) continue;
+                if (part) {
+                    if (n < ldp) *(f32x4 *)(part + (blockIdx.y * x.rows + t) * ldp + n) = v;
+                } else {
+                    mx_put4(o, t, n, w.rows, v);
+                }
+            }
         }
     }
 }
@@ -1136,8 +1316,8 @@ namespace {
 
 // How a product is cut: tiles, and parts of the rows' length.
 struct Plan {
-    bool few;                     // k_mx_few
-    int bw, bx, parts, per;       // per: stages of a part
+    enum { FEW, STREAM, TILES } kernel;
+    int bw, bx, parts, per;       // per: stages (STREAM: steps) of a part
     int64_t m_tiles, n_tiles, ldp;
 };
 // Tiles of 16 weight rows to a workgroup of k_mx_few: the most that leave 150
@@ -1147,25 +1327,52 @@ int few_tiles(const Fh3kMx *w, const Fh3kMx *x, bool swiglu) {
     return swiglu || (n16 >= 600 && x->rows <= 16) ? 4 : n16 >= 300 ? 2 : 1;
 }
 
-Plan plan_of(const Fh3kMx *w, const Fh3kMx *x, bool swiglu) {
-    Plan p = {};
-    // k_mx_few where what its workgroups read of x stays below 3 * 2^24 values; FP8 rows
-    // to bf16, us, it and the tiles: 4096 -> 4096, 64 rows (2^26) 13.7, 15.4; 5120 -> 5120, 64 rows (50 M) 16.8, 15.8;
-    // 5120 -> 15360, 17 rows (42 M) 18.6, 21.9, 32 rows (79 M) 22.4, 21.9; 8192 -> 5120, 33 rows (43 M) 21.0, 18.2;
-    // 5120 -> 51200 SwiGLU, 16 rows (66 M) 42, 47, 32 rows 57, 47
+// Each kernel's time in us by what was measured (weights from memory), of which the least is taken.
+// FP8 rows to bf16, k_mx_few, k_mx_stream and the tiles:
+//    rows of 5120 -> 5120:  1 row 6.5, 8.1, 18;    32 rows 10.7, 12.6, 19
+//    5120 -> 15360:         1 row 12.9, 11.4, 18;  17 rows 18.5, 14.2, 19; 64 rows -, 22.1, 21.3
+//    25600 -> 5120:         1 row 20.7, 20.0, 27;  16 rows 29, 21.7, 27
+//    5120 -> 51200 SwiGLU:  1 row 35.7, 28.2, 45;  32 rows 57, 33.8, 45.5
+double few_us(const Fh3kMx *w, const Fh3kMx *x, bool swiglu, bool split) {
     const int64_t rows = 16 * few_tiles(w, x, swiglu), groups = (w->rows + rows - 1) / rows;
-    if (x->rows <= 64 && groups * x->rows * w->in <= 3 << 24) {
-        p.few = true;
-        p.parts = 1;
-        return p;
-    }
-    // Otherwise the tile size and the number of parts with the least time by what was
-    // measured: us for a stage on a CU that has one workgroup of 128 x 128, two, or one of 256 x 256, and for a round's
-    // beginning and end; parts are written and read at 4 MB a us and joined by a launch of 3.5 us.
+    const double row = (double)w->in * (x->type == FH3K_MX_FP8 ? 1.0 : 0.5), each = (double)rows * w->in / 2 + x->rows * row;
+    // a workgroup's bytes through one CU, or all weights from memory and the rows for each workgroup from L2
+    const double one = each / (x->rows <= 16 ? 38e3 : x->rows <= 32 ? 36e3 : 26e3);
+    const double all = (double)w->rows * w->in * 0.53 / (4.4e6 * (groups < 200 ? groups / 200.0 : 1.0)) + groups * x->rows * row / 12e6;
+    return 3.9 + (one > all ? one : all) * (!split ? 1 : x->rows <= 16 ? 1.1 : x->rows <= 32 ? 1.35 : 1.8);
+}
+// Steps of 128 values that a wavefront of k_mx_stream holds of x: what fits its registers
+int stream_steps(const Fh3kMx *x) {
+    const int steps = (int)((x->in + 127) / 128);
+    return x->rows <= 32 || (x->type == FH3K_MX_FP4 && steps <= 5 * MX_STREAM) ? 5 : 3;
+}
+double stream_us(const Fh3kMx *w, const Fh3kMx *x, bool swiglu, bool split, Plan &p) {
+    const int steps = (int)((w->in + 127) / 128), most = MX_STREAM * stream_steps(x);
+    p.kernel = Plan::STREAM;
+    p.per = (steps + (steps + most - 1) / most - 1) / ((steps + most - 1) / most);
+    p.parts = (steps + p.per - 1) / p.per;
+    // a workgroup to a CU; tiles of 16 rows, or blocks of 32 outputs
+    const bool blocks = swiglu && p.parts == 1;
+    p.n_tiles = blocks ? w->rows / 64 : (w->rows + 15) / 16;
+    p.m_tiles = p.parts < 256 ? 256 / p.parts : 1;
+    if (p.m_tiles > p.n_tiles) p.m_tiles = p.n_tiles;
+    p.ldp = (w->rows + 7) / 8 * 8;
+    const int tt = x->rows <= 16 ? 1 : x->rows <= 32 ? 2 : 4;
+    const double each = (double)((p.n_tiles + p.m_tiles - 1) / p.m_tiles) * (blocks ? 4 : 1) * p.per;
+    const double held = (double)x->rows * p.per * (x->type == FH3K_MX_FP8 ? 128 : 64);
+    double t = 5 + each * 0.038 + held / 45e3 + (tt == 4 ? 1.5 : 0);
+    if (split && tt > 1) t += tt * (1 + each * 0.01);
+    if (p.parts > 1) t += 2.5 + (double)p.parts * x->rows * w->rows * 8 / 4e6;
+    return t;
+}
+// Tiles: for a stage on a CU that has one workgroup of 128 x 128, two, or one of 256 x 256, and for a round's
+// beginning and end; parts are written and read at 4 MB a us and joined by a launch of 3.5 us.
+double tiles_us(const Fh3kMx *w, const Fh3kMx *x, bool split, Plan &p) {
     const bool f8 = x->type == FH3K_MX_FP8;
     const int ks = f8 ? 128 : 256, stages = (int)((w->in + ks - 1) / ks);
-    const double one = f8 ? 0.65 : 1.05, two = f8 ? 1.0 : 1.42, big = f8 ? 1.45 : 2.1;
+    const double more = split ? 1.4 : 1, one = f8 ? 0.65 * more : 1.05, two = f8 ? 1.0 * more : 1.42, big = f8 ? 1.45 * more : 2.1;
     double least = 0;
+    p.kernel = Plan::TILES;
     for (int b = 128; b <= 256; b += 128) {
         const int64_t m = (x->rows + b - 1) / b, n = (w->rows + b - 1) / b;
         for (int parts = 1; parts <= 32 && (parts == 1 || parts * 4 <= stages); parts++) {
@@ -1186,7 +1393,21 @@ Plan plan_of(const Fh3kMx *w, const Fh3kMx *x, bool swiglu) {
         }
     }
     p.ldp = (w->rows + 7) / 8 * 8;
-    return p;
+    return least;
+}
+// split: FP8 rows to fp32, in two products
+Plan plan_of(const Fh3kMx *w, const Fh3kMx *x, bool swiglu, bool split) {
+    Plan tiles = {}, stream = {};
+    const double t = tiles_us(w, x, split, tiles);
+    if (x->rows > 64) return tiles;
+    const double s = stream_us(w, x, swiglu, split, stream), f = few_us(w, x, swiglu, split);
+    if (f <= s && f <= t) {
+        Plan few = {};
+        few.kernel = Plan::FEW;
+        few.parts = 1;
+        return few;
+    }
+    return s <= t ? stream : tiles;
 }
 
 template <class G, bool SPLIT = false> void launch_gemm(const Fh3kMx *w, const Fh3kMx *x, const Fh3kMxOut *o, const Plan &p, float *part, bool vec,
@@ -1219,51 +1440,70 @@ bool sixteens(const void *p, int64_t ld, int size) { return !p || ((uintptr_t)p 
 }  // namespace
 
 extern "C" int fh3k_mx_matmul_fits(const Fh3kMx *w, const Fh3kMx *x) {
-    const Plan p = plan_of(w, x, false);
-    return p.m_tiles * p.n_tiles < ((int64_t)1 << 23) && p.ldp * x->rows <= ((int64_t)1 << 40);
+    const Plan p = plan_of(w, x, false, false);
+    return (p.kernel != Plan::TILES || p.m_tiles * p.n_tiles < ((int64_t)1 << 23)) && p.ldp * x->rows <= ((int64_t)1 << 40);
 }
 
 extern "C" size_t fh3k_mx_matmul_ws_bytes(const Fh3kMx *w, const Fh3kMx *x, int swiglu) {
-    const Plan p = plan_of(w, x, swiglu);
-    return p.parts > 1 ? (size_t)p.parts * p.ldp * x->rows * sizeof(float) : 0;
+    // the output's type is not known here: for either
+    size_t most = 0;
+    for (int split = 0; split < (x->type == FH3K_MX_FP8 && !swiglu ? 2 : 1); split++) {
+        const Plan p = plan_of(w, x, swiglu, split);
+        const size_t n = p.parts > 1 ? (size_t)p.parts * p.ldp * x->rows * sizeof(float) : 0;
+        most = n > most ? n : most;
+    }
+    return most;
 }
 
 extern "C" hipError_t fh3k_mx_matmul(const Fh3kMx *w, const Fh3kMx *x, const Fh3kMxOut *o, void *ws, hipStream_t st) {
-    const Plan p = plan_of(w, x, o->y.codes);
+    const bool f8 = x->type == FH3K_MX_FP8, split = f8 && o->type == FH3K_F32 && !o->y.codes;
+    const Plan p = plan_of(w, x, o->y.codes, split);
     float *part = p.parts > 1 ? (float *)ws : nullptr;
     const int size = o->type == FH3K_F32 ? 4 : 2;
     const bool vec = sixteens(o->out, o->ldo, size) && sixteens(o->res, o->ldres, size) && sixteens(o->gate, w->rows, 4);
-    const bool f8 = x->type == FH3K_MX_FP8, split = f8 && o->type == FH3K_F32 && !o->y.codes;
-    if (p.few) {
-        auto go = [&](auto f, auto sp, auto tt) {
-            const int r = few_tiles(w, x, o->y.codes);
-            if (r == 4) launch_few<f(), sp(), tt(), 4>(w, x, o, st);
-            else if (r == 2) launch_few<f(), sp(), tt(), 2>(w, x, o, st);
-            else launch_few<f(), sp(), tt(), 1>(w, x, o, st);
-        };
-        auto by_rows = [&](auto f, auto sp) {
-            if (x->rows <= 16) go(f, sp, std::integral_constant<int, 1>{});
-            else if (x->rows <= 32) go(f, sp, std::integral_constant<int, 2>{});
-            else go(f, sp, std::integral_constant<int, 4>{});
-        };
-        if (!f8) by_rows(std::false_type{}, std::false_type{});
-        else if (!split) by_rows(std::true_type{}, std::false_type{});
-        else by_rows(std::true_type{}, std::true_type{});
-        return hipGetLastError();
-    }
+    using N1 = std::integral_constant<int, 1>;
+    using N2 = std::integral_constant<int, 2>;
+    using N3 = std::integral_constant<int, 3>;
+    using N4 = std::integral_constant<int, 4>;
+    using N5 = std::integral_constant<int, 5>;
     using Big4 = Gemm<4, 2, 2, 4, false, 256, 2>;
     using Big8 = Gemm<4, 2, 2, 4, true, 128, 3>;
     using Small4 = Gemm<2, 2, 2, 2, false, 256, 2>;
     using Small8 = Gemm<2, 2, 2, 2, true, 128, 3>;
-    if (p.bw == 256) {
-        if (!f8) launch_gemm<Big4>(w, x, o, p, part, vec, st);
-        else if (!split) launch_gemm<Big8>(w, x, o, p, part, vec, st);
-        else launch_gemm<Big8, true>(w, x, o, p, part, vec, st);
-    } else {
-        if (!f8) launch_gemm<Small4>(w, x, o, p, part, vec, st);
-        else if (!split) launch_gemm<Small8>(w, x, o, p, part, vec, st);
-        else launch_gemm<Small8, true>(w, x, o, p, part, vec, st);
-    }
+    auto few = [&](auto f, auto sp) {
+        const int r = few_tiles(w, x, o->y.codes);
+        auto go = [&](auto tt) {
+            if (r == 4) launch_few<f(), sp(), tt(), 4>(w, x, o, st);
+            else if (r == 2) launch_few<f(), sp(), tt(), 2>(w, x, o, st);
+            else launch_few<f(), sp(), tt(), 1>(w, x, o, st);
+        };
+        if (x->rows <= 16) go(N1{});
+        else if (x->rows <= 32) go(N2{});
+        else go(N4{});
+    };
+    auto stream = [&](auto f, auto sp) {
+        auto go = [&](auto tt, auto ns) {
+            const dim3 grid((unsigned)p.m_tiles, (unsigned)p.parts);
+            k_mx_stream<f(), sp(), tt(), ns()><<<grid, 64 * MX_STREAM, 0, st>>>(*w, *x, *o, part, p.ldp, (int)p.n_tiles, p.per);
+        };
+        if (x->rows <= 16) go(N1{}, N5{});
+        else if (x->rows <= 32) go(N2{}, N5{});
+        else if (stream_steps(x) == 3) go(N4{}, N3{});
+        else if constexpr (!f()) go(N4{}, N5{});
+    };
+    auto by_rows = [&](auto go) {
+        if (!f8) go(std::false_type{}, std::false_type{});
+        else if (!split) go(std::true_type{}, std::false_type{});
+        else go(std::true_type{}, std::true_type{});
+    };
+    if (p.kernel == Plan::FEW) by_rows(few);
+    else if (p.kernel == Plan::STREAM) by_rows(stream);
+    else if (p.bw == 256 && !f8) launch_gemm<Big4>(w, x, o, p, part, vec, st);
+    else if (p.bw == 256 && !split) launch_gemm<Big8>(w, x, o, p, part, vec, st);
+    else if (p.bw == 256) launch_gemm<Big8, true>(w, x, o, p, part, vec, st);
+    else if (!f8) launch_gemm<Small4>(w, x, o, p, part, vec, st);
+    else if (!split) launch_gemm<Small8>(w, x, o, p, part, vec, st);
+    else launch_gemm<Small8, true>(w, x, o, p, part, vec, st);
     if (!part) return hipGetLastError();
     if (o->y.codes) {
         const dim3 grid((unsigned)x->rows, (unsigned)((o->y.in + 2047) / 2048));

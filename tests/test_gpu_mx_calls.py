@@ -334,6 +334,73 @@ class Repeated:
         return y[at] * k, b[at] * k * 2.0 ** -12
 
 
+def _scaled_back(c, rows):
+    """Case-like rows of c for the bias, gate and residual of tests."""
+    rng = np.random.default_rng(rows)
+    return rng.standard_normal(c.out).astype(np.float32), rng.standard_normal((rows, c.out)).astype(np.float32), rng.standard_normal((rows, c.out))
+
+
+# few rows against many weights, whole and in parts of the rows' length, ragged in both directions
+MANY_WEIGHTS = [(5088, 15361), (25632, 5130), (2080, 40003)]
+
+
+@pytest.mark.parametrize("fmt", [FP8, FP4])
+@pytest.mark.parametrize("t,extra", [(F32, False), (F32, True), (BF16, True)])
+@pytest.mark.parametrize("n,out", MANY_WEIGHTS)
+@pytest.mark.parametrize("rows", [1, 15, 17, 33, 64])
+def test_few_rows_many_weights(gpu, rows, n, out, t, extra, fmt):
+    F, c = gpu, Repeated(rows + n, rows, n, out, fmt, base_x=rows)
+    x, w = c.arrays(F)
+    want, b = c.exact(t)
+    kind, ld = to_type(np.zeros(1, np.float32), t).dtype, out + 5
+    full = np.full(3 + rows * ld, 77, kind)
+    kw, size, at = {}, np.abs(want), 3 * kind.itemsize
+    y = F.DeviceBuffer.from_array(full)
+    if extra:
+        bias, gate, res = _scaled_back(c, rows)
+        res = to_type(4 * res, t)
+        r = from_type(res, t).astype(np.float64)
+        want, b, size = r + gate * (want + bias), b * np.abs(gate), np.abs(r) + np.abs(gate) * (size + np.abs(bias))
+        full[3:].reshape(rows, ld)[:, :out] = res
+        y = buf(F, full)
+        kw = dict(d_bias=buf(F, bias), d_gate=buf(F, gate), d_res=y.ptr + at, ldres=ld)
+    need = F.mx_matmul_workspace_bytes(w.mx, x.mx)
+    ws = F.DeviceBuffer(need + 1024)
+    ws.fill(0xFF)
+    F.mx_matmul_dev(w.mx, x.mx, t, y.ptr + at, ws, need, ldy=ld, **kw)
+    F.synchronize()
+    got = y.download(kind, full.shape)
+    rest = got[3:].reshape(rows, ld)
+    assert (got[:3] == 77).all() and (rest[:, out:] == 77).all() and (ws.download(np.uint8, (need + 1024,))[need:] == 0xFF).all()
+    bad = np.abs(from_type(rest[:, :out], t).astype(np.float64) - want) - (b + 2.0 ** -22 * size + HALF[t] * np.abs(want))
+    assert (bad <= 0).all(), (float(bad.max()), np.argwhere(~(bad <= 0))[:3])
+
+
+@pytest.mark.parametrize("fmt", [FP8, FP4])
+@pytest.mark.parametrize("n,out", MANY_WEIGHTS)
+@pytest.mark.parametrize("rows", [2, 30, 50])
+def test_few_rows_many_weights_nan_rows(gpu, rows, n, out, fmt):
+    F, c = gpu, Repeated(rows + n, rows, n, out, fmt, base_x=rows)
+    x, w = c.arrays(F)
+    y, need = F.DeviceBuffer(rows * out * 4), F.mx_matmul_workspace_bytes(w.mx, x.mx)
+    ws = F.DeviceBuffer(max(1, need))
+
+    def run():
+        y.fill(0)
+        F.mx_matmul_dev(w.mx, x.mx, F32, y, ws, need)
+        F.synchronize()
+        return y.download(np.float32, (rows, out))
+
+    clean = run()
+    _tail(F, x.ds, (rows - 1) * strides(fmt, n)[1] + n // 32 - 1, np.array([255], np.uint8))
+    _tail(F, w.ds, (out - 1) * strides(FP4, n)[1], np.array([255], np.uint8))
+    _tail(F, w.ds, 700 * strides(FP4, n)[1] + 33, np.array([255], np.uint8))
+    bad = run()
+    nan = np.zeros(clean.shape, bool)
+    nan[rows - 1], nan[:, out - 1], nan[:, 700] = True, True, True
+    assert np.array_equal(np.isnan(bad), nan) and np.array_equal(bad[~nan], clean[~nan])
+
+
 # many tiles, whole and in parts of the rows' length: the larger tiles
 LARGE = [(1930, 1824, 4401), (422, 16480, 5532)]
 
@@ -372,14 +439,15 @@ def test_large_products(gpu, rows, n, out, t, off, more, extra, fmt):
 
 @pytest.mark.parametrize("fmt", [FP8, FP4])
 @pytest.mark.parametrize("to", [FP8, FP4])
-@pytest.mark.parametrize("rows,n,out", [(1930, 1824, 4480), (422, 16480, 5504)])
+@pytest.mark.parametrize("rows,n,out", [(1930, 1824, 4480), (422, 16480, 5504), (1, 5088, 40064), (19, 5088, 40064), (40, 5088, 40064), (64, 2080, 40064),
+                                        (12, 13856, 20096), (30, 13856, 20096), (60, 13856, 20096)])
 def test_large_swiglu(gpu, rows, n, out, to, fmt):
     F, c, f = gpu, Repeated(rows + 1, rows, n, out, fmt), out // 2
     x, w = c.arrays(F)
     y, b = c.exact(BF16)
     o = Mx(F, to, rows, f)
     need = F.mx_matmul_workspace_bytes(w.mx, x.mx, True)
-    assert (need > 0) == (rows == 422)
+    assert rows not in (422, 1930) or (need > 0) == (rows == 422)
     ws = F.DeviceBuffer(max(1, need))
     ws.fill(0xFF)
     F.mx_matmul_swiglu_dev(w.mx, x.mx, o.mx, ws, need)
