@@ -39,11 +39,15 @@ template <int T> __device__ __forceinline__ uint16_t to_half(float v) {
     else return __builtin_bit_cast(uint16_t, (__bf16)v);
 }
 
+// What is written once and not read here goes past L2's other lines: 13824 x 5120 fp32 to FP4 and back 99.6 -> 91.3 us,
+// norm of 14430 x 5376 204 -> 198, 8192 x 5120 -> 15360 360 -> 328 (the tiles' operands stay in L2).
+template <class V> __device__ __forceinline__ void put_past(const V &v, void *p) { __builtin_nontemporal_store(v, (V *)p); }
+
 // Stores eight values, each rounded once to the type, and leaves them as they were stored.
 template <int T> __device__ __forceinline__ void store8(void *p, int64_t i, float (&v)[8]) {
     if constexpr (T == FH3K_F32) {
-        *(f32x4 *)((float *)p + i) = f32x4{v[0], v[1], v[2], v[3]};
-        *(f32x4 *)((float *)p + i + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        put_past(f32x4{v[0], v[1], v[2], v[3]}, (float *)p + i);
+        put_past(f32x4{v[4], v[5], v[6], v[7]}, (float *)p + i + 4);
     } else {
         u32x4 a;
 #pragma unroll
@@ -58,7 +62,7 @@ template <int T> __device__ __forceinline__ void store8(void *p, int64_t i, floa
                 v[2 * k + 1] = __builtin_bit_cast(float, hi << 16);
             }
         }
-        *(u32x4 *)((uint16_t *)p + i) = a;
+        put_past(a, (uint16_t *)p + i);
     }
 }
 
@@ -113,8 +117,8 @@ template <bool F8> __device__ __forceinline__ void mx_store(const Fh3kMx &y, int
     }
     const uint32_t s = mx_scale<F8>(quad_max(u));
     const u32x2 code = mx_encode<F8>(v, s);
-    if constexpr (F8) *(u32x2 *)(y.codes + row * y.ld + col) = code;
-    else *(uint32_t *)(y.codes + row * y.ld + col / 2) = code.x;
+    if constexpr (F8) put_past(code, y.codes + row * y.ld + col);
+    else put_past((uint32_t)code.x, y.codes + row * y.ld + col / 2);
     if ((col & (MX_BLOCK - 1)) == 0) y.scales[row * y.lds + col / MX_BLOCK] = (uint8_t)s;
 }
 
@@ -665,22 +669,26 @@ template <int T, int TX, int TW> __device__ __forceinline__ void mx_rows_out(con
     if (o.res) mx_rows_out<T, true>(o, acc, stg, lane, t0, rows, n0, cols, vec);
     else mx_rows_out<T, false>(o, acc, stg, lane, t0, rows, n0, cols, vec);
 }
-// The same where the wavefront's first tiles are values and the others their gates: SwiGLU to codes.  A block is a tile's 32 columns.
-template <bool F8, int TX, int TW> __device__ __forceinline__ void mx_swiglu_out(const Fh3kMxOut &o, const f32x16 (&acc)[TX][TW], int lane,
+// The same where the wavefront's first tiles are values and the others their gates: SwiGLU to codes.  A block is a
+// tile's 32 columns.  Codes and scales come together in the wavefront's piece of LDS, [32 TX][BYTES], and leave 16 bytes
+// to a lane and a row's scales at once: from the registers a store covered 16 bytes of 32 rows (3016 x 5376 -> 28672 402 -> 391 us).
+template <bool F8, int TX, int TW> __device__ __forceinline__ void mx_swiglu_out(const Fh3kMxOut &o, const f32x16 (&acc)[TX][TW], uint8_t *stg, int lane,
                                                                                  int64_t t0, int64_t rows, int f0) {
+    constexpr int J = TW / 2, BYTES = F8 ? 32 * J : 16 * J, LD = BYTES + 16, L = BYTES / 16, TOKENS = 32 * TX;   // + 16: other banks for each row
+    static_assert(TOKENS == 64 && J <= 2, "scales: a token to a lane");
     const int64_t f = o.y.in;
     const int g = lane >> 5;
+    if (f0 >= f) return;                      // f is a multiple of 64: all of the wavefront's columns or none
+    uint8_t *sc = stg + TOKENS * LD;
 #pragma unroll 1
-    for (int idx = 0; idx < TX * TW / 2; idx++) {
-        const int i = idx / (TW / 2), j = idx % (TW / 2), col = f0 + 32 * j;
-        const int64_t t = t0 + 32 * i + (lane & 31);
+    for (int idx = 0; idx < TX * J; idx++) {
+        const int i = idx / J, j = idx % J, col = f0 + 32 * j, t = 32 * i + (lane & 31);
         f32x16 a, b;
         float v[2][8], q[2][8];
         mx_pick<TX, TW>(a, acc, i * TW + j);
-        mx_pick<TX, TW>(b, acc, i * TW + j + TW / 2);
+        mx_pick<TX, TW>(b, acc, i * TW + j + J);
         mx_columns(a, v);
         mx_columns(b, q);
-        if (col >= f) continue;               // the whole wavefront
         uint32_t u = 0;
 #pragma unroll
         for (int m = 0; m < 2; m++)
@@ -694,14 +702,25 @@ template <bool F8, int TX, int TW> __device__ __forceinline__ void mx_swiglu_out
             }
         const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
         const uint32_t r0 = r[0], r1 = r[1], s = mx_scale<F8>(r0 > r1 ? r0 : r1);
-        if (t >= rows) continue;
 #pragma unroll
         for (int m = 0; m < 2; m++) {
             const u32x2 c = mx_encode<F8>(v[m], s);
-            if constexpr (F8) *(u32x2 *)(o.y.codes + t * o.y.ld + col + 16 * m + 8 * g) = c;
-            else *(uint32_t *)(o.y.codes + t * o.y.ld + (col + 16 * m + 8 * g) / 2) = c.x;
+            if constexpr (F8) *(u32x2 *)(stg + t * LD + 32 * j + 16 * m + 8 * g) = c;
+            else *(uint32_t *)(stg + t * LD + 16 * j + 8 * m + 4 * g) = c.x;
         }
-        if (!g) o.y.scales[t * o.y.lds + col / MX_BLOCK] = (uint8_t)s;
+        if (!g) sc[t * J + j] = (uint8_t)s;
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int it = 0; it < TOKENS; it += 64 / L) {
+        const int t = it + lane / L, p = 16 * (lane % L);
+        const u32x4 c = *(const u32x4 *)(stg + t * LD + p);
+        if (t0 + t < rows) put_past(c, o.y.codes + (t0 + t) * o.y.ld + (F8 ? f0 : f0 / 2) + p);
+    }
+    if (t0 + lane < rows) {
+        uint8_t *p = o.y.scales + (t0 + lane) * o.y.lds + f0 / MX_BLOCK;
+        if constexpr (J == 2) *(uint16_t *)p = *(const uint16_t *)(sc + lane * 2);
+        else *p = sc[lane];
     }
 }
 
@@ -800,7 +819,7 @@ template <class G, bool SPLIT> __global__ __launch_bounds__(64 * G::WAVES, 8 / G
     // nothing more comes to LDS, and nobody reads it
     mx_barrier<0>();
     constexpr int PIECE = TW * 32 * 32 / 4, PER = sizeof(typename G::Buf) / 16 / PIECE;   // 16-byte words of a wavefront, wavefronts to a buffer
-    static_assert(G::NBUF * PER >= G::WAVES, "the sums' room");
+    static_assert(G::NBUF * PER >= G::WAVES && PIECE * 16 >= 64 * (TW * 16 + 16 + 2), "the sums' room");
     f32x4 *stg = (f32x4 *)(wave < PER ? b0.x : wave < 2 * PER || G::NBUF == 2 ? b1.x : (u32x4 *)&b2) + wave % PER * PIECE;
     if (part) {
         o = Fh3kMxOut{};
@@ -810,8 +829,8 @@ template <class G, bool SPLIT> __global__ __launch_bounds__(64 * G::WAVES, 8 / G
     const int64_t t0 = m0 + wm * (G::BX / G::NX);
     const int n0 = nt * G::BW + wn * CW;
     if (swiglu) {
-        if (o.y.type == FH3K_MX_FP8) mx_swiglu_out<true>(o, acc, lane, t0, x.rows, n0 / 2);
-        else mx_swiglu_out<false>(o, acc, lane, t0, x.rows, n0 / 2);
+        if (o.y.type == FH3K_MX_FP8) mx_swiglu_out<true>(o, acc, (uint8_t *)stg, lane, t0, x.rows, n0 / 2);
+        else mx_swiglu_out<false>(o, acc, (uint8_t *)stg, lane, t0, x.rows, n0 / 2);
     } else if (o.type == FH3K_F32) mx_rows_out<FH3K_F32>(o, acc, stg, lane, t0, x.rows, n0, part ? ldp : w.rows, vec);
     else if (o.type == FH3K_F16) mx_rows_out<FH3K_F16>(o, acc, stg, lane, t0, x.rows, n0, w.rows, vec);
     else mx_rows_out<FH3K_BF16>(o, acc, stg, lane, t0, x.rows, n0, w.rows, vec);
@@ -1329,10 +1348,10 @@ int few_tiles(const Fh3kMx *w, const Fh3kMx *x, bool swiglu) {
 
 // Each kernel's time in us by what was measured (weights from memory), of which the least is taken.
 // FP8 rows to bf16, k_mx_few, k_mx_stream and the tiles:
-//    rows of 5120 -> 5120:  1 row 6.5, 8.1, 18;    32 rows 10.7, 12.6, 19
-//    5120 -> 15360:         1 row 12.9, 11.4, 18;  17 rows 18.5, 14.2, 19; 64 rows -, 22.1, 21.3
-//    25600 -> 5120:         1 row 20.7, 20.0, 27;  16 rows 29, 21.7, 27
-//    5120 -> 51200 SwiGLU:  1 row 35.7, 28.2, 45;  32 rows 57, 33.8, 45.5
+//    5120 -> 5120           1 row 6.5, 8.1, -    32 rows 10.7, 12.6, -     64 rows -, 14.9, 15.0
+//    5120 -> 15360          1 row 12.9, 11.3, -  17 rows 18.5, 14.2, -     64 rows -, 22.1, 21.3
+//    25600 -> 5120          1 row 20.7, 19.0, -  16 rows -, 21.3, 27.3     64 rows -, 29.0, 31.0
+//    5120 -> 51200 SwiGLU   1 row 35.7, 28.2, -  17 rows 57, 32.0, 44.3    64 rows -, 47.5, 48.3
 double few_us(const Fh3kMx *w, const Fh3kMx *x, bool swiglu, bool split) {
     const int64_t rows = 16 * few_tiles(w, x, swiglu), groups = (w->rows + rows - 1) / rows;
     const double row = (double)w->in * (x->type == FH3K_MX_FP8 ? 1.0 : 0.5), each = (double)rows * w->in / 2 + x->rows * row;
