@@ -58,7 +58,15 @@ Workloads (each launch sequence is preceded by one untimed warmup launch):
          500 bf16 tokens over 2 x 14000 and of 250 fp32 tokens over 2 x 16000:
          fh3_hip_kv_append_dev, _read_dev, _attention_dev -> k_kv_*
 
-seqs and cache take --only NAME,NAME of their cases.
+  mx     microscaled operands: one FP8 row of 5120 -> 15360 (fp32), 16 of 25600
+         -> 5120, 600 of 5120 -> 17408, 8192 FP4 rows of 5120 -> 15360, 3016 FP8
+         rows of 7168 -> 5376 (fp32, gated residual), 32768 of 13824 -> 5120
+         (gated residual), SwiGLU of 20 x 5120 -> 51200 and 3016 x 5376 ->
+         28672, quantisation of 13824 x 5120 fp32 to FP4 and its read-back, of
+         37 x 25600 bf16 to FP8, the norm of one fp32 row of 5120 and of 14430
+         bf16 rows of 5376, modulated: fh3_hip_mx_* -> k_mx_*; weights rotated
+
+seqs, cache and mx take --only NAME,NAME of their cases.
 """
 import argparse
 import sys
@@ -360,15 +368,91 @@ def cache(reps, only=None):
             b.close()
 
 
+def _mx_rows(rng, fmt, rows, n):
+    """Random codes (FP8: without NaN) and scales of 2^-3 to 2^3."""
+    codes, scales = (np.empty(b, np.uint8) for b in F.mx_bytes(fmt, rows, n))
+    codes[:] = rng.integers(0, 256, codes.size, dtype=np.uint8) & (0xFF if fmt == F.FH3_MX_FP4 else 0xF7)
+    scales[:] = rng.integers(124, 131, scales.size, dtype=np.uint8)
+    c, s = F.DeviceBuffer.from_array(codes), F.DeviceBuffer.from_array(scales)
+    return F.mx(fmt, rows, n, c, s), [c, s]
+
+
+def mx(reps, only=None):
+    rng = np.random.default_rng(5)
+    fp4, fp8 = F.FH3_MX_FP4, F.FH3_MX_FP8
+    products = [("token", fp8, 1, 5120, 15360, "F32", False), ("tokens", fp8, 16, 25600, 5120, "BF16", False),
+                ("prompt", fp8, 600, 5120, 17408, "BF16", False), ("clip", fp4, 8192, 5120, 15360, "BF16", False),
+                ("out", fp8, 3016, 7168, 5376, "F32", True), ("long", fp8, 32768, 13824, 5120, "BF16", True),
+                ("prompt_swiglu", fp8, 20, 5120, 51200, None, False), ("clip_swiglu", fp8, 3016, 5376, 28672, None, False)]
+    for name, fmt, rows, n, out, t, gated in products:
+        if only and name not in only:
+            continue
+        used = []
+        x, b = _mx_rows(rng, fmt, rows, n)
+        used += b
+        ws = []
+        for _ in range(max(1, min(8, MALL_BYTES // (out * n // 2))) + 1 if rows <= 64 else 1):
+            w, b = _mx_rows(rng, fp4, out, n)
+            ws.append(w)
+            used += b
+        size = F.mx_matmul_workspace_bytes(ws[0], x, t is None)
+        work = F.DeviceBuffer(max(1, size))
+        used.append(work)
+        if t is None:
+            y, b = _mx_rows(rng, fp8, rows, out // 2)
+            used += b
+        else:
+            y = F.DeviceBuffer(rows * out * (4 if t == "F32" else 2))
+            used.append(y)
+        res, gate = None, None
+        if gated:
+            res, gate = _typed(rng, rows, out, t), _typed(rng, rows, out, "F32")
+            used += [res, gate]
+        for i in range(reps + 1):
+            if t is None:
+                F.mx_matmul_swiglu_dev(ws[i % len(ws)], x, y, work, size)
+            else:
+                F.mx_matmul_dev(ws[i % len(ws)], x, _TYPES[t], y, work, size, d_gate=gate, d_res=res)
+        F.synchronize()
+        print("mx %s: %d x %d -> %d, %d launches" % (name, rows, n, out, reps), flush=True)
+        for b in used:
+            b.close()
+    for name, fmt, rows, n, t in (("weights", fp4, 13824, 5120, "F32"), ("rows", fp8, 37, 25600, "BF16")):
+        if only and name not in only:
+            continue
+        x, back = _typed(rng, rows, n, t), F.DeviceBuffer(rows * n * 2)
+        y, used = _mx_rows(rng, fmt, rows, n)
+        for _ in range(reps + 1):
+            F.mx_quantize_dev(_TYPES[t], x, y)
+            F.mx_dequant_dev(y, F.FH3_QUANT_BF16, back)
+        F.synchronize()
+        print("mx %s: %d x %d, %d launches" % (name, rows, n, reps), flush=True)
+        for b in [x, back] + used:
+            b.close()
+    for name, rows, n, t, mod in (("token_norm", 1, 5120, "F32", False), ("clip_norm", 14430, 5376, "BF16", True)):
+        if only and name not in only:
+            continue
+        x, add, w = _typed(rng, rows, n, t), _typed(rng, rows, n, t), _typed(rng, 1, n, "F32")
+        shift, scale = (_typed(rng, rows, n, "F32") for _ in range(2)) if mod else (None, None)
+        y, used = _mx_rows(rng, fp8, rows, n)
+        total = F.DeviceBuffer(x.nbytes)
+        for _ in range(reps + 1):
+            F.mx_norm_dev(_TYPES[t], x, w, 1e-6, y, d_add=add, d_sum=total, d_shift=shift, d_scale=scale)
+        F.synchronize()
+        print("mx %s: %d x %d, %d launches" % (name, rows, n, reps), flush=True)
+        for b in [x, add, w, total] + used + ([shift, scale] if mod else []):
+            b.close()
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser()
     ap.add_argument("workload", choices=("gemv", "te", "prompt", "mid", "single", "q56", "gemm", "mlp", "copy", "attn", "vsa",
-                                         "seqs", "cache", "all"))
+                                         "seqs", "cache", "mx", "all"))
     ap.add_argument("--reps", type=int, default=20)
-    ap.add_argument("--only", help="seqs, cache: these cases")
+    ap.add_argument("--only", help="seqs, cache, mx: these cases")
     args = ap.parse_args(argv)
     F.init(0)
-    if args.workload in ("seqs", "cache"):
+    if args.workload in ("seqs", "cache", "mx"):
         globals()[args.workload](args.reps, args.only.split(",") if args.only else None)
         return 0
     for name in (("gemv", "gemm", "copy") if args.workload == "all" else (args.workload,)):
