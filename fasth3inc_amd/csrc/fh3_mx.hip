@@ -276,8 +276,8 @@ __device__ __forceinline__ void set4(i32x8 &v, int at, const u32x4 &a) {
 // e4m3 codes whose magnitude is 2 or more (bit 6 set); the others are c ^ that.  Within
 // each part the products with e2m1 codes span no more than 13 bits, so both are summed exactly.
 __device__ __forceinline__ uint32_t fp8_large(uint32_t c) {
-    const uint32_t m = c & 0x40404040u, t = m << 1;
-    return c & (t | (t - (m >> 6)));
+    // each byte's bit 6 in all of the byte's bits: the permutation's selectors 8 .. 11 are the signs of bytes 1, 3, 5, 7
+    return c & __builtin_amdgcn_perm(c << 1, c << 9, 0x0B090A08u);
 }
 
 // ---------------------------------------------------------------------------
@@ -1366,9 +1366,10 @@ double few_us(const Fh3kMx *w, const Fh3kMx *x, bool swiglu, bool split) {
     const int64_t rows = 16 * few_tiles(w, x, swiglu), groups = (w->rows + rows - 1) / rows;
     const double row = (double)w->in * (x->type == FH3K_MX_FP8 ? 1.0 : 0.5), each = (double)rows * w->in / 2 + x->rows * row;
     // a workgroup's bytes through one CU, or all weights from memory and the rows for each workgroup from L2
-    const double one = each / (x->rows <= 16 ? 38e3 : x->rows <= 32 ? 36e3 : 26e3);
+    const double one = each / (x->rows <= 16 ? 38e3 : x->rows <= 32 ? 36e3 : 30e3);
     const double all = (double)w->rows * w->in * 0.53 / (4.4e6 * (groups < 200 ? groups / 200.0 : 1.0)) + groups * x->rows * row / 12e6;
-    return 3.9 + (one > all ? one : all) * (!split ? 1 : x->rows <= 16 ? 1.1 : x->rows <= 32 ? 1.35 : 1.8);
+    const double more = !split || x->rows <= 16 ? 1 : x->rows <= 32 ? 1.35 : 1.8, a = 3.9 + one * more, b = (swiglu || x->rows > 32 ? 3.9 : 2.6) + all * more;
+    return a > b ? a : b;
 }
 // Steps of 128 values that a wavefront of k_mx_stream holds of x: what fits its registers
 int stream_steps(const Fh3kMx *x) {
