@@ -1239,7 +1239,7 @@ template <bool F8, bool SPLIT, int TT, int NS> __global__ __launch_bounds__(64 *
                 }
             }
             // the sums of the last trip are read
-            if (d == 0) asm volatile("s_barrier" : : : "memory");
+            if (d == 0) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -1427,17 +1427,16 @@ double tiles_us(const Fh3kMx *w, const Fh3kMx *x, bool split, Plan &p) {
 }
 // split: FP8 rows to fp32, in two products
 Plan plan_of(const Fh3kMx *w, const Fh3kMx *x, bool swiglu, bool split) {
-    Plan tiles = {}, stream = {};
-    const double t = tiles_us(w, x, split, tiles);
-    if (x->rows > 64) return tiles;
-    const double s = stream_us(w, x, swiglu, split, stream), f = few_us(w, x, swiglu, split);
-    if (f <= s && f <= t) {
-        Plan few = {};
-        few.kernel = Plan::FEW;
-        few.parts = 1;
-        return few;
+    Plan few = {}, tiles = {}, stream = {};
+    few.kernel = Plan::FEW;
+    few.parts = 1;
+    if (x->rows > 64) {
+        tiles_us(w, x, split, tiles);
+        return tiles;
     }
-    return s <= t ? stream : tiles;
+    const double s = stream_us(w, x, swiglu, split, stream), f = few_us(w, x, swiglu, split), least = s < f ? s : f;
+    if (x->rows > 16 && tiles_us(w, x, split, tiles) < least) return tiles;   // (16 rows: never the least)
+    return f <= s ? few : stream;
 }
 
 template <class G, bool SPLIT = false> void launch_gemm(const Fh3kMx *w, const Fh3kMx *x, const Fh3kMxOut *o, const Plan &p, float *part, bool vec,
@@ -1470,6 +1469,7 @@ bool sixteens(const void *p, int64_t ld, int size) { return !p || ((uintptr_t)p 
 }  // namespace
 
 extern "C" int fh3k_mx_matmul_fits(const Fh3kMx *w, const Fh3kMx *x) {
+    if ((x->rows + 127) / 128 * ((w->rows + 127) / 128) < ((int64_t)1 << 23) && (w->rows + 7) / 8 * 8 * x->rows <= ((int64_t)1 << 40)) return 1;
     const Plan p = plan_of(w, x, false, false);
     return (p.kernel != Plan::TILES || p.m_tiles * p.n_tiles < ((int64_t)1 << 23)) && p.ldp * x->rows <= ((int64_t)1 << 40);
 }

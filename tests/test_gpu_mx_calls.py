@@ -486,3 +486,47 @@ def test_large_products_nan_rows(gpu, fmt):
     nan = np.zeros(clean.shape, bool)
     nan[1000], nan[:, 4400] = True, True
     assert np.array_equal(np.isnan(bad), nan) and np.array_equal(bad[~nan], clean[~nan])
+
+
+@pytest.mark.parametrize("fmt", [FP8, FP4])
+@pytest.mark.parametrize("rows,out", [(1, 20), (20, 33), (40, 300), (70, 20), (300, 130)])
+def test_the_longest_rows(gpu, rows, out, fmt):
+    F, n = gpu, 1 << 20
+    c = Repeated(rows, rows, n, out, fmt, base_x=3, base_w=5)
+    x, w = c.arrays(F)
+    need = F.mx_matmul_workspace_bytes(w.mx, x.mx)
+    ws, y = F.DeviceBuffer(max(1, need)), F.DeviceBuffer(rows * out * 4)
+    ws.fill(0xFF)
+    for t in (F32, BF16):
+        want, b = c.exact(t)
+        F.mx_matmul_dev(w.mx, x.mx, t, y, ws, need)
+        F.synchronize()
+        got = from_type(y.download(to_type(np.zeros(1, np.float32), t).dtype, (rows, out)), t)
+        assert (np.abs(got - want) <= b + 2.0 ** -22 * np.abs(want) + HALF[t] * np.abs(want)).all()
+
+
+def test_many_threads_query_and_call(gpu):
+    """Plans, workspaces and launches from many threads: nothing is kept between calls."""
+    F, errors = gpu, []
+    cases = [Case(r, r, n, o, FP8) for r, n, o in ((1, 5120, 130), (20, 1024, 300), (70, 4096, 200), (300, 512, 260))]
+    want = [c.run(F, F32) for c in cases]
+    streams = _streams(F, len(cases))
+
+    def work(c, y, st):
+        try:
+            for _ in range(10):
+                x, w = Mx(F, FP8, c.rows, c.n, *c.x[:2]), Mx(F, FP4, c.out, c.n, *c.w[:2])
+                need, out = F.mx_matmul_workspace_bytes(w.mx, x.mx), F.DeviceBuffer(y.nbytes)
+                ws = F.DeviceBuffer(max(1, need))
+                F.mx_matmul_dev(w.mx, x.mx, F32, out, ws, need, stream_ptr=st)
+                assert F.lib().hipStreamSynchronize(st) == 0
+                assert np.array_equal(out.download(np.float32, y.shape), y)
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(cases, want, streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
