@@ -293,9 +293,9 @@ __device__ __forceinline__ uint32_t fp8_large(uint32_t c) {
 // p of sixteen rows lie in different banks.  Scales come for CH stages at a time (a
 // request to L2 for each row's 8 or 4 bytes of a stage took as many requests as the
 // codes) and are held in registers.
-// 8192 x 5120 -> 15360 FP4 321 us (4.0 PFLOP/s: products alone 190, DMA alone 193, with the
+// 8192 x 5120 -> 15360 FP4 322 us (4.0 PFLOP/s: products alone 190, DMA alone 193, with the
 // operands' reads 280), 32768 x 13824 -> 5120 FP8 1855 (2.5; the library's FP8 product 2.6),
-// 3016 x 5376 -> 28672 SwiGLU 391, 3016 x 7168 -> 5376 fp32 in two products 180.
+// 3016 x 5376 -> 28672 SwiGLU 380, 3016 x 7168 -> 5376 fp32 in two products 178.
 // ---------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) void lds_void;
 
@@ -734,7 +734,7 @@ template <bool F8, int TX, int TW> __device__ __forceinline__ void mx_swiglu_out
 }
 
 template <class G, bool SPLIT> __global__ __launch_bounds__(64 * G::WAVES, 8 / G::WAVES) void k_mx_gemm(
-    Fh3kMx w, Fh3kMx x, Fh3kMxOut o, float *part, int64_t ldp, int m_tiles, int n_tiles, int per, bool vec) {
+    Fh3kMx w, Fh3kMx x, Fh3kMxOut o, float *part, int64_t ldp, int m_tiles, int n_tiles, int first, int per, bool vec) {
     constexpr int TW = G::TW, TX = G::TX;
     __shared__ typename G::Buf b0, b1;
     __shared__ typename std::conditional<G::NBUF == 3, typename G::Buf, int>::type b2;
@@ -746,7 +746,7 @@ template <class G, bool SPLIT> __global__ __launch_bounds__(64 * G::WAVES, 8 / G
     const int total = m_tiles * n_tiles, id = blockIdx.x, share = total >> 3;
     const int L = id < share * 8 ? (id & 7) * share + (id >> 3) : id;
     const int band = L / (GB * n_tiles), gs = min(GB, m_tiles - band * GB), in = L - band * GB * n_tiles;
-    const int nt = in / gs, mt = band * GB + in - nt * gs;
+    const int mt = band * GB + in % gs, nt = first + in / gs;   // columns of tiles from the first on
     const int64_t m0 = (int64_t)mt * G::BX;
     const bool swiglu = o.y.codes != nullptr && !part;
 
@@ -1348,6 +1348,7 @@ struct Plan {
     enum { FEW, STREAM, TILES } kernel;
     int bw, bx, parts, per;       // per: stages (STREAM: steps) of a part
     int64_t m_tiles, n_tiles, ldp;
+    int64_t large;                // columns of larger tiles, where the others are left to smaller ones
 };
 // Tiles of 16 weight rows to a workgroup of k_mx_few: the most that leave 150
 // workgroups, since each reads all rows of x.  SwiGLU: a block of 32 outputs.
@@ -1366,7 +1367,7 @@ double few_us(const Fh3kMx *w, const Fh3kMx *x, bool swiglu, bool split) {
     const int64_t rows = 16 * few_tiles(w, x, swiglu), groups = (w->rows + rows - 1) / rows;
     const double row = (double)w->in * (x->type == FH3K_MX_FP8 ? 1.0 : 0.5), each = (double)rows * w->in / 2 + x->rows * row;
     // a workgroup's bytes through one CU, or all weights from memory and the rows for each workgroup from L2
-    const double one = each / (x->rows <= 16 ? 38e3 : x->rows <= 32 ? 36e3 : 30e3);
+    const double one = each / (x->rows <= 16 ? 38e3 : x->rows <= 32 ? 36e3 : rows == 64 ? 20e3 : 32e3);
     const double all = (double)w->rows * w->in * 0.53 / (4.4e6 * (groups < 200 ? groups / 200.0 : 1.0)) + groups * x->rows * row / 12e6;
     const double more = !split || x->rows <= 16 ? 1 : x->rows <= 32 ? 1.35 : 1.8, a = 3.9 + one * more, b = (swiglu || x->rows > 32 ? 3.9 : 2.6) + all * more;
     return a > b ? a : b;
@@ -1391,29 +1392,46 @@ double stream_us(const Fh3kMx *w, const Fh3kMx *x, bool swiglu, bool split, Plan
     const double each = (double)((p.n_tiles + p.m_tiles - 1) / p.m_tiles) * (blocks ? 4 : 1) * p.per;
     const double held = (double)x->rows * p.per * (x->type == FH3K_MX_FP8 ? 128 : 64);
     double t = 5 + each * 0.038 + held / 45e3 + (tt == 4 ? 1.5 : 0);
-    if (split && tt > 1) t += tt * (1 + each * 0.01);
+    if (split && tt > 1) t += tt * (1 + each * 0.008);
     if (p.parts > 1) t += 2.5 + (double)p.parts * x->rows * w->rows * 8 / 4e6;
     return t;
 }
 // Tiles: for a stage on a CU that has one workgroup of 128 x 128, two, or one of 256 x 256, and for a round's
-// beginning and end; parts are written and read at 4 MB a us and joined by a launch of 3.5 us.
+// beginning and end; parts are written and read at 4 MB a us and joined by a launch of 3.5 us.  FP8 rows of 5120, weights
+// in the caches, small and large tiles: 600 rows -> 5120 23.3, 37 us; 400 -> 17408 57, 50; 1000 -> 15360 85, 63;
+// 13824 -> 5120: 600 rows 53.6, 64, 1000 rows 92, 85.
 double tiles_us(const Fh3kMx *w, const Fh3kMx *x, bool split, Plan &p) {
     const bool f8 = x->type == FH3K_MX_FP8;
     const int ks = f8 ? 128 : 256, stages = (int)((w->in + ks - 1) / ks);
-    const double more = split ? 1.4 : 1, one = f8 ? 0.65 * more : 1.05, two = f8 ? 1.0 * more : 1.42, big = f8 ? 1.45 * more : 2.1;
+    const double more = split ? 1.5 : 1, one = f8 ? 0.51 * more : 0.88, few = f8 ? 0.78 * more : 0.95, two = f8 ? 0.95 * more : 1.15,
+                 big = f8 ? 1.2 * more : 1.6;
     double least = 0;
     p.kernel = Plan::TILES;
+    // a last round of smaller tiles: one to a CU, two to a few or to all
+    auto some = [&](int64_t n, int per) { return n <= 256 ? per * one + 3 : per * (few + (two - few) * (n - 256) / 256) + 4; };
     for (int b = 128; b <= 256; b += 128) {
         const int64_t m = (x->rows + b - 1) / b, n = (w->rows + b - 1) / b;
         for (int parts = 1; parts <= 32 && (parts == 1 || parts * 4 <= stages); parts++) {
             const int per = (stages + parts - 1) / parts;
             if (parts > 1 && (stages + per - 1) / per != parts) continue;
             const int64_t groups = m * n * parts, slots = b == 128 ? 512 : 256, rest = groups % slots;
-            const double round = b == 256 ? per * big + 9 : per * two + 4, last = b == 256 || rest > 256 ? round : per * one + 3;
+            const double round = b == 256 ? per * big + 8 : per * two + 4, last = b == 256 ? round : some(rest, per);
             double t = (double)(groups / slots) * round + (rest ? last : 0);
             if (parts > 1) t += 3.5 + (double)parts * x->rows * w->rows * 8 / 4e6;
+            // the last round, where it is not full, in smaller tiles: a launch of its own for the last columns
+            // (4096 x 13824 -> 5120, 1.25 rounds, 257 -> 216 us, 3016 x 5376 -> 28672 SwiGLU, 5.25 rounds, 389 -> 378)
+            const int64_t large = b == 256 && parts == 1 ? groups / 256 * 256 / m : 0;
+            bool mixed = false;
+            if (large > 0 && large < n) {
+                const int64_t small = (x->rows + 127) / 128 * ((w->rows + 127) / 128 - 2 * large), over = small % 512;
+                const double both = (double)(groups / 256) * round + (double)(small / 512) * (per * two + 4) +
+                                    (over ? some(over, per) : 0) + 3;
+                mixed = both * 1.02 < t;
+                if (mixed) t = both;
+            }
             if (least == 0 || t < least) {
                 least = t;
+                p.large = mixed ? large : 0;
                 p.bw = p.bx = b;
                 p.parts = parts;
                 p.per = per;
@@ -1435,14 +1453,17 @@ Plan plan_of(const Fh3kMx *w, const Fh3kMx *x, bool swiglu, bool split) {
         return tiles;
     }
     const double s = stream_us(w, x, swiglu, split, stream), f = few_us(w, x, swiglu, split), least = s < f ? s : f;
-    if (x->rows > 16 && tiles_us(w, x, split, tiles) < least) return tiles;   // (16 rows: never the least)
+    // tiles: no less than the weights' way from memory (16 rows: never the least)
+    if (x->rows > 16 && 8 + (double)w->rows * w->in * 0.53 / 3.2e6 < least && tiles_us(w, x, split, tiles) < least) return tiles;
     return f <= s ? few : stream;
 }
 
-template <class G, bool SPLIT = false> void launch_gemm(const Fh3kMx *w, const Fh3kMx *x, const Fh3kMxOut *o, const Plan &p, float *part, bool vec,
-                                                       hipStream_t st) {
-    const dim3 grid((unsigned)(p.m_tiles * p.n_tiles), (unsigned)p.parts);
-    k_mx_gemm<G, SPLIT><<<grid, 64 * G::WAVES, 0, st>>>(*w, *x, *o, part, p.ldp, (int)p.m_tiles, (int)p.n_tiles, p.per, vec || part);
+// Columns first .. of tiles, all or those before `end`.
+template <class G, bool SPLIT> void launch_gemm(const Fh3kMx *w, const Fh3kMx *x, const Fh3kMxOut *o, const Plan &p, int64_t first, int64_t end,
+                                                float *part, bool vec, hipStream_t st) {
+    const int64_t m = (x->rows + G::BX - 1) / G::BX, all = (w->rows + G::BW - 1) / G::BW, n = (end ? end : all) - first;
+    const dim3 grid((unsigned)(m * n), (unsigned)p.parts);
+    k_mx_gemm<G, SPLIT><<<grid, 64 * G::WAVES, 0, st>>>(*w, *x, *o, part, p.ldp, (int)m, (int)n, (int)first, p.per, vec || part);
 }
 
 template <bool F8, bool SPLIT, int TT, int R> void launch_few(const Fh3kMx *w, const Fh3kMx *x, const Fh3kMxOut *o, hipStream_t st) {
@@ -1521,6 +1542,10 @@ extern "C" hipError_t fh3k_mx_matmul(const Fh3kMx *w, const Fh3kMx *x, const Fh3
         else if (stream_steps(x) == 3) go(N4{}, N3{});
         else if constexpr (!f()) go(N4{}, N5{});
     };
+    auto tiles = [&](auto large, auto small, auto sp) {
+        if (p.bw == 256) launch_gemm<decltype(large), sp()>(w, x, o, p, 0, p.large, part, vec, st);
+        if (p.bw == 128 || p.large) launch_gemm<decltype(small), sp()>(w, x, o, p, 2 * p.large, 0, part, vec, st);
+    };
     auto by_rows = [&](auto go) {
         if (!f8) go(std::false_type{}, std::false_type{});
         else if (!split) go(std::true_type{}, std::false_type{});
@@ -1528,12 +1553,9 @@ extern "C" hipError_t fh3k_mx_matmul(const Fh3kMx *w, const Fh3kMx *x, const Fh3
     };
     if (p.kernel == Plan::FEW) by_rows(few);
     else if (p.kernel == Plan::STREAM) by_rows(stream);
-    else if (p.bw == 256 && !f8) launch_gemm<Big4>(w, x, o, p, part, vec, st);
-    else if (p.bw == 256 && !split) launch_gemm<Big8>(w, x, o, p, part, vec, st);
-    else if (p.bw == 256) launch_gemm<Big8, true>(w, x, o, p, part, vec, st);
-    else if (!f8) launch_gemm<Small4>(w, x, o, p, part, vec, st);
-    else if (!split) launch_gemm<Small8>(w, x, o, p, part, vec, st);
-    else launch_gemm<Small8, true>(w, x, o, p, part, vec, st);
+    else if (!f8) tiles(Big4{}, Small4{}, std::false_type{});
+    else if (!split) tiles(Big8{}, Small8{}, std::false_type{});
+    else tiles(Big8{}, Small8{}, std::true_type{});
     if (!part) return hipGetLastError();
     if (o->y.codes) {
         const dim3 grid((unsigned)x->rows, (unsigned)((o->y.in + 2047) / 2048));
