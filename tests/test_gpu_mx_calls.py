@@ -401,8 +401,8 @@ def test_few_rows_many_weights_nan_rows(gpu, rows, n, out, fmt):
     assert np.array_equal(np.isnan(bad), nan) and np.array_equal(bad[~nan], clean[~nan])
 
 
-# many tiles, whole and in parts of the rows' length: the larger tiles
-LARGE = [(1930, 1824, 4401), (422, 16480, 5532)]
+# many tiles, whole, in parts of the rows' length, and with a last round of smaller ones: the larger tiles
+LARGE = [(1930, 1824, 4401), (422, 16480, 5532), (2100, 1824, 8101)]
 
 
 @pytest.mark.parametrize("fmt", [FP8, FP4])
@@ -439,7 +439,7 @@ def test_large_products(gpu, rows, n, out, t, off, more, extra, fmt):
 
 @pytest.mark.parametrize("fmt", [FP8, FP4])
 @pytest.mark.parametrize("to", [FP8, FP4])
-@pytest.mark.parametrize("rows,n,out", [(1930, 1824, 4480), (422, 16480, 5504), (1, 5088, 40064), (19, 5088, 40064), (40, 5088, 40064), (64, 2080, 40064),
+@pytest.mark.parametrize("rows,n,out", [(1930, 1824, 4480), (422, 16480, 5504), (2100, 1824, 8192), (1, 5088, 40064), (19, 5088, 40064), (40, 5088, 40064), (64, 2080, 40064),
                                         (12, 13856, 20096), (30, 13856, 20096), (60, 13856, 20096)])
 def test_large_swiglu(gpu, rows, n, out, to, fmt):
     F, c, f = gpu, Repeated(rows + 1, rows, n, out, fmt), out // 2
@@ -468,23 +468,24 @@ def test_large_swiglu(gpu, rows, n, out, to, fmt):
 
 
 @pytest.mark.parametrize("fmt", [FP8, FP4])
-def test_large_products_nan_rows(gpu, fmt):
-    F, c = gpu, Repeated(3, 1930, 1824, 4401, fmt)
+@pytest.mark.parametrize("rows,out", [(1930, 4401), (2100, 8101)])
+def test_large_products_nan_rows(gpu, rows, out, fmt):
+    F, c = gpu, Repeated(3, rows, 1824, out, fmt)
     x, w = c.arrays(F)
-    y = F.DeviceBuffer(1930 * 4401 * 4)
+    y = F.DeviceBuffer(rows * out * 4)
 
     def run():
         y.fill(0)
         F.mx_matmul_dev(w.mx, x.mx, F32, y, None, 0)
         F.synchronize()
-        return y.download(np.float32, (1930, 4401))
+        return y.download(np.float32, (rows, out))
 
     clean = run()
     _tail(F, x.ds, 1000 * strides(fmt, 1824)[1] + 56, np.array([255], np.uint8))
-    _tail(F, w.ds, 4400 * strides(FP4, 1824)[1], np.array([255], np.uint8))
+    _tail(F, w.ds, (out - 1) * strides(FP4, 1824)[1], np.array([255], np.uint8))
     bad = run()
     nan = np.zeros(clean.shape, bool)
-    nan[1000], nan[:, 4400] = True, True
+    nan[1000], nan[:, out - 1] = True, True
     assert np.array_equal(np.isnan(bad), nan) and np.array_equal(bad[~nan], clean[~nan])
 
 
