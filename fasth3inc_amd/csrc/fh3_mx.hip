@@ -12,6 +12,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef short i16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int MX_BLOCK = 32;
+constexpr float LOG2E_REST = 1.92596299e-08f;   // of log2(e) below LOG2E
 
 // ---------------------------------------------------------------------------
 // Values, eight to a lane: a block of 32 is the four lanes of a quad
@@ -271,8 +272,9 @@ __device__ __forceinline__ void set4(i32x8 &v, int at, const u32x4 &a) {
 }
 // The instruction aligns eight products to the largest one's power of two 2^E and cuts
 // off what lies below 2^(E - 13): with FP8 codes 4e-6 to 1.2e-5 of the result (FP4: nothing).
-// Outputs of 16 bits and SwiGLU's codes, whose own rounding is 2^-11 and more, take that;
-// fp32 outputs come from two products, at half the rate:
+// Outputs of 16 bits, whose own rounding is 2^-11 and more, take that.  fp32 outputs and
+// SwiGLU, whose codes it would move (3016 x 5376 -> 28672: 3e-3 of the codes' norm, scales
+// among them, where fp32 sums give 1e-4), come from two products, at half the rate:
 // e4m3 codes whose magnitude is 2 or more (bit 6 set); the others are c ^ that.  Within
 // each part the products with e2m1 codes span no more than 13 bits, so both are summed exactly.
 __device__ __forceinline__ uint32_t fp8_large(uint32_t c) {
@@ -295,7 +297,7 @@ __device__ __forceinline__ uint32_t fp8_large(uint32_t c) {
 // codes) and are held in registers.
 // 8192 x 5120 -> 15360 FP4 322 us (4.0 PFLOP/s: products alone 190, DMA alone 193, with the
 // operands' reads 280), 32768 x 13824 -> 5120 FP8 1855 (2.5; the library's FP8 product 2.6),
-// 3016 x 5376 -> 28672 SwiGLU 380, 3016 x 7168 -> 5376 fp32 in two products 178.
+// in two products 3016 x 5376 -> 28672 SwiGLU 635 (2.9 PFLOP/s of them) and 3016 x 7168 -> 5376 fp32 178.
 // ---------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) void lds_void;
 
@@ -549,8 +551,17 @@ template <int TX, int TW> __device__ __forceinline__ void mx_settle(f32x16 (&acc
         for (int j = 0; j < TW; j++) asm volatile("" : "+a"(acc[i][j]));
 }
 
-// g / (1 + exp(-g)), to two units in the last place and those of exp2's argument
-__device__ __forceinline__ float silu(float g) { return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-LOG2E * g)); }
+// g / (1 + exp(-g)) to about two units in the last place: from e = exp(-|g|), which cannot overflow, with the rest of
+// exp2's rounded argument (up to 1e-6 of e at |g| = 20) and the reciprocal's error taken out.
+__device__ __forceinline__ float silu(float g) {
+    const float m = -fminf(fabsf(g), 200.f), a = m * LOG2E, rest = __builtin_fmaf(m, LOG2E, -a) + m * LOG2E_REST;
+    float e = __builtin_amdgcn_exp2f(a);
+    e = __builtin_fmaf(e, rest * 0.69314718f, e);
+    const float d = 1.f + e;
+    float r = __builtin_amdgcn_rcpf(d);
+    r = __builtin_fmaf(r, __builtin_fmaf(-d, r, 1.f), r);
+    return (g < 0.f ? g * e : g) * r;
+}
 
 // Eight values of a row, or one, to where they go; Beside: what is read for them.
 struct Beside {
@@ -680,7 +691,7 @@ template <int T, int TX, int TW> __device__ __forceinline__ void mx_rows_out(con
 }
 // The same where the wavefront's first tiles are values and the others their gates: SwiGLU to codes.  A block is a
 // tile's 32 columns.  Codes and scales come together in the wavefront's piece of LDS, [32 TX][BYTES], and leave 16 bytes
-// to a lane and a row's scales at once: from the registers a store covered 16 bytes of 32 rows (3016 x 5376 -> 28672 402 -> 391 us).
+// to a lane and a row's scales at once: from the registers a store covered 16 bytes of 32 rows (3016 x 5376 -> 28672 in one product 402 -> 391 us).
 template <bool F8, int TX, int TW> __device__ __forceinline__ void mx_swiglu_out(const Fh3kMxOut &o, const f32x16 (&acc)[TX][TW], uint8_t *stg, int lane,
                                                                                  int64_t t0, int64_t rows, int f0) {
     constexpr int J = TW / 2, BYTES = F8 ? 32 * J : 16 * J, LD = BYTES + 16, L = BYTES / 16, TOKENS = 32 * TX;   // + 16: other banks for each row
@@ -1111,10 +1122,11 @@ template <bool F8, bool SPLIT, int TT, int R, bool AHEAD> __global__ __launch_bo
 // 128 values) and takes tile after tile of 16 weight rows, straight from memory, two of
 // them while the next two are on their way; the wavefronts' sums meet in LDS four tiles at a time.
 // k_mx_few reads all of x for each 16 R weight rows: 20 rows x 5120 -> 51200 SwiGLU, 139 MB
-// of weights, took it 57 us, the tiles 43, this 32 (27.5 with one row: 5.1 TB/s).
+// of weights, took it 57 us, the tiles 43, this 32 (27.5 with one row: 5.1 TB/s), each in one
+// product; in two 39: 40 more VALU instructions for 32 codes (16 rows: the halves stay in registers, 30).
 // Where x is longer than 40 steps (24), each part of it has its own workgroups, and the
 // parts' sums are joined: 16 rows x 25600 -> 5120 29 us, tiles 24, this 19.
-// Two tiles to each splitting of FP8 codes (fp32 outputs): with one, that took longer than the loads.
+// Two tiles to each splitting of FP8 codes (fp32 outputs, SwiGLU): with one, that took longer than the loads.
 // Nothing that is known before the loop is kept over it (the asm statements): the
 // registers are full of loads, and a reload from scratch waits for all loads before it.
 // ---------------------------------------------------------------------------
@@ -1362,7 +1374,7 @@ int few_tiles(const Fh3kMx *w, const Fh3kMx *x, bool swiglu) {
 //    5120 -> 5120           1 row 6.5, 8.1, -    32 rows 10.7, 12.6, -     64 rows -, 14.9, 15.0
 //    5120 -> 15360          1 row 12.9, 11.3, -  17 rows 18.5, 14.2, -     64 rows -, 22.1, 21.3
 //    25600 -> 5120          1 row 20.7, 19.0, -  16 rows -, 21.3, 27.3     64 rows -, 29.0, 31.0
-//    5120 -> 51200 SwiGLU   1 row 35.7, 28.2, -  17 rows 57, 32.0, 44.3    64 rows -, 47.5, 48.3
+//    5120 -> 51200 in one   1 row 35.7, 28.2, -  17 rows 57, 32.0, 44.3    64 rows -, 47.5, 48.3
 double few_us(const Fh3kMx *w, const Fh3kMx *x, bool swiglu, bool split) {
     const int64_t rows = 16 * few_tiles(w, x, swiglu), groups = (w->rows + rows - 1) / rows;
     const double row = (double)w->in * (x->type == FH3K_MX_FP8 ? 1.0 : 0.5), each = (double)rows * w->in / 2 + x->rows * row;
@@ -1419,7 +1431,7 @@ double tiles_us(const Fh3kMx *w, const Fh3kMx *x, bool split, Plan &p) {
             double t = (double)(groups / slots) * round + (rest ? last : 0);
             if (parts > 1) t += 3.5 + (double)parts * x->rows * w->rows * 8 / 4e6;
             // the last round, where it is not full, in smaller tiles: a launch of its own for the last columns
-            // (4096 x 13824 -> 5120, 1.25 rounds, 257 -> 216 us, 3016 x 5376 -> 28672 SwiGLU, 5.25 rounds, 389 -> 378)
+            // (4096 x 13824 -> 5120, 1.25 rounds, 257 -> 216 us, 3016 x 5376 -> 28672, 5.25 rounds, in one product 389 -> 378)
             const int64_t large = b == 256 && parts == 1 ? groups / 256 * 256 / m : 0;
             bool mixed = false;
             if (large > 0 && large < n) {
@@ -1443,7 +1455,7 @@ double tiles_us(const Fh3kMx *w, const Fh3kMx *x, bool split, Plan &p) {
     p.ldp = (w->rows + 7) / 8 * 8;
     return least;
 }
-// split: FP8 rows to fp32, in two products
+// split: FP8 rows to fp32 or through SwiGLU, in two products
 Plan plan_of(const Fh3kMx *w, const Fh3kMx *x, bool swiglu, bool split) {
     Plan few = {}, tiles = {}, stream = {};
     few.kernel = Plan::FEW;
@@ -1496,9 +1508,10 @@ extern "C" int fh3k_mx_matmul_fits(const Fh3kMx *w, const Fh3kMx *x) {
 }
 
 extern "C" size_t fh3k_mx_matmul_ws_bytes(const Fh3kMx *w, const Fh3kMx *x, int swiglu) {
-    // the output's type is not known here: for either
+    // the output's type is not known here: for either (SwiGLU: its own)
     size_t most = 0;
-    for (int split = 0; split < (x->type == FH3K_MX_FP8 && !swiglu ? 2 : 1); split++) {
+    const bool f8 = x->type == FH3K_MX_FP8;
+    for (int split = f8 && swiglu ? 1 : 0; split < (f8 ? 2 : 1); split++) {
         const Plan p = plan_of(w, x, swiglu, split);
         const size_t n = p.parts > 1 ? (size_t)p.parts * p.ldp * x->rows * sizeof(float) : 0;
         most = n > most ? n : most;
@@ -1507,7 +1520,7 @@ extern "C" size_t fh3k_mx_matmul_ws_bytes(const Fh3kMx *w, const Fh3kMx *x, int 
 }
 
 extern "C" hipError_t fh3k_mx_matmul(const Fh3kMx *w, const Fh3kMx *x, const Fh3kMxOut *o, void *ws, hipStream_t st) {
-    const bool f8 = x->type == FH3K_MX_FP8, split = f8 && o->type == FH3K_F32 && !o->y.codes;
+    const bool f8 = x->type == FH3K_MX_FP8, split = f8 && o->type == FH3K_F32;   // SwiGLU: F32 too
     const Plan p = plan_of(w, x, o->y.codes, split);
     float *part = p.parts > 1 ? (float *)ws : nullptr;
     const int size = o->type == FH3K_F32 ? 4 : 2;

@@ -531,3 +531,52 @@ def test_many_threads_query_and_call(gpu):
     for t in threads:
         t.join()
     assert not errors, errors
+
+
+@pytest.mark.parametrize("rows,n,out", [(1, 5120, 640), (20, 1024, 640), (50, 2080, 512), (130, 1056, 640), (300, 4096, 1280), (2100, 1824, 8192)])
+def test_swiglu_codes_are_those_of_exact_sums(gpu, rows, n, out):
+    """FP8 rows: but for values within fp32 sums' error of a border between two codes, the formula's codes and scales."""
+    F, c, f = gpu, Repeated(rows + 5, rows, n, out, FP8), out // 2
+    x, w = c.arrays(F)
+    y, b = c.exact(F32)
+    o = Mx(F, FP8, rows, f)
+    need = F.mx_matmul_workspace_bytes(w.mx, x.mx, True)
+    ws = F.DeviceBuffer(max(1, need))
+    F.mx_matmul_swiglu_dev(w.mx, x.mx, o.mx, ws, need)
+    F.synchronize()
+    codes, s = o.read()
+    val, gate = y[:, :f], y[:, f:]
+    with np.errstate(over="ignore"):
+        act = val * gate / (1 + np.exp(-gate))
+    tol = np.abs(gate) * b[:, :f] + 1.1 * np.abs(val) * b[:, f:] + 1.1 * b[:, :f] * b[:, f:] + np.abs(act) * (8 + np.abs(gate)) * 2.0 ** -23
+    lo, hi = quantize(act - tol, FP8), quantize(act + tol, FP8)
+    amax, blocks = np.abs(act).reshape(rows, -1, 32), tol.reshape(rows, -1, 32)
+    s_lo, s_hi = scale_bytes(np.maximum(amax - blocks, 0).max(-1), FP8), scale_bytes((amax + blocks).max(-1), FP8)
+    assert ((s >= s_lo) & (s <= s_hi)).all()
+    sure = np.repeat((s_lo == s_hi) & (lo[1] == s) & (hi[1] == s), 32, 1)
+    got, least, most = (values(a, b, FP8) for a, b in ((codes, s), lo, hi))
+    assert ((got >= least) & (got <= most))[sure].all()
+
+
+@pytest.mark.parametrize("to", [FP8, FP4])
+@pytest.mark.parametrize("rows", [1, 20, 50, 300])
+def test_swiglu_of_fp8_rows_is_exact(gpu, rows, to):
+    """Eight products of very different sizes: large ones that cancel beside small ones that are the value; what a single
+    block-scaled instruction cuts off would change the codes.  The gates are 512 and more, where silu(g) is g."""
+    F, n, f = gpu, 256, 128
+    x = np.zeros((rows, n), np.uint8)
+    x[:, ::8], x[:, 1::8], x[:, 2::8], x[:, 3::8] = 0x7E, 0x01, 0x09, 0x58     # 448, 2^-9, 1.125 * 2^-6, 16
+    w = np.zeros((2 * f, n), np.uint8)
+    w[:f, ::16], w[:f, 8::16] = 2, 10                                          # 1 and -1: the large ones cancel
+    w[:f, 1::8], w[:f, 2::8] = 1, (np.arange(f) % 7 + 1)[:, None]
+    w[f:, 3::8] = 2
+    one = np.full((rows, n // 32), 127, np.uint8)
+    xm, wm, o = Mx(F, FP8, rows, n, x, one), Mx(F, FP4, 2 * f, n, w, one[:1].repeat(2 * f, 0)), Mx(F, to, rows, f)
+    need = F.mx_matmul_workspace_bytes(wm.mx, xm.mx, True)
+    ws = F.DeviceBuffer(max(1, need))
+    F.mx_matmul_swiglu_dev(wm.mx, xm.mx, o.mx, ws, need)
+    F.synchronize()
+    y = values(x, one, FP8) @ values(w, one[:1].repeat(2 * f, 0), FP4).T
+    assert (y[:, f:] == 512).all() and (y[:, :f] < 4).all()
+    got, want = o.read(), quantize(y[:, :f] * y[:, f:], to)
+    assert np.array_equal(got[1], want[1]) and np.array_equal(got[0], want[0])
