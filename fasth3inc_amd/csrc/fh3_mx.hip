@@ -275,11 +275,13 @@ __device__ __forceinline__ void set4(i32x8 &v, int at, const u32x4 &a) {
 // Outputs of 16 bits, whose own rounding is 2^-11 and more, take that.  fp32 outputs and
 // SwiGLU, whose codes it would move (3016 x 5376 -> 28672: 3e-3 of the codes' norm, scales
 // among them, where fp32 sums give 1e-4), come from two products, at half the rate:
-// e4m3 codes whose magnitude is 2 or more (bit 6 set); the others are c ^ that.  Within
-// each part the products with e2m1 codes span no more than 13 bits, so both are summed exactly.
-__device__ __forceinline__ uint32_t fp8_large(uint32_t c) {
-    // each byte's bit 6 in all of the byte's bits: the permutation's selectors 8 .. 11 are the signs of bytes 1, 3, 5, 7
-    return c & __builtin_amdgcn_perm(c << 1, c << 9, 0x0B090A08u);
+// e4m3 codes whose magnitude is 2 or more (bit 6 set), and the others.  Within each
+// part the products with e2m1 codes span no more than 13 bits, so both are summed exactly.
+// The selector of a byte is its place, in the permutation's second word or (+ 4) its first.
+__device__ __forceinline__ void fp8_split(uint32_t c, int &large, int &small) {
+    const uint32_t sel = (c >> 4 & 0x04040404u) | 0x03020100u;
+    large = (int)__builtin_amdgcn_perm(c, 0u, sel);
+    small = (int)__builtin_amdgcn_perm(0u, c, sel);
 }
 
 // ---------------------------------------------------------------------------
@@ -522,8 +524,10 @@ template <class G, bool SPLIT, int t, int tn, bool SC, int Q, int j = 0> __devic
             i32x8 h, l;
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                h[k] = (int)fp8_large((uint32_t)f.x[j][k]);
-                l[k] = f.x[j][k] ^ h[k];
+                int large, small;
+                fp8_split((uint32_t)f.x[j][k], large, small);
+                h[k] = large;
+                l[k] = small;
             }
             mx_mfma<t>(acc[j], f.w, s.w, h, s.x[j]);
             between();
@@ -912,7 +916,7 @@ template <bool F8> __global__ __launch_bounds__(256) void k_mx_join_swiglu(const
 // values, straight from memory into 16x16x128 products, and their sums meet in LDS.
 // Lane (r, g), g = 0 .. 3, holds of row r the FP4 codes 32 g .. + 31 of a step's 128, or
 // the FP8 codes 16 g .. + 15 and 64 + 16 g .. + 15, and the scale of block g.
-// FP8 rows to fp32 enter as two products (fp8_large).
+// FP8 rows to fp32 enter as two products (fp8_split).
 // SwiGLU: half of the R tiles are values' rows, half their gates'.
 // ---------------------------------------------------------------------------
 constexpr int MX_WAVES = 12, MX_WAVES_AHEAD = 8;   // the most wavefronts to a workgroup
@@ -1002,8 +1006,10 @@ template <bool F8, int TT, int R> struct Window {
                 if constexpr (SPLIT) {
 #pragma unroll
                     for (int k = 0; k < 8; k++) {
-                        h[k] = (int)fp8_large((uint32_t)v[k]);
-                        v[k] ^= h[k];
+                        int large, small;
+                        fp8_split((uint32_t)v[k], large, small);
+                        h[k] = large;
+                        v[k] = small;
                     }
 #pragma unroll
                     for (int i = 0; i < R; i++) acc[i][j] = mx_mfma16(w[i][s], h, acc[i][j], sw[i], sx, true);
@@ -1123,7 +1129,7 @@ template <bool F8, bool SPLIT, int TT, int R, bool AHEAD> __global__ __launch_bo
 // them while the next two are on their way; the wavefronts' sums meet in LDS four tiles at a time.
 // k_mx_few reads all of x for each 16 R weight rows: 20 rows x 5120 -> 51200 SwiGLU, 139 MB
 // of weights, took it 57 us, the tiles 43, this 32 (27.5 with one row: 5.1 TB/s), each in one
-// product; in two 39: 40 more VALU instructions for 32 codes (16 rows: the halves stay in registers, 30).
+// product; in two 38.5: 32 more VALU instructions for 32 codes (16 rows: the halves stay in registers, 30).
 // Where x is longer than 40 steps (24), each part of it has its own workgroups, and the
 // parts' sums are joined: 16 rows x 25600 -> 5120 29 us, tiles 24, this 19.
 // Two tiles to each splitting of FP8 codes (fp32 outputs, SwiGLU): with one, that took longer than the loads.
@@ -1240,8 +1246,10 @@ template <bool F8, bool SPLIT, int TT, int NS> __global__ __launch_bounds__(64 *
                     if constexpr (SPLIT) {
 #pragma unroll
                         for (int e = 0; e < 8; e++) {
-                            h[e] = (int)fp8_large((uint32_t)c[e]);
-                            c[e] ^= h[e];
+                            int large, small;
+                            fp8_split((uint32_t)c[e], large, small);
+                            h[e] = large;
+                            c[e] = small;
                         }
 #pragma unroll
                         for (int i = 0; i < 2; i++) acc[i][j] = mx_mfma16(v[d][i].w[s], h, acc[i][j], sw[i], (int)xs[j][s >> 2], s & 3, true);
