@@ -270,13 +270,16 @@ __device__ __forceinline__ void set4(i32x8 &v, int at, const u32x4 &a) {
 #pragma unroll
     for (int k = 0; k < 4; k++) v[at + k] = (int)a[k];
 }
-// The instruction aligns eight products to the largest one's power of two 2^E and cuts
-// off what lies below 2^(E - 13): with FP8 codes 4e-6 to 1.2e-5 of the result (FP4: nothing).
-// Outputs of 16 bits, whose own rounding is 2^-11 and more, take that.  fp32 outputs and
-// SwiGLU, whose codes it would move (3016 x 5376 -> 28672: 3e-3 of the codes' norm, scales
-// among them, where fp32 sums give 1e-4), come from two products, at half the rate:
-// e4m3 codes whose magnitude is 2 or more (bit 6 set), and the others.  Within each
-// part the products with e2m1 codes span no more than 13 bits, so both are summed exactly.
+// The instruction aligns eight products to 2^E, E the largest sum of two codes' exponents
+// among them, and cuts off what lies below 2^(E - 13): up to seven times 2^-13 of the
+// largest product, and where large ones cancel, all that is left (FP4 rows lose nothing:
+// their products span 2^4 to 2^-2).  So FP8 rows come in two products, at half the rate:
+// e4m3 codes whose magnitude is 2 or more (bit 6 set), and the others.  The first part's
+// products have E of 10 at most (448 = 1.75 * 2^8, 6 = 1.5 * 2^2) and are multiples of
+// 2^-3 (2.25 * 0.5), the second's E of 2 (1.875, 6) and multiples of 2^-10 (2^-9 * 0.5): 13 bits
+// or less below 2^E, so eight of them are summed exactly.  In one product 600 x 5120 -> 17408
+// bf16 took 56 us in place of 95, 32768 x 13824 -> 5120 1839 in place of 2980 and 16 x 25600 -> 5120
+// 19.1 in place of 19.8, but differed from rounded fp32 sums by 2e-4 of their norm (in two: by 1e-6).
 // The selector of a byte is its place, in the permutation's second word or (+ 4) its first.
 __device__ __forceinline__ void fp8_split(uint32_t c, int &large, int &small) {
     const uint32_t sel = (c >> 4 & 0x04040404u) | 0x03020100u;
@@ -298,8 +301,8 @@ __device__ __forceinline__ void fp8_split(uint32_t c, int &large, int &small) {
 // request to L2 for each row's 8 or 4 bytes of a stage took as many requests as the
 // codes) and are held in registers.
 // 8192 x 5120 -> 15360 FP4 322 us (4.0 PFLOP/s: products alone 190, DMA alone 193, with the
-// operands' reads 280), 32768 x 13824 -> 5120 FP8 1855 (2.5; the library's FP8 product 2.6),
-// in two products 3016 x 5376 -> 28672 SwiGLU 635 (2.9 PFLOP/s of them) and 3016 x 7168 -> 5376 fp32 178.
+// operands' reads 280); FP8 rows, in two products: 32768 x 13824 -> 5120 2980 (3.1 PFLOP/s of them),
+// 3016 x 5376 -> 28672 SwiGLU 635 (2.9), 3016 x 7168 -> 5376 fp32 175, 600 x 5120 -> 17408 95.
 // ---------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) void lds_void;
 
@@ -508,19 +511,19 @@ template <class G, int t, bool SC, int n, int end> __device__ __forceinline__ vo
 // next chunk's scales), and where Q is 0 or 1 that half of stage `to`'s loads into lb.
 // Loads are issued a few at a time: all at once they kept the matrix instructions behind
 // them waiting for the address unit.  Over one step or two: 8192 x 5120 -> 15360 FP4 362,
-// 353 us; 32768 x 13824 -> 5120 FP8 1826, 1850.
-template <class G, bool SPLIT, int t, int tn, bool SC, int Q, int j = 0> __device__ __forceinline__ void mx_step(
+// 353 us; FP8, of half as many steps to a stage, 815-826, 842, and 32768 x 13824 -> 5120 2860, 2890.
+template <class G, int t, int tn, bool SC, int Q, int j = 0> __device__ __forceinline__ void mx_step(
     f32x16 (&acc)[G::TX][G::TW], const Frags<G> &f, const StageScales<G> &s, Frags<G> &nf, Scales<G> &ns, const typename G::Buf &nb,
     const typename G::ScaleBuf &sb, const Load<G> &ld, typename G::Buf &lb, int to, int wr, int xr, int g) {
     if constexpr (j < G::TX) {
         constexpr int gap = Q * G::TX + j, gaps = G::HALVES * G::TX;
         auto between = [&]() {
             // (FP8 codes split in two leave registers for half of them)
-            constexpr int N = G::TW + G::TX, n0 = SPLIT ? j * N / G::TX : j ? N : 0, n1 = SPLIT ? (j + 1) * N / G::TX : N;
+            constexpr int N = G::TW + G::TX, n0 = G::F8 ? j * N / G::TX : j ? N : 0, n1 = G::F8 ? (j + 1) * N / G::TX : N;
             mx_reads<G, tn, SC, n0, n1>(nf, ns, nb, sb, wr, xr, g);
             if constexpr (Q >= 0 && Q < G::HALVES) ld.template codes<gap * G::D / gaps, (gap + 1) * G::D / gaps>(lb, to);
         };
-        if constexpr (SPLIT) {
+        if constexpr (G::F8) {
             i32x8 h, l;
 #pragma unroll
             for (int k = 0; k < 8; k++) {
@@ -538,7 +541,7 @@ template <class G, bool SPLIT, int t, int tn, bool SC, int Q, int j = 0> __devic
             between();
         }
         __builtin_amdgcn_sched_barrier(0);
-        mx_step<G, SPLIT, t, tn, SC, Q, j + 1>(acc, f, s, nf, ns, nb, sb, ld, lb, to, wr, xr, g);
+        mx_step<G, t, tn, SC, Q, j + 1>(acc, f, s, nf, ns, nb, sb, ld, lb, to, wr, xr, g);
     }
 }
 
@@ -748,7 +751,7 @@ template <bool F8, int TX, int TW> __device__ __forceinline__ void mx_swiglu_out
     }
 }
 
-template <class G, bool SPLIT> __global__ __launch_bounds__(64 * G::WAVES, 8 / G::WAVES) void k_mx_gemm(
+template <class G> __global__ __launch_bounds__(64 * G::WAVES, 8 / G::WAVES) void k_mx_gemm(
     Fh3kMx w, Fh3kMx x, Fh3kMxOut o, float *part, int64_t ldp, int m_tiles, int n_tiles, int first, int per, bool vec) {
     constexpr int TW = G::TW, TX = G::TX;
     __shared__ typename G::Buf b0, b1;
@@ -805,15 +808,15 @@ template <class G, bool SPLIT> __global__ __launch_bounds__(64 * G::WAVES, 8 / G
         constexpr int c = ci();
         const int left = ld.blocks - s * G::NB - g * G::T;   // blocks of the row for this lane's scale bytes
         mx_stage_scales<G, c>(ss, sc, g, left >= G::T ? -1 : left <= 0 ? 0 : (int)((1u << (8 * left)) - 1));
-        mx_step<G, SPLIT, 0, 1, false, 1>(acc, fr[0], ss, fr[1], sc, cur, sb, ld, prev, s + G::NBUF - 1, wr, xr, g);
+        mx_step<G, 0, 1, false, 1>(acc, fr[0], ss, fr[1], sc, cur, sb, ld, prev, s + G::NBUF - 1, wr, xr, g);
         if constexpr (G::T == 4) {
-            mx_step<G, SPLIT, 1, 2, false, -1>(acc, fr[1], ss, fr[0], sc, cur, sb, ld, prev, 0, wr, xr, g);
-            mx_step<G, SPLIT, 2, 3, false, -1>(acc, fr[0], ss, fr[1], sc, cur, sb, ld, prev, 0, wr, xr, g);
+            mx_step<G, 1, 2, false, -1>(acc, fr[1], ss, fr[0], sc, cur, sb, ld, prev, 0, wr, xr, g);
+            mx_step<G, 2, 3, false, -1>(acc, fr[0], ss, fr[1], sc, cur, sb, ld, prev, 0, wr, xr, g);
         }
         // this stage's operands are all read, the next one's have landed
         mx_barrier<(G::NBUF - 2) * G::D>();
         if constexpr (c == 0) ld.scales(sb, s + G::CH);   // this chunk's are all in registers
-        mx_step<G, SPLIT, G::T - 1, 0, c == G::CH - 1, 0>(acc, fr[1], ss, fr[0], sc, nxt, sb, ld, cur, s + G::NBUF, wr, xr, g);
+        mx_step<G, G::T - 1, 0, c == G::CH - 1, 0>(acc, fr[1], ss, fr[0], sc, nxt, sb, ld, cur, s + G::NBUF, wr, xr, g);
     };
     mx_settle(acc);
     using I0 = std::integral_constant<int, 0>;
@@ -911,12 +914,12 @@ template <bool F8> __global__ __launch_bounds__(256) void k_mx_join_swiglu(const
 
 // ---------------------------------------------------------------------------
 // Few rows (up to 16 TT), not too many weights: bound by the weights' way from memory and,
-// with x for each workgroup, from L2 (5120 -> 5120: 1 row 6.5 us, 32 rows 10.7).  A workgroup
+// with x for each workgroup, from L2 (5120 -> 5120: 1 row 7.2 us, 32 rows 11.3).  A workgroup
 // takes 16 R weight rows, its wavefronts a share each of the rows' windows of 128 S
 // values, straight from memory into 16x16x128 products, and their sums meet in LDS.
 // Lane (r, g), g = 0 .. 3, holds of row r the FP4 codes 32 g .. + 31 of a step's 128, or
 // the FP8 codes 16 g .. + 15 and 64 + 16 g .. + 15, and the scale of block g.
-// FP8 rows to fp32 enter as two products (fp8_split).
+// FP8 rows enter as two products (fp8_split).
 // SwiGLU: half of the R tiles are values' rows, half their gates'.
 // ---------------------------------------------------------------------------
 constexpr int MX_WAVES = 12, MX_WAVES_AHEAD = 8;   // the most wavefronts to a workgroup
@@ -991,7 +994,7 @@ template <bool F8, int TT, int R> struct Window {
     // the scale of step s's block g; past the row's end 0, whatever stands there
     __device__ __forceinline__ static int scale(uint32_t d, int s, int left, int g) { return 4 * s + g < left ? (int)(d >> (8 * g)) : 0; }
 
-    template <bool SPLIT> __device__ __forceinline__ void products(f32x4 (&acc)[R][TT], int left, int g) const {
+    __device__ __forceinline__ void products(f32x4 (&acc)[R][TT], int left, int g) const {
 #pragma unroll
         for (int s = 0; s < S; s++) {
             int sw[R];
@@ -1002,8 +1005,8 @@ template <bool F8, int TT, int R> struct Window {
                 const int sx = scale(xs[j][s], s, left, g);
                 i32x8 v = {}, h;
                 set4(v, 0, x[j][s][0]);
-                if constexpr (F8) set4(v, 4, x[j][s][1]);
-                if constexpr (SPLIT) {
+                if constexpr (F8) {
+                    set4(v, 4, x[j][s][1]);
 #pragma unroll
                     for (int k = 0; k < 8; k++) {
                         int large, small;
@@ -1065,7 +1068,7 @@ __device__ __forceinline__ void mx_put4(const Fh3kMxOut &o, int64_t t, int64_t n
     }
 }
 
-template <bool F8, bool SPLIT, int TT, int R, bool AHEAD> __global__ __launch_bounds__(64 * (AHEAD || TT == 4 || R * TT == 8 ? MX_WAVES_AHEAD : MX_WAVES)) void k_mx_few(Fh3kMx w, Fh3kMx x, Fh3kMxOut o) {
+template <bool F8, int TT, int R, bool AHEAD> __global__ __launch_bounds__(64 * (AHEAD || TT == 4 || R * TT == 8 ? MX_WAVES_AHEAD : MX_WAVES)) void k_mx_few(Fh3kMx w, Fh3kMx x, Fh3kMxOut o) {
     extern __shared__ f32x4 parts[];         // [wavefront][R][TT][64]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int r = lane & 15, g = lane >> 4;
@@ -1090,7 +1093,7 @@ template <bool F8, bool SPLIT, int TT, int R, bool AHEAD> __global__ __launch_bo
             if (a >= windows) break;
             if (!AHEAD) v[0].load(fw, fx, a, blocks - WBL * a, g);
             else if (b < windows) v[AHEAD ? 1 - h : 0].load(fw, fx, b, blocks - WBL * b, g);
-            v[AHEAD ? h : 0].template products<SPLIT>(acc, blocks - WBL * a, g);
+            v[AHEAD ? h : 0].products(acc, blocks - WBL * a, g);
         }
     }
 #pragma unroll
@@ -1128,11 +1131,11 @@ template <bool F8, bool SPLIT, int TT, int R, bool AHEAD> __global__ __launch_bo
 // 128 values) and takes tile after tile of 16 weight rows, straight from memory, two of
 // them while the next two are on their way; the wavefronts' sums meet in LDS four tiles at a time.
 // k_mx_few reads all of x for each 16 R weight rows: 20 rows x 5120 -> 51200 SwiGLU, 139 MB
-// of weights, took it 57 us, the tiles 43, this 32 (27.5 with one row: 5.1 TB/s), each in one
-// product; in two 38.5: 32 more VALU instructions for 32 codes (16 rows: the halves stay in registers, 30).
+// of weights, take it 58 us, the tiles 65, this 39 (FP4 rows 48, 34, 30; one FP8 row 29): the splitting
+// of FP8 codes is 32 VALU instructions to 32 codes (up to 16 rows the halves stay in registers: 31).
 // Where x is longer than 40 steps (24), each part of it has its own workgroups, and the
-// parts' sums are joined: 16 rows x 25600 -> 5120 29 us, tiles 24, this 19.
-// Two tiles to each splitting of FP8 codes (fp32 outputs, SwiGLU): with one, that took longer than the loads.
+// parts' sums are joined: 16 rows x 25600 -> 5120 30 us, tiles 39, this 21 with weights from memory.
+// Two tiles to each splitting of FP8 codes: with one, that took longer than the loads.
 // Nothing that is known before the loop is kept over it (the asm statements): the
 // registers are full of loads, and a reload from scratch waits for all loads before it.
 // ---------------------------------------------------------------------------
@@ -1176,7 +1179,7 @@ template <int NS> struct Streamed {
     }
 };
 
-template <bool F8, bool SPLIT, int TT, int NS> __global__ __launch_bounds__(64 * MX_STREAM, 2) void k_mx_stream(
+template <bool F8, int TT, int NS> __global__ __launch_bounds__(64 * MX_STREAM, 2) void k_mx_stream(
     Fh3kMx w, Fh3kMx x, Fh3kMxOut o, float *part, int64_t ldp, int units, int per) {
     __shared__ f32x4 sums[4][TT][MX_STREAM][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1240,10 +1243,10 @@ template <bool F8, bool SPLIT, int TT, int NS> __global__ __launch_bounds__(64 *
                 for (int j = 0; j < TT; j++) {
                     i32x8 c = {}, h;
                     // split here each time: kept, the halves take twice the registers (one tile of rows: there is room for them)
-                    if constexpr (SPLIT && TT > 1) asm volatile("" : "+v"(xc[j][s][0]), "+v"(xc[j][s][1]));
+                    if constexpr (F8 && TT > 1) asm volatile("" : "+v"(xc[j][s][0]), "+v"(xc[j][s][1]));
                     set4(c, 0, xc[j][s][0]);
-                    if constexpr (F8) set4(c, 4, xc[j][s][1]);
-                    if constexpr (SPLIT) {
+                    if constexpr (F8) {
+                        set4(c, 4, xc[j][s][1]);
 #pragma unroll
                         for (int e = 0; e < 8; e++) {
                             int large, small;
@@ -1379,17 +1382,21 @@ int few_tiles(const Fh3kMx *w, const Fh3kMx *x, bool swiglu) {
 
 // Each kernel's time in us by what was measured (weights from memory), of which the least is taken.
 // FP8 rows to bf16, k_mx_few, k_mx_stream and the tiles:
-//    5120 -> 5120           1 row 6.5, 8.1, -    32 rows 10.7, 12.6, -     64 rows -, 14.9, 15.0
-//    5120 -> 15360          1 row 12.9, 11.3, -  17 rows 18.5, 14.2, -     64 rows -, 22.1, 21.3
-//    25600 -> 5120          1 row 20.7, 19.0, -  16 rows -, 21.3, 27.3     64 rows -, 29.0, 31.0
-//    5120 -> 51200 in one   1 row 35.7, 28.2, -  17 rows 57, 32.0, 44.3    64 rows -, 47.5, 48.3
-double few_us(const Fh3kMx *w, const Fh3kMx *x, bool swiglu, bool split) {
+//    5120 -> 5120           1 row 7.3, 8.5, 14.7     32 rows 11.3, 15.0, 15.9   64 rows 20.6, 18.7, 17.5
+//    5120 -> 15360          1 row 13.3, 11.6, 24.6   17 rows 20.5, 16.7, 26.6   64 rows 43.5, 29.0, 28.4
+//    25600 -> 5120          1 row 21.2, 19.5, 36.5   16 rows 30.3, 21.6, 38.7   64 rows 78.4, 39.0, 40.7
+//    5120 -> 51200 SwiGLU   1 row 39.1, 29.1, 64.4   17 rows 56.5, 39.2, 65.5   64 rows 79.6, 68.6, 66.8
+// and FP4 rows:
+//    5120 -> 5120           1 row 6.2, 7.6, 10.8     32 rows 8.7, 9.8, 12.2     64 rows 12.3, 13.8, 13.7
+//    5120 -> 15360          1 row 12.9, 10.9, 16.8   17 rows 15.0, 12.2, 17.5   64 rows 27.6, 18.3, 20.5
+//    25600 -> 5120          1 row 19.1, 18.6, 24.4   16 rows 24.5, 20.1, 25.7   64 rows 50.6, 25.5, 28.5
+double few_us(const Fh3kMx *w, const Fh3kMx *x, bool swiglu) {
     const int64_t rows = 16 * few_tiles(w, x, swiglu), groups = (w->rows + rows - 1) / rows;
     const double row = (double)w->in * (x->type == FH3K_MX_FP8 ? 1.0 : 0.5), each = (double)rows * w->in / 2 + x->rows * row;
     // a workgroup's bytes through one CU, or all weights from memory and the rows for each workgroup from L2
     const double one = each / (x->rows <= 16 ? 38e3 : x->rows <= 32 ? 36e3 : rows == 64 ? 20e3 : 32e3);
     const double all = (double)w->rows * w->in * 0.53 / (4.4e6 * (groups < 200 ? groups / 200.0 : 1.0)) + groups * x->rows * row / 12e6;
-    const double more = !split || x->rows <= 16 ? 1 : x->rows <= 32 ? 1.35 : 1.8, a = 3.9 + one * more, b = (swiglu || x->rows > 32 ? 3.9 : 2.6) + all * more;
+    const double more = x->type == FH3K_MX_FP4 || x->rows <= 16 ? 1 : x->rows <= 32 ? 1.35 : 1.8, a = 3.9 + one * more, b = (swiglu || x->rows > 32 ? 3.9 : 2.6) + all * more;
     return a > b ? a : b;
 }
 // Steps of 128 values that a wavefront of k_mx_stream holds of x: what fits its registers
@@ -1397,7 +1404,7 @@ int stream_steps(const Fh3kMx *x) {
     const int steps = (int)((x->in + 127) / 128);
     return x->rows <= 32 || (x->type == FH3K_MX_FP4 && steps <= 5 * MX_STREAM) ? 5 : 3;
 }
-double stream_us(const Fh3kMx *w, const Fh3kMx *x, bool swiglu, bool split, Plan &p) {
+double stream_us(const Fh3kMx *w, const Fh3kMx *x, bool swiglu, Plan &p) {
     const int steps = (int)((w->in + 127) / 128), most = MX_STREAM * stream_steps(x);
     p.kernel = Plan::STREAM;
     p.per = (steps + (steps + most - 1) / most - 1) / ((steps + most - 1) / most);
@@ -1412,19 +1419,18 @@ double stream_us(const Fh3kMx *w, const Fh3kMx *x, bool swiglu, bool split, Plan
     const double each = (double)((p.n_tiles + p.m_tiles - 1) / p.m_tiles) * (blocks ? 4 : 1) * p.per;
     const double held = (double)x->rows * p.per * (x->type == FH3K_MX_FP8 ? 128 : 64);
     double t = 5 + each * 0.038 + held / 45e3 + (tt == 4 ? 1.5 : 0);
-    if (split && tt > 1) t += tt * (1 + each * 0.008);
+    if (x->type == FH3K_MX_FP8 && tt > 1) t += tt * (1 + each * 0.008);
     if (p.parts > 1) t += 2.5 + (double)p.parts * x->rows * w->rows * 8 / 4e6;
     return t;
 }
 // Tiles: for a stage on a CU that has one workgroup of 128 x 128, two, or one of 256 x 256, and for a round's
 // beginning and end; parts are written and read at 4 MB a us and joined by a launch of 3.5 us.  FP8 rows of 5120, weights
-// in the caches, small and large tiles: 600 rows -> 5120 23.3, 37 us; 400 -> 17408 57, 50; 1000 -> 15360 85, 63;
-// 13824 -> 5120: 600 rows 53.6, 64, 1000 rows 92, 85.
-double tiles_us(const Fh3kMx *w, const Fh3kMx *x, bool split, Plan &p) {
+// in the caches, small and large tiles: 600 rows -> 5120 39, 52 us; 400 -> 17408 93, 91; 1000 -> 15360 129, 108;
+// 13824 -> 5120: 600 rows 96, 91, 1000 rows 148, 122.  FP4 rows: 21, 31; 40, 32; 53, 41; 42, 46, 56, 65.
+double tiles_us(const Fh3kMx *w, const Fh3kMx *x, Plan &p) {
     const bool f8 = x->type == FH3K_MX_FP8;
     const int ks = f8 ? 128 : 256, stages = (int)((w->in + ks - 1) / ks);
-    const double more = split ? 1.5 : 1, one = f8 ? 0.51 * more : 0.88, few = f8 ? 0.78 * more : 0.95, two = f8 ? 0.95 * more : 1.15,
-                 big = f8 ? 1.2 * more : 1.6;
+    const double one = f8 ? 0.765 : 0.88, few = f8 ? 1.17 : 0.95, two = f8 ? 1.425 : 1.15, big = f8 ? 1.8 : 1.6;
     double least = 0;
     p.kernel = Plan::TILES;
     // a last round of smaller tiles: one to a CU, two to a few or to all
@@ -1439,7 +1445,7 @@ double tiles_us(const Fh3kMx *w, const Fh3kMx *x, bool split, Plan &p) {
             double t = (double)(groups / slots) * round + (rest ? last : 0);
             if (parts > 1) t += 3.5 + (double)parts * x->rows * w->rows * 8 / 4e6;
             // the last round, where it is not full, in smaller tiles: a launch of its own for the last columns
-            // (4096 x 13824 -> 5120, 1.25 rounds, 257 -> 216 us, 3016 x 5376 -> 28672, 5.25 rounds, in one product 389 -> 378)
+            // (4096 x 13824 -> 5120, 1.25 rounds, FP8 432 -> 380 us, FP4 170 -> 146; 3016 x 5376 -> 28672, 5.25 rounds, 678 -> 644)
             const int64_t large = b == 256 && parts == 1 ? groups / 256 * 256 / m : 0;
             bool mixed = false;
             if (large > 0 && large < n) {
@@ -1463,30 +1469,29 @@ double tiles_us(const Fh3kMx *w, const Fh3kMx *x, bool split, Plan &p) {
     p.ldp = (w->rows + 7) / 8 * 8;
     return least;
 }
-// split: FP8 rows to fp32 or through SwiGLU, in two products
-Plan plan_of(const Fh3kMx *w, const Fh3kMx *x, bool swiglu, bool split) {
+Plan plan_of(const Fh3kMx *w, const Fh3kMx *x, bool swiglu) {
     Plan few = {}, tiles = {}, stream = {};
     few.kernel = Plan::FEW;
     few.parts = 1;
     if (x->rows > 64) {
-        tiles_us(w, x, split, tiles);
+        tiles_us(w, x, tiles);
         return tiles;
     }
-    const double s = stream_us(w, x, swiglu, split, stream), f = few_us(w, x, swiglu, split), least = s < f ? s : f;
+    const double s = stream_us(w, x, swiglu, stream), f = few_us(w, x, swiglu), least = s < f ? s : f;
     // tiles: no less than the weights' way from memory (16 rows: never the least)
-    if (x->rows > 16 && 8 + (double)w->rows * w->in * 0.53 / 3.2e6 < least && tiles_us(w, x, split, tiles) < least) return tiles;
+    if (x->rows > 16 && 8 + (double)w->rows * w->in * 0.53 / 3.2e6 < least && tiles_us(w, x, tiles) < least) return tiles;
     return f <= s ? few : stream;
 }
 
 // Columns first .. of tiles, all or those before `end`.
-template <class G, bool SPLIT> void launch_gemm(const Fh3kMx *w, const Fh3kMx *x, const Fh3kMxOut *o, const Plan &p, int64_t first, int64_t end,
+template <class G> void launch_gemm(const Fh3kMx *w, const Fh3kMx *x, const Fh3kMxOut *o, const Plan &p, int64_t first, int64_t end,
                                                 float *part, bool vec, hipStream_t st) {
     const int64_t m = (x->rows + G::BX - 1) / G::BX, all = (w->rows + G::BW - 1) / G::BW, n = (end ? end : all) - first;
     const dim3 grid((unsigned)(m * n), (unsigned)p.parts);
-    k_mx_gemm<G, SPLIT><<<grid, 64 * G::WAVES, 0, st>>>(*w, *x, *o, part, p.ldp, (int)m, (int)n, (int)first, p.per, vec || part);
+    k_mx_gemm<G><<<grid, 64 * G::WAVES, 0, st>>>(*w, *x, *o, part, p.ldp, (int)m, (int)n, (int)first, p.per, vec || part);
 }
 
-template <bool F8, bool SPLIT, int TT, int R> void launch_few(const Fh3kMx *w, const Fh3kMx *x, const Fh3kMxOut *o, hipStream_t st) {
+template <bool F8, int TT, int R> void launch_few(const Fh3kMx *w, const Fh3kMx *x, const Fh3kMxOut *o, hipStream_t st) {
     const int64_t n = o->y.codes ? w->rows / 2 : w->rows, per = o->y.codes ? 8 * R : 16 * R;
     // as many wavefronts as share the windows evenly, and whose sums fit 64 KiB; where
     // that leaves each more than one, eight that load ahead
@@ -1495,7 +1500,7 @@ template <bool F8, bool SPLIT, int TT, int R> void launch_few(const Fh3kMx *w, c
     auto go = [&](auto ahead, int most) {
         if (most > room) most = room;
         const int each = (windows + most - 1) / most, waves = (windows + each - 1) / each;
-        k_mx_few<F8, SPLIT, TT, R, ahead()><<<(unsigned)((n + per - 1) / per), 64 * waves, waves * R * TT * 1024, st>>>(*w, *x, *o);
+        k_mx_few<F8, TT, R, ahead()><<<(unsigned)((n + per - 1) / per), 64 * waves, waves * R * TT * 1024, st>>>(*w, *x, *o);
     };
     // (registers for two windows)
     if constexpr (Window<F8, TT, R>::S * (R + TT * (F8 ? 2 : 1)) <= 20) {
@@ -1511,25 +1516,18 @@ bool sixteens(const void *p, int64_t ld, int size) { return !p || ((uintptr_t)p 
 
 extern "C" int fh3k_mx_matmul_fits(const Fh3kMx *w, const Fh3kMx *x) {
     if ((x->rows + 127) / 128 * ((w->rows + 127) / 128) < ((int64_t)1 << 23) && (w->rows + 7) / 8 * 8 * x->rows <= ((int64_t)1 << 40)) return 1;
-    const Plan p = plan_of(w, x, false, false);
+    const Plan p = plan_of(w, x, false);
     return (p.kernel != Plan::TILES || p.m_tiles * p.n_tiles < ((int64_t)1 << 23)) && p.ldp * x->rows <= ((int64_t)1 << 40);
 }
 
 extern "C" size_t fh3k_mx_matmul_ws_bytes(const Fh3kMx *w, const Fh3kMx *x, int swiglu) {
-    // the output's type is not known here: for either (SwiGLU: its own)
-    size_t most = 0;
-    const bool f8 = x->type == FH3K_MX_FP8;
-    for (int split = f8 && swiglu ? 1 : 0; split < (f8 ? 2 : 1); split++) {
-        const Plan p = plan_of(w, x, swiglu, split);
-        const size_t n = p.parts > 1 ? (size_t)p.parts * p.ldp * x->rows * sizeof(float) : 0;
-        most = n > most ? n : most;
-    }
-    return most;
+    const Plan p = plan_of(w, x, swiglu);
+    return p.parts > 1 ? (size_t)p.parts * p.ldp * x->rows * sizeof(float) : 0;
 }
 
 extern "C" hipError_t fh3k_mx_matmul(const Fh3kMx *w, const Fh3kMx *x, const Fh3kMxOut *o, void *ws, hipStream_t st) {
-    const bool f8 = x->type == FH3K_MX_FP8, split = f8 && o->type == FH3K_F32;   // SwiGLU: F32 too
-    const Plan p = plan_of(w, x, o->y.codes, split);
+    const bool f8 = x->type == FH3K_MX_FP8;
+    const Plan p = plan_of(w, x, o->y.codes);
     float *part = p.parts > 1 ? (float *)ws : nullptr;
     const int size = o->type == FH3K_F32 ? 4 : 2;
     const bool vec = sixteens(o->out, o->ldo, size) && sixteens(o->res, o->ldres, size) && sixteens(o->gate, w->rows, 4);
@@ -1542,41 +1540,39 @@ extern "C" hipError_t fh3k_mx_matmul(const Fh3kMx *w, const Fh3kMx *x, const Fh3
     using Big8 = Gemm<4, 2, 2, 4, true, 128, 3>;
     using Small4 = Gemm<2, 2, 2, 2, false, 256, 2>;
     using Small8 = Gemm<2, 2, 2, 2, true, 128, 3>;
-    auto few = [&](auto f, auto sp) {
+    auto few = [&](auto f) {
         const int r = few_tiles(w, x, o->y.codes);
         auto go = [&](auto tt) {
-            if (r == 4) launch_few<f(), sp(), tt(), 4>(w, x, o, st);
-            else if (r == 2) launch_few<f(), sp(), tt(), 2>(w, x, o, st);
-            else launch_few<f(), sp(), tt(), 1>(w, x, o, st);
+            if (r == 4) launch_few<f(), tt(), 4>(w, x, o, st);
+            else if (r == 2) launch_few<f(), tt(), 2>(w, x, o, st);
+            else launch_few<f(), tt(), 1>(w, x, o, st);
         };
         if (x->rows <= 16) go(N1{});
         else if (x->rows <= 32) go(N2{});
         else go(N4{});
     };
-    auto stream = [&](auto f, auto sp) {
+    auto stream = [&](auto f) {
         auto go = [&](auto tt, auto ns) {
             const dim3 grid((unsigned)p.m_tiles, (unsigned)p.parts);
-            k_mx_stream<f(), sp(), tt(), ns()><<<grid, 64 * MX_STREAM, 0, st>>>(*w, *x, *o, part, p.ldp, (int)p.n_tiles, p.per);
+            k_mx_stream<f(), tt(), ns()><<<grid, 64 * MX_STREAM, 0, st>>>(*w, *x, *o, part, p.ldp, (int)p.n_tiles, p.per);
         };
         if (x->rows <= 16) go(N1{}, N5{});
         else if (x->rows <= 32) go(N2{}, N5{});
         else if (stream_steps(x) == 3) go(N4{}, N3{});
         else if constexpr (!f()) go(N4{}, N5{});
     };
-    auto tiles = [&](auto large, auto small, auto sp) {
-        if (p.bw == 256) launch_gemm<decltype(large), sp()>(w, x, o, p, 0, p.large, part, vec, st);
-        if (p.bw == 128 || p.large) launch_gemm<decltype(small), sp()>(w, x, o, p, 2 * p.large, 0, part, vec, st);
+    auto tiles = [&](auto large, auto small) {
+        if (p.bw == 256) launch_gemm<decltype(large)>(w, x, o, p, 0, p.large, part, vec, st);
+        if (p.bw == 128 || p.large) launch_gemm<decltype(small)>(w, x, o, p, 2 * p.large, 0, part, vec, st);
     };
     auto by_rows = [&](auto go) {
-        if (!f8) go(std::false_type{}, std::false_type{});
-        else if (!split) go(std::true_type{}, std::false_type{});
-        else go(std::true_type{}, std::true_type{});
+        if (f8) go(std::true_type{});
+        else go(std::false_type{});
     };
     if (p.kernel == Plan::FEW) by_rows(few);
     else if (p.kernel == Plan::STREAM) by_rows(stream);
-    else if (!f8) tiles(Big4{}, Small4{}, std::false_type{});
-    else if (!split) tiles(Big8{}, Small8{}, std::false_type{});
-    else tiles(Big8{}, Small8{}, std::true_type{});
+    else if (f8) tiles(Big8{}, Small8{});
+    else tiles(Big4{}, Small4{});
     if (!part) return hipGetLastError();
     if (o->y.codes) {
         const dim3 grid((unsigned)x->rows, (unsigned)((o->y.in + 2047) / 2048));
