@@ -302,7 +302,7 @@ __device__ __forceinline__ void fp8_split(uint32_t c, int &large, int &small) {
 // codes) and are held in registers.
 // 8192 x 5120 -> 15360 FP4 322 us (4.0 PFLOP/s: products alone 190, DMA alone 193, with the
 // operands' reads 280); FP8 rows, in two products: 32768 x 13824 -> 5120 2980 (3.1 PFLOP/s of them),
-// 3016 x 5376 -> 28672 SwiGLU 635 (2.9), 3016 x 7168 -> 5376 fp32 175, 600 x 5120 -> 17408 95.
+// 3016 x 5376 -> 28672 SwiGLU 639 (2.9), 3016 x 7168 -> 5376 fp32 175, 600 x 5120 -> 17408 95.
 // ---------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) void lds_void;
 
@@ -558,16 +558,20 @@ template <int TX, int TW> __device__ __forceinline__ void mx_settle(f32x16 (&acc
         for (int j = 0; j < TW; j++) asm volatile("" : "+a"(acc[i][j]));
 }
 
-// g / (1 + exp(-g)) to about two units in the last place: from e = exp(-|g|), which cannot overflow, with the rest of
-// exp2's rounded argument (up to 1e-6 of e at |g| = 20) and the reciprocal's error taken out.
-__device__ __forceinline__ float silu(float g) {
-    const float m = -fminf(fabsf(g), 200.f), a = m * LOG2E, rest = __builtin_fmaf(m, LOG2E, -a) + m * LOG2E_REST;
-    float e = __builtin_amdgcn_exp2f(a);
+// v * g / (1 + exp(-g)) to a few units in the last place: from e = exp(-|g|), which cannot overflow, with the rest of
+// exp2's rounded argument (up to 1e-6 of e at |g| = 20) and the reciprocal's error taken out.  exp2's results below 2^-126 are
+// zero, which with g from -87 on and large v would be seen (-88: -5e-37 v): where e is below 2^-100, it is kept 2^160 times as large, and
+// that is taken from v and from the product in two halves, neither of which leaves fp32's range where a code is not zero anyway.
+__device__ __forceinline__ float swiglu(float v, float g) {
+    const float m = -fminf(fabsf(g), 230.f), a = m * LOG2E, rest = __builtin_fmaf(m, LOG2E, -a) + m * LOG2E_REST;
+    const bool far = a < -100.f;
+    float e = __builtin_amdgcn_exp2f(far ? a + 160.f : a);   // (exact: multiples of a's last place)
     e = __builtin_fmaf(e, rest * 0.69314718f, e);
-    const float d = 1.f + e;
+    const float d = far ? 1.f : 1.f + e;
     float r = __builtin_amdgcn_rcpf(d);
     r = __builtin_fmaf(r, __builtin_fmaf(-d, r, 1.f), r);
-    return (g < 0.f ? g * e : g) * r;
+    const float s = (g < 0.f ? g * e : g) * r;
+    return far && g < 0.f ? v * 0x1p-80f * s * 0x1p-80f : v * s;
 }
 
 // Eight values of a row, or one, to where they go; Beside: what is read for them.
@@ -723,7 +727,7 @@ template <bool F8, int TX, int TW> __device__ __forceinline__ void mx_swiglu_out
             for (int k = 0; k < 8; k++) {
                 const int n = col + 16 * m + 8 * g + k;
                 const float bv = o.bias ? o.bias[n] : 0.f, bg = o.bias ? o.bias[f + n] : 0.f;
-                v[m][k] = (v[m][k] + bv) * silu(q[m][k] + bg);
+                v[m][k] = swiglu(v[m][k] + bv, q[m][k] + bg);
                 const uint32_t w = __builtin_bit_cast(uint32_t, v[m][k]) & 0x7FFFFFFFu;
                 u = u > w ? u : w;
             }
@@ -908,7 +912,7 @@ template <bool F8> __global__ __launch_bounds__(256) void k_mx_join_swiglu(const
     mx_add_parts(part, S, rows * ldp, t * ldp + col, v);
     mx_add_parts(part, S, rows * ldp, t * ldp + f + col, q);
 #pragma unroll
-    for (int k = 0; k < 8; k++) a[k] = (v[k] + (o.bias ? o.bias[col + k] : 0.f)) * silu(q[k] + (o.bias ? o.bias[f + col + k] : 0.f));
+    for (int k = 0; k < 8; k++) a[k] = swiglu(v[k] + (o.bias ? o.bias[col + k] : 0.f), q[k] + (o.bias ? o.bias[f + col + k] : 0.f));
     mx_store<F8>(o.y, t, col, a);
 }
 
@@ -1034,7 +1038,7 @@ __device__ __forceinline__ void mx_swiglu16(const Fh3kMxOut &o, const f32x4 &v0,
     for (int k = 0; k < 8; k++) {
         const int64_t n = n0 + 16 * (k >> 2) + 4 * g + (k & 3);
         const float v = k < 4 ? v0[k & 3] : v1[k & 3], q = k < 4 ? q0[k & 3] : q1[k & 3];
-        a[k] = (v + (o.bias ? o.bias[n] : 0.f)) * silu(q + (o.bias ? o.bias[f + n] : 0.f));
+        a[k] = swiglu(v + (o.bias ? o.bias[n] : 0.f), q + (o.bias ? o.bias[f + n] : 0.f));
         const float c = a[k];
         const uint32_t b = __builtin_bit_cast(uint32_t, c) & 0x7FFFFFFFu;
         u = u > b ? u : b;
@@ -1445,7 +1449,7 @@ double tiles_us(const Fh3kMx *w, const Fh3kMx *x, Plan &p) {
             double t = (double)(groups / slots) * round + (rest ? last : 0);
             if (parts > 1) t += 3.5 + (double)parts * x->rows * w->rows * 8 / 4e6;
             // the last round, where it is not full, in smaller tiles: a launch of its own for the last columns
-            // (4096 x 13824 -> 5120, 1.25 rounds, FP8 432 -> 380 us, FP4 170 -> 146; 3016 x 5376 -> 28672, 5.25 rounds, 678 -> 644)
+            // (4096 x 13824 -> 5120, 1.25 rounds, FP8 432 -> 380 us, FP4 170 -> 146; 3016 x 5376 -> 28672, 5.25 rounds, 678 -> 643)
             const int64_t large = b == 256 && parts == 1 ? groups / 256 * 256 / m : 0;
             bool mixed = false;
             if (large > 0 && large < n) {

@@ -108,3 +108,36 @@ def test_swiglu(gpu, rows, n, out, to, fmt):
     got, want = y.read(), quantize(val * gate, to)
     assert np.array_equal(got[1], want[1])
     assert np.array_equal(got[0], want[0])
+
+
+# gates from where exp(g) leaves fp32's normal numbers on, beside values that bring the result back among the codes
+FAR = [(1.0, -87.4, 4.0), (-3.0, -92.0, 3.0), (2.0 ** 40, -110.0, 20.0), (-(2.0 ** 100), -150.0, 20.0), (3e38, -186.0, 30.0), (1.0, -20.0, 40.0),
+       (2.0 ** -20, -80.0, 12.0), (1e38, -400.0, 100.0)]
+
+
+@pytest.mark.parametrize("to", [FP8, FP4])
+@pytest.mark.parametrize("rows,n,out", [(1, 96, 1024), (19, 5088, 40064), (12, 13856, 20096), (130, 1056, 1280), (300, 4096, 1280), (1930, 1824, 4480)])
+def test_swiglu_of_far_negative_gates(gpu, rows, n, out, to):
+    """Rows of zeros and a bias that holds values and gates.  Relative errors: exp2 and the reciprocal a unit in the last place
+    (2^-23) each, seven roundings of 2^-24; below 2^-126 two steps of 2^-149."""
+    f, rng = out // 2, np.random.default_rng(out)
+    kind = np.arange(f) // 32 % len(FAR)
+    v, g, w = (np.array([c[i] for c in FAR])[kind] for i in range(3))
+    bias = np.concatenate([v, g - w * rng.random(f)]).astype(np.float32)
+    x = Mx(gpu, FP8, rows, n, np.zeros((rows, n), np.uint8), np.full((rows, n // 32), 127, np.uint8))
+    wm = Mx(gpu, FP4, out, n, rng.integers(0, 16, (1, n)).astype(np.uint8).repeat(out, 0), np.full((out, n // 32), 127, np.uint8))
+    y, need = Mx(gpu, to, rows, f), gpu.mx_matmul_workspace_bytes(wm.mx, x.mx, True)
+    ws = gpu.DeviceBuffer(max(1, need))
+    gpu.mx_matmul_swiglu_dev(wm.mx, x.mx, y.mx, ws, need, d_bias=buf(gpu, bias))
+    gpu.synchronize()
+    codes, s = y.read()
+    assert (codes == codes[:1]).all() and (s == s[:1]).all()
+    b = bias.astype(np.float64)
+    act = (b[:f] * b[f:] / (1 + np.exp(-b[f:])))[None]
+    off = np.abs(act) * 2.0 ** -20 + 2.0 ** -148
+    low, high = quantize(np.sign(act) * (np.abs(act) - off).clip(0), to), quantize(np.sign(act) * (np.abs(act) + off), to)
+    assert ((s[:1] >= low[1]) & (s[:1] <= high[1])).all()
+    sure = np.repeat(low[1] == high[1], 32, 1)
+    a, lo, hi = (np.abs(values(*c, to)) for c in ((codes[:1], s[:1]), low, high))
+    assert ((a >= lo) & (a <= hi))[sure].all() and sure.mean() > 0.9
+    assert codes[0].reshape(-1, 32).any(1)[kind[::32] < 4].all()
