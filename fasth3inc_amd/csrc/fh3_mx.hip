@@ -194,12 +194,12 @@ template <int T, bool F8> __global__ __launch_bounds__(256) void k_mx_dequant(Fh
 }
 
 // A 64-bit value cut to fp32, the last bit set where anything was cut off: rounding
-// that to a code gives what rounding the value itself gives.
+// that to a code gives what rounding the value itself gives.  Past fp32's range: infinite.
 __device__ __forceinline__ float cut(double d) {
     const float f = (float)d;
     const double b = (double)f;
     uint32_t u = __builtin_bit_cast(uint32_t, f);
-    if (b != d) u = (u - (fabs(b) > fabs(d) ? 1u : 0u)) | 1u;
+    if (b != d && fabs(b) <= 3.4028234663852886e38) u = (u - (fabs(b) > fabs(d) ? 1u : 0u)) | 1u;
     return __builtin_bit_cast(float, u);
 }
 

@@ -372,7 +372,8 @@ int fh3_hip_mx_dequant_dev(const Fh3Mx *x, int type, void *d_y, int64_t ldy, voi
  * ([rows][in] fp32, both or neither) n * (1 + scale) + shift, as
  * fh3_hip_rownorm_dev; quantised to y as above.  d_add NULL: h = x, and d_sum may be
  * NULL (else it gets a copy).  d_sum may be d_x or d_add itself (with its row stride).
- * y->in at most 32768.  Sums of squares are in 64 bits: rows of any finite size. */
+ * y->in at most 32768.  Sums of squares are in 64 bits: rows of any finite size.  A
+ * value that leaves fp32's range on its way to y is an infinity. */
 int fh3_hip_mx_norm_dev(int type, const void *d_x, int64_t ldx, const void *d_add, int64_t ldadd, void *d_sum,
                         int64_t ldsum, const float *d_norm_w, float eps, const float *d_shift, const float *d_scale,
                         const Fh3Mx *y, void *stream);

@@ -141,3 +141,26 @@ def test_swiglu_of_far_negative_gates(gpu, rows, n, out, to):
     a, lo, hi = (np.abs(values(*c, to)) for c in ((codes[:1], s[:1]), low, high))
     assert ((a >= lo) & (a <= hi))[sure].all() and sure.mean() > 0.9
     assert codes[0].reshape(-1, 32).any(1)[kind[::32] < 4].all()
+
+
+@pytest.mark.parametrize("to", [FP8, FP4])
+@pytest.mark.parametrize("modulate", [False, True])
+def test_norm_past_fp32(gpu, modulate, to):
+    """Values that fp32 cannot hold (through a weight, or a modulation) make their block NaN, as infinities do, and no other."""
+    rows, n = 3, 256
+    x, w = np.ones((rows, n), np.float32), np.ones(n, np.float32)
+    x[1], x[1, 40] = 0, 4                                     # 16 after the norm
+    w[40] = 3e37
+    scale, shift = np.zeros((rows, n), np.float32), np.zeros((rows, n), np.float32)
+    if modulate:
+        w[40], scale[1, 40], shift[2, 200], scale[2, 200] = 1, 3e37, -3e38, -3e38
+    y, d = Mx(gpu, to, rows, n), [buf(gpu, a) for a in (x, w, shift, scale)]
+    gpu.mx_norm_dev(F32, d[0], d[1], 0.0, y.mx, d_shift=d[2] if modulate else None, d_scale=d[3] if modulate else None)
+    gpu.synchronize()
+    codes, s = y.read()
+    nan = np.zeros(s.shape, bool)
+    nan[1, 1], nan[2, 6] = True, modulate
+    assert np.array_equal(s == 255, nan) and not codes[np.repeat(nan, 32, 1)].any()
+    e = x / np.sqrt((x.astype(np.float64) ** 2).mean(-1, keepdims=True)) * w.astype(np.float64)
+    want = quantize(np.where(np.repeat(nan, 32, 1), 0, e * (1 + scale.astype(np.float64)) + shift), to)
+    assert np.array_equal(s[~nan], want[1][~nan]) and np.array_equal(codes[~np.repeat(nan, 32, 1)], want[0][~np.repeat(nan, 32, 1)])
