@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 
 from mx_ref import BF16, F16, F32, FP4, FP8, Mx, buf, from_type, quantize, to_type, values
+from test_gpu_mx_calls import test_swiglu_codes_are_those_of_exact_sums as codes_of_exact_sums
 
 pytestmark = pytest.mark.gpu
 
@@ -164,3 +165,9 @@ def test_norm_past_fp32(gpu, modulate, to):
     e = x / np.sqrt((x.astype(np.float64) ** 2).mean(-1, keepdims=True)) * w.astype(np.float64)
     want = quantize(np.where(np.repeat(nan, 32, 1), 0, e * (1 + scale.astype(np.float64)) + shift), to)
     assert np.array_equal(s[~nan], want[1][~nan]) and np.array_equal(codes[~np.repeat(nan, 32, 1)], want[0][~np.repeat(nan, 32, 1)])
+
+
+@pytest.mark.parametrize("rows,n,out", [(19, 5088, 40064), (40, 5088, 40064), (12, 13856, 20096), (30, 13856, 20096), (422, 16480, 5504)])
+def test_swiglu_codes_of_random_rows(gpu, rows, n, out):
+    """Streamed weights, whole and in parts, and large tiles in parts: the formula's codes but where fp32 sums leave two."""
+    codes_of_exact_sums(gpu, rows, n, out)
