@@ -278,7 +278,7 @@ __device__ __forceinline__ void set4(i32x8 &v, int at, const u32x4 &a) {
 // products have E of 10 at most (448 = 1.75 * 2^8, 6 = 1.5 * 2^2) and are multiples of
 // 2^-3 (2.25 * 0.5), the second's E of 2 (1.875, 6) and multiples of 2^-10 (2^-9 * 0.5): 13 bits
 // or less below 2^E, so eight of them are summed exactly.  In one product 600 x 5120 -> 17408
-// bf16 took 56 us in place of 95, 32768 x 13824 -> 5120 1839 in place of 2980 and 16 x 25600 -> 5120
+// bf16 took 56 us in place of 95, 32768 x 13824 -> 5120 1839 in place of 2980, and 16 x 25600 -> 5120
 // 19.1 in place of 19.8, but differed from rounded fp32 sums by 2e-4 of their norm (in two: by 1e-6).
 // The selector of a byte is its place, in the permutation's second word or (+ 4) its first.
 __device__ __forceinline__ void fp8_split(uint32_t c, int &large, int &small) {
@@ -301,7 +301,7 @@ __device__ __forceinline__ void fp8_split(uint32_t c, int &large, int &small) {
 // request to L2 for each row's 8 or 4 bytes of a stage took as many requests as the
 // codes) and are held in registers.
 // 8192 x 5120 -> 15360 FP4 322 us (4.0 PFLOP/s: products alone 190, DMA alone 193, with the
-// operands' reads 280); FP8 rows, in two products: 32768 x 13824 -> 5120 2980 (3.1 PFLOP/s of them),
+// operands' reads 280); FP8 rows, in two products: 32768 x 13824 -> 5120 2980 (3.1 PFLOP/s of both),
 // 3016 x 5376 -> 28672 SwiGLU 639 (2.9), 3016 x 7168 -> 5376 fp32 175, 600 x 5120 -> 17408 95.
 // ---------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) void lds_void;
@@ -702,7 +702,7 @@ template <int T, int TX, int TW> __device__ __forceinline__ void mx_rows_out(con
 }
 // The same where the wavefront's first tiles are values and the others their gates: SwiGLU to codes.  A block is a
 // tile's 32 columns.  Codes and scales come together in the wavefront's piece of LDS, [32 TX][BYTES], and leave 16 bytes
-// to a lane and a row's scales at once: from the registers a store covered 16 bytes of 32 rows (3016 x 5376 -> 28672 in one product 402 -> 391 us).
+// to a lane and a row's scales at once: from the registers a store covered 16 bytes of 32 rows (3016 x 5376 -> 28672, FP8 rows in one product, 402 -> 391 us).
 template <bool F8, int TX, int TW> __device__ __forceinline__ void mx_swiglu_out(const Fh3kMxOut &o, const f32x16 (&acc)[TX][TW], uint8_t *stg, int lane,
                                                                                  int64_t t0, int64_t rows, int f0) {
     constexpr int J = TW / 2, BYTES = F8 ? 32 * J : 16 * J, LD = BYTES + 16, L = BYTES / 16, TOKENS = 32 * TX;   // + 16: other banks for each row

@@ -372,8 +372,8 @@ int fh3_hip_mx_dequant_dev(const Fh3Mx *x, int type, void *d_y, int64_t ldy, voi
  * ([rows][in] fp32, both or neither) n * (1 + scale) + shift, as
  * fh3_hip_rownorm_dev; quantised to y as above.  d_add NULL: h = x, and d_sum may be
  * NULL (else it gets a copy).  d_sum may be d_x or d_add itself (with its row stride).
- * y->in at most 32768.  Sums of squares are in 64 bits: rows of any finite size.  A
- * value that leaves fp32's range on its way to y is an infinity. */
+ * y->in at most 32768.  Sums of squares are in 64 bits: rows of any finite size.
+ * What is quantised counts as an infinity where it is past fp32's range. */
 int fh3_hip_mx_norm_dev(int type, const void *d_x, int64_t ldx, const void *d_add, int64_t ldadd, void *d_sum,
                         int64_t ldsum, const float *d_norm_w, float eps, const float *d_shift, const float *d_scale,
                         const Fh3Mx *y, void *stream);
@@ -395,9 +395,11 @@ int fh3_hip_mx_norm_dev(int type, const void *d_x, int64_t ldx, const void *d_ad
  *
  * fh3_hip_mx_matmul_swiglu_dev: W's rows are [val (F) | gate (F)], 2 F == w->rows a
  * multiple of 128, as FH3_EPI_SWIGLU; y [x->rows][F] = val * silu(gate), bias
- * included, quantised as above for the product that follows.  The workspace is that
- * of (w, x, 1).  Only the sizes and types in w and x are read for its size; 0 is
- * also the answer for sizes that are refused. */
+ * included, quantised as above for the product that follows; where the fp32 sums'
+ * rounding puts a value on the other side of a border between two codes, or a block's
+ * largest value on that of one between two scales, the codes are that side's.  The
+ * workspace is that of (w, x, 1).  Only the sizes and types in w and x are read for
+ * its size; 0 is also the answer for sizes that are refused. */
 size_t fh3_hip_mx_matmul_workspace_bytes(const Fh3Mx *w, const Fh3Mx *x, int swiglu);
 int fh3_hip_mx_matmul_dev(const Fh3Mx *w, const Fh3Mx *x, const float *d_bias, const float *d_gate, const void *d_res,
                           int64_t ldres, int type, void *d_y, int64_t ldy, void *d_ws, size_t ws_bytes, void *stream);
